@@ -71,8 +71,17 @@ enum {
  * block, the 16 slots of each 32-element group are adjacent, so one kv
  * head's scales of a block are one contiguous run).
  * kv_dim must be a multiple of 32 (head_dim too for the RoPE append). Gather
- * and rows have no Q8_0 form (LTKV_ERR_ARG). */
-enum { LTKV_F16 = 0, LTKV_F32 = 1, LTKV_Q8_0 = 2 };
+ * and rows have no Q8_0 form (LTKV_ERR_ARG; ltkv_gather_values).
+ * Q4_0 stores each 32-element run as 32 4-bit quants q in -8 .. 7 plus an f16
+ * scale d and reads q * d back: d is minus an eighth of the run's element of
+ * largest magnitude (the positive one where both signs reach it), rounded to 8
+ * significant bits (bf16, then f16, nearest even), q the nearest integer to
+ * x / d, ties to even (0 where d is 0). Magnitudes over 65280 are held as 65280,
+ * NaN as 0. A value q * d is exactly an f16 number. Quants: two a byte, in
+ * tiles [n_blocks][kv_dim/32][16 slots][16 bytes]; scales as Q8_0's. The same
+ * entry points and limits as Q8_0; planned attention reads every query's own
+ * context (no groups), the fused append runs as ltkv_write, then attention. */
+enum { LTKV_F16 = 0, LTKV_F32 = 1, LTKV_Q8_0 = 2, LTKV_Q4_0 = 3 };
 
 /* Thread-local message of the last failing call on this thread. */
 LTKV_API const char *ltkv_last_error(void);
@@ -81,7 +90,7 @@ LTKV_API const char *ltkv_last_error(void);
 
 /* KvCache::new(n_layers, kv_dim, n_tokens) (kv.rs:35-48): ceil(n_tokens/16)
  * blocks, zero-filled K and V pools on HIP device `device` (or none for
- * LTKV_NO_DEVICE), free stack (0..n_blocks).rev(). Any kv_dim >= 1 (Q8_0:
+ * LTKV_NO_DEVICE), free stack (0..n_blocks).rev(). Any kv_dim >= 1 (Q8_0, Q4_0:
  * a multiple of 32); rows whose byte length is a multiple of 16 take the
  * vectorised kernels, others element-wise ones.
  * A device cache also holds memory for attention partials (ltkv_bytes does
@@ -153,7 +162,8 @@ LTKV_API int ltkv_init_free_order(ltkv_cache *c, const uint32_t *order, size_t n
  * block*16+slot of `layer`, rounded f32->f16 RNE (F16), stored as is
  * (F32) or quantised per 32 elements (Q8_0: amax = max |x| ignoring NaN,
  * d = amax / 127, q = round-half-away(x / d) saturated to int8, NaN -> 0,
- * d stored as f16 RNE). Negative or out-of-range slots are skipped. */
+ * d stored as f16 RNE; Q4_0: as its storage type says). Negative or
+ * out-of-range slots are skipped. */
 LTKV_API int ltkv_write(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_slot_mapping,
                const float *d_k, const float *d_v, size_t src_stride);
 
@@ -192,7 +202,7 @@ LTKV_API int ltkv_rope_init(ltkv_cache *c, float base, size_t rope_dim, size_t h
  * ([n][q_stride], n_heads heads) in place; V appended unrotated. Tokens with
  * a position outside the table are skipped (nothing written). Bit-identical
  * to the reference's f32 rotation (no fused multiply-add) and f16 rounding
- * (Q8_0 cells: the rotated K row quantised as ltkv_write does). */
+ * (Q8_0 and Q4_0 cells: the rotated K row quantised as ltkv_write does). */
 LTKV_API int ltkv_write_rope(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_slot_mapping,
                     const int32_t *d_positions, const float *d_k, const float *d_v, size_t src_stride,
                     float *d_q, size_t q_stride, size_t n_heads);
@@ -216,6 +226,14 @@ LTKV_API int ltkv_copy_blocks(ltkv_cache *c, size_t n, const int32_t *d_pairs);
 LTKV_API int ltkv_gather(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_tables,
                 size_t table_stride, const int32_t *d_lens, const int64_t *d_out_offsets,
                 void *d_k_out, void *d_v_out);
+
+/* ltkv_gather with the rows as f32 values, for pools of every type (quants as
+ * d * q, f16 widened): rows go to row d_out_offsets[i] onward of d_k_out /
+ * d_v_out ([rows][kv_dim] f32, 16-byte aligned). The reference holds f16 only
+ * and reads rows where they lie (kv.rs:133-150). */
+LTKV_API int ltkv_gather_values(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_tables,
+                                size_t table_stride, const int32_t *d_lens, const int64_t *d_out_offsets,
+                                float *d_k_out, float *d_v_out);
 
 /* Kernel 4, GQA paged decode attention: the attention closure of
  * model.rs:431-475 for n queries. Query i (d_q row i, [n_heads*head_dim] f32)
@@ -288,6 +306,44 @@ LTKV_API int ltkv_append_decode_attention(ltkv_cache *c, size_t layer, size_t n,
                                           const float *d_k, const float *d_v, size_t src_stride,
                                           float *d_out);
 
+/* ---- scored attention -------------------------------------------------- */
+
+/* Types of the rows of a scored attention call (its Q and output). */
+#define LTKV_ROWS_F32 0
+#define LTKV_ROWS_F16 1
+#define LTKV_ROWS_BF16 2
+
+/* Attention with capped scores, distance biases and masks, over single tokens
+ * and prompt chunks alike. Sequence i (of n) has the rows [d_row_starts[i],
+ * d_row_starts[i+1]) of d_q and d_out ([n_rows][n_heads*head_dim] of row_type),
+ * which are the last of its d_lens[i] positions: row r of m stands at position
+ * p = lens[i] - m + r. (Write this step's K and V first: ltkv_write.) Without
+ * d_row_starts every sequence has one row, and n_rows is n. A row sees the
+ * positions t < lens[i] with
+ *   t <= p, or t < d_prefix[i] (a bidirectional prefix; d_prefix may be null);
+ *   t >= d_first[row] (the start of the row's document; d_first may be null);
+ *   with window > 0, t > p - window or t - d_first[row] < sinks.
+ * The score of a position is s = scale * q.k, capped to softcap * tanh(s /
+ * softcap) where softcap > 0, minus d_slopes[h] * |p - t| for query head h
+ * (d_slopes may be null); the output is V weighted by the softmax of the
+ * scores over the visible positions, zeros where there are none. Positions a
+ * row does not see do not enter its result, whatever they hold.
+ * f32 rows are computed to f32 accuracy; f16 and bf16 rows take Q as it is
+ * and weights rounded to f16, summed in f32.
+ * max_rows: the most rows of one sequence, which chooses the kernels; one with
+ * more rows is computed all the same. Rows before the first start or behind
+ * the last are left as they were. Tables, lengths and faults as
+ * ltkv_decode_attention; q and out 16-byte aligned; head_dim up to 1024.
+ * Summation orders depend on the call's shape, not only on a row's own length.
+ * No reference counterpart: the reference's models have neither (model.rs:431-475
+ * is plain causal attention). */
+LTKV_API int ltkv_scored_attention(ltkv_cache *c, size_t layer, size_t n, size_t n_rows, size_t max_rows,
+                                   size_t n_heads, size_t head_dim, float scale, float softcap,
+                                   const float *d_slopes, size_t window, size_t sinks,
+                                   const int32_t *d_prefix, const int32_t *d_first, int row_type,
+                                   const void *d_q, const int32_t *d_tables, size_t table_stride,
+                                   const int32_t *d_lens, const int32_t *d_row_starts, void *d_out);
+
 /* Tokens per context partition of the decode attention split (multiple of
  * 64), or 0 (the default) for the per-query policy: a query is split into
  * four partitions of ceil(len/4) rounded up to 64 tokens (at least 64) up to
@@ -310,7 +366,7 @@ LTKV_API int ltkv_set_attention_partition(ltkv_cache *c, size_t tokens);
  * append then runs as ltkv_write followed by attention, and group partials
  * are folded by the merge. Results match the reference within the same
  * tolerance either way, and a query's result stays independent of the rest
- * of the batch. Refused (LTKV_ERR_ARG) on Q8_0 pools. No reference
+ * of the batch. Refused (LTKV_ERR_ARG) on Q8_0 and Q4_0 pools. No reference
  * counterpart: it keeps the two kernel designs measurable against each
  * other on one build. */
 LTKV_API int ltkv_set_attention_engine(ltkv_cache *c, int engine);
@@ -412,12 +468,12 @@ LTKV_API int ltkv_table_uploads(const ltkv_cache *c, uint64_t *entries);
 LTKV_API int ltkv_read_resident_tables(ltkv_cache *c, int32_t *h_tables, int32_t *h_lengths);
 
 /* Copy one layer's K and V pools ([n_blocks][16][kv_dim]) to host: f16 bits,
- * f32, or Q8_0 int8 quants (stored on the device offset by 128, one byte
- * q + 128 each; this copy gives back q). */
+ * f32, or Q8_0 and Q4_0 quants as int8 (stored on the device offset by 128 and
+ * by 8; this copy gives back q). */
 LTKV_API int ltkv_read_pool(ltkv_cache *c, size_t layer, void *h_k, void *h_v);
 
 /* Copy one layer's K and V scale pools ([n_blocks][kv_dim/32][16] f16 bits)
- * of a Q8_0 cache to host. */
+ * of a Q8_0 or Q4_0 cache to host. */
 LTKV_API int ltkv_read_scales(ltkv_cache *c, size_t layer, uint16_t *h_k, uint16_t *h_v);
 
 /* KvCache::rows(layer, seq, n) collected to host [n][kv_dim] buffers. */

@@ -31,6 +31,10 @@ pub mod ffi {
     pub const LTKV_F16: c_int = 0;
     pub const LTKV_F32: c_int = 1;
     pub const LTKV_Q8_0: c_int = 2;
+    pub const LTKV_Q4_0: c_int = 3;
+    pub const LTKV_ROWS_F32: c_int = 0;
+    pub const LTKV_ROWS_F16: c_int = 1;
+    pub const LTKV_ROWS_BF16: c_int = 2;
     pub const LTKV_PLAN_SHARED_PREFIX: c_uint = 1;
     pub const LTKV_PLAN_F16_PRODUCTS: c_uint = 2;
     pub const LTKV_NOALLOC_SCRATCH_BYTES: usize = 32 << 20;
@@ -86,6 +90,9 @@ pub mod ffi {
         pub fn ltkv_gather(c: *mut ltkv_cache, layer: usize, n: usize, d_tables: *const i32, table_stride: usize,
                            d_lens: *const i32, d_out_offsets: *const i64, d_k_out: *mut c_void,
                            d_v_out: *mut c_void) -> c_int;
+        pub fn ltkv_gather_values(c: *mut ltkv_cache, layer: usize, n: usize, d_tables: *const i32,
+                                  table_stride: usize, d_lens: *const i32, d_out_offsets: *const i64,
+                                  d_k_out: *mut f32, d_v_out: *mut f32) -> c_int;
         pub fn ltkv_decode_attention(c: *mut ltkv_cache, layer: usize, n: usize, n_heads: usize, head_dim: usize,
                                      scale: f32, d_q: *const f32, d_tables: *const i32, table_stride: usize,
                                      d_lens: *const i32, d_out: *mut f32) -> c_int;
@@ -97,6 +104,12 @@ pub mod ffi {
                                             table_stride: usize, d_lens: *const i32, d_slot_mapping: *const i32,
                                             d_k: *const f32, d_v: *const f32, src_stride: usize,
                                             d_out: *mut f32) -> c_int;
+        pub fn ltkv_scored_attention(c: *mut ltkv_cache, layer: usize, n: usize, n_rows: usize, max_rows: usize,
+                                     n_heads: usize, head_dim: usize, scale: f32, softcap: f32,
+                                     d_slopes: *const f32, window: usize, sinks: usize, d_prefix: *const i32,
+                                     d_first: *const i32, row_type: c_int, d_q: *const c_void,
+                                     d_tables: *const i32, table_stride: usize, d_lens: *const i32,
+                                     d_row_starts: *const i32, d_out: *mut c_void) -> c_int;
         pub fn ltkv_set_attention_partition(c: *mut ltkv_cache, tokens: usize) -> c_int;
         pub fn ltkv_set_attention_engine(c: *mut ltkv_cache, engine: c_int) -> c_int;
 
@@ -139,6 +152,28 @@ pub enum Dtype {
     F16,
     F32,
     Q8_0,
+    Q4_0,
+}
+
+/// Type of the rows (Q and output) of `KvCache::scored_attention`.
+#[derive(Clone, Copy, Debug, PartialEq, Eq)]
+pub enum RowType {
+    F32,
+    F16,
+    BF16,
+}
+
+/// What `KvCache::scored_attention` does to scores and which positions a row
+/// sees (`ltkv_scored_attention`); null pointers leave a part out.
+#[derive(Clone, Copy, Debug)]
+pub struct Scoring {
+    pub scale: f32,
+    pub softcap: f32,
+    pub d_slopes: *const f32,
+    pub window: usize,
+    pub sinks: usize,
+    pub d_prefix: *const i32,
+    pub d_first: *const i32,
 }
 
 /// An error returned by the C ABI: its `LTKV_ERR_*` code and the library's
@@ -195,6 +230,7 @@ impl KvCache {
             Dtype::F16 => LTKV_F16,
             Dtype::F32 => LTKV_F32,
             Dtype::Q8_0 => LTKV_Q8_0,
+            Dtype::Q4_0 => LTKV_Q4_0,
         };
         let mut raw = std::ptr::null_mut();
         check(unsafe { ltkv_create(n_layers, kv_dim, n_tokens, code, device, &mut raw) })?;
@@ -271,7 +307,7 @@ impl KvCache {
     }
 
     /// kv.rs:133-150 collected: the first `n` K and V rows of `seq` (f16 bits)
-    /// of an F16 cache (`rows_f32` for an F32 cache; Q8_0 has no rows form).
+    /// of an F16 cache (`rows_f32` for an F32 cache; Q8_0 and Q4_0 have no rows form).
     pub fn rows(&mut self, layer: usize, seq: u32, n: usize) -> anyhow::Result<(Vec<u16>, Vec<u16>)> {
         anyhow::ensure!(self.dtype == Dtype::F16, "rows gives f16 rows: the cache holds {:?}", self.dtype);
         let mut k = vec![0u16; n * self.kv_dim];
@@ -387,12 +423,12 @@ impl KvCache {
     }
 
     /// One layer's K and V pools to host ([n_blocks][16][kv_dim] elements of
-    /// the cache's dtype: f16 bits, f32, or Q8_0 quants).
+    /// the cache's dtype: f16 bits, f32, or Q8_0 and Q4_0 quants as int8).
     pub unsafe fn read_pool(&mut self, layer: usize, h_k: *mut c_void, h_v: *mut c_void) -> anyhow::Result<()> {
         check(ltkv_read_pool(self.raw, layer, h_k, h_v))
     }
 
-    /// One layer's K and V scale pools of a Q8_0 cache: n_blocks * (kv_dim / 32)
+    /// One layer's K and V scale pools of a Q8_0 or Q4_0 cache: n_blocks * (kv_dim / 32)
     /// * 16 f16 bits each, [block][group][slot].
     pub fn read_scales(&mut self, layer: usize, h_k: &mut [u16], h_v: &mut [u16]) -> anyhow::Result<()> {
         let need = self.n_blocks() * (self.kv_dim / 32) * 16;
@@ -450,6 +486,30 @@ impl KvCache {
                          d_lens: *const i32, d_out_offsets: *const i64, d_k_out: *mut c_void,
                          d_v_out: *mut c_void) -> anyhow::Result<()> {
         check(ltkv_gather(self.raw, layer, n, d_tables, table_stride, d_lens, d_out_offsets, d_k_out, d_v_out))
+    }
+
+    /// `gather` with the rows as f32 values, for caches of every type.
+    pub unsafe fn gather_values(&mut self, layer: usize, n: usize, d_tables: *const i32, table_stride: usize,
+                                d_lens: *const i32, d_out_offsets: *const i64, d_k_out: *mut f32,
+                                d_v_out: *mut f32) -> anyhow::Result<()> {
+        check(ltkv_gather_values(self.raw, layer, n, d_tables, table_stride, d_lens, d_out_offsets, d_k_out, d_v_out))
+    }
+
+    /// Attention with capped scores, distance biases and masks: sequence i has
+    /// rows d_row_starts[i]..d_row_starts[i+1] of n_rows (null: one each), at
+    /// most about max_rows each.
+    pub unsafe fn scored_attention(&mut self, layer: usize, n: usize, n_rows: usize, max_rows: usize, n_heads: usize,
+                                   head_dim: usize, how: &Scoring, rows: RowType, d_q: *const c_void,
+                                   d_tables: *const i32, table_stride: usize, d_lens: *const i32,
+                                   d_row_starts: *const i32, d_out: *mut c_void) -> anyhow::Result<()> {
+        let row_type = match rows {
+            RowType::F32 => LTKV_ROWS_F32,
+            RowType::F16 => LTKV_ROWS_F16,
+            RowType::BF16 => LTKV_ROWS_BF16,
+        };
+        check(ltkv_scored_attention(self.raw, layer, n, n_rows, max_rows, n_heads, head_dim, how.scale, how.softcap,
+                                    how.d_slopes, how.window, how.sinks, how.d_prefix, how.d_first, row_type, d_q,
+                                    d_tables, table_stride, d_lens, d_row_starts, d_out))
     }
 
     /// Kernel 4 (the attention closure of model.rs:431-475).

@@ -12,7 +12,8 @@ import os
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libltkv.so")
 
 OK, ERR_FULL, ERR_NONCONTIG, ERR_RANGE, ERR_HIP, ERR_ARG = 0, 1, 2, 3, 4, 5
-F16, F32, Q8_0 = 0, 1, 2
+F16, F32, Q8_0, Q4_0 = 0, 1, 2, 3
+ROWS_F32, ROWS_F16, ROWS_BF16 = 0, 1, 2
 PLAN_SHARED_PREFIX, PLAN_F16_PRODUCTS = 1, 2
 ENGINE_AUTO, ENGINE_VALU = 0, 1
 NO_DEVICE = -1
@@ -51,10 +52,13 @@ SIGNATURES = {
     "ltkv_write_rope": (_int, [_vp, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _sz]),
     "ltkv_copy_blocks": (_int, [_vp, _sz, _vp]),
     "ltkv_gather": (_int, [_vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp]),
+    "ltkv_gather_values": (_int, [_vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp]),
     "ltkv_decode_attention": (_int, [_vp, _sz, _sz, _sz, _sz, _f32, _vp, _vp, _sz, _vp, _vp]),
     "ltkv_decode_attention_noalloc": (_int, [_vp, _sz, _sz, _sz, _sz, _f32, _vp, _vp, _sz, _vp, _vp]),
     "ltkv_append_decode_attention": (_int, [_vp, _sz, _sz, _sz, _sz, _f32, _vp, _vp, _sz, _vp, _vp, _vp, _vp,
                                             _sz, _vp]),
+    "ltkv_scored_attention": (_int, [_vp, _sz, _sz, _sz, _sz, _sz, _sz, _f32, _f32, _vp, _sz, _sz, _vp, _vp, _int,
+                                     _vp, _vp, _sz, _vp, _vp, _vp]),
     "ltkv_set_attention_partition": (_int, [_vp, _sz]),
     "ltkv_set_attention_engine": (_int, [_vp, _int]),
     "ltkv_plan_attention": (_int, [_vp, _sz, _vp, _vp, _sz, _sz, _u32]),

@@ -115,7 +115,7 @@ struct ltkv_cache {
   size_t n_layers = 0, kv_dim = 0, n_blocks = 0, elem = 2;
   ltkv::PoolGeom geom{};
   void *k = nullptr, *v = nullptr;  // [layer][block][slot][kv_dim]
-  // Q8_0: per-32-element f16 scales, [layer][block][slot][kv_dim / 32].
+  // Q8_0 and Q4_0: per-32-element f16 scales, [layer][block][kv_dim / 32][slot].
   void *ks = nullptr, *vs = nullptr;
   ltkv::PoolGeom sgeom{};  // the scale pools as a pool of 2-byte elements
   hipStream_t stream = nullptr;
@@ -188,9 +188,23 @@ struct ltkv_cache {
   uint64_t rt_uploaded = 0;                      // triples uploaded so far (statistics)
 
   size_t layer_elems() const { return n_blocks * LTKV_BLOCK * kv_dim; }
-  uint8_t *k_layer(size_t l) const { return (uint8_t *)k + l * layer_elems() * elem; }
-  uint8_t *v_layer(size_t l) const { return (uint8_t *)v + l * layer_elems() * elem; }
+  size_t layer_bytes() const { return q4() ? layer_elems() / 2 : layer_elems() * elem; }
+  uint8_t *k_layer(size_t l) const { return (uint8_t *)k + l * layer_bytes(); }
+  uint8_t *v_layer(size_t l) const { return (uint8_t *)v + l * layer_bytes(); }
   bool q8() const { return dtype == LTKV_Q8_0; }
+  bool q4() const { return dtype == LTKV_Q4_0; }
+  bool quantised() const { return q8() || q4(); }
+  // The pools as block copies see them: a q4_0 block is 16 rows of kv_dim / 2 bytes.
+  ltkv::PoolGeom copy_geom() const {
+    ltkv::PoolGeom g = geom;
+    if (q4()) {
+      g.elem = 1;
+      g.kv_dim = (int)(kv_dim / 2);
+      g.slot_stride /= 2;
+      g.block_stride /= 2;
+    }
+    return g;
+  }
   size_t layer_scales() const { return n_blocks * LTKV_BLOCK * (kv_dim / 32); }
   uint16_t *k_scales(size_t l) const { return ks ? (uint16_t *)ks + l * layer_scales() : nullptr; }
   uint16_t *v_scales(size_t l) const { return vs ? (uint16_t *)vs + l * layer_scales() : nullptr; }
@@ -336,9 +350,9 @@ struct ltkv_cache {
     HIP_TRY(hipEventRecord(pairs_done, stream), "hipEventRecord");
     pairs_in_flight = true;
     const bool bulk = n >= kCopyOrderMinPairs;
-    HIP_TRY(ltkv::launch_copy_blocks(geom, (int)n_layers, k, v, d_pairs, (int64_t)n, bulk, stream),
+    HIP_TRY(ltkv::launch_copy_blocks(copy_geom(), (int)n_layers, k, v, d_pairs, (int64_t)n, bulk, stream),
             "copy_blocks launch");
-    if (q8())
+    if (quantised())
       HIP_TRY(ltkv::launch_copy_blocks(sgeom, (int)n_layers, ks, vs, d_pairs, (int64_t)n, bulk, stream),
               "copy_blocks launch (scales)");
     return LTKV_OK;
@@ -434,7 +448,7 @@ int ensure_workspace(ltkv_cache *c, size_t bytes) {
 // the cache took ~150 us more to create, as any allocation of 2 MiB and more
 // does; smaller ones ~1 us.)
 size_t held_size(const ltkv_cache *c) {
-  const size_t quarter = c->layer_elems() * c->elem / 2;
+  const size_t quarter = c->layer_bytes() / 2;
   return std::min<size_t>(std::max<size_t>(quarter, size_t{1} << 20), size_t{16} << 20);
 }
 
@@ -1056,10 +1070,10 @@ int ltkv_create(size_t n_layers, size_t kv_dim, size_t n_tokens, int dtype, int 
   if (!out) return fail(LTKV_ERR_ARG, "out is null");
   *out = nullptr;
   if (n_layers == 0 || kv_dim == 0) return fail(LTKV_ERR_ARG, "n_layers and kv_dim must be > 0");
-  if (dtype != LTKV_F16 && dtype != LTKV_F32 && dtype != LTKV_Q8_0)
-    return fail(LTKV_ERR_ARG, "dtype must be F16, F32 or Q8_0");
-  if (dtype == LTKV_Q8_0 && kv_dim % 32 != 0)
-    return fail(LTKV_ERR_ARG, "Q8_0 needs kv_dim a multiple of 32 (one scale per 32 elements)");
+  if (dtype != LTKV_F16 && dtype != LTKV_F32 && dtype != LTKV_Q8_0 && dtype != LTKV_Q4_0)
+    return fail(LTKV_ERR_ARG, "dtype must be F16, F32, Q8_0 or Q4_0");
+  if ((dtype == LTKV_Q8_0 || dtype == LTKV_Q4_0) && kv_dim % 32 != 0)
+    return fail(LTKV_ERR_ARG, "Q8_0 and Q4_0 need kv_dim a multiple of 32 (one scale per 32 elements)");
   const size_t n_blocks = (n_tokens + LTKV_BLOCK - 1) / LTKV_BLOCK;  // kv.rs:36
   if (n_blocks > (size_t)INT32_MAX / LTKV_BLOCK)
     return fail(LTKV_ERR_ARG, "n_tokens too large for 32-bit cell indices");
@@ -1077,7 +1091,7 @@ int ltkv_create(size_t n_layers, size_t kv_dim, size_t n_tokens, int dtype, int 
   c->n_layers = n_layers;
   c->kv_dim = kv_dim;
   c->n_blocks = n_blocks;
-  c->elem = dtype == LTKV_F16 ? 2 : dtype == LTKV_F32 ? 4 : 1;
+  c->elem = dtype == LTKV_F16 ? 2 : dtype == LTKV_F32 ? 4 : dtype == LTKV_Q8_0 ? 1 : (size_t)ltkv::kElemQ4;
   c->geom.n_blocks = (int64_t)n_blocks;
   c->geom.block_stride = (int64_t)(LTKV_BLOCK * kv_dim);
   c->geom.slot_stride = (int64_t)kv_dim;
@@ -1115,21 +1129,21 @@ int ltkv_create(size_t n_layers, size_t kv_dim, size_t n_tokens, int dtype, int 
     c->scratch = static_cast<uint8_t *>(p);
   }
 
-  const size_t bytes = n_layers * c->layer_elems() * c->elem;
+  const size_t bytes = n_layers * c->layer_bytes();
+  const int zero = c->q8() ? 0x80 : c->q4() ? 0x88 : 0;  // quants are stored offset by 128 and by 8
   int rc = LTKV_OK;
   hipError_t e;
   if (bytes > 0) {
     if ((e = hipMalloc(&c->k, bytes)) != hipSuccess) rc = hip_fail(e, "hipMalloc(K pool)");
     else if ((e = hipMalloc(&c->v, bytes)) != hipSuccess) rc = hip_fail(e, "hipMalloc(V pool)");
-    // zero cells; q8_0 quants are stored offset by 128, so a zero quant is 0x80
-    else if ((e = hipMemset(c->k, c->q8() ? 0x80 : 0, bytes)) != hipSuccess) rc = hip_fail(e, "hipMemset(K pool)");
-    else if ((e = hipMemset(c->v, c->q8() ? 0x80 : 0, bytes)) != hipSuccess) rc = hip_fail(e, "hipMemset(V pool)");
+    else if ((e = hipMemset(c->k, zero, bytes)) != hipSuccess) rc = hip_fail(e, "hipMemset(K pool)");
+    else if ((e = hipMemset(c->v, zero, bytes)) != hipSuccess) rc = hip_fail(e, "hipMemset(V pool)");
   }
   if (rc == LTKV_OK) {
     if ((e = hipMalloc((void **)&c->d_status, 4 * sizeof(int32_t))) != hipSuccess) rc = hip_fail(e, "hipMalloc(status)");
     else if ((e = hipMemset(c->d_status, 0, 4 * sizeof(int32_t))) != hipSuccess) rc = hip_fail(e, "hipMemset(status)");
   }
-  const size_t sbytes = c->q8() ? n_layers * c->layer_scales() * 2 : 0;
+  const size_t sbytes = c->quantised() ? n_layers * c->layer_scales() * 2 : 0;
   if (rc == LTKV_OK && sbytes > 0) {
     if ((e = hipMalloc(&c->ks, sbytes)) != hipSuccess) rc = hip_fail(e, "hipMalloc(K scales)");
     else if ((e = hipMalloc(&c->vs, sbytes)) != hipSuccess) rc = hip_fail(e, "hipMalloc(V scales)");
@@ -1197,7 +1211,7 @@ int ltkv_set_stream(ltkv_cache *c, void *hip_stream) {
 size_t ltkv_capacity(const ltkv_cache *c) { return c ? c->n_blocks * LTKV_BLOCK : 0; }
 size_t ltkv_bytes(const ltkv_cache *c) {
   if (!c) return 0;
-  return 2 * c->n_layers * (c->layer_elems() * c->elem + (c->q8() ? c->layer_scales() * 2 : 0));
+  return 2 * c->n_layers * (c->layer_bytes() + (c->quantised() ? c->layer_scales() * 2 : 0));
 }
 size_t ltkv_len(const ltkv_cache *c, uint32_t seq) {
   if (!c) return 0;
@@ -1314,10 +1328,10 @@ int write_rows(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_slot_mapp
   if ((uint64_t)n * c->kv_dim >= (1ull << 40)) return fail(LTKV_ERR_ARG, "too many rows for one launch");
   DeviceGuard dg(c->device);
   if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
-  if (c->q8())
-    HIP_TRY(ltkv::launch_write_q8(c->geom, c->k_layer(layer), c->v_layer(layer), c->k_scales(layer),
-                                  c->v_scales(layer), d_slot_mapping, d_k, d_v, (int64_t)n,
-                                  (int64_t)src_stride, c->stream, d_order, (int64_t)n_rows),
+  if (c->quantised())
+    HIP_TRY(ltkv::launch_write_quant(c->geom, c->k_layer(layer), c->v_layer(layer), c->k_scales(layer),
+                                     c->v_scales(layer), d_slot_mapping, d_k, d_v, (int64_t)n,
+                                     (int64_t)src_stride, c->stream, d_order, (int64_t)n_rows),
             "write launch");
   else
     HIP_TRY(ltkv::launch_write(c->geom, c->k_layer(layer), c->v_layer(layer), d_slot_mapping, d_k,
@@ -1426,8 +1440,8 @@ int ltkv_write_rope(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_slot
   if (src_stride < c->kv_dim || src_stride % 4 != 0)
     return fail(LTKV_ERR_ARG, "src_stride must be >= kv_dim and a multiple of 4");
   const size_t hd = (size_t)c->rope_geom.head_dim;
-  if (c->q8() && hd % 32 != 0)
-    return fail(LTKV_ERR_ARG, "the Q8_0 RoPE append needs head_dim a multiple of 32 (whole scale groups per head)");
+  if (c->quantised() && hd % 32 != 0)
+    return fail(LTKV_ERR_ARG, "the Q8_0 and Q4_0 RoPE appends need head_dim a multiple of 32 (whole scale groups per head)");
   if (d_q && (n_heads == 0 || q_stride < n_heads * hd || q_stride % 4 != 0))
     return fail(LTKV_ERR_ARG, "q_stride must be >= n_heads * head_dim and a multiple of 4");
   if (((uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_q) % 16 != 0)
@@ -1436,11 +1450,11 @@ int ltkv_write_rope(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_slot
   if ((uint64_t)n * per >= (1ull << 32) - 256) return fail(LTKV_ERR_ARG, "too many rows for one launch");
   DeviceGuard dg(c->device);
   if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
-  if (c->q8())
-    HIP_TRY(ltkv::launch_write_rope_q8(c->geom, c->k_layer(layer), c->v_layer(layer), c->k_scales(layer),
-                                       c->v_scales(layer), d_slot_mapping, d_positions, d_k, d_v, d_q,
-                                       (int64_t)n, (int64_t)src_stride, (int64_t)q_stride, (int)n_heads,
-                                       c->rope_geom, c->stream),
+  if (c->quantised())
+    HIP_TRY(ltkv::launch_write_rope_quant(c->geom, c->k_layer(layer), c->v_layer(layer), c->k_scales(layer),
+                                          c->v_scales(layer), d_slot_mapping, d_positions, d_k, d_v, d_q,
+                                          (int64_t)n, (int64_t)src_stride, (int64_t)q_stride, (int)n_heads,
+                                          c->rope_geom, c->stream),
             "write_rope launch");
   else
     HIP_TRY(ltkv::launch_write_rope(c->geom, c->k_layer(layer), c->v_layer(layer), d_slot_mapping,
@@ -1458,7 +1472,7 @@ int ltkv_copy_blocks(ltkv_cache *c, size_t n, const int32_t *d_pairs) {
   DeviceGuard dg(c->device);
   if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
   if (n > (size_t)INT32_MAX) return fail(LTKV_ERR_ARG, "%zu copy pairs exceed 2^31 - 1", n);
-  const int64_t max_pairs = ltkv::copy_max_pairs(c->geom, (int)c->n_layers, n >= kCopyOrderMinPairs);
+  const int64_t max_pairs = ltkv::copy_max_pairs(c->copy_geom(), (int)c->n_layers, n >= kCopyOrderMinPairs);
   if ((int64_t)n > max_pairs)
     return fail(LTKV_ERR_ARG, "%zu copy pairs exceed the %lld one launch takes at this pool shape", n,
                 (long long)max_pairs);
@@ -1499,9 +1513,9 @@ int ltkv_copy_blocks(ltkv_cache *c, size_t n, const int32_t *d_pairs) {
     pairs = c->d_order_pairs;
   }
   const bool bulk = n >= kCopyOrderMinPairs;
-  HIP_TRY(ltkv::launch_copy_blocks(c->geom, (int)c->n_layers, c->k, c->v, pairs, (int64_t)n, bulk, c->stream),
+  HIP_TRY(ltkv::launch_copy_blocks(c->copy_geom(), (int)c->n_layers, c->k, c->v, pairs, (int64_t)n, bulk, c->stream),
           "copy_blocks launch");
-  if (c->q8())
+  if (c->quantised())
     HIP_TRY(ltkv::launch_copy_blocks(c->sgeom, (int)c->n_layers, c->ks, c->vs, pairs, (int64_t)n, bulk,
                                      c->stream),
             "copy_blocks launch (scales)");
@@ -1514,7 +1528,7 @@ int ltkv_gather(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_tables,
   if (!c) return fail(LTKV_ERR_ARG, "cache is null");
   if (c->device == LTKV_NO_DEVICE) return no_device();
   if (layer >= c->n_layers) return fail(LTKV_ERR_RANGE, "layer %zu out of range (%zu)", layer, c->n_layers);
-  if (c->q8()) return fail(LTKV_ERR_ARG, "gather has no Q8_0 form");
+  if (c->quantised()) return fail(LTKV_ERR_ARG, "gather has no Q8_0 or Q4_0 form (ltkv_gather_values)");
   if (n == 0 || table_stride == 0) return LTKV_OK;
   if (!d_tables || !d_lens || !d_out_offsets || !d_k_out || !d_v_out)
     return fail(LTKV_ERR_ARG, "null device pointer");
@@ -1534,12 +1548,34 @@ int ltkv_gather(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_tables,
   return LTKV_OK;
 }
 
+int ltkv_gather_values(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_tables, size_t table_stride,
+                       const int32_t *d_lens, const int64_t *d_out_offsets, float *d_k_out, float *d_v_out) {
+  if (!c) return fail(LTKV_ERR_ARG, "cache is null");
+  if (c->device == LTKV_NO_DEVICE) return no_device();
+  if (layer >= c->n_layers) return fail(LTKV_ERR_RANGE, "layer %zu out of range (%zu)", layer, c->n_layers);
+  if (n == 0 || table_stride == 0) return LTKV_OK;
+  if (!d_tables || !d_lens || !d_out_offsets || !d_k_out || !d_v_out)
+    return fail(LTKV_ERR_ARG, "null device pointer");
+  if (((uintptr_t)d_k_out | (uintptr_t)d_v_out) % 16 != 0)
+    return fail(LTKV_ERR_ARG, "outputs must be 16-byte aligned");
+  // One work-group of 256 threads per block's K or V.
+  if (n >= (size_t{1} << 32) || table_stride >= (size_t{1} << 32) || n * table_stride * 2 * 256 >= (size_t{1} << 32))
+    return fail(LTKV_ERR_ARG, "n * table_stride too large for one launch");
+  DeviceGuard dg(c->device);
+  if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
+  HIP_TRY(ltkv::launch_gather_values(c->geom, c->k_layer(layer), c->v_layer(layer), c->k_scales(layer),
+                                     c->v_scales(layer), d_tables, (int64_t)table_stride, d_lens, d_out_offsets,
+                                     (int64_t)n, d_k_out, d_v_out, c->d_status, c->stream),
+          "gather launch");
+  return LTKV_OK;
+}
+
 int ltkv_set_attention_engine(ltkv_cache *c, int engine) {
   if (!c) return fail(LTKV_ERR_ARG, "cache is null");
   if (engine != LTKV_ENGINE_AUTO && engine != LTKV_ENGINE_VALU)
     return fail(LTKV_ERR_ARG, "unknown attention engine %d", engine);
-  if (engine == LTKV_ENGINE_VALU && c->elem == 1)
-    return fail(LTKV_ERR_ARG, "the vector-ALU engine serves f16 and f32 pools, not Q8_0");
+  if (engine == LTKV_ENGINE_VALU && c->quantised())
+    return fail(LTKV_ERR_ARG, "the vector-ALU engine serves f16 and f32 pools, not Q8_0 or Q4_0");
   c->attn_engine = engine;
   return LTKV_OK;
 }
@@ -1553,6 +1589,59 @@ int ltkv_set_attention_partition(ltkv_cache *c, size_t tokens) {
 }
 
 namespace {
+
+// The pool, device and queries' layout of a scored attention call, or of a
+// decode call on a q4_0 pool.
+ltkv::ScoredArgs scored_args(ltkv_cache *c, size_t layer, size_t n, size_t n_rows, size_t n_heads, size_t head_dim,
+                             float scale, const void *d_q, const int32_t *d_tables, size_t table_stride,
+                             size_t max_len, const int32_t *d_lens, void *d_out) {
+  ltkv::ScoredArgs a{};
+  a.k_layer = c->k_layer(layer);
+  a.v_layer = c->v_layer(layer);
+  a.k_scale = c->k_scales(layer);
+  a.v_scale = c->v_scales(layer);
+  a.q = d_q;
+  a.out = d_out;
+  a.row_type = LTKV_ROWS_F32;
+  a.tables = d_tables;
+  a.table_stride = (int64_t)table_stride;
+  a.lens = d_lens;
+  a.n = (int64_t)n;
+  a.n_rows = (int64_t)n_rows;
+  a.max_rows = 1;
+  a.max_len = (int64_t)std::min<size_t>(max_len, (size_t)INT32_MAX - 15);
+  a.n_heads = (int)n_heads;
+  a.n_kv_heads = (int)(c->kv_dim / head_dim);
+  a.head_dim = (int)head_dim;
+  a.scale = scale;
+  a.status = c->d_status;
+  a.cu_count = c->device_count_cu;
+  a.part_tokens = (int)c->attn_part_tokens;
+  return a;
+}
+
+// Launches it, its partials in the cache's memory, or with use_scratch in the
+// device's static scratch (which allocates nothing).
+int scored_attention(ltkv_cache *c, ltkv::ScoredArgs &a, bool use_scratch = false) {
+  const ltkv::ScoredWorkspace ws = ltkv::scored_workspace((int)c->elem, a);
+  if (use_scratch && (size_t)ws.bytes > ltkv::kScratchBytes)
+    return fail(LTKV_ERR_ARG,
+                "attention needs %lld bytes of partition partials, more than the %zu bytes of the "
+                "no-allocation scratch",
+                (long long)ws.bytes, ltkv::kScratchBytes);
+  if (ws.bytes > 0) {
+    uint8_t *base = c->scratch;
+    if (!use_scratch)
+      if (int rc = workspace(c, (size_t)ws.bytes, &base)) return rc;
+    a.part_o = (float *)(base + ws.part_o_off);
+    a.part_ml = (float *)(base + ws.part_ml_off);
+    a.part_n = (int32_t *)(base + ws.part_n_off);
+  }
+  const hipError_t e = ltkv::launch_scored_attention(head_geom(c, (size_t)a.head_dim), a, c->stream);
+  if (e == hipErrorInvalidValue) return fail(LTKV_ERR_ARG, "attention grid too large for one launch");
+  if (e != hipSuccess) return hip_fail(e, "attention launch");
+  return LTKV_OK;
+}
 
 // Decode attention over explicit tables (rows == nullptr: query i reads row
 // i) or over the resident tables (query i reads row rows[i]); lengths are cut
@@ -1570,6 +1659,13 @@ int decode_attention(ltkv_cache *c, size_t layer, size_t n, size_t n_heads, size
   // ltkv_set_attention_partition), so its result is bit-identical whatever
   // else is in the batch (the reference's property, engine/README.md:102).
   // max_len only bounds the grid.
+  if (c->q4()) {  // (a fused append is two launches on these pools: never here)
+    ltkv::ScoredArgs a = scored_args(c, layer, n, n, n_heads, head_dim, scale, d_q, d_tables, table_stride, max_len,
+                                     d_lens, d_out);
+    a.rows = d_rows;
+    a.table_rows = (int64_t)n_rows;
+    return scored_attention(c, a, use_scratch);
+  }
   int part = (int)c->attn_part_tokens;  // 0: the shape's per-query policy
   const bool valu = c->attn_engine == LTKV_ENGINE_VALU && c->elem == 2;
   if (part == 0) part = ltkv::attention_part_policy((int)c->elem, (int)group, (int)(c->kv_dim / head_dim), valu);
@@ -1715,6 +1811,47 @@ int ltkv_decode_attention_rows(ltkv_cache *c, size_t layer, size_t n, size_t n_h
                           c->rt_rows, max_len, d_lens, d_out, group);
 }
 
+int ltkv_scored_attention(ltkv_cache *c, size_t layer, size_t n, size_t n_rows, size_t max_rows, size_t n_heads,
+                          size_t head_dim, float scale, float softcap, const float *d_slopes, size_t window,
+                          size_t sinks, const int32_t *d_prefix, const int32_t *d_first, int row_type,
+                          const void *d_q, const int32_t *d_tables, size_t table_stride, const int32_t *d_lens,
+                          const int32_t *d_row_starts, void *d_out) {
+  if (!c) return fail(LTKV_ERR_ARG, "cache is null");
+  if (c->device == LTKV_NO_DEVICE) return no_device();
+  if (layer >= c->n_layers) return fail(LTKV_ERR_RANGE, "layer %zu out of range (%zu)", layer, c->n_layers);
+  size_t group = 0;
+  if (int rc = check_attention_shape(c, n_heads, head_dim, &group)) return rc;
+  if (row_type != LTKV_ROWS_F32 && row_type != LTKV_ROWS_F16 && row_type != LTKV_ROWS_BF16)
+    return fail(LTKV_ERR_ARG, "unknown row type %d", row_type);
+  if (!(softcap >= 0.f) || std::isinf(softcap)) return fail(LTKV_ERR_ARG, "softcap must be 0 (none) or positive");
+  if (!std::isfinite(scale)) return fail(LTKV_ERR_ARG, "scale must be finite");
+  if (sinks > 0 && window == 0) return fail(LTKV_ERR_ARG, "sinks need a window");
+  if (!d_row_starts && n_rows != n)
+    return fail(LTKV_ERR_ARG, "without row starts each of the %zu sequences has one row, not %zu in all", n, n_rows);
+  if (n_rows > (size_t)INT32_MAX / 2 || n > (size_t)INT32_MAX / 2)
+    return fail(LTKV_ERR_ARG, "%zu rows of %zu sequences are too many for one call", n_rows, n);
+  if (n == 0 || n_rows == 0) return LTKV_OK;
+  if (max_rows == 0) return fail(LTKV_ERR_ARG, "max_rows must be > 0");
+  if (table_stride == 0) return fail(LTKV_ERR_ARG, "table_stride must be > 0");
+  if (!d_q || !d_tables || !d_lens || !d_out) return fail(LTKV_ERR_ARG, "null device pointer");
+  if (((uintptr_t)d_q | (uintptr_t)d_out) % 16 != 0) return fail(LTKV_ERR_ARG, "q and out must be 16-byte aligned");
+  DeviceGuard dg(c->device);
+  if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
+  const size_t max_len = table_stride >= (size_t)INT32_MAX / LTKV_BLOCK ? (size_t)INT32_MAX : table_stride * LTKV_BLOCK;
+  ltkv::ScoredArgs a =
+      scored_args(c, layer, n, n_rows, n_heads, head_dim, scale, d_q, d_tables, table_stride, max_len, d_lens, d_out);
+  a.row_type = row_type;
+  a.row_starts = d_row_starts;
+  a.max_rows = d_row_starts ? (int64_t)std::min(max_rows, n_rows) : 1;
+  a.softcap = softcap;
+  a.slopes = d_slopes;
+  a.window = (int64_t)std::min<size_t>(window, (size_t)INT32_MAX);
+  a.sinks = (int64_t)std::min<size_t>(sinks, (size_t)INT32_MAX);
+  a.prefix = d_prefix;
+  a.first = d_first;
+  return scored_attention(c, a);
+}
+
 int ltkv_seq_rows(const ltkv_cache *c, size_t n, const uint32_t *seqs, int32_t *rows) {
   if (!c) return fail(LTKV_ERR_ARG, "cache is null");
   if (n > 0 && (!seqs || !rows)) return fail(LTKV_ERR_ARG, "null argument");
@@ -1802,6 +1939,19 @@ PlanShape plan_shape(const ltkv_cache *c) {
   const int group = (int)P.n_heads / n_kv;
   const bool grouped = P.groups > 0;
   PlanShape L{};
+  if (c->q4()) {
+    ltkv::ScoredArgs a{};
+    a.n = a.n_rows = (int64_t)P.n;
+    a.max_rows = 1;
+    a.max_len = (int64_t)(P.sstride * LTKV_BLOCK);
+    a.n_heads = (int)P.n_heads;
+    a.n_kv_heads = n_kv;
+    a.head_dim = (int)P.head_dim;
+    a.part_tokens = (int)c->attn_part_tokens;
+    a.cu_count = c->device_count_cu;
+    L.bytes = (size_t)ltkv::scored_workspace((int)c->elem, a).bytes;
+    return L;
+  }
   // Grouped plans are batch-dependent anyway: when every query's remainder is
   // short (forks reading a few private blocks), their per-query pass takes
   // the plan's partition unless one is fixed; long remainders keep the
@@ -1874,6 +2024,14 @@ int ltkv_planned_attention(ltkv_cache *c, size_t layer, float scale, const float
   if (((uintptr_t)d_q) % 16 != 0) return fail(LTKV_ERR_ARG, "q must be 16-byte aligned");
   const size_t group = P.n_heads / (c->kv_dim / P.head_dim);
   const bool grouped = P.groups > 0;
+  if (c->q4()) {  // no groups: every query its whole context
+    DeviceGuard dg(c->device);
+    if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
+    const int32_t *d = reinterpret_cast<const int32_t *>(P.d);
+    ltkv::ScoredArgs a = scored_args(c, layer, P.n, P.n, P.n_heads, P.head_dim, scale, d_q, d + P.off_stables,
+                                     P.sstride, P.sstride * LTKV_BLOCK, d + P.off_slens, d_out);
+    return scored_attention(c, a);
+  }
   const PlanShape L = plan_shape(c);
   if (L.too_large) return fail(LTKV_ERR_ARG, "attention grid too large for one launch");
   const int part = L.part, split = L.split;
@@ -2000,6 +2158,41 @@ int ltkv_synchronize(ltkv_cache *c) {
   return take_status(c);
 }
 
+namespace {
+
+// The quants of a q4_0 layer as int8 rows [n_blocks][16][kv_dim] (device of
+// the cache current).
+int read_pool_q4(ltkv_cache *c, size_t layer, int8_t *h_k, int8_t *h_v) {
+  const size_t bytes = c->layer_bytes(), groups = c->kv_dim / 32;
+  std::vector<uint8_t> packed;
+  try {
+    packed.resize(bytes);
+  } catch (const std::bad_alloc &) {
+    return fail(LTKV_ERR_ARG, "out of host memory");
+  }
+  for (int is_v = 0; is_v < 2; ++is_v) {
+    int8_t *out = is_v ? h_v : h_k;
+    if (bytes == 0) break;
+    HIP_TRY(hipMemcpyAsync(packed.data(), is_v ? c->v_layer(layer) : c->k_layer(layer), bytes, hipMemcpyDeviceToHost,
+                           c->stream),
+            "read pool");
+    HIP_TRY(c->stream ? hipStreamSynchronize(c->stream) : hipDeviceSynchronize(), "synchronize");
+    for (size_t b = 0; b < c->n_blocks; ++b)
+      for (size_t g = 0; g < groups; ++g)
+        for (size_t slot = 0; slot < LTKV_BLOCK; ++slot) {
+          const uint8_t *src = packed.data() + ((b * groups + g) * LTKV_BLOCK + slot) * 16;
+          int8_t *dst = out + (b * LTKV_BLOCK + slot) * c->kv_dim + g * 32;
+          for (int e = 0; e < 32; ++e) {  // element e: bit 4 * (e % 8 / 2) + 16 * (e % 2) of dword e / 8
+            const int bit = 4 * (e % 8 / 2) + 16 * (e % 2);
+            dst[e] = (int8_t)((src[e / 8 * 4 + bit / 8] >> (bit % 8) & 15) - 8);
+          }
+        }
+  }
+  return LTKV_OK;
+}
+
+}  // namespace
+
 int ltkv_read_pool(ltkv_cache *c, size_t layer, void *h_k, void *h_v) {
   if (!c) return fail(LTKV_ERR_ARG, "cache is null");
   if (c->device == LTKV_NO_DEVICE) return no_device();
@@ -2007,6 +2200,7 @@ int ltkv_read_pool(ltkv_cache *c, size_t layer, void *h_k, void *h_v) {
   if (!h_k || !h_v) return fail(LTKV_ERR_ARG, "null host pointer");
   DeviceGuard dg(c->device);
   if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
+  if (c->q4()) return read_pool_q4(c, layer, static_cast<int8_t *>(h_k), static_cast<int8_t *>(h_v));
   const size_t bytes = c->layer_elems() * c->elem;
   HIP_TRY(hipMemcpyAsync(h_k, c->k_layer(layer), bytes, hipMemcpyDeviceToHost, c->stream), "read K pool");
   HIP_TRY(hipMemcpyAsync(h_v, c->v_layer(layer), bytes, hipMemcpyDeviceToHost, c->stream), "read V pool");
@@ -2021,7 +2215,7 @@ int ltkv_read_pool(ltkv_cache *c, size_t layer, void *h_k, void *h_v) {
 int ltkv_read_scales(ltkv_cache *c, size_t layer, uint16_t *h_k, uint16_t *h_v) {
   if (!c) return fail(LTKV_ERR_ARG, "cache is null");
   if (c->device == LTKV_NO_DEVICE) return no_device();
-  if (!c->q8()) return fail(LTKV_ERR_ARG, "only Q8_0 caches have scale pools");
+  if (!c->quantised()) return fail(LTKV_ERR_ARG, "only Q8_0 and Q4_0 caches have scale pools");
   if (layer >= c->n_layers) return fail(LTKV_ERR_RANGE, "layer %zu out of range (%zu)", layer, c->n_layers);
   if (!h_k || !h_v) return fail(LTKV_ERR_ARG, "null host pointer");
   DeviceGuard dg(c->device);
@@ -2036,7 +2230,8 @@ int ltkv_read_scales(ltkv_cache *c, size_t layer, uint16_t *h_k, uint16_t *h_v) 
 int ltkv_rows(ltkv_cache *c, size_t layer, uint32_t seq, size_t n, void *h_k, void *h_v) {
   if (!c) return fail(LTKV_ERR_ARG, "cache is null");
   if (c->device == LTKV_NO_DEVICE) return no_device();
-  if (c->q8()) return fail(LTKV_ERR_ARG, "rows has no Q8_0 form (ltkv_read_pool, ltkv_read_scales)");
+  if (c->quantised())
+    return fail(LTKV_ERR_ARG, "rows has no Q8_0 or Q4_0 form (ltkv_read_pool, ltkv_read_scales, ltkv_gather_values)");
   if (layer >= c->n_layers) return fail(LTKV_ERR_RANGE, "layer %zu out of range (%zu)", layer, c->n_layers);
   if (n == 0) return LTKV_OK;
   if (!h_k || !h_v) return fail(LTKV_ERR_ARG, "null host pointer");
@@ -2097,10 +2292,10 @@ int ltkv_write_row(ltkv_cache *c, size_t layer, uint32_t block, uint32_t slot, c
   uint8_t *d = nullptr;
   HIP_TRY(hipMalloc((void **)&d, total), "hipMalloc(row staging)");
   hipError_t e = hipMemcpyAsync(d, h.data(), total, hipMemcpyHostToDevice, c->stream);
-  if (e == hipSuccess && c->q8())
-    e = ltkv::launch_write_q8(c->geom, c->k_layer(layer), c->v_layer(layer), c->k_scales(layer),
-                              c->v_scales(layer), (const int32_t *)d, (const float *)(d + 16),
-                              (const float *)(d + 16 + row), 1, (int64_t)c->kv_dim, c->stream);
+  if (e == hipSuccess && c->quantised())
+    e = ltkv::launch_write_quant(c->geom, c->k_layer(layer), c->v_layer(layer), c->k_scales(layer),
+                                 c->v_scales(layer), (const int32_t *)d, (const float *)(d + 16),
+                                 (const float *)(d + 16 + row), 1, (int64_t)c->kv_dim, c->stream);
   else if (e == hipSuccess)
     e = ltkv::launch_write(c->geom, c->k_layer(layer), c->v_layer(layer), (const int32_t *)d,
                            (const float *)(d + 16), (const float *)(d + 16 + row), 1,

@@ -18,17 +18,21 @@ struct PoolGeom {
   int64_t slot_stride;   // elements between consecutive slots of a block
   int64_t head_stride;   // elements between consecutive kv heads of a block
   int kv_dim;
-  int elem;              // bytes per element: 1 (q8_0 quants), 2 (f16) or 4 (f32)
+  int elem;              // bytes per element: 1 (q8_0 quants), 2 (f16) or 4 (f32); kElemQ4
 };
 
-// Kernel 1 for q8_0 cells (elem 1): quants into k/v_layer, per-32 f16 scales
-// into k/v_scale ([cell][kv_dim / 32]).
+// PoolGeom::elem of q4_0 pools (half a byte per element). Their quants lie in
+// tiles [block][kv_dim / 32][16 slots][16 bytes], not in token-major rows.
+constexpr int kElemQ4 = 0;
+
+// Kernel 1 for q8_0 and q4_0 cells: quants into k/v_layer, per-32 f16 scales
+// into k/v_scale ([block][kv_dim / 32][16 slots]).
 // With order (n entries), launch row i is source row order[i]; entries outside
 // [0, n_rows) are skipped.
-hipError_t launch_write_q8(const PoolGeom &g, void *k_layer, void *v_layer, void *k_scale,
-                           void *v_scale, const int32_t *slots, const float *k, const float *v,
-                           int64_t n, int64_t src_stride, hipStream_t s, const int32_t *order = nullptr,
-                           int64_t n_rows = 0);
+hipError_t launch_write_quant(const PoolGeom &g, void *k_layer, void *v_layer, void *k_scale,
+                              void *v_scale, const int32_t *slots, const float *k, const float *v,
+                              int64_t n, int64_t src_stride, hipStream_t s, const int32_t *order = nullptr,
+                              int64_t n_rows = 0);
 
 hipError_t launch_write(const PoolGeom &g, void *k_layer, void *v_layer, const int32_t *slots,
                         const float *k, const float *v, int64_t n, int64_t src_stride,
@@ -47,12 +51,12 @@ hipError_t launch_write_rope(const PoolGeom &g, void *k_layer, void *v_layer, co
                             int64_t n, int64_t src_stride, int64_t q_stride, int n_heads,
                             const RopeGeom &r, hipStream_t s);
 
-// The same for q8_0 cells: K rotated then quantised per 32 elements, V
-// quantised, Q rotated in place.
-hipError_t launch_write_rope_q8(const PoolGeom &g, void *k_layer, void *v_layer, void *k_scale, void *v_scale,
-                               const int32_t *slots, const int32_t *positions, const float *k, const float *v,
-                               float *q, int64_t n, int64_t src_stride, int64_t q_stride, int n_heads,
-                               const RopeGeom &r, hipStream_t s);
+// The same for q8_0 and q4_0 cells: K rotated then quantised per 32 elements,
+// V quantised, Q rotated in place.
+hipError_t launch_write_rope_quant(const PoolGeom &g, void *k_layer, void *v_layer, void *k_scale, void *v_scale,
+                                   const int32_t *slots, const int32_t *positions, const float *k, const float *v,
+                                   float *q, int64_t n, int64_t src_stride, int64_t q_stride, int n_heads,
+                                   const RopeGeom &r, hipStream_t s);
 
 // Kernel 2 over (src, dst) block pairs of every layer; `bulk` selects the
 // form for large batches (pairs in destination order, see launch_copy_order).
@@ -358,6 +362,56 @@ struct MqArgs {
 };
 bool mq_supported(int elem, int head_dim, int group);
 hipError_t launch_mq_attention(const PoolGeom &g, const MqArgs &a, hipStream_t s);
+
+// ---- q4_0 decode attention and scored attention (ltkv_scored.hip) ----------
+
+// Rows of a scored attention call (ltkv_scored_attention), or the queries of a
+// decode call on a q4_0 pool (row_starts == nullptr: row i is query i at the
+// last position of its context).
+struct ScoredArgs {
+  const void *k_layer, *v_layer;
+  const void *k_scale, *v_scale;  // quantised pools: per-32 f16 scales of the layer
+  const void *q;                  // [n_rows][n_heads * head_dim] of row_type
+  void *out;                      // likewise
+  int row_type;                   // LTKV_ROWS_*
+  const int32_t *tables;
+  int64_t table_stride;
+  const int32_t *rows;  // resident tables: sequence i reads table row rows[i] (nullptr: row i)
+  int64_t table_rows;
+  const int32_t *lens;        // [n] context lengths, this call's rows included
+  const int32_t *row_starts;  // [n + 1], or nullptr
+  int64_t n, n_rows;
+  int64_t max_rows;  // most rows of a sequence
+  int64_t max_len;   // lengths are cut to it
+  int n_heads, n_kv_heads, head_dim;
+  float scale, softcap;  // softcap 0: none
+  const float *slopes;   // [n_heads], or nullptr
+  int64_t window, sinks; // window 0: none
+  const int32_t *prefix; // [n], or nullptr
+  const int32_t *first;  // [n_rows], or nullptr
+  int32_t *status;       // fault word, as AttnArgs::status
+  int cu_count;
+  int part_tokens;       // 0: the per-length policy of decode partitions
+  // Partials of rows split over their context: part_o [row][head][max_parts]
+  // [head_dim], part_ml [row][head][max_parts][2], part_n [row] parts used.
+  float *part_o, *part_ml;
+  int32_t *part_n;
+  int max_parts;
+};
+
+// Partials of a call (offsets and bytes; 0 bytes: none needed); sets max_parts.
+struct ScoredWorkspace {
+  int64_t part_o_off, part_ml_off, part_n_off, bytes;
+};
+ScoredWorkspace scored_workspace(int elem, ScoredArgs &a);
+hipError_t launch_scored_attention(const PoolGeom &g, const ScoredArgs &a, hipStream_t s);
+
+// Rows 0 .. lens[i] - 1 behind each table as f32 values, at row out_offsets[i]
+// onward of k_out / v_out ([rows][kv_dim]); table faults as launch_gather.
+hipError_t launch_gather_values(const PoolGeom &g, const void *k_layer, const void *v_layer, const void *k_scale,
+                                const void *v_scale, const int32_t *tables, int64_t table_stride,
+                                const int32_t *lens, const int64_t *out_offsets, int64_t n, float *k_out,
+                                float *v_out, int32_t *status, hipStream_t s);
 
 // Scratch of the allocation-free decode attention: a static device array of
 // kScratchBytes on every device the library runs on. scratch_address gives

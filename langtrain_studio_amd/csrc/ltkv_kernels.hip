@@ -1,8 +1,8 @@
 // gfx950 (MI355X, CDNA4) kernels of the paged KV-cache path.
 //
-//   write_kernel / write_q8_kernel      slot-mapped K/V append (kv.rs:123-131 write,
-//                                       per model.rs:414-429; q8_0 per quant.rs:785-791)
-//   write_rope_kernel / write_rope_q8_kernel  RoPE of K and Q (model.rs:291-308) fused
+//   write_kernel / write_quant_kernel   slot-mapped K/V append (kv.rs:123-131 write,
+//                                       per model.rs:414-429; q8_0 per quant.rs:785-791; q4_0)
+//   write_rope_kernel / write_rope_quant_kernel  RoPE of K and Q (model.rs:291-308) fused
 //                                       into the append
 //   copy_blocks_kernel                  copy-on-write block copy (kv.rs:99-110)
 //   gather_kernel                       block-table gather (kv.rs:133-150 rows, collected)
@@ -33,6 +33,7 @@
 #include <mutex>
 #include <type_traits>
 
+#include "ltkv_device.h"
 #include "ltkv_kernels.h"
 
 // Scratch of the allocation-free decode attention (ltkv_decode_attention_noalloc):
@@ -62,45 +63,6 @@ static __device__ unsigned long long g_timeline[kTimelineWaves * 8];
 
 namespace ltkv {
 namespace {
-
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-typedef __fp16 hf4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
-typedef __attribute__((address_space(3))) hf4 lds_hf4;
-typedef __attribute__((address_space(3))) char lds_char;
-
-// Fault bits of a cache's status word (reported by ltkv_synchronize).
-constexpr int kFaultTable = 1;      // a block-table entry outside the pool
-constexpr int kFaultFusedCell = 2;  // a fused append's cell is not position len - 1 of its table
-
-// ds_read_b64_tr_b16: within each 16-lane group, lane i receives element
-// i % 4 of the 8 bytes addressed by lane 4 j + i / 4 as its element j.
-__device__ __forceinline__ hf4 lds_read_tr(const char *p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_hf4 *)(lds_char *)p);
-}
-
-// ----------------------------------------------------------------------------
-// f32 -> f16, IEEE round-to-nearest-even (the conversion of f16::from_f32).
-// v_cvt_f16_f32 rounds to nearest even in the default mode; NaN is rewritten
-// explicitly so the result is sign | 0x7e00 | top payload bits on every part.
-// ----------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t f16_bits(float x) {
-  const _Float16 h = (_Float16)x;
-  uint32_t b = (uint32_t)__builtin_bit_cast(uint16_t, h);
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  if ((u & 0x7fffffffu) > 0x7f800000u) b = ((u >> 16) & 0x8000u) | 0x7e00u | ((u >> 13) & 0x3ffu);
-  return b;
-}
-
-__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
-  return f16_bits(a) | (f16_bits(b) << 16);
-}
 
 // ----------------------------------------------------------------------------
 // Kernel 1: slot-mapped append. One thread moves 8 consecutive elements of
@@ -209,13 +171,6 @@ write_kernel(uint8_t *__restrict__ kpool, uint8_t *__restrict__ vpool,
 // int8 quants in the cell and its scale d, rounded to f16, in the scale pool
 // (the Q8_0 block of quant.rs:188-193: f16 d + 32 int8).
 // ----------------------------------------------------------------------------
-// DPP move of x (row_mask and bank_mask all set).
-template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-  return __builtin_bit_cast(
-      float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
-}
-
 // quant.rs:785-791 on one 32-element group spread over 4 aligned lanes of
 // a wave, 8 elements each (lane j of the group holds elements 8j .. 8j+7):
 // amax folded with fmaxf from 0 (a NaN element is skipped, as f32::max; an
@@ -246,16 +201,66 @@ __device__ __forceinline__ void quantize_store4(const float (&x)[8], int j, int8
   if (j == 0) *ds = (uint16_t)f16_bits(d);
 }
 
-// Scale entry of (cell s, group g): layout [block][kv_dim / 32][16 slots],
-// so the scales of one kv head of a block are one contiguous run.
-__device__ __forceinline__ int64_t scale_index(int32_t s, int g, int kg) {
-  return (((int64_t)(s >> 4) * kg + g) << 4) + (s & 15);
+// A 32-element group as 4-bit quants, spread over 4 aligned lanes like
+// quantize_store4's. The scale is minus an eighth of the element of largest
+// magnitude (the positive one where both signs reach it), so that element
+// becomes -8 exactly and the levels -8 .. 7 are all used; magnitudes over
+// 65280 count as 65280 and NaN as 0. The scale is rounded to 8 significant
+// bits (bf16, nearest even) before it becomes an f16: q then has at most 3
+// bits (or is -8) and d at most 8, so q * d is exactly an f16 number (subnormal
+// ones too) and the readers multiply in f16 without rounding. q is the nearest
+// integer to x / d, ties to even: the division is correctly rounded and d has
+// 8 bits, so its rounding never moves a quotient onto or across a tie. Quants
+// are stored offset by 8, element 2 i of a lane's 8 at bits 4 i of its dword
+// and element 2 i + 1 at bits 16 + 4 i: a shift and a mask give two f16 lanes.
+// A group's 16 bytes lie in its block's tile [kv_dim / 32][16 slots][16 bytes]
+// (a head's rows of a block are one contiguous run, as its scales are).
+__device__ __forceinline__ void quantize_store4_q4(const float (&x)[8], int j, uint8_t *__restrict__ tile,
+                                                   uint16_t *__restrict__ ds) {
+  constexpr float kLimit = 65280.f;  // 8 * the largest 8-bit scale whose products are finite f16 numbers
+  float c[8], top = -kLimit, low = kLimit;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    c[i] = x[i] == x[i] ? __builtin_fminf(__builtin_fmaxf(x[i], -kLimit), kLimit) : 0.f;
+    top = __builtin_fmaxf(top, c[i]);
+    low = __builtin_fminf(low, c[i]);
+  }
+  top = __builtin_fmaxf(top, dpp<0xB1>(top));
+  low = __builtin_fminf(low, dpp<0xB1>(low));
+  top = __builtin_fmaxf(top, dpp<0x4E>(top));
+  low = __builtin_fminf(low, dpp<0x4E>(low));
+  const float e = (top >= -low ? top : low) * -0.125f;
+  const uint32_t u = __builtin_bit_cast(uint32_t, e);
+  const _Float16 dh = (_Float16)__builtin_bit_cast(float, (u + 0x7fffu + ((u >> 16) & 1u)) & 0xffff0000u);
+  const float d = (float)dh;
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float r = d != 0.f ? __builtin_rintf(c[i] / d) : 0.f;
+    const int q = (int)__builtin_fminf(__builtin_fmaxf(r, -8.f), 7.f);
+    w |= (uint32_t)(q + 8) << (4 * (i >> 1) + 16 * (i & 1));
+  }
+  reinterpret_cast<uint32_t *>(tile)[j] = w;
+  if (j == 0) *ds = d != 0.f ? __builtin_bit_cast(uint16_t, dh) : (uint16_t)0;
 }
 
-// Kernel 1 for q8_0 cells: 4 lanes per 32-element group of K or V, two
-// 16-byte loads and one 8-byte store per lane.
+// A lane's 8 elements of row element e (K or V row of cell s) into the pools of
+// BITS-bit quants.
+template <int BITS>
+__device__ __forceinline__ void store_quants(const float (&x)[8], int32_t s, int e, int kv_dim, int8_t *pool,
+                                             uint16_t *scales) {
+  const int64_t at = scale_index(s, e >> 5, kv_dim >> 5);
+  if constexpr (BITS == 8)
+    quantize_store4(x, (e >> 3) & 3, pool + (int64_t)s * kv_dim + (e & ~31), scales + at);
+  else
+    quantize_store4_q4(x, (e >> 3) & 3, reinterpret_cast<uint8_t *>(pool) + at * 16, scales + at);
+}
+
+// Kernel 1 for q8_0 and q4_0 cells: 4 lanes per 32-element group of K or V, two
+// 16-byte loads and one 8-byte (4-byte) store per lane.
+template <int BITS>
 __global__ void __launch_bounds__(256)
-write_q8_kernel(int8_t *__restrict__ kpool, int8_t *__restrict__ vpool, uint16_t *__restrict__ kscale,
+write_quant_kernel(int8_t *__restrict__ kpool, int8_t *__restrict__ vpool, uint16_t *__restrict__ kscale,
                 uint16_t *__restrict__ vscale, const int32_t *__restrict__ slots,
                 const float *__restrict__ k, const float *__restrict__ v, int64_t n, int64_t src_stride,
                 int kv_dim, int64_t n_slots, const int32_t *__restrict__ order, int64_t n_rows) {
@@ -273,8 +278,7 @@ write_q8_kernel(int8_t *__restrict__ kpool, int8_t *__restrict__ vpool, uint16_t
   const f32x4 *src = reinterpret_cast<const f32x4 *>((is_v ? v : k) + row * src_stride + e);
   const f32x4 t0 = src[0], t1 = src[1];
   const float x[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
-  quantize_store4(x, (e >> 3) & 3, (is_v ? vpool : kpool) + (int64_t)s * kv_dim + (e & ~31),
-                  (is_v ? vscale : kscale) + scale_index(s, e >> 5, kv_dim >> 5));
+  store_quants<BITS>(x, s, e, kv_dim, is_v ? vpool : kpool, is_v ? vscale : kscale);
 }
 
 // ----------------------------------------------------------------------------
@@ -409,16 +413,17 @@ write_rope_kernel(uint8_t *__restrict__ kpool, uint8_t *__restrict__ vpool,
 }
 
 // ----------------------------------------------------------------------------
-// Kernel 1 with RoPE for q8_0 cells: 4 lanes per 32-element group of K
-// (rotated, then quantised as write_q8_kernel) or of V (quantised), 8
+// Kernel 1 with RoPE for q8_0 and q4_0 cells: 4 lanes per 32-element group of K
+// (rotated, then quantised as write_quant_kernel) or of V (quantised), 8
 // elements a lane; and a thread per 8-element unit of Q (rotated in place,
 // as write_rope_kernel). A lane's K elements rotate with the products of
 // rope_pairs, 4 at a time: (2i, 2i+1) partners lie in the lane, NeoX
 // partners (i, i + rope_dim/2) are the 4 elements rope_dim/2 away (rope_dim
 // is a multiple of 8, so each 4 lie on one side).
 // ----------------------------------------------------------------------------
+template <int BITS>
 __global__ void __launch_bounds__(256)
-write_rope_q8_kernel(int8_t *__restrict__ kpool, int8_t *__restrict__ vpool, uint16_t *__restrict__ kscale,
+write_rope_quant_kernel(int8_t *__restrict__ kpool, int8_t *__restrict__ vpool, uint16_t *__restrict__ kscale,
                      uint16_t *__restrict__ vscale, const int32_t *__restrict__ slots,
                      const int32_t *__restrict__ positions, const float *__restrict__ k,
                      const float *__restrict__ v, float *__restrict__ q, int64_t n, int64_t src_stride,
@@ -485,8 +490,7 @@ write_rope_q8_kernel(int8_t *__restrict__ kpool, int8_t *__restrict__ vpool, uin
       }
     }
   }
-  quantize_store4(x, (e >> 3) & 3, (is_v ? vpool : kpool) + (int64_t)s * kv_dim + (e & ~31),
-                  (is_v ? vscale : kscale) + scale_index(s, e >> 5, kv_dim >> 5));
+  store_quants<BITS>(x, s, e, kv_dim, is_v ? vpool : kpool, is_v ? vscale : kscale);
 }
 // ----------------------------------------------------------------------------
 // Kernel 2: block copy. Work item = one chunk of THREADS x VEC 16-byte
@@ -701,58 +705,6 @@ struct Tile<float> {
 constexpr int kAttnWaves = 4;
 constexpr int kBufferWord3 = 0x00020000;  // buffer descriptor word 3 for gfx9-family raw buffers
 constexpr int kNt = 2;                    // buffer load cache policy: non-temporal
-constexpr float kLog2e = 1.4426950408889634f;
-
-// Block table of query qi: row qi of `tables`, or, with resident tables, row
-// rows[qi] (a row outside [0, n_rows) reads row 0: such a query must have
-// length 0, and nothing is read then).
-__device__ __forceinline__ const int32_t *table_of(const int32_t *tables, int64_t stride,
-                                                   const int32_t *rows, int64_t n_rows, int64_t qi) {
-  int64_t r = qi;
-  if (rows) {
-    r = ((const __attribute__((address_space(4))) int32_t *)rows)[qi];  // uniform: the scalar cache
-    if (r < 0 || r >= n_rows) r = 0;
-  }
-  return tables + r * stride;
-}
-
-// Faults a device op met, for ltkv_synchronize to report (the reference
-// panics at the same places): status[0] ORs the fault bits, status[1] holds
-// the query of one of them. The op goes on safely (a bad entry reads block
-// 0), so nothing faults on the GPU.
-// A wave-uniform read of memory no thread writes during the launch (block
-// tables, lengths), through the scalar cache: the constant address space
-// tells the compiler so, where stores elsewhere in the kernel would keep it
-// from proving it.
-__device__ __forceinline__ int32_t scalar_read(const int32_t *p, int64_t i) {
-  return ((const __attribute__((address_space(4))) int32_t *)p)[i];
-}
-
-// Every calling lane stores the same bits and query: no lane test, so values
-// the caller computes around a report stay uniform over the wave.
-__device__ __forceinline__ void report_fault(int32_t *status, int code, int64_t qi) {
-  if (!status) return;
-  __hip_atomic_fetch_or(status, code, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  status[1] = (int32_t)qi;
-}
-
-// Checks the table entries of blocks [b0, b1) (the positions a work-group
-// reads: kv.rs:147 indexes the sequence's blocks with them) and the query's
-// row in the resident tables; run once before the tile loop, one wave.
-__device__ __forceinline__ void check_table(const int32_t *tab, int b0, int b1, int64_t n_blocks,
-                                            const int32_t *rows, int64_t n_rows, int64_t qi, int32_t *status) {
-  if (!status || b1 <= b0) return;
-  bool bad = false;
-  if (rows) {
-    const int32_t r = rows[qi];
-    bad = r < 0 || r >= n_rows;  // such a query must have length 0
-  }
-  for (int b = b0 + (int)(threadIdx.x & 63); b < b1 && !bad; b += 64) {
-    const int32_t blk = tab[b];
-    bad = blk < 0 || blk >= n_blocks;
-  }
-  if (__builtin_amdgcn_ballot_w64(bad)) report_fault(status, kFaultTable, qi);
-}
 
 // Fused append of the f32 decode kernels: the work-group of the query's last
 // partition writes the new row of its kv head (position len - 1, cell
@@ -1665,36 +1617,6 @@ struct BufVec<4> {
   }
 };
 
-// Stored quants x 8 (bytes u = x + 128) -> f16 x 8 of x, exact: each byte
-// becomes the mantissa of an f16 in [1024, 1280) (bits 0x6400 | u, value
-// 1024 + u), and 1152 is subtracted: two v_perm_b32 and two packed f16
-// subtractions per four elements.
-__device__ __forceinline__ h8 i8x8_to_h8(const u32x2 &w) {
-  constexpr uint32_t kHi = 0x64646464u;
-  const uint32_t a = w.x, b = w.y;
-  const h2 bias = {(_Float16)1152.f, (_Float16)1152.f};
-  const h2 p0 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(kHi, a, 0x04010400u)) - bias;
-  const h2 p1 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(kHi, a, 0x04030402u)) - bias;
-  const h2 p2 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(kHi, b, 0x04010400u)) - bias;
-  const h2 p3 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(kHi, b, 0x04030402u)) - bias;
-  return h8{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
-}
-
-// Sum / maximum of a value over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (the
-// four 16-lane rows of the wave), in every lane: v_permlane16_swap and
-// v_permlane32_swap of x with itself give the even and odd rows (the lower
-// and upper halves) in both places, so no exchange goes through LDS.
-template <bool MAX>
-__device__ __forceinline__ float rows_reduce(float x) {
-  auto op = [](float a, float b) { return MAX ? __builtin_fmaxf(a, b) : a + b; };
-  uint32_t u = __builtin_bit_cast(uint32_t, x);
-  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  x = op(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
-  u = __builtin_bit_cast(uint32_t, x);
-  const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return op(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
-}
-
 constexpr float kDecodeSlack = 8.f;  // log2 headroom of the softmax reference
 // q8_0 weights enter their products times a V scale (~0.02 for rows of N(0, 1)),
 // so the lo parts of most are subnormal, multiples of 2^-24. Their reference lies
@@ -2454,7 +2376,7 @@ attn_mfma_kernel(const T *__restrict__ kpool, const T *__restrict__ vpool, const
     }
     if constexpr (Q8) {
       // Fused append into q8_0 cells: the wave quantises the row of its heads
-      // (write_q8_kernel's 4 lanes per group, the same bits), stores it and
+      // (write_quant_kernel's 4 lanes per group, the same bits), stores it and
       // waits for the stores, and its tiles' loads find the row in the pool.
       if (new_slots && it.tok1 == len && len > 0) {  // uniform
         const int32_t cell = scalar_read(new_slots, qi);
@@ -3804,21 +3726,6 @@ constexpr int kAnyThreads = 256;
 constexpr int kAnyMaxHeadDim = 1024;  // four output elements per thread
 constexpr int kAnyD = kAnyMaxHeadDim / kAnyThreads;
 
-// Block-wide max / sum over the 256 threads (every thread gets it).
-template <bool MAX>
-__device__ __forceinline__ float block_reduce(float x, float *red) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    const float y = __shfl_xor(x, off, 64);
-    x = MAX ? __builtin_fmaxf(x, y) : x + y;
-  }
-  __syncthreads();  // red may still be read by the previous reduction
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-  __syncthreads();
-  const float a = red[0], b = red[1], c = red[2], d = red[3];
-  return MAX ? __builtin_fmaxf(__builtin_fmaxf(a, b), __builtin_fmaxf(c, d)) : (a + b) + (c + d);
-}
-
 // Element e of a pool row of cell `cell` (block * 16 + slot) as f32: f16 and
 // f32 as stored, q8_0 as d * q (quant byte q + 128, scale d of the element's
 // 32-element group, [block][kv_dim / 32][16 slots]).
@@ -4396,14 +4303,15 @@ slot_mapping_kernel(const int32_t *__restrict__ tables, const int32_t *__restric
 
 }  // namespace
 
-hipError_t launch_write_q8(const PoolGeom &g, void *k_layer, void *v_layer, void *k_scale,
-                           void *v_scale, const int32_t *slots, const float *k, const float *v,
-                           int64_t n, int64_t src_stride, hipStream_t s, const int32_t *order,
-                           int64_t n_rows) {
+hipError_t launch_write_quant(const PoolGeom &g, void *k_layer, void *v_layer, void *k_scale,
+                              void *v_scale, const int32_t *slots, const float *k, const float *v,
+                              int64_t n, int64_t src_stride, hipStream_t s, const int32_t *order,
+                              int64_t n_rows) {
   if (n <= 0) return hipSuccess;
   const int64_t threads = n * (g.kv_dim >> 2);
   const int64_t blocks = (threads + 255) / 256;
-  write_q8_kernel<<<(unsigned)blocks, 256, 0, s>>>(
+  const auto kernel = g.elem == kElemQ4 ? write_quant_kernel<4> : write_quant_kernel<8>;
+  kernel<<<(unsigned)blocks, 256, 0, s>>>(
       static_cast<int8_t *>(k_layer), static_cast<int8_t *>(v_layer), static_cast<uint16_t *>(k_scale),
       static_cast<uint16_t *>(v_scale), slots, k, v, n, src_stride, g.kv_dim, g.n_blocks * 16, order, n_rows);
   return hipGetLastError();
@@ -4478,14 +4386,15 @@ hipError_t launch_write_rope(const PoolGeom &g, void *k_layer, void *v_layer, co
   return hipGetLastError();
 }
 
-hipError_t launch_write_rope_q8(const PoolGeom &g, void *k_layer, void *v_layer, void *k_scale, void *v_scale,
-                               const int32_t *slots, const int32_t *positions, const float *k, const float *v,
-                               float *q, int64_t n, int64_t src_stride, int64_t q_stride, int n_heads,
-                               const RopeGeom &r, hipStream_t s) {
+hipError_t launch_write_rope_quant(const PoolGeom &g, void *k_layer, void *v_layer, void *k_scale, void *v_scale,
+                                   const int32_t *slots, const int32_t *positions, const float *k, const float *v,
+                                   float *q, int64_t n, int64_t src_stride, int64_t q_stride, int n_heads,
+                                   const RopeGeom &r, hipStream_t s) {
   if (n <= 0) return hipSuccess;
   const int64_t per = 2 * (int64_t)(g.kv_dim >> 3) + (q ? (int64_t)n_heads * (r.head_dim >> 3) : 0);
   const int64_t blocks = (n * per + 255) / 256;
-  write_rope_q8_kernel<<<(unsigned)blocks, 256, 0, s>>>(
+  const auto kernel = g.elem == kElemQ4 ? write_rope_quant_kernel<4> : write_rope_quant_kernel<8>;
+  kernel<<<(unsigned)blocks, 256, 0, s>>>(
       static_cast<int8_t *>(k_layer), static_cast<int8_t *>(v_layer), static_cast<uint16_t *>(k_scale),
       static_cast<uint16_t *>(v_scale), slots, positions, k, v, q, n, src_stride, q_stride, g.kv_dim, n_heads,
       g.n_blocks * 16, r.table, r.max_pos, r.rope_dim, r.head_dim, r.neox);
@@ -4608,7 +4517,8 @@ AttnWorkspace attention_workspace(int64_t n, int n_heads, int head_dim, int max_
 }
 
 bool attention_supported(int elem, int head_dim, int group) {
-  return (elem == 1 || elem == 2 || elem == 4) && head_dim >= 1 && head_dim <= kAnyMaxHeadDim && group >= 1;
+  return (elem == kElemQ4 || elem == 1 || elem == 2 || elem == 4) && head_dim >= 1 && head_dim <= kAnyMaxHeadDim &&
+         group >= 1;
 }
 
 bool attention_wide(int elem, int head_dim, int group, bool valu) {

@@ -1,0 +1,333 @@
+// gfx950 (MI355X, CDNA4) kernels of scored attention and of q4_0 pools.
+//
+//   scored_any_kernel       scored attention and q4_0 decode attention of any shape
+//   gather_values_kernel    rows behind block tables as f32 values
+//
+// Scored attention (ltkv_scored_attention): row r of a sequence with m rows and
+// L positions stands at position p = L - m + r and sees the positions t with
+//   t < L, first_r <= t, (t <= p or t < prefix), and, with a window of w,
+//   (t > p - w or t < first_r + sinks).
+// Its weights are the softmax over these of
+//   s = scale q.k;  s <- cap tanh(s / cap) with a cap;  s <- s - slope_h |p - t|,
+// and a row that sees nothing (or stands before the context) gives zeros.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <type_traits>
+
+#include "../../include/ltkv.h"
+#include "ltkv_device.h"
+#include "ltkv_kernels.h"
+
+namespace ltkv {
+namespace {
+
+struct Q4 {};  // element tag of q4_0 pools
+
+// A sequence's rows of a call: `count` rows from row `row0`, which stand at
+// positions len - count ... len - 1.
+struct SeqRows {
+  int64_t row0;
+  int32_t count, len;
+};
+
+__device__ __forceinline__ SeqRows seq_rows(const ScoredArgs &a, int64_t seq) {
+  SeqRows s;
+  const int64_t len = scalar_read(a.lens, seq);
+  s.len = (int32_t)(len < 0 ? 0 : len > a.max_len ? a.max_len : len);
+  if (!a.row_starts) {
+    s.row0 = seq;
+    s.count = 1;
+    return s;
+  }
+  // starts outside [0, n_rows], or falling ones, give fewer rows, never a row
+  // outside the call's
+  const int64_t lo = scalar_read(a.row_starts, seq), hi = scalar_read(a.row_starts, seq + 1);
+  s.row0 = lo < 0 ? 0 : lo > a.n_rows ? a.n_rows : lo;
+  const int64_t end = hi > a.n_rows ? a.n_rows : hi;
+  s.count = (int32_t)(end > s.row0 ? end - s.row0 : 0);
+  return s;
+}
+
+// The positions a row sees: [first, sink_end) and [from, end) without those
+// before `from` again, masked by sees().
+struct RowView {
+  int32_t pos;       // the row's position
+  int32_t first;     // first position of its document
+  int32_t sink_end;  // sink positions lie before it
+  int32_t from;      // first position inside the window
+  int32_t end;       // positions from here on are not visible
+  __device__ __forceinline__ bool sees(int32_t t) const {
+    return t >= first && t < end && (t >= from || t < sink_end);
+  }
+};
+
+__device__ __forceinline__ RowView row_view(const ScoredArgs &a, const SeqRows &s, int64_t seq, int32_t r) {
+  RowView v;
+  v.pos = s.len - s.count + r;
+  v.first = a.first ? max(a.first[s.row0 + r], 0) : 0;
+  int32_t end = v.pos + 1;
+  if (a.prefix) end = max(end, min(a.prefix[seq], s.len));
+  v.end = v.pos >= 0 ? end : 0;
+  v.from = v.first;
+  v.sink_end = v.first;
+  if (a.window > 0) {
+    v.from = max(v.first, (int32_t)max((int64_t)v.pos - a.window + 1, (int64_t)0));
+    // (first may be anything: no sum past the last position)
+    v.sink_end = v.first < s.len ? v.first + (int32_t)min(a.sinks, (int64_t)(s.len - v.first)) : v.first;
+  }
+  return v;
+}
+
+// Sequence of launch row `row`: the last one whose first row is not behind it.
+__device__ __forceinline__ int64_t seq_of_row(const ScoredArgs &a, int64_t row) {
+  if (!a.row_starts) return row;
+  int64_t lo = 0, hi = a.n;  // starts[lo] <= row, or lo == 0
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) / 2;
+    if ((int64_t)scalar_read(a.row_starts, mid) <= row) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ float row_load(const ScoredArgs &a, int64_t i) {
+  if (a.row_type == LTKV_ROWS_F32) return static_cast<const float *>(a.q)[i];
+  const uint16_t u = static_cast<const uint16_t *>(a.q)[i];
+  return a.row_type == LTKV_ROWS_F16 ? (float)__builtin_bit_cast(_Float16, u)
+                                     : __builtin_bit_cast(float, (uint32_t)u << 16);
+}
+
+// f32 -> bf16, nearest even (NaN stays NaN).
+__device__ __forceinline__ uint16_t bf16_bits(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
+  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+
+__device__ __forceinline__ void row_store(const ScoredArgs &a, int64_t i, float x) {
+  if (a.row_type == LTKV_ROWS_F32) static_cast<float *>(a.out)[i] = x;
+  else
+    static_cast<uint16_t *>(a.out)[i] = a.row_type == LTKV_ROWS_F16 ? (uint16_t)f16_bits(x) : bf16_bits(x);
+}
+
+// Element e of the pool row of cell `cell` (block * 16 + slot) as f32.
+template <typename T>
+__device__ __forceinline__ float cell_value(const void *pool, const void *scales, int64_t cell, int64_t kv_dim,
+                                            int64_t e) {
+  if constexpr (std::is_same_v<T, Q4>) {
+    const int64_t at = (((cell >> 4) * (kv_dim >> 5) + (e >> 5)) << 4) + (cell & 15);
+    const int i = (int)e & 31;
+    const uint32_t w = static_cast<const uint32_t *>(pool)[at * 4 + (i >> 3)];
+    const int q = (int)(w >> (4 * ((i & 7) >> 1) + 16 * (i & 1)) & 15u) - 8;
+    return (float)q * (float)static_cast<const _Float16 *>(scales)[at];
+  } else if constexpr (std::is_same_v<T, int8_t>) {
+    const int q = (int)static_cast<const uint8_t *>(pool)[cell * kv_dim + e] - 128;
+    const int64_t at = (((cell >> 4) * (kv_dim >> 5) + (e >> 5)) << 4) + (cell & 15);
+    return (float)q * (float)static_cast<const _Float16 *>(scales)[at];
+  } else {
+    return (float)static_cast<const T *>(pool)[cell * kv_dim + e];
+  }
+}
+
+// The score of a visible position from q.k, in the log2 domain.
+__device__ __forceinline__ float score_of(float qk, float scale, float softcap, float slope, int32_t dist) {
+  float s = qk * scale;
+  if (softcap > 0.f) s = softcap * tanhf(s / softcap);
+  return (s - slope * (float)dist) * kLog2e;
+}
+
+constexpr int kAnyThreads = 256;
+constexpr int kAnyMaxHeadDim = 1024;  // four output elements per thread
+constexpr int kAnyD = kAnyMaxHeadDim / kAnyThreads;
+
+// Any shape and pool. Work-group = (row, query head): 256 positions a round,
+// one score a thread, the softmax of the round against the running maximum
+// (exp2 domain), then each thread accumulates up to four output elements over
+// the round's positions. Positions a row does not see are skipped, not
+// multiplied by zero: they may hold infinities or NaN.
+template <typename T>
+__global__ void __launch_bounds__(kAnyThreads) scored_any_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim) {
+  __shared__ float sq[kAnyMaxHeadDim];
+  __shared__ float sp[kAnyThreads];
+  __shared__ int32_t sblk[kAnyThreads / 16];
+  __shared__ float red[4];
+  const int t = (int)threadIdx.x;
+  const int h = (int)(blockIdx.x % a.n_heads);
+  const int64_t row = blockIdx.x / a.n_heads;
+  const int64_t seq = seq_of_row(a, row);
+  const SeqRows s = seq_rows(a, seq);
+  if (row < s.row0 || row >= s.row0 + s.count) return;  // no sequence's row: left as it is
+  const RowView view = row_view(a, s, seq, (int32_t)(row - s.row0));
+  const int64_t head_off = (int64_t)(h / (a.n_heads / a.n_kv_heads)) * a.head_dim;
+  const int64_t qh = (row * a.n_heads + h) * a.head_dim;
+  for (int d = t; d < a.head_dim; d += kAnyThreads) sq[d] = row_load(a, qh + d);
+  const int32_t *tab = table_of(a.tables, a.table_stride, a.rows, a.table_rows, seq);
+  if (t < 64) {
+    check_table(tab, view.first >> 4, (min(view.sink_end, view.end) + 15) >> 4, n_blocks, a.rows, a.table_rows, seq,
+                a.status);
+    check_table(tab, view.from >> 4, (view.end + 15) >> 4, n_blocks, a.rows, a.table_rows, seq, a.status);
+  }
+  const float slope = a.slopes ? a.slopes[h] : 0.f;
+  float m = -INFINITY, l = 0.f, o[kAnyD];
+#pragma unroll
+  for (int k = 0; k < kAnyD; ++k) o[k] = 0.f;
+  // rounds of 16-position blocks, from the sinks on to the window
+  int32_t t0 = (view.sink_end > view.first ? view.first : view.from) & ~15;
+  for (; t0 < view.end; t0 += kAnyThreads) {
+    if (t0 >= view.sink_end && t0 + 16 <= view.from) t0 = view.from & ~15;
+    const int n_tok = min(view.end - t0, kAnyThreads);
+    if (t < (n_tok + 15) / 16) {
+      int32_t blk = tab[(t0 >> 4) + t];
+      if (blk < 0 || blk >= n_blocks) blk = 0;  // reported by check_table
+      sblk[t] = blk;
+    }
+    __syncthreads();
+    float sc = -INFINITY;
+    const bool seen = t < n_tok && view.sees(t0 + t);
+    if (seen) {
+      const int64_t cell = (int64_t)sblk[t >> 4] * 16 + (t & 15);
+      float acc = 0.f;
+      for (int d = 0; d < a.head_dim; ++d)
+        acc += sq[d] * cell_value<T>(a.k_layer, a.k_scale, cell, kv_dim, head_off + d);
+      sc = score_of(acc, a.scale, a.softcap, slope, abs(view.pos - (t0 + t)));
+    }
+    const float mx = block_reduce<true>(sc, red);
+    const float mn = __builtin_fmaxf(m, mx);
+    const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
+    const float alpha = __builtin_amdgcn_exp2f(m - ref);
+    const float p = seen ? __builtin_amdgcn_exp2f(sc - ref) : 0.f;
+    sp[t] = seen ? p : -1.f;
+    l = l * alpha + block_reduce<false>(p, red);
+    m = mn;
+#pragma unroll
+    for (int k = 0; k < kAnyD; ++k) o[k] *= alpha;
+    __syncthreads();
+    for (int j = 0; j < n_tok; ++j) {
+      const float pj = sp[j];
+      if (pj < 0.f) continue;
+      const int64_t cell = (int64_t)sblk[j >> 4] * 16 + (j & 15);
+#pragma unroll
+      for (int k = 0; k < kAnyD; ++k) {
+        const int d = t + kAnyThreads * k;
+        if (d < a.head_dim) o[k] += pj * cell_value<T>(a.v_layer, a.v_scale, cell, kv_dim, head_off + d);
+      }
+    }
+    __syncthreads();  // sblk and sp are rewritten next round
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;  // (a NaN sum stays one)
+#pragma unroll
+  for (int k = 0; k < kAnyD; ++k) {
+    const int d = t + kAnyThreads * k;
+    if (d < a.head_dim) row_store(a, qh + d, o[k] * inv);
+  }
+}
+
+// Rows of a block as f32 values: a work-group per (table entry, K or V), four
+// elements a thread and 16-byte stores (one element where kv_dim is not a
+// multiple of four), consecutive threads on consecutive elements of a row.
+constexpr int kValuesThreads = 256;
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kValuesThreads)
+gather_values_kernel(const void *__restrict__ kpool, const void *__restrict__ vpool, const void *__restrict__ kscale,
+                     const void *__restrict__ vscale, const int32_t *__restrict__ tables, int64_t table_stride,
+                     const int32_t *__restrict__ lens, const int64_t *__restrict__ out_offsets,
+                     float *__restrict__ kout, float *__restrict__ vout, int64_t n_blocks, int64_t kv_dim,
+                     int32_t *__restrict__ status) {
+  const int is_v = (int)(blockIdx.x & 1);
+  const int64_t entry = blockIdx.x >> 1;
+  const int64_t seq = entry / table_stride;
+  const int64_t j = entry - seq * table_stride;
+  int64_t len = lens[seq];
+  if (len > table_stride * 16) len = table_stride * 16;
+  const int64_t start = j * 16;
+  if (start >= len) return;
+  const int rows = (int)(len - start < 16 ? len - start : 16);
+  const int32_t blk = tables[entry];
+  if (blk < 0 || blk >= n_blocks) {
+    if (threadIdx.x == 0) report_fault(status, kFaultTable, seq);
+    return;
+  }
+  const void *pool = is_v ? vpool : kpool, *scale = is_v ? vscale : kscale;
+  float *dst = (is_v ? vout : kout) + (out_offsets[seq] + start) * kv_dim;
+  const int per_row = (int)(kv_dim / VEC);
+  for (int u = (int)threadIdx.x; u < rows * per_row; u += kValuesThreads) {
+    const int slot = u / per_row;
+    const int64_t e = (int64_t)(u - slot * per_row) * VEC, cell = (int64_t)blk * 16 + slot;
+    float x[VEC];
+    if constexpr (VEC == 4 && std::is_same_v<T, Q4>) {
+      const int64_t at = (((cell >> 4) * (kv_dim >> 5) + (e >> 5)) << 4) + (cell & 15);
+      const uint32_t w = static_cast<const uint32_t *>(pool)[at * 4 + (((int)e & 31) >> 3)] >> (2 * ((int)e & 4));
+      const float d = (float)static_cast<const _Float16 *>(scale)[at];
+      x[0] = (float)((int)(w & 15u) - 8) * d;
+      x[1] = (float)((int)(w >> 16 & 15u) - 8) * d;
+      x[2] = (float)((int)(w >> 4 & 15u) - 8) * d;
+      x[3] = (float)((int)(w >> 20 & 15u) - 8) * d;
+    } else if constexpr (VEC == 4 && std::is_same_v<T, int8_t>) {
+      const uint32_t w = *reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(pool) + cell * kv_dim + e);
+      const float d =
+          (float)static_cast<const _Float16 *>(scale)[(((cell >> 4) * (kv_dim >> 5) + (e >> 5)) << 4) + (cell & 15)];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = (float)((int)(w >> (8 * i) & 255u) - 128) * d;
+    } else if constexpr (VEC == 4 && std::is_same_v<T, _Float16>) {
+      const h4 w = *reinterpret_cast<const h4 *>(static_cast<const _Float16 *>(pool) + cell * kv_dim + e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = (float)w[i];
+    } else if constexpr (VEC == 4) {
+      const f32x4 w = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(pool) + cell * kv_dim + e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = w[i];
+    } else {
+      x[0] = cell_value<T>(pool, scale, cell, kv_dim, e);
+    }
+    if constexpr (VEC == 4) *reinterpret_cast<f32x4 *>(dst + slot * kv_dim + e) = f32x4{x[0], x[1], x[2], x[3]};
+    else dst[slot * kv_dim + e] = x[0];
+  }
+}
+
+template <typename F>
+hipError_t by_element(int elem, F &&f) {
+  if (elem == kElemQ4) return f(Q4{});
+  if (elem == 1) return f(int8_t{});
+  if (elem == 2) return f(_Float16{});
+  return f(float{});
+}
+
+}  // namespace
+
+ScoredWorkspace scored_workspace(int elem, ScoredArgs &a) {
+  (void)elem;
+  a.max_parts = 1;
+  return ScoredWorkspace{};
+}
+
+hipError_t launch_scored_attention(const PoolGeom &g, const ScoredArgs &a, hipStream_t s) {
+  if (a.n <= 0 || a.n_rows <= 0) return hipSuccess;
+  const int64_t grid = a.n_rows * a.n_heads;
+  if (grid * kAnyThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
+  return by_element(g.elem, [&](auto tag) {
+    scored_any_kernel<decltype(tag)><<<(unsigned)grid, kAnyThreads, 0, s>>>(a, g.n_blocks, g.kv_dim);
+    return hipGetLastError();
+  });
+}
+
+hipError_t launch_gather_values(const PoolGeom &g, const void *k_layer, const void *v_layer, const void *k_scale,
+                                const void *v_scale, const int32_t *tables, int64_t table_stride,
+                                const int32_t *lens, const int64_t *out_offsets, int64_t n, float *k_out,
+                                float *v_out, int32_t *status, hipStream_t s) {
+  if (n <= 0 || table_stride <= 0) return hipSuccess;
+  const int64_t wgs = n * table_stride * 2;
+  if (wgs * kValuesThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
+  return by_element(g.elem, [&](auto tag) {
+    using T = decltype(tag);
+    const auto kernel = g.kv_dim % 4 == 0 ? gather_values_kernel<T, 4> : gather_values_kernel<T, 1>;
+    kernel<<<(unsigned)wgs, kValuesThreads, 0, s>>>(k_layer, v_layer, k_scale, v_scale, tables, table_stride, lens,
+                                                    out_offsets, k_out, v_out, g.n_blocks, g.kv_dim, status);
+    return hipGetLastError();
+  });
+}
+
+}  // namespace ltkv

@@ -76,17 +76,17 @@ class KvCache:
     """kv.rs KvCache with its pools in HBM.
 
     ``KvCache(n_layers, kv_dim, n_tokens)`` is ``KvCache::new`` (kv.rs:35-48);
-    ``dtype`` selects the storage ("f16" as the reference, "f32", or
-    "q8_0": int8 quants with one f16 scale per 32 elements, quant.rs:785-791)
-    and ``device`` the HIP device (``None`` = a metadata-only cache with no
+    ``dtype`` selects the storage ("f16" as the reference, "f32", "q8_0":
+    int8 quants with one f16 scale per 32 elements, quant.rs:785-791, or
+    "q4_0": 4-bit quants with one) and ``device`` the HIP device (``None`` = a metadata-only cache with no
     pools, whose device ops raise).
     """
 
     def __init__(self, n_layers: int, kv_dim: int, n_tokens: int, dtype: str = "f16",
                  device: Optional[int] = 0, stream=None):
-        codes = {"f16": _lib.F16, "f32": _lib.F32, "q8_0": _lib.Q8_0}
+        codes = {"f16": _lib.F16, "f32": _lib.F32, "q8_0": _lib.Q8_0, "q4_0": _lib.Q4_0}
         if dtype not in codes:
-            raise ValueError("dtype must be 'f16', 'f32' or 'q8_0'")
+            raise ValueError("dtype must be 'f16', 'f32', 'q8_0' or 'q4_0'")
         self._lib = _lib.load()
         h = C.c_void_p()
         dev = _lib.NO_DEVICE if device is None else int(device)
@@ -94,7 +94,7 @@ class KvCache:
         self._h = h
         self.n_layers = n_layers
         self.dtype = dtype
-        self.elem = {"f16": 2, "f32": 4, "q8_0": 1}[dtype]
+        self.elem = {"f16": 2, "f32": 4, "q8_0": 1, "q4_0": 0.5}[dtype]  # bytes per element, scales apart
         self.device = device
         self.n_blocks = self._lib.ltkv_n_blocks(h)
         self._kv_dim = self._lib.ltkv_kv_dim(h)
@@ -294,17 +294,89 @@ class KvCache:
         """Kernel 3: rows 0..lens[i] of each table to k_out/v_out rows out_offsets[i]..."""
         import torch
 
-        dt = {1: torch.int8, 2: torch.float16, 4: torch.float32}[self.elem]
-        n = lens.numel()
-        if tables.dim() != 2 or tables.shape[0] != n or out_offsets.numel() != n:
-            raise ValueError("tables must be [n][stride]; lens and out_offsets [n]")
-        if k_out.dim() != 2 or k_out.shape[1] != self.kv_dim or v_out.shape != k_out.shape:
-            raise ValueError("k_out and v_out must be [rows][kv_dim]")
+        dt = {0.5: torch.int8, 1: torch.int8, 2: torch.float16, 4: torch.float32}[self.elem]
+        n = self._gather_args(tables, lens, out_offsets, k_out, v_out)
         _check(self._lib.ltkv_gather(
             self._h, layer, n, _dev_ptr(tables, torch.int32, "tables", self.device), tables.shape[1],
             _dev_ptr(lens, torch.int32, "lens", self.device),
             _dev_ptr(out_offsets, torch.int64, "out_offsets", self.device),
             _dev_ptr(k_out, dt, "k_out", self.device), _dev_ptr(v_out, dt, "v_out", self.device)))
+
+    def _gather_args(self, tables, lens, out_offsets, k_out, v_out) -> int:
+        n = lens.numel()
+        if tables.dim() != 2 or tables.shape[0] != n or out_offsets.numel() != n:
+            raise ValueError("tables must be [n][stride]; lens and out_offsets [n]")
+        if k_out.dim() != 2 or k_out.shape[1] != self.kv_dim or v_out.shape != k_out.shape:
+            raise ValueError("k_out and v_out must be [rows][kv_dim]")
+        return n
+
+    def gather_values(self, layer: int, tables, lens, out_offsets, k_out, v_out) -> None:
+        """gather with the rows as f32 values, for caches of every dtype: rows
+        0..lens[i] of each table to the f32 k_out/v_out rows out_offsets[i]..."""
+        import torch
+
+        n = self._gather_args(tables, lens, out_offsets, k_out, v_out)
+        _check(self._lib.ltkv_gather_values(
+            self._h, layer, n, _dev_ptr(tables, torch.int32, "tables", self.device), tables.shape[1],
+            _dev_ptr(lens, torch.int32, "lens", self.device),
+            _dev_ptr(out_offsets, torch.int64, "out_offsets", self.device),
+            _dev_ptr(k_out, torch.float32, "k_out", self.device),
+            _dev_ptr(v_out, torch.float32, "v_out", self.device)))
+
+    def scored_attention(self, layer: int, q, tables, lens, n_heads: int, head_dim: int, row_starts=None,
+                         max_rows: Optional[int] = None, scale: Optional[float] = None, softcap: float = 0.0,
+                         slopes=None, window: int = 0, sinks: int = 0, prefix=None, first=None, out=None):
+        """Attention with capped scores, distance biases and masks
+        (ltkv_scored_attention) for single tokens and prompt chunks: sequence i
+        has rows row_starts[i]..row_starts[i+1] of q ([n_rows][n_heads*head_dim],
+        f32, f16 or bf16; row_starts int32 [n+1], None: one row each), the last
+        of its lens[i] positions. softcap > 0: scores become softcap *
+        tanh(score / softcap). slopes (f32 [n_heads]): score minus slope *
+        distance. window > 0: a row sees that many positions up to its own, and
+        the first `sinks`. prefix (int32 [n]): positions every row of the
+        sequence sees. first (int32 [n_rows]): the first position of the row's
+        document. max_rows: the most rows of one sequence (a hint; default: as
+        many as there are). Rows of no sequence are left as they were."""
+        import torch
+
+        n = lens.numel()
+        types = {torch.float32: _lib.ROWS_F32, torch.float16: _lib.ROWS_F16, torch.bfloat16: _lib.ROWS_BF16}
+        if q.dim() != 2 or q.shape[1] != n_heads * head_dim:
+            raise ValueError("q must be [n_rows][n_heads*head_dim]")
+        if q.dtype not in types:
+            raise TypeError(f"q must be float32, float16 or bfloat16, got {q.dtype}")
+        if tables.dim() != 2 or tables.shape[0] != n:
+            raise ValueError("tables must be [n][stride]")
+        n_rows = q.shape[0]
+        if row_starts is None:
+            if n_rows != n:
+                raise ValueError("without row_starts q must have one row per sequence")
+        elif row_starts.numel() != n + 1:
+            raise ValueError("row_starts must have one entry per sequence and one more")
+        if out is None:
+            out = torch.zeros_like(q) if row_starts is not None else torch.empty_like(q)
+        elif out.shape != q.shape:
+            raise ValueError("out must match q")
+        if scale is None:
+            scale = 1.0 / math.sqrt(head_dim)  # model.rs:402
+        if window < 0 or sinks < 0 or (max_rows is not None and max_rows < 0):
+            raise ValueError("window, sinks and max_rows must not be negative")
+
+        def given(t, dtype, name, size):
+            if t is None:
+                return None
+            if t.numel() != size:
+                raise ValueError(f"{name} must have {size} entries")
+            return _dev_ptr(t, dtype, name, self.device)
+
+        _check(self._lib.ltkv_scored_attention(
+            self._h, layer, n, n_rows, n_rows if max_rows is None else max_rows, n_heads, head_dim, float(scale),
+            float(softcap), given(slopes, torch.float32, "slopes", n_heads), window, sinks,
+            given(prefix, torch.int32, "prefix", n), given(first, torch.int32, "first", n_rows), types[q.dtype],
+            _dev_ptr(q, q.dtype, "q", self.device), _dev_ptr(tables, torch.int32, "tables", self.device),
+            tables.shape[1], _dev_ptr(lens, torch.int32, "lens", self.device),
+            given(row_starts, torch.int32, "row_starts", n + 1), _dev_ptr(out, q.dtype, "out", self.device)))
+        return out
 
     def decode_attention(self, layer: int, q, tables, lens, n_heads: int, head_dim: int,
                          scale: Optional[float] = None, out=None, noalloc: bool = False):
@@ -489,8 +561,8 @@ class KvCache:
 
     def read_pool(self, layer: int = 0) -> tuple[np.ndarray, np.ndarray]:
         """Raw K and V pools of one layer, [n_blocks][16][kv_dim] on the host
-        (f16 bits as uint16, float32, or q8_0 quants as int8)."""
-        dt = {1: np.int8, 2: np.uint16, 4: np.float32}[self.elem]
+        (f16 bits as uint16, float32, or q8_0 and q4_0 quants as int8)."""
+        dt = {0.5: np.int8, 1: np.int8, 2: np.uint16, 4: np.float32}[self.elem]
         shape = (self.n_blocks, BLOCK, self.kv_dim)
         k = np.empty(shape, dtype=dt)
         v = np.empty(shape, dtype=dt)
@@ -498,7 +570,7 @@ class KvCache:
         return k, v
 
     def read_scales(self, layer: int = 0) -> tuple[np.ndarray, np.ndarray]:
-        """K and V scale pools of one layer of a q8_0 cache,
+        """K and V scale pools of one layer of a q8_0 or q4_0 cache,
         [n_blocks][kv_dim/32][16] f16 bits (uint16) on the host: the scale of
         slot s, 32-element group g of block b is [b][g][s]."""
         shape = (self.n_blocks, self.kv_dim // 32, BLOCK)
