@@ -1609,7 +1609,7 @@ ltkv::ScoredArgs scored_args(ltkv_cache *c, size_t layer, size_t n, size_t n_row
   a.n = (int64_t)n;
   a.n_rows = (int64_t)n_rows;
   a.max_rows = 1;
-  a.max_len = (int64_t)std::min<size_t>(max_len, (size_t)INT32_MAX - 15);
+  a.max_len = c->n_blocks == 0 ? 0 : (int64_t)std::min<size_t>(max_len, (size_t)INT32_MAX - 15);  // no pool: no context
   a.n_heads = (int)n_heads;
   a.n_kv_heads = (int)(c->kv_dim / head_dim);
   a.head_dim = (int)head_dim;

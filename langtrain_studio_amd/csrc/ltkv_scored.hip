@@ -1,16 +1,8 @@
 // gfx950 (MI355X, CDNA4) kernels of scored attention and of q4_0 pools.
 //
 //   scored_any_kernel       scored attention and q4_0 decode attention of any shape
+//   scored_merge_kernel     fold of the parts of rows that were split
 //   gather_values_kernel    rows behind block tables as f32 values
-//
-// Scored attention (ltkv_scored_attention): row r of a sequence with m rows and
-// L positions stands at position p = L - m + r and sees the positions t with
-//   t < L, first_r <= t, (t <= p or t < prefix), and, with a window of w,
-//   (t > p - w or t < first_r + sinks).
-// Its weights are the softmax over these of
-//   s = scale q.k;  s <- cap tanh(s / cap) with a cap;  s <- s - slope_h |p - t|,
-// and a row that sees nothing (or stands before the context) gives zeros.
-
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -20,98 +12,10 @@
 #include "../../include/ltkv.h"
 #include "ltkv_device.h"
 #include "ltkv_kernels.h"
+#include "ltkv_scored.h"
 
 namespace ltkv {
 namespace {
-
-struct Q4 {};  // element tag of q4_0 pools
-
-// A sequence's rows of a call: `count` rows from row `row0`, which stand at
-// positions len - count ... len - 1.
-struct SeqRows {
-  int64_t row0;
-  int32_t count, len;
-};
-
-__device__ __forceinline__ SeqRows seq_rows(const ScoredArgs &a, int64_t seq) {
-  SeqRows s;
-  const int64_t len = scalar_read(a.lens, seq);
-  s.len = (int32_t)(len < 0 ? 0 : len > a.max_len ? a.max_len : len);
-  if (!a.row_starts) {
-    s.row0 = seq;
-    s.count = 1;
-    return s;
-  }
-  // starts outside [0, n_rows], or falling ones, give fewer rows, never a row
-  // outside the call's
-  const int64_t lo = scalar_read(a.row_starts, seq), hi = scalar_read(a.row_starts, seq + 1);
-  s.row0 = lo < 0 ? 0 : lo > a.n_rows ? a.n_rows : lo;
-  const int64_t end = hi > a.n_rows ? a.n_rows : hi;
-  s.count = (int32_t)(end > s.row0 ? end - s.row0 : 0);
-  return s;
-}
-
-// The positions a row sees: [first, sink_end) and [from, end) without those
-// before `from` again, masked by sees().
-struct RowView {
-  int32_t pos;       // the row's position
-  int32_t first;     // first position of its document
-  int32_t sink_end;  // sink positions lie before it
-  int32_t from;      // first position inside the window
-  int32_t end;       // positions from here on are not visible
-  __device__ __forceinline__ bool sees(int32_t t) const {
-    return t >= first && t < end && (t >= from || t < sink_end);
-  }
-};
-
-__device__ __forceinline__ RowView row_view(const ScoredArgs &a, const SeqRows &s, int64_t seq, int32_t r) {
-  RowView v;
-  v.pos = s.len - s.count + r;
-  v.first = a.first ? max(a.first[s.row0 + r], 0) : 0;
-  int32_t end = v.pos + 1;
-  if (a.prefix) end = max(end, min(a.prefix[seq], s.len));
-  v.end = v.pos >= 0 ? end : 0;
-  v.from = v.first;
-  v.sink_end = v.first;
-  if (a.window > 0) {
-    v.from = max(v.first, (int32_t)max((int64_t)v.pos - a.window + 1, (int64_t)0));
-    // (first may be anything: no sum past the last position)
-    v.sink_end = v.first < s.len ? v.first + (int32_t)min(a.sinks, (int64_t)(s.len - v.first)) : v.first;
-  }
-  return v;
-}
-
-// Sequence of launch row `row`: the last one whose first row is not behind it.
-__device__ __forceinline__ int64_t seq_of_row(const ScoredArgs &a, int64_t row) {
-  if (!a.row_starts) return row;
-  int64_t lo = 0, hi = a.n;  // starts[lo] <= row, or lo == 0
-  while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) / 2;
-    if ((int64_t)scalar_read(a.row_starts, mid) <= row) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
-__device__ __forceinline__ float row_load(const ScoredArgs &a, int64_t i) {
-  if (a.row_type == LTKV_ROWS_F32) return static_cast<const float *>(a.q)[i];
-  const uint16_t u = static_cast<const uint16_t *>(a.q)[i];
-  return a.row_type == LTKV_ROWS_F16 ? (float)__builtin_bit_cast(_Float16, u)
-                                     : __builtin_bit_cast(float, (uint32_t)u << 16);
-}
-
-// f32 -> bf16, nearest even (NaN stays NaN).
-__device__ __forceinline__ uint16_t bf16_bits(float x) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
-
-__device__ __forceinline__ void row_store(const ScoredArgs &a, int64_t i, float x) {
-  if (a.row_type == LTKV_ROWS_F32) static_cast<float *>(a.out)[i] = x;
-  else
-    static_cast<uint16_t *>(a.out)[i] = a.row_type == LTKV_ROWS_F16 ? (uint16_t)f16_bits(x) : bf16_bits(x);
-}
 
 // Element e of the pool row of cell `cell` (block * 16 + slot) as f32.
 template <typename T>
@@ -225,6 +129,37 @@ __global__ void __launch_bounds__(kAnyThreads) scored_any_kernel(ScoredArgs a, i
   }
 }
 
+// Rows whose positions were taken in several parts: the parts' numerators and
+// sums folded in order by their references. A work-group per 256 elements of a
+// row, for the first `most` rows of each sequence (and every most-th after).
+constexpr int kMergeThreads = 256;
+
+__global__ void __launch_bounds__(kMergeThreads) scored_merge_kernel(ScoredArgs a, int slices, int64_t most) {
+  const int64_t item = blockIdx.x / (uint32_t)slices;
+  const int i = (int)(blockIdx.x % (uint32_t)slices) * kMergeThreads + (int)threadIdx.x;
+  const int64_t seq = item / most;
+  const SeqRows s = seq_rows(a, seq);
+  if (i >= a.n_heads * a.head_dim) return;
+  const int h = i / a.head_dim, e = i - h * a.head_dim;
+  for (int64_t r = item - seq * most; r < s.count; r += most) {
+    const int64_t row = s.row0 + r;
+    const int n_parts = scalar_read(a.part_n, row);
+    if (n_parts <= 1) continue;
+    const int64_t at = (row * a.n_heads + h) * a.max_parts;
+    const float *ml = a.part_ml + 2 * at, *o = a.part_o + at * a.head_dim + e;
+    float mx = -INFINITY;
+    for (int p = 0; p < n_parts; ++p) mx = __builtin_fmaxf(mx, ml[2 * p]);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float l = 0.f, x = 0.f;
+    for (int p = 0; p < n_parts; ++p) {
+      const float f = __builtin_amdgcn_exp2f(ml[2 * p] - base);
+      l = __builtin_fmaf(ml[2 * p + 1], f, l);
+      x = __builtin_fmaf(o[(int64_t)p * a.head_dim], f, x);
+    }
+    row_store(a, row * a.n_heads * a.head_dim + i, l != 0.f ? x / l : 0.f);
+  }
+}
+
 // Rows of a block as f32 values: a work-group per (table entry, K or V), four
 // elements a thread and 16-byte stores (one element where kv_dim is not a
 // multiple of four), consecutive threads on consecutive elements of a row.
@@ -288,24 +223,39 @@ gather_values_kernel(const void *__restrict__ kpool, const void *__restrict__ vp
   }
 }
 
-template <typename F>
-hipError_t by_element(int elem, F &&f) {
-  if (elem == kElemQ4) return f(Q4{});
-  if (elem == 1) return f(int8_t{});
-  if (elem == 2) return f(_Float16{});
-  return f(float{});
-}
-
 }  // namespace
 
+// The span of positions a row can see, rounded up to whole steps of both ranges.
+static int64_t span_bound(const ScoredArgs &a) {
+  int64_t span = a.max_len;
+  // (a prefix may show more than the window)
+  if (a.window > 0 && !a.prefix) span = std::min(span, a.window + std::min(a.sinks, a.max_len) + 2 * 16);
+  return (span + 31) / 32 * 32 + 32;
+}
+
 ScoredWorkspace scored_workspace(int elem, ScoredArgs &a) {
-  (void)elem;
+  ScoredWorkspace w{};
   a.max_parts = 1;
-  return ScoredWorkspace{};
+  if (!scored_rows_supported(elem, a.head_dim)) return w;
+  a.max_parts = (int)scored_max_parts(span_bound(a), a.part_tokens);
+  if (a.max_parts <= 1) return w;
+  const int64_t parts = a.n_rows * a.n_heads * (int64_t)a.max_parts;
+  w.part_ml_off = parts * a.head_dim * 4;
+  w.part_n_off = w.part_ml_off + parts * 2 * 4;
+  w.bytes = w.part_n_off + a.n_rows * 4;
+  return w;
 }
 
 hipError_t launch_scored_attention(const PoolGeom &g, const ScoredArgs &a, hipStream_t s) {
   if (a.n <= 0 || a.n_rows <= 0) return hipSuccess;
+  if (a.max_rows <= kRowsKernelMax && scored_rows_supported(g.elem, a.head_dim)) {
+    if (const hipError_t e = launch_scored_rows(g, a, a.n_rows, s); e != hipSuccess || a.max_parts == 1) return e;
+    const int slices = (a.n_heads * a.head_dim + kMergeThreads - 1) / kMergeThreads;
+    const int64_t grid = a.n * a.max_rows * slices;
+    if (grid * kMergeThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
+    scored_merge_kernel<<<(unsigned)grid, kMergeThreads, 0, s>>>(a, slices, a.max_rows);
+    return hipGetLastError();
+  }
   const int64_t grid = a.n_rows * a.n_heads;
   if (grid * kAnyThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
   return by_element(g.elem, [&](auto tag) {

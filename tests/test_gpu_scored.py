@@ -7,7 +7,13 @@ two f16 parts, the scale, the cap and the bias), a tanh by a few half-steps of
 the cap. A weight is then off by as much relatively, twice (numerator and sum),
 the f32 sums over L positions by L + 32 half-steps (32: exp2, the weights as
 two f16 parts, the folds), and f16 / bf16 rows by one f16 rounding per weight
-(2^-11, in numerator and sum) and the rounding of the result to its type."""
+(2^-11, in numerator and sum) and the rounding of the result to its type.
+Small weights are off absolutely: the lo part of a weight is an f16 number, a
+multiple of 2^-24, and a largest weight enters the products as at least 2^6 (8-bit
+pools: as at least 2^6 over the largest scale, times quants of up to 127), so a
+weight is off by at most 2^-25 / 2^6 = 2^-31 of the largest, times at most the
+largest |V| the position could hold: 2^-30 w_max L max |V| in all, where a
+position with a tiny weight holds the only value of its column."""
 
 from __future__ import annotations
 
@@ -112,7 +118,8 @@ def expect(q, held, tables, lens, starts, heads, hd, scale=None, softcap=0.0, sl
                     o, m = w @ v[:, a:a + hd], w @ np.abs(v[:, a:a + hd])
                     out[r, h * hd:(h + 1) * hd] = o
                     mass[r, h * hd:(h + 1) * hd] = m
-                    bound[r, h * hd:(h + 1) * hd] = (2 * off.max() + (t.size + 32) * H) * m
+                    small = 2.0 ** -30 * w.max() * t.size * np.abs(v[:, a:a + hd]).max()
+                    bound[r, h * hd:(h + 1) * hd] = (2 * off.max() + (t.size + 32) * H) * m + small
     return out, bound, mass
 
 
