@@ -18,7 +18,8 @@ LIB = os.path.join(PKG, "libltkv.so")
 # workloads; the product never loads it.
 TIMELINE_LIB = os.path.join(PKG, "libltkv_timeline.so")
 SOURCES = [os.path.join(CSRC, "ltkv_cache.cpp"), os.path.join(CSRC, "ltkv_kernels.hip"),
-           os.path.join(CSRC, "ltkv_scored.hip"), os.path.join(CSRC, "ltkv_scored_rows.hip")]
+           os.path.join(CSRC, "ltkv_scored.hip"), os.path.join(CSRC, "ltkv_scored_rows.hip"),
+           os.path.join(CSRC, "ltkv_scored_chunk.hip")]
 HEADERS = [os.path.join(CSRC, "ltkv_kernels.h"), os.path.join(CSRC, "ltkv_device.h"),
            os.path.join(CSRC, "ltkv_scored.h"), os.path.join(os.path.dirname(PKG), "include", "ltkv.h")]
 

@@ -151,6 +151,10 @@ struct ltkv_cache {
   // ltkv::kPartsBytes, allocated by the first of those and then kept.
   uint8_t *held = nullptr, *states = nullptr;
   size_t held_bytes = 0;
+  // Partials of scored attention and q4_0 decodes (kept_memory): the last buffer
+  // is the one in use.
+  std::vector<uint8_t *> kept;
+  size_t kept_bytes = 0;
   // The device's static scratch (ltkv_decode_attention_noalloc), looked up at
   // creation; shared by every cache on the device.
   uint8_t *scratch = nullptr;
@@ -474,6 +478,36 @@ bool capturing(const ltkv_cache *c) {
     return true;
   }
   return st != hipStreamCaptureStatusNone;
+}
+
+// Memory for the partials of scored attention and of q4_0 decodes: the held
+// memory, or a buffer that grows on demand. An outgrown buffer is kept until the
+// cache is destroyed, since a captured launch may still name it; a capture
+// itself allocates nothing.
+int kept_memory(ltkv_cache *c, size_t bytes, uint8_t **base) {
+  if (bytes <= c->held_bytes) {
+    *base = c->held;
+    return LTKV_OK;
+  }
+  if (c->kept.empty() || bytes > c->kept_bytes) {
+    if (capturing(c))
+      return fail(LTKV_ERR_ARG,
+                  "attention needs %zu bytes of partials, which a stream capture cannot allocate: make the call once "
+                  "before capturing it",
+                  bytes);
+    const size_t size = std::max(bytes, 2 * c->kept_bytes);
+    try {
+      c->kept.reserve(c->kept.size() + 1);
+    } catch (const std::bad_alloc &) {
+      return fail(LTKV_ERR_ARG, "out of host memory");
+    }
+    uint8_t *p = nullptr;
+    HIP_TRY(hipMalloc((void **)&p, size), "hipMalloc(partials)");
+    c->kept.push_back(p);
+    c->kept_bytes = size;
+  }
+  *base = c->kept.back();
+  return LTKV_OK;
 }
 
 // Memory for `bytes` (at most kPartsBytes) of part states, `used` bytes of the
@@ -1184,6 +1218,7 @@ void ltkv_destroy(ltkv_cache *c) {
     if (c->ws) (void)hipFree(c->ws);
     if (c->held) (void)hipFree(c->held);
     if (c->states) (void)hipFree(c->states);
+    for (uint8_t *p : c->kept) (void)hipFree(p);
     if (c->d_status) (void)hipFree(c->d_status);
     if (c->rope) (void)hipFree(c->rope);
     if (c->plan.done) (void)hipEventDestroy(c->plan.done);
@@ -1632,10 +1667,17 @@ int scored_attention(ltkv_cache *c, ltkv::ScoredArgs &a, bool use_scratch = fals
   if (ws.bytes > 0) {
     uint8_t *base = c->scratch;
     if (!use_scratch)
-      if (int rc = workspace(c, (size_t)ws.bytes, &base)) return rc;
-    a.part_o = (float *)(base + ws.part_o_off);
-    a.part_ml = (float *)(base + ws.part_ml_off);
-    a.part_n = (int32_t *)(base + ws.part_n_off);
+      if (int rc = kept_memory(c, (size_t)ws.bytes, &base)) return rc;
+    if (a.max_parts > 1) {
+      a.part_o = (float *)(base + ws.part_o_off);
+      a.part_ml = (float *)(base + ws.part_ml_off);
+      a.part_n = (int32_t *)(base + ws.part_n_off);
+    }
+    if (a.splits > 1) {
+      a.chunk_o = (float *)(base + ws.chunk_o_off);
+      a.chunk_ml = (float *)(base + ws.chunk_ml_off);
+      a.chunk_n = (int32_t *)(base + ws.chunk_n_off);
+    }
   }
   const hipError_t e = ltkv::launch_scored_attention(head_geom(c, (size_t)a.head_dim), a, c->stream);
   if (e == hipErrorInvalidValue) return fail(LTKV_ERR_ARG, "attention grid too large for one launch");
@@ -2001,9 +2043,12 @@ int ltkv_plan_attention(ltkv_cache *c, size_t n, const uint32_t *seqs, const uin
     uint8_t *base = nullptr;
     if (n > 0 && dg.ok) {
       const PlanShape L = plan_shape(c);
-      if (!L.too_large && L.bytes > c->held_bytes && L.bytes > c->ws_bytes && !capturing(c) &&
-          workspace(c, L.bytes, &base) != LTKV_OK)
+      if (c->q4()) {
+        if (!capturing(c) && kept_memory(c, L.bytes, &base) != LTKV_OK) (void)hipGetLastError();
+      } else if (!L.too_large && L.bytes > c->held_bytes && L.bytes > c->ws_bytes && !capturing(c) &&
+                 workspace(c, L.bytes, &base) != LTKV_OK) {
         (void)hipGetLastError();
+      }
     }
   }
   c->plan.valid = true;

@@ -381,7 +381,7 @@ struct ScoredArgs {
   const int32_t *lens;        // [n] context lengths, this call's rows included
   const int32_t *row_starts;  // [n + 1], or nullptr
   int64_t n, n_rows;
-  int64_t max_rows;  // most rows of a sequence
+  int64_t max_rows;  // expected most rows of a sequence
   int64_t max_len;   // lengths are cut to it
   int n_heads, n_kv_heads, head_dim;
   float scale, softcap;  // softcap 0: none
@@ -392,16 +392,24 @@ struct ScoredArgs {
   int32_t *status;       // fault word, as AttnArgs::status
   int cu_count;
   int part_tokens;       // 0: the per-length policy of decode partitions
-  // Partials of rows split over their context: part_o [row][head][max_parts]
-  // [head_dim], part_ml [row][head][max_parts][2], part_n [row] parts used.
+  // Set by scored_workspace: whether the chunk kernel takes sequences, whether
+  // the rows kernel takes rows one by one (not sequences), and the most parts of
+  // a row in either.
+  bool chunks, row_items;
+  int max_parts, splits;
+  // Partials of rows split over their positions: part_o [slot][head][max_parts]
+  // [head_dim], part_ml [slot][head][max_parts][2] (reference, sum), part_n
+  // [slot] parts used, a slot per row (row_items) or max_rows per sequence; the
+  // chunk kernel's with a slot per row.
   float *part_o, *part_ml;
   int32_t *part_n;
-  int max_parts;
+  float *chunk_o, *chunk_ml;
+  int32_t *chunk_n;
 };
 
-// Partials of a call (offsets and bytes; 0 bytes: none needed); sets max_parts.
+// Partials of a call (offsets and bytes; 0 bytes: none needed).
 struct ScoredWorkspace {
-  int64_t part_o_off, part_ml_off, part_n_off, bytes;
+  int64_t part_o_off, part_ml_off, part_n_off, chunk_o_off, chunk_ml_off, chunk_n_off, bytes;
 };
 ScoredWorkspace scored_workspace(int elem, ScoredArgs &a);
 hipError_t launch_scored_attention(const PoolGeom &g, const ScoredArgs &a, hipStream_t s);

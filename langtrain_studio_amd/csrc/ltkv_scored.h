@@ -33,6 +33,16 @@ constexpr int kRowsKernelMax = 2;
 bool scored_rows_supported(int elem, int head_dim);
 hipError_t launch_scored_rows(const PoolGeom &g, const ScoredArgs &a, int64_t most_rows, hipStream_t s);
 
+// The chunk kernel (ltkv_scored_chunk.hip): sequences of more than `min_rows`
+// rows. A work-group takes kChunkColumns (row, query head) pairs of a kv head.
+constexpr int kChunkWaves = 4;
+constexpr int kChunkColumns = 32 * kChunkWaves;
+inline bool scored_chunks_supported(int elem, int head_dim, int group) {
+  return elem != 4 && (head_dim == 64 || head_dim == 128) && group <= kChunkColumns;
+}
+inline int chunk_rows(const ScoredArgs &a) { return kChunkColumns / (a.n_heads / a.n_kv_heads); }
+hipError_t launch_scored_chunks(const PoolGeom &g, const ScoredArgs &a, int64_t min_rows, hipStream_t s);
+
 namespace {
 
 struct Q4 {};  // element tag of q4_0 pools
@@ -125,6 +135,117 @@ __device__ __forceinline__ void row_store(const ScoredArgs &a, int64_t i, float 
 }
 
 
+// Element e of the pool row of cell `cell` (block * 16 + slot) as f32.
+template <typename T>
+__device__ __forceinline__ float cell_value(const void *pool, const void *scales, int64_t cell, int64_t kv_dim,
+                                            int64_t e) {
+  if constexpr (std::is_same_v<T, Q4>) {
+    const int64_t at = (((cell >> 4) * (kv_dim >> 5) + (e >> 5)) << 4) + (cell & 15);
+    const int i = (int)e & 31;
+    const uint32_t w = static_cast<const uint32_t *>(pool)[at * 4 + (i >> 3)];
+    const int q = (int)(w >> (4 * ((i & 7) >> 1) + 16 * (i & 1)) & 15u) - 8;
+    return (float)q * (float)static_cast<const _Float16 *>(scales)[at];
+  } else if constexpr (std::is_same_v<T, int8_t>) {
+    const int q = (int)static_cast<const uint8_t *>(pool)[cell * kv_dim + e] - 128;
+    const int64_t at = (((cell >> 4) * (kv_dim >> 5) + (e >> 5)) << 4) + (cell & 15);
+    return (float)q * (float)static_cast<const _Float16 *>(scales)[at];
+  } else {
+    return (float)static_cast<const T *>(pool)[cell * kv_dim + e];
+  }
+}
+
+// Quants of q4_0, 8 a dword: a nibble becomes the low mantissa bits of an f16
+// in [1024, 1040) (0x6400 | u), 1032 is subtracted and the scale multiplied,
+// both exactly (the scale's 8 bits).
+__device__ __forceinline__ h8 q4x8_to_h8(uint32_t w, h2 d) {
+  const h2 bias = {(_Float16)1032.f, (_Float16)1032.f};
+  h2 p[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    p[i] = (__builtin_bit_cast(h2, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) - bias) * d;
+  return h8{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
+}
+
+// hi + lo f16 parts of x: 22 bits together.
+__device__ __forceinline__ void split2(float x, _Float16 &hi, _Float16 &lo) {
+  // x as an f32 number: folded into a product's conversion it could be rounded
+  // once for hi and twice for what lo is the rest of
+  asm("" : "+v"(x));
+  hi = (_Float16)x;
+  lo = (_Float16)(x - (float)hi);
+}
+
+// Score references are raised only when a score exceeds them by kSlack (log2),
+// so most steps need no exchange between lanes and no rescaling; weights carry
+// 2^lift, so that the largest (2^(kSlack + lift)) lie near the top of f16 and the
+// lo parts of small ones stay out of its subnormals: kLift for values V that are
+// f16 numbers themselves. q8_0 weights are multiplied by V's scales first: the
+// lift follows the largest scale met, whatever its magnitude.
+constexpr float kSlack = 8.f;
+constexpr float kLift = 6.f;
+
+// tanh, to a few units of f32 at any size: odd polynomial below 0.35 (the next
+// term is below 2^-26 there), 1 - 2 / (exp(2 |x|) + 1) beyond.
+__device__ __forceinline__ float tanh_f32(float x) {
+  const float y = x * x;
+  float p = __builtin_fmaf(y, -0.008863235529902197f, 0.021869488536155203f);
+  p = __builtin_fmaf(y, p, -0.05396825396825397f);
+  p = __builtin_fmaf(y, p, 0.13333333333333333f);
+  p = __builtin_fmaf(y, p, -0.3333333333333333f);
+  const float small = __builtin_fmaf(x * y, p, x);
+  const float ax = __builtin_fabsf(x);
+  const float e = __builtin_amdgcn_exp2f(ax * (2.f * kLog2e));
+  const float large = __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
+  return ax < 0.35f ? small : __builtin_copysignf(large, x);
+}
+
+// tanh to a few units of f32 in absolute terms, for rows of 16 bits.
+__device__ __forceinline__ float tanh_f16(float x) {
+  return __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * (2.f * kLog2e)) + 1.f), 1.f);
+}
+
+// Elements i ... i + 7 of Q as f32 (zeros where `live` is false).
+__device__ __forceinline__ void load_row8(const ScoredArgs &a, int64_t i, bool live, float (&x)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) x[k] = 0.f;
+  if (!live) return;
+  if (a.row_type == LTKV_ROWS_F32) {
+    const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(a.q) + i);
+    const f32x4 u = p[0], v = p[1];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[k] = u[k];
+      x[4 + k] = v[k];
+    }
+    return;
+  }
+  const u32x4 u = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.q) + i);
+  const h8 h = __builtin_bit_cast(h8, u);
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    x[k] = a.row_type == LTKV_ROWS_F16
+               ? (float)h[k]
+               : __builtin_bit_cast(float, k & 1 ? u[k >> 1] & 0xffff0000u : u[k >> 1] << 16);
+}
+
+// Elements i ... i + 3 of the output.
+__device__ __forceinline__ void store_row4(const ScoredArgs &a, int64_t i, const f32x4 &x) {
+  if (a.row_type == LTKV_ROWS_F32) {
+    *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + i) = x;
+    return;
+  }
+  uint32_t u[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) u[k] = a.row_type == LTKV_ROWS_F16 ? f16_bits(x[k]) : bf16_bits(x[k]);
+  *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + i) = u32x2{u[0] | u[1] << 16, u[2] | u[3] << 16};
+}
+
+// Two ds_read_b64_tr_b16 as one operand: positions at p and `step` bytes on.
+__device__ __forceinline__ h8 read_tr2(const char *p, int step) {
+  const h4 x = __builtin_bit_cast(h4, lds_read_tr(p)), y = __builtin_bit_cast(h4, lds_read_tr(p + step));
+  return h8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+}
+
 template <typename F>
 hipError_t by_element(int elem, F &&f) {
   if (elem == kElemQ4) return f(Q4{});
@@ -152,20 +273,22 @@ inline int64_t scored_max_parts(int64_t span, int fixed) {
   return parts;
 }
 
-// The 32-token steps over a row's visible positions: those of its sinks, then
-// those of its window (one range where the two meet). Steps begin at block
-// borders; a step's positions end at its range's end.
+// The STEP-position steps over what a row (or rows together) sees: those of the
+// sinks, then those of the window (one range where the two meet). Steps begin
+// at block borders; a step's positions end at its range's end.
+template <int STEP>
 struct StepRange {
   int32_t a0, a_end, b0, b_end;
   int32_t n_a, n;
   __device__ __forceinline__ int32_t start(int32_t step) const {
-    return step < n_a ? a0 + 32 * step : b0 + 32 * (step - n_a);
+    return step < n_a ? a0 + STEP * step : b0 + STEP * (step - n_a);
   }
   __device__ __forceinline__ int32_t end(int32_t step) const { return step < n_a ? a_end : b_end; }
 };
 
-__device__ __forceinline__ StepRange step_range(const RowView &v) {
-  StepRange s;
+template <int STEP>
+__device__ __forceinline__ StepRange<STEP> step_range(const RowView &v) {
+  StepRange<STEP> s;
   s.a0 = v.first & ~15;
   s.a_end = min(v.sink_end, v.end);
   s.b0 = v.from & ~15;
@@ -174,8 +297,8 @@ __device__ __forceinline__ StepRange step_range(const RowView &v) {
     s.b0 = s.a0;
     s.a_end = s.a0;
   }
-  s.n_a = s.a_end > v.first ? (s.a_end - s.a0 + 31) / 32 : 0;
-  s.n = s.n_a + (s.b_end > v.from || (s.b0 == s.a0 && s.b_end > v.first) ? (s.b_end - s.b0 + 31) / 32 : 0);
+  s.n_a = s.a_end > v.first ? (s.a_end - s.a0 + STEP - 1) / STEP : 0;
+  s.n = s.n_a + (s.b_end > v.from || (s.b0 == s.a0 && s.b_end > v.first) ? (s.b_end - s.b0 + STEP - 1) / STEP : 0);
   return s;
 }
 

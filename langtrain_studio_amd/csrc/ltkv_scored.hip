@@ -17,25 +17,6 @@
 namespace ltkv {
 namespace {
 
-// Element e of the pool row of cell `cell` (block * 16 + slot) as f32.
-template <typename T>
-__device__ __forceinline__ float cell_value(const void *pool, const void *scales, int64_t cell, int64_t kv_dim,
-                                            int64_t e) {
-  if constexpr (std::is_same_v<T, Q4>) {
-    const int64_t at = (((cell >> 4) * (kv_dim >> 5) + (e >> 5)) << 4) + (cell & 15);
-    const int i = (int)e & 31;
-    const uint32_t w = static_cast<const uint32_t *>(pool)[at * 4 + (i >> 3)];
-    const int q = (int)(w >> (4 * ((i & 7) >> 1) + 16 * (i & 1)) & 15u) - 8;
-    return (float)q * (float)static_cast<const _Float16 *>(scales)[at];
-  } else if constexpr (std::is_same_v<T, int8_t>) {
-    const int q = (int)static_cast<const uint8_t *>(pool)[cell * kv_dim + e] - 128;
-    const int64_t at = (((cell >> 4) * (kv_dim >> 5) + (e >> 5)) << 4) + (cell & 15);
-    return (float)q * (float)static_cast<const _Float16 *>(scales)[at];
-  } else {
-    return (float)static_cast<const T *>(pool)[cell * kv_dim + e];
-  }
-}
-
 // The score of a visible position from q.k, in the log2 domain.
 __device__ __forceinline__ float score_of(float qk, float scale, float softcap, float slope, int32_t dist) {
   float s = qk * scale;
@@ -129,35 +110,55 @@ __global__ void __launch_bounds__(kAnyThreads) scored_any_kernel(ScoredArgs a, i
   }
 }
 
-// Rows whose positions were taken in several parts: the parts' numerators and
-// sums folded in order by their references. A work-group per 256 elements of a
-// row, for the first `most` rows of each sequence (and every most-th after).
+// Rows whose positions were taken in several parts (or splits): their numerators
+// and sums folded in order by their references. A work-group per 256 elements
+// of a row: first the part slots of the rows kernel (ScoredArgs::part_n), then
+// every launch row for the chunk kernel's.
 constexpr int kMergeThreads = 256;
 
-__global__ void __launch_bounds__(kMergeThreads) scored_merge_kernel(ScoredArgs a, int slices, int64_t most) {
+__global__ void __launch_bounds__(kMergeThreads) scored_merge_kernel(ScoredArgs a, int slices, int64_t part_slots,
+                                                                     int64_t min_rows) {
   const int64_t item = blockIdx.x / (uint32_t)slices;
   const int i = (int)(blockIdx.x % (uint32_t)slices) * kMergeThreads + (int)threadIdx.x;
-  const int64_t seq = item / most;
-  const SeqRows s = seq_rows(a, seq);
   if (i >= a.n_heads * a.head_dim) return;
   const int h = i / a.head_dim, e = i - h * a.head_dim;
-  for (int64_t r = item - seq * most; r < s.count; r += most) {
-    const int64_t row = s.row0 + r;
-    const int n_parts = scalar_read(a.part_n, row);
-    if (n_parts <= 1) continue;
-    const int64_t at = (row * a.n_heads + h) * a.max_parts;
-    const float *ml = a.part_ml + 2 * at, *o = a.part_o + at * a.head_dim + e;
-    float mx = -INFINITY;
-    for (int p = 0; p < n_parts; ++p) mx = __builtin_fmaxf(mx, ml[2 * p]);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float l = 0.f, x = 0.f;
-    for (int p = 0; p < n_parts; ++p) {
-      const float f = __builtin_amdgcn_exp2f(ml[2 * p] - base);
-      l = __builtin_fmaf(ml[2 * p + 1], f, l);
-      x = __builtin_fmaf(o[(int64_t)p * a.head_dim], f, x);
-    }
-    row_store(a, row * a.n_heads * a.head_dim + i, l != 0.f ? x / l : 0.f);
+  int64_t row, slot;
+  int n_parts, stride;
+  const float *o, *ml;
+  if (item < part_slots) {
+    slot = item;
+    const int64_t seq = a.row_items ? seq_of_row(a, item) : item / a.max_rows;
+    const SeqRows s = seq_rows(a, seq);
+    row = a.row_items ? item : s.row0 + (item - seq * a.max_rows);
+    // (slots of rows that no kernel took hold nothing)
+    if (row < s.row0 || row >= s.row0 + s.count || s.count > min_rows) return;
+    n_parts = scalar_read(a.part_n, slot);
+    stride = a.max_parts;
+    o = a.part_o;
+    ml = a.part_ml;
+  } else {
+    slot = row = item - part_slots;
+    const SeqRows s = seq_rows(a, seq_of_row(a, row));
+    if (row < s.row0 || row >= s.row0 + s.count || s.count <= min_rows) return;
+    n_parts = scalar_read(a.chunk_n, slot);
+    stride = a.splits;
+    o = a.chunk_o;
+    ml = a.chunk_ml;
   }
+  if (n_parts <= 1) return;
+  const int64_t at = (slot * a.n_heads + h) * stride;
+  ml += 2 * at;
+  o += at * a.head_dim + e;
+  float mx = -INFINITY;
+  for (int p = 0; p < n_parts; ++p) mx = __builtin_fmaxf(mx, ml[2 * p]);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float l = 0.f, x = 0.f;
+  for (int p = 0; p < n_parts; ++p) {
+    const float f = __builtin_amdgcn_exp2f(ml[2 * p] - base);
+    l = __builtin_fmaf(ml[2 * p + 1], f, l);
+    x = __builtin_fmaf(o[(int64_t)p * a.head_dim], f, x);
+  }
+  row_store(a, row * a.n_heads * a.head_dim + i, l != 0.f ? x / l : 0.f);
 }
 
 // Rows of a block as f32 values: a work-group per (table entry, K or V), four
@@ -225,43 +226,89 @@ gather_values_kernel(const void *__restrict__ kpool, const void *__restrict__ vp
 
 }  // namespace
 
-// The span of positions a row can see, rounded up to whole steps of both ranges.
-static int64_t span_bound(const ScoredArgs &a) {
+namespace {
+
+// Most positions that the steps of a row cover.
+int64_t span_bound(const ScoredArgs &a) {
   int64_t span = a.max_len;
   // (a prefix may show more than the window)
   if (a.window > 0 && !a.prefix) span = std::min(span, a.window + std::min(a.sinks, a.max_len) + 2 * 16);
   return (span + 31) / 32 * 32 + 32;
 }
 
+// Which kernels a call takes: the rows kernel where no sequence is expected to
+// have more than kRowsKernelMax rows (or every row by itself where the chunk
+// kernel does not serve the shape), the chunk kernel else, with the rows kernel
+// for the short sequences beside it; the generic kernel for the other shapes.
+struct Kernels {
+  bool rows, row_items, chunks;
+};
+
+Kernels kernels_of(int elem, const ScoredArgs &a) {
+  const int group = a.n_heads / a.n_kv_heads;
+  if (!scored_rows_supported(elem, a.head_dim)) return {false, false, false};
+  if (a.max_rows <= kRowsKernelMax) return {true, false, false};
+  if (!scored_chunks_supported(elem, a.head_dim, group)) return {true, true, false};
+  return {a.n > 1, false, true};
+}
+
+}  // namespace
+
 ScoredWorkspace scored_workspace(int elem, ScoredArgs &a) {
   ScoredWorkspace w{};
-  a.max_parts = 1;
-  if (!scored_rows_supported(elem, a.head_dim)) return w;
-  a.max_parts = (int)scored_max_parts(span_bound(a), a.part_tokens);
-  if (a.max_parts <= 1) return w;
-  const int64_t parts = a.n_rows * a.n_heads * (int64_t)a.max_parts;
-  w.part_ml_off = parts * a.head_dim * 4;
-  w.part_n_off = w.part_ml_off + parts * 2 * 4;
-  w.bytes = w.part_n_off + a.n_rows * 4;
+  const Kernels k = kernels_of(elem, a);
+  a.row_items = k.row_items;
+  a.chunks = k.chunks;
+  if (k.chunks && k.rows) a.max_rows = kRowsKernelMax;  // of the sequences that the rows kernel takes
+  a.max_parts = a.splits = 1;
+  const int64_t span = span_bound(a);
+  int64_t at = 0;
+  if (k.rows && (a.max_parts = (int)scored_max_parts(span, a.part_tokens)) > 1) {
+    const int64_t slots = a.row_items ? a.n_rows : a.n * a.max_rows, parts = slots * a.n_heads * (int64_t)a.max_parts;
+    w.part_o_off = at;
+    w.part_ml_off = at + parts * a.head_dim * 4;
+    w.part_n_off = w.part_ml_off + parts * 2 * 4;
+    at = (w.part_n_off + slots * 4 + 255) / 256 * 256;
+  }
+  if (k.chunks) {
+    // as many work-groups as are resident (two a CU), at least 256 positions each
+    const int64_t tiles = (a.n_rows / chunk_rows(a) + 1) * a.n_kv_heads;
+    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({2 * a.cu_count / tiles, span / 256, 32}));
+    if (a.splits > 1) {
+      const int64_t parts = a.n_rows * a.n_heads * (int64_t)a.splits;
+      w.chunk_o_off = at;
+      w.chunk_ml_off = at + parts * a.head_dim * 4;
+      w.chunk_n_off = w.chunk_ml_off + parts * 2 * 4;
+      at = w.chunk_n_off + a.n_rows * 4;
+    }
+  }
+  w.bytes = at;
   return w;
 }
 
 hipError_t launch_scored_attention(const PoolGeom &g, const ScoredArgs &a, hipStream_t s) {
   if (a.n <= 0 || a.n_rows <= 0) return hipSuccess;
-  if (a.max_rows <= kRowsKernelMax && scored_rows_supported(g.elem, a.head_dim)) {
-    if (const hipError_t e = launch_scored_rows(g, a, a.n_rows, s); e != hipSuccess || a.max_parts == 1) return e;
-    const int slices = (a.n_heads * a.head_dim + kMergeThreads - 1) / kMergeThreads;
-    const int64_t grid = a.n * a.max_rows * slices;
-    if (grid * kMergeThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
-    scored_merge_kernel<<<(unsigned)grid, kMergeThreads, 0, s>>>(a, slices, a.max_rows);
-    return hipGetLastError();
+  if (!scored_rows_supported(g.elem, a.head_dim)) {
+    const int64_t grid = a.n_rows * a.n_heads;
+    if (grid * kAnyThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
+    return by_element(g.elem, [&](auto tag) {
+      scored_any_kernel<decltype(tag)><<<(unsigned)grid, kAnyThreads, 0, s>>>(a, g.n_blocks, g.kv_dim);
+      return hipGetLastError();
+    });
   }
-  const int64_t grid = a.n_rows * a.n_heads;
-  if (grid * kAnyThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
-  return by_element(g.elem, [&](auto tag) {
-    scored_any_kernel<decltype(tag)><<<(unsigned)grid, kAnyThreads, 0, s>>>(a, g.n_blocks, g.kv_dim);
-    return hipGetLastError();
-  });
+  const int64_t all = INT64_MAX;
+  const int64_t border = a.chunks ? (a.n > 1 ? kRowsKernelMax : 0) : all;  // most rows of the rows kernel's sequences
+  if (a.chunks)
+    if (const hipError_t e = launch_scored_chunks(g, a, border, s); e != hipSuccess) return e;
+  if (border > 0)
+    if (const hipError_t e = launch_scored_rows(g, a, border, s); e != hipSuccess) return e;
+  const int64_t part_slots = border > 0 && a.max_parts > 1 ? (a.row_items ? a.n_rows : a.n * a.max_rows) : 0;
+  const int64_t items = part_slots + (a.splits > 1 ? a.n_rows : 0);
+  if (items == 0) return hipSuccess;
+  const int slices = (a.n_heads * a.head_dim + kMergeThreads - 1) / kMergeThreads;
+  if (items * slices * kMergeThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
+  scored_merge_kernel<<<(unsigned)(items * slices), kMergeThreads, 0, s>>>(a, slices, part_slots, border);
+  return hipGetLastError();
 }
 
 hipError_t launch_gather_values(const PoolGeom &g, const void *k_layer, const void *v_layer, const void *k_scale,

@@ -1,0 +1,559 @@
+// gfx950 (MI355X, CDNA4) kernel of scored attention for prompt chunks: many rows
+// of a sequence against tiles of its positions that they share, on the matrix
+// cores.
+
+#include "ltkv_scored.h"
+
+namespace ltkv {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kChunkTokens = 64;  // positions of a tile
+
+// A thread's share of a tile on its way from the pool to LDS: a quarter of the
+// head (NC = HD / 32 chunks of 8 elements) of one position, K and V. planes()
+// gives the chunk as f16 numbers: f16 and q4_0 cells are f16 numbers; q8_0
+// cells times a power of two (which keeps the tile's largest scale at the top
+// of f16) as f16 hi + lo pairs.
+template <typename T, int NC>
+struct Share;
+
+template <int NC>
+struct Share<_Float16, NC> {
+  u32x4 x[NC];
+  // chunk of the head that x[j] is: 64 consecutive bytes of a position a load
+  __device__ static __forceinline__ int chunk(int part, int j) { return part + 4 * j; }
+  __device__ __forceinline__ void load(const void *pool, const void *, int64_t kv_dim, int32_t blk, int slot, int part,
+                                       int64_t head_off) {
+    const _Float16 *row = static_cast<const _Float16 *>(pool) + ((int64_t)blk * 16 + slot) * kv_dim + head_off;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) x[j] = *reinterpret_cast<const u32x4 *>(row + chunk(part, j) * 8);
+  }
+  __device__ __forceinline__ h8 get(int j) const { return __builtin_bit_cast(h8, x[j]); }
+};
+
+template <int NC>
+struct Share<Q4, NC> {
+  uint32_t x[NC];
+  uint16_t s;
+  __device__ static __forceinline__ int chunk(int part, int j) { return part * NC + j; }
+  __device__ __forceinline__ void load(const void *pool, const void *scales, int64_t kv_dim, int32_t blk, int slot,
+                                       int part, int64_t head_off) {
+    const int e = (int)head_off + part * NC * 8;
+    const int64_t at = ((int64_t)blk * (kv_dim >> 5) + (e >> 5)) * 16 + slot;
+    s = static_cast<const uint16_t *>(scales)[at];
+    const uint32_t *p = static_cast<const uint32_t *>(pool) + at * 4 + ((e & 31) >> 3);
+    if constexpr (NC == 4) {
+      const u32x4 w = *reinterpret_cast<const u32x4 *>(p);
+      x[0] = w.x;
+      x[1] = w.y;
+      x[2] = w.z;
+      x[3] = w.w;
+    } else {
+      const u32x2 w = *reinterpret_cast<const u32x2 *>(p);
+      x[0] = w.x;
+      x[1] = w.y;
+    }
+  }
+  __device__ __forceinline__ h8 get(int j) const {
+    const _Float16 d = __builtin_bit_cast(_Float16, s);
+    return q4x8_to_h8(x[j], h2{d, d});
+  }
+};
+
+template <int NC>
+struct Share<int8_t, NC> {
+  u32x2 x[NC];
+  uint16_t s;
+  __device__ static __forceinline__ int chunk(int part, int j) { return part * NC + j; }
+  __device__ __forceinline__ void load(const void *pool, const void *scales, int64_t kv_dim, int32_t blk, int slot,
+                                       int part, int64_t head_off) {
+    const int64_t e = head_off + part * NC * 8;
+    s = static_cast<const uint16_t *>(scales)[((int64_t)blk * (kv_dim >> 5) + (e >> 5)) * 16 + slot];
+    const uint8_t *p = static_cast<const uint8_t *>(pool) + ((int64_t)blk * 16 + slot) * kv_dim + e;
+#pragma unroll
+    for (int j = 0; j < NC; j += 2) {
+      const u32x4 w = *reinterpret_cast<const u32x4 *>(p + 8 * j);
+      x[j] = u32x2{w.x, w.y};
+      x[j + 1] = u32x2{w.z, w.w};
+    }
+  }
+  __device__ __forceinline__ float scale() const { return (float)__builtin_bit_cast(_Float16, s); }
+  // chunk j times d (the scale times a power of two), as hi + lo parts
+  __device__ __forceinline__ void get2(int j, float d, h8 &hi, h8 &lo) const {
+    const h8 q = i8x8_to_h8(x[j]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      _Float16 a, b;
+      split2((float)q[i] * d, a, b);
+      hi[i] = a;
+      lo[i] = b;
+    }
+  }
+};
+
+// True if an element is infinite or NaN.
+__device__ __forceinline__ bool not_finite(const h8 &x) {
+  const u32x4 u = __builtin_bit_cast(u32x4, x);
+  uint32_t bad = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= ((u[i] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
+  return bad != 0;
+}
+
+__device__ __forceinline__ h8 finite_or_zero(const h8 &x) {
+  h8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = __builtin_fabsf((float)x[i]) <= 65504.f ? x[i] : (_Float16)0.f;
+  return r;
+}
+
+// Sum / maximum of a value over lanes l and l ^ 32.
+template <bool MAX>
+__device__ __forceinline__ float halves_reduce(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const float p = __builtin_bit_cast(float, (uint32_t)b[0]), q = __builtin_bit_cast(float, (uint32_t)b[1]);
+  return MAX ? __builtin_fmaxf(p, q) : p + q;
+}
+
+// Work-group barrier that orders LDS only: loads from global memory stay in
+// flight across it.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// The least and largest of what the rows of a wave (or work-group) see.
+struct Bounds {
+  int32_t first_min, first_max, from_min, from_max, sink_min, sink_max, end_min, end_max;
+  __device__ __forceinline__ bool none(int32_t t, int32_t n) const {  // of positions [t, t + n)
+    return t >= end_max || t + n <= first_min || (t + n <= from_min && t >= sink_max);
+  }
+  __device__ __forceinline__ bool all(int32_t t, int32_t n) const {
+    return t >= first_max && t + n <= end_min && (t >= from_max || t + n <= sink_min);
+  }
+};
+
+// A work-group takes 128 columns, which are (row, query head) pairs of one kv
+// head: 128 / group rows; each of its four waves 32 of them. Tiles of 64
+// positions go through LDS as f16 numbers; a wave takes 32 positions at a time
+// on 32x32x16 products: scores^T = K Q^T, weights in place, numerators^T += V^T W
+// (a lane's scores are positions 8 (r / 4) + 4 (lane / 32) + r % 4 of its column,
+// which is the second product's operand layout when its 16 positions are taken
+// as 4 (lane / 32) ... + 3 and 8 + 4 (lane / 32) ... + 3: no exchange). FULL
+// (f32 rows): Q and the weights as hi + lo pairs; else Q as it is (times a power
+// of two) and the weights rounded to f16.
+template <typename T, int HD, bool FULL>
+__global__ void __launch_bounds__(64 * kChunkWaves, 2)
+scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per_tile, int64_t min_rows,
+                    int64_t n_slots) {
+  constexpr int NC = HD / 32, NK = HD / 16;
+  constexpr bool Q8 = std::is_same_v<T, int8_t>;
+  constexpr int K_PLANES = Q8 ? 2 : 1, V_PLANES = Q8 && FULL ? 2 : 1;
+  constexpr int K_PITCH = HD * 2 + 16;  // rows 4 banks apart: 16-byte reads of 16 rows without conflicts
+  constexpr int V_PITCH = HD * 2 + 64;  // rows 16 banks apart, for the transposing reads
+  constexpr int K_BYTES = kChunkTokens * K_PITCH, V_BYTES = kChunkTokens * V_PITCH;
+  __shared__ __align__(16) char lds[K_PLANES * K_BYTES + V_PLANES * V_BYTES];
+  __shared__ Bounds s_bounds[kChunkWaves];
+  __shared__ float s_scale[kChunkWaves][2];  // q8_0: largest K and V scales of the next tile
+  __shared__ uint32_t s_bad[kChunkWaves];    // a V element of the tile is infinite or NaN
+  char *const lds_k = lds, *const lds_v = lds + K_PLANES * K_BYTES;
+
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int group = a.n_heads / a.n_kv_heads;
+  uint32_t b = blockIdx.x;
+  const int kvh = (int)(b % (uint32_t)a.n_kv_heads);
+  b /= (uint32_t)a.n_kv_heads;
+  const int split = (int)(b % (uint32_t)a.splits);
+  // late slots first: under a causal mask a chunk's last rows see most
+  const int64_t slot = n_slots - 1 - (int64_t)(b / (uint32_t)a.splits);
+
+  // Slots of sequence i begin at starts[i] / rows_per_tile + i: room for all of
+  // its tiles whatever its first row's place in a tile.
+  auto slot0 = [&](int64_t i) {
+    const int64_t st = a.row_starts[i];
+    return (st < 0 ? 0 : st > a.n_rows ? a.n_rows : st) / rows_per_tile + i;
+  };
+  int64_t seq = 0;
+  for (int64_t size = a.n; size > 1;) {  // the last sequence whose slots begin at or before this one
+    const int64_t step = (size + 63) / 64, i = seq + lane * step;
+    const bool before = i < seq + size && slot0(i) <= slot;
+    const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before));
+    if (n == 0) return;
+    const int64_t skip = (n - 1) * step;
+    seq += skip;
+    size = size - skip < step ? size - skip : step;
+  }
+  seq = ((int64_t)__builtin_amdgcn_readfirstlane((int)(seq >> 32)) << 32) |
+        (uint32_t)__builtin_amdgcn_readfirstlane((int)seq);
+  const SeqRows rows = seq_rows(a, seq);
+  const int64_t tile64 = slot - slot0(seq);
+  if (rows.count <= min_rows || tile64 < 0 || tile64 * rows_per_tile >= rows.count) return;
+  const int32_t r0 = (int32_t)tile64 * rows_per_tile;
+
+  // the lane's column
+  const int c128 = wave * 32 + col, rr = c128 / group;
+  const bool live = rr < rows_per_tile && r0 + rr < rows.count;
+  const int head = kvh * group + c128 - rr * group;
+  const int64_t row = rows.row0 + r0 + (live ? rr : 0);
+  RowView view = row_view(a, rows, seq, r0 + (live ? rr : 0));
+  if (!live) view.end = 0;
+  Bounds wb, gb;
+  {
+    auto reduce = [](int32_t x, bool most) {
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) {
+        const int32_t y = __shfl_xor(x, off, 64);
+        x = most ? max(x, y) : min(x, y);
+      }
+      return __builtin_amdgcn_readfirstlane(x);
+    };
+    const int32_t lo = INT32_MIN, hi = INT32_MAX;
+    // rows that see nothing bound nothing
+    const bool any = live && view.end > view.first;
+    wb.first_min = reduce(any ? view.first : hi, false);
+    wb.first_max = reduce(any ? view.first : lo, true);
+    wb.from_min = reduce(any ? view.from : hi, false);
+    wb.from_max = reduce(any ? view.from : lo, true);
+    wb.sink_min = reduce(any ? view.sink_end : hi, false);
+    wb.sink_max = reduce(any ? view.sink_end : lo, true);
+    wb.end_min = reduce(any ? view.end : live ? lo : hi, false);  // (but they keep tiles from being whole)
+    wb.end_max = reduce(any ? view.end : lo, true);
+    if (lane == 0) s_bounds[wave] = wb;
+    __syncthreads();
+    gb = s_bounds[0];
+#pragma unroll
+    for (int w = 1; w < kChunkWaves; ++w) {
+      const Bounds o = s_bounds[w];
+      gb.first_min = min(gb.first_min, o.first_min);
+      gb.from_min = min(gb.from_min, o.from_min);
+      gb.sink_max = max(gb.sink_max, o.sink_max);
+      gb.end_max = max(gb.end_max, o.end_max);
+    }
+  }
+  StepRange<kChunkTokens> range{0, 0, 0, 0, 0, 0};
+  if (gb.end_max > 0) {
+    const RowView all{0, gb.first_min, gb.sink_max, gb.from_min, gb.end_max};
+    range = step_range<kChunkTokens>(all);
+  }
+  const int per_part = (range.n + a.splits - 1) / a.splits;
+  const int n_parts = per_part > 0 ? (range.n + per_part - 1) / per_part : 1;
+  if (split >= n_parts) return;
+  const int s_begin = split * per_part, s_end = min(range.n, s_begin + per_part);
+
+  // Q columns (as scored_rows_kernel's)
+  h8 qh[NK], ql[FULL ? NK : 1];
+  float qscale;
+  {
+    float x[NK][8], amax = 0.f;
+    const int64_t at = (row * a.n_heads + head) * (int64_t)HD;
+#pragma unroll
+    for (int j = 0; j < NK; ++j) {
+      load_row8(a, at + 16 * j + 8 * half, live, x[j]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = __builtin_fmaxf(amax, __builtin_fabsf(x[j][i]));
+    }
+    amax = halves_reduce<true>(amax);
+    const int up = amax > 0.f && amax < INFINITY ? 10 - __builtin_amdgcn_frexp_expf(amax) : 0;
+#pragma unroll
+    for (int j = 0; j < NK; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        _Float16 hi, lo;
+        split2(__builtin_amdgcn_ldexpf(x[j][i], up), hi, lo);
+        qh[j][i] = hi;
+        if constexpr (FULL) ql[j][i] = lo;
+      }
+    qscale = __builtin_amdgcn_ldexpf(a.scale, -up);
+  }
+  const bool cap = a.softcap > 0.f;
+  const float in_scale = cap ? qscale / a.softcap : qscale * kLog2e;
+  const float cap_scale = a.softcap * kLog2e;
+  const float slope = a.slopes && live ? a.slopes[head] * kLog2e : 0.f;
+  const bool biased = a.slopes != nullptr;
+
+  f32x16 o[NC];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) o[i] = f32x16{};
+  float ref = -INFINITY, sum = 0.f;
+  int v_exp = -1000;  // q8_0: V enters the products times 2^-v_exp
+
+  // staging
+  const int32_t *tab = table_of(a.tables, a.table_stride, a.rows, a.table_rows, seq);
+  const int64_t head_off = (int64_t)kvh * HD;
+  const int tok = tid >> 2, part = tid & 3;
+  auto entry_of = [&](int s) {
+    const int32_t t = range.start(s) + tok;
+    int32_t e = s < s_end && t < range.end(s) ? tab[t >> 4] : 0;
+    if (e < 0 || e >= n_blocks) {
+      report_fault(a.status, kFaultTable, seq);
+      e = 0;
+    }
+    return e;
+  };
+  Share<T, NC> ks, vs;
+  int32_t next = 0;
+  if (s_begin < s_end) {
+    const int32_t e = entry_of(s_begin);
+    ks.load(a.k_layer, a.k_scale, kv_dim, e, tok & 15, part, head_off);
+    vs.load(a.v_layer, a.v_scale, kv_dim, e, tok & 15, part, head_off);
+    next = entry_of(s_begin + 1);
+  }
+
+  for (int s = s_begin; s < s_end; ++s) {
+    const int32_t t0 = range.start(s), t_end = range.end(s);
+    if constexpr (Q8) {
+      float dk = ks.scale(), dv = vs.scale();
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) {
+        dk = __builtin_fmaxf(dk, __shfl_xor(dk, off, 64));
+        dv = __builtin_fmaxf(dv, __shfl_xor(dv, off, 64));
+      }
+      if (lane == 0) {
+        s_scale[wave][0] = dk;
+        s_scale[wave][1] = dv;
+      }
+    }
+    lds_barrier();  // the last tile has been read
+    int k_exp = 0;
+    if constexpr (Q8) {
+      float dk = 0.f, dv = 0.f;
+#pragma unroll
+      for (int w = 0; w < kChunkWaves; ++w) {
+        dk = __builtin_fmaxf(dk, s_scale[w][0]);
+        dv = __builtin_fmaxf(dv, s_scale[w][1]);
+      }
+      // quants of up to 128 times the largest scale stay below 2^15
+      k_exp = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(__builtin_fminf(dk, 65504.f))) - 8;
+      if (dk == 0.f) k_exp = 0;
+      const int e = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(__builtin_fminf(dv, 65504.f))) - 8;
+      if (dv > 0.f && e > v_exp) {
+        if (v_exp > -1000) {
+          const float f = __builtin_amdgcn_ldexpf(1.f, v_exp - e);
+#pragma unroll
+          for (int i = 0; i < NC; ++i) o[i] *= f;
+        }
+        v_exp = e;
+      }
+    }
+    bool bad = false;
+    {
+      float dk = 0.f, dv = 0.f;
+      if constexpr (Q8) {
+        dk = __builtin_amdgcn_ldexpf(ks.scale(), -k_exp);
+        dv = __builtin_amdgcn_ldexpf(vs.scale(), -(v_exp > -1000 ? v_exp : 0));
+      }
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const int c = Share<T, NC>::chunk(part, j) * 16;
+        if constexpr (Q8) {
+          h8 hi, lo;
+          ks.get2(j, dk, hi, lo);
+          *reinterpret_cast<h8 *>(lds_k + tok * K_PITCH + c) = hi;
+          *reinterpret_cast<h8 *>(lds_k + K_BYTES + tok * K_PITCH + c) = lo;
+          vs.get2(j, dv, hi, lo);
+          if (not_finite(hi)) {
+            bad = true;
+            hi = h8{};
+            lo = h8{};
+          }
+          *reinterpret_cast<h8 *>(lds_v + tok * V_PITCH + c) = hi;
+          if constexpr (V_PLANES == 2) *reinterpret_cast<h8 *>(lds_v + V_BYTES + tok * V_PITCH + c) = lo;
+        } else {
+          *reinterpret_cast<h8 *>(lds_k + tok * K_PITCH + c) = ks.get(j);
+          h8 x = vs.get(j);
+          if constexpr (std::is_same_v<T, _Float16>)
+            if (not_finite(x)) {
+              bad = true;
+              x = finite_or_zero(x);
+            }
+          *reinterpret_cast<h8 *>(lds_v + tok * V_PITCH + c) = x;
+        }
+      }
+    }
+    if constexpr (!std::is_same_v<T, Q4>) {
+      const bool any_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+      if (lane == 0) s_bad[wave] = any_bad;
+    }
+    if (s + 1 < s_end) {
+      ks.load(a.k_layer, a.k_scale, kv_dim, next, tok & 15, part, head_off);
+      vs.load(a.v_layer, a.v_scale, kv_dim, next, tok & 15, part, head_off);
+      next = entry_of(s + 2);
+    }
+    lds_barrier();
+    bool tile_bad = false;
+    if constexpr (!std::is_same_v<T, Q4>) tile_bad = (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) != 0;
+
+#pragma unroll 1
+    for (int u = 0; u < kChunkTokens; u += 32) {
+      const int32_t tb = t0 + u;
+      if (tb >= t_end || wb.none(tb, 32)) continue;
+      f32x16 c = {};
+      const char *kp = lds_k + (u + col) * K_PITCH + 16 * half;
+#pragma unroll
+      for (int j = 0; j < NK; ++j) {
+        const h8 x = *reinterpret_cast<const h8 *>(kp + 32 * j);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[j], c, 0, 0, 0);
+        if constexpr (FULL) c = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[j], c, 0, 0, 0);
+        if constexpr (Q8) {
+          const h8 y = *reinterpret_cast<const h8 *>(kp + K_BYTES + 32 * j);
+          c = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[j], c, 0, 0, 0);
+        }
+      }
+      const float to_x = Q8 ? __builtin_amdgcn_ldexpf(in_scale, k_exp) : in_scale;
+      if (cap) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float x = c[i] * to_x;
+          if constexpr (FULL) c[i] = tanh_f32(x) * cap_scale;
+          else c[i] = tanh_f16(x) * cap_scale;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) c[i] *= to_x;
+      }
+      const int32_t tl = tb + 4 * half;  // the lane's positions: tl + 8 (i / 4) + i % 4
+      if (biased) {
+        const float d0 = (float)(view.pos - tl);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          c[i] = __builtin_fmaf(-slope, __builtin_fabsf(d0 - (float)(8 * (i / 4) + i % 4)), c[i]);
+      }
+      if (tb + 32 > t_end || !wb.all(tb, 32)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int32_t t = tl + 8 * (i / 4) + i % 4;
+          if (!(view.sees(t) && t < t_end)) c[i] = -INFINITY;
+        }
+      }
+      float top = c[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = __builtin_fmaxf(top, c[i]);
+      if (__builtin_amdgcn_ballot_w64(top > ref + kSlack)) {
+        const float nr = __builtin_fmaxf(ref, halves_reduce<true>(top));
+        const float f = nr == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - nr);
+        sum *= f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) o[i] *= f;
+        ref = nr;
+      }
+      const float base = (ref == -INFINITY ? 0.f : ref) - kLift;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        c[i] = __builtin_amdgcn_exp2f(c[i] - base);
+        sum += c[i];
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        h8 wh, wl;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          _Float16 hi, lo;
+          split2(c[8 * p + i], hi, lo);
+          wh[i] = hi;
+          wl[i] = lo;
+        }
+        const char *vp = lds_v + (u + 16 * p + 4 * half + ((lane & 15) >> 2)) * V_PITCH +
+                         (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const h8 x = read_tr2(vp + 64 * i, 8 * V_PITCH);
+          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wh, o[i], 0, 0, 0);
+          if constexpr (FULL) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wl, o[i], 0, 0, 0);
+          if constexpr (V_PLANES == 2) {
+            const h8 y = read_tr2(vp + V_BYTES + 64 * i, 8 * V_PITCH);
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, wh, o[i], 0, 0, 0);
+          }
+        }
+      }
+      if constexpr (!std::is_same_v<T, Q4>) {
+        if (tile_bad) {
+          // V elements that are infinite or NaN entered as zeros: the rows that
+          // see their positions get them here, the others do not
+          for (int j = 0; j < 32; ++j) {
+            const int32_t t = tb + j;
+            if (t >= t_end) break;
+            int32_t e = tab[t >> 4];
+            if (e < 0 || e >= n_blocks) e = 0;
+            float w = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)  // position j is element i of lane (column, j / 4 % 2)
+              if (i == (j >> 3) * 4 + (j & 3)) w = __shfl(c[i], col + 32 * ((j >> 2) & 1), 64);
+            if (!view.sees(t)) continue;
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+#pragma unroll
+              for (int k = 0; k < 16; ++k) {
+                const int64_t d = head_off + 32 * i + 8 * (k / 4) + 4 * half + k % 4;
+                const float x = cell_value<T>(a.v_layer, a.v_scale, (int64_t)e * 16 + (t & 15), kv_dim, d);
+                if (!(__builtin_fabsf(x) < INFINITY)) o[i][k] += w * x;
+              }
+          }
+        }
+      }
+    }
+  }
+
+  sum = halves_reduce<false>(sum);
+  if constexpr (Q8) {
+    const float f = __builtin_amdgcn_ldexpf(1.f, v_exp > -1000 ? v_exp : 0);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) o[i] *= f;
+  }
+  if (live) {
+    const int64_t rh = row * a.n_heads + head;
+    if (n_parts == 1) {
+      const float inv = sum != 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; k += 4)
+          store_row4(a, rh * HD + 32 * i + 2 * k + 4 * half,
+                     f32x4{o[i][k] * inv, o[i][k + 1] * inv, o[i][k + 2] * inv, o[i][k + 3] * inv});
+    } else {
+      const int64_t at = rh * a.splits + split;
+      float *dst = a.chunk_o + at * HD + 4 * half;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; k += 4)
+          *reinterpret_cast<f32x4 *>(dst + 32 * i + 2 * k) = f32x4{o[i][k], o[i][k + 1], o[i][k + 2], o[i][k + 3]};
+      if (half == 0) {
+        a.chunk_ml[2 * at] = ref;
+        a.chunk_ml[2 * at + 1] = sum;
+      }
+    }
+    if (a.chunk_n && split == 0 && half == 0 && kvh == 0 && c128 - rr * group == 0) a.chunk_n[row] = n_parts;
+  }
+}
+
+template <typename T, int HD>
+hipError_t launch_chunk_t(const PoolGeom &g, const ScoredArgs &a, int64_t min_rows, hipStream_t s) {
+  const int rows_per_tile = chunk_rows(a);
+  const int64_t n_slots = a.n_rows / rows_per_tile + a.n;
+  const int64_t wgs = n_slots * a.splits * a.n_kv_heads;
+  if (wgs * 64 * kChunkWaves >= (int64_t{1} << 32)) return hipErrorInvalidValue;
+  const auto kernel =
+      a.row_type == LTKV_ROWS_F32 ? scored_chunk_kernel<T, HD, true> : scored_chunk_kernel<T, HD, false>;
+  kernel<<<(unsigned)wgs, 64 * kChunkWaves, 0, s>>>(a, g.n_blocks, g.kv_dim, rows_per_tile, min_rows, n_slots);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_chunk_hd(const PoolGeom &g, const ScoredArgs &a, int64_t min_rows, hipStream_t s) {
+  return a.head_dim == 64 ? launch_chunk_t<T, 64>(g, a, min_rows, s) : launch_chunk_t<T, 128>(g, a, min_rows, s);
+}
+
+}  // namespace
+
+hipError_t launch_scored_chunks(const PoolGeom &g, const ScoredArgs &a, int64_t min_rows, hipStream_t s) {
+  if (g.elem == kElemQ4) return launch_chunk_hd<Q4>(g, a, min_rows, s);
+  if (g.elem == 1) return launch_chunk_hd<int8_t>(g, a, min_rows, s);
+  return launch_chunk_hd<_Float16>(g, a, min_rows, s);
+}
+
+}  // namespace ltkv

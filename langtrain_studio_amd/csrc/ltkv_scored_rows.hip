@@ -7,6 +7,7 @@ namespace ltkv {
 namespace {
 
 constexpr int kRowsWaves = 4;
+constexpr int kTopExp = 15;  // q8_0 weights times V scales stay below 2^kTopExp
 
 // K or V of 16 positions as a wave loads them: lane (t, quad) = (lane & 15,
 // lane >> 4) holds NC chunks of 8 elements of position t. Chunk j of a lane is
@@ -30,18 +31,6 @@ struct Cells<_Float16, NC, SPAN> {
   }
   __device__ __forceinline__ h8 get(int j) const { return __builtin_bit_cast(h8, x[j]); }
 };
-
-// Quants of q4_0, 8 a dword: a nibble becomes the low mantissa bits of an f16
-// in [1024, 1040) (0x6400 | u), 1032 is subtracted and the scale multiplied,
-// both exactly (the scale's 8 bits).
-__device__ __forceinline__ h8 q4x8_to_h8(uint32_t w, h2 d) {
-  const h2 bias = {(_Float16)1032.f, (_Float16)1032.f};
-  h2 p[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    p[i] = (__builtin_bit_cast(h2, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) - bias) * d;
-  return h8{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
-}
 
 template <int NC, bool SPAN>
 struct Cells<Q4, NC, SPAN> {
@@ -117,37 +106,6 @@ struct Cells<int8_t, NC, SPAN> {
   __device__ __forceinline__ h4 scale(int j) const { return __builtin_bit_cast(h4, s[j]); }
 };
 
-// hi + lo f16 parts of x: 22 bits together.
-__device__ __forceinline__ void split2(float x, _Float16 &hi, _Float16 &lo) {
-  hi = (_Float16)x;
-  lo = (_Float16)(x - (float)hi);
-}
-
-// Score references are raised only when a score exceeds them by kSlack (log2),
-// so most steps need no exchange between lanes and no rescaling; weights carry
-// 2^lift, so that the largest (2^(kSlack + lift)) lie near the top of f16 and the
-// lo parts of small ones stay out of its subnormals: kLift for values V that are
-// f16 numbers themselves. q8_0 weights are multiplied by V's scales first: the
-// lift follows the largest scale met, whatever its magnitude.
-constexpr float kSlack = 8.f;
-constexpr float kLift = 6.f;
-constexpr int kTopExp = 15;  // largest weights are below 2^kTopExp
-
-// tanh, to a few units of f32 at any size: odd polynomial below 0.35 (the next
-// term is below 2^-26 there), 1 - 2 / (exp(2 |x|) + 1) beyond.
-__device__ __forceinline__ float tanh_f32(float x) {
-  const float y = x * x;
-  float p = __builtin_fmaf(y, -0.008863235529902197f, 0.021869488536155203f);
-  p = __builtin_fmaf(y, p, -0.05396825396825397f);
-  p = __builtin_fmaf(y, p, 0.13333333333333333f);
-  p = __builtin_fmaf(y, p, -0.3333333333333333f);
-  const float small = __builtin_fmaf(x * y, p, x);
-  const float ax = __builtin_fabsf(x);
-  const float e = __builtin_amdgcn_exp2f(ax * (2.f * kLog2e));
-  const float large = __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
-  return ax < 0.35f ? small : __builtin_copysignf(large, x);
-}
-
 // A work-group takes one part of one row's visible positions for one kv head:
 // its four waves take 32-position steps in turn. Per step and wave, on 16x16x32
 // products: scores^T = K Q^T (16 positions x the group's query heads as
@@ -178,9 +136,13 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
   const int kvh = (int)(b % (uint32_t)a.n_kv_heads);
   b /= (uint32_t)a.n_kv_heads;
   const int part = (int)(b % (uint32_t)a.max_parts);
-  const int64_t seq = b / (uint32_t)a.max_parts;
+  const int64_t item = b / (uint32_t)a.max_parts;
+  // an item is a sequence, whose rows are taken one after the other, or a row
+  const int64_t seq = a.row_items ? seq_of_row(a, item) : item;
   const SeqRows rows = seq_rows(a, seq);
   if (rows.count > most_rows) return;
+  if (a.row_items && (item < rows.row0 || item >= rows.row0 + rows.count)) return;
+  const int r_begin = a.row_items ? (int)(item - rows.row0) : 0, r_end = a.row_items ? r_begin + 1 : rows.count;
   const int cols = min(16, group - head_tile * 16);
   const int head0 = kvh * group + head_tile * 16;
   const bool live = col < cols;
@@ -192,16 +154,19 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
   }
   char *const my = lds + wave * V_BYTES;
 
-  for (int r = 0; r < rows.count; ++r) {
+  for (int r = r_begin; r < r_end; ++r) {
     const RowView view = row_view(a, rows, seq, r);
-    const StepRange range = step_range(view);
+    const StepRange<32> range = step_range<32>(view);
     int per_part = scored_part_tokens((int64_t)range.n * 32, a.part_tokens) >> 5;
-    if ((int64_t)per_part * a.max_parts < range.n) per_part = (range.n + a.max_parts - 1) / a.max_parts;
+    // no memory for the parts of rows past the expected most: one part
+    const bool parted = a.row_items || r < a.max_rows;
+    if (!parted) per_part = range.n;
+    else if ((int64_t)per_part * a.max_parts < range.n) per_part = (range.n + a.max_parts - 1) / a.max_parts;
     const int n_parts = range.n > per_part ? (range.n + per_part - 1) / per_part : 1;
     if (part >= n_parts) continue;
     const int s_end = min(range.n, (part + 1) * per_part);
     const int s_first = part * per_part + wave;
-    const int64_t row = rows.row0 + r;
+    const int64_t row = rows.row0 + r, slot = a.row_items ? row : seq * a.max_rows + r;
 
     // block ids of the wave's next 32 steps, two a step, one a lane
     int entry = 0;
@@ -225,27 +190,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
         const int e = (SPAN ? quad * NC + j : 4 * j + quad) * 8;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
-        if (live && (SPAN || e < a.head_dim)) {
-          if (a.row_type == LTKV_ROWS_F32) {
-            const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(a.q) + at + e);
-            const f32x4 u = p[0], v = p[1];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              x[j][i] = u[i];
-              x[j][4 + i] = v[i];
-            }
-          } else {
-            const u32x4 u = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.q) + at + e);
-            const h8 hx = __builtin_bit_cast(h8, u);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              x[j][i] = a.row_type == LTKV_ROWS_F16
-                            ? (float)hx[i]
-                            : __builtin_bit_cast(float, i & 1 ? u[i >> 1] & 0xffff0000u : u[i >> 1] << 16);
-          }
-        }
+        load_row8(a, at + e, live && (SPAN || e < a.head_dim), x[j]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) amax = __builtin_fmaxf(amax, __builtin_fabsf(x[j][i]));
       }
@@ -428,8 +373,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
           }
         }
         const char *p = my + (4 * quad + (col >> 2)) * PITCH + (16 * i + 4 * (col & 3)) * 2;
-        const h4 x0 = __builtin_bit_cast(h4, lds_read_tr(p)), x1 = __builtin_bit_cast(h4, lds_read_tr(p + 16 * PITCH));
-        const h8 x = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+        const h8 x = read_tr2(p, 16 * PITCH);
         o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, wh, o[i], 0, 0, 0);
         o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, wl, o[i], 0, 0, 0);
       }
@@ -472,7 +416,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
       if (n_parts == 1) {
         row_store(a, rh * a.head_dim + e, l != 0.f ? x / l : 0.f);
       } else {
-        const int64_t at = rh * a.max_parts + part;
+        const int64_t at = (slot * a.n_heads + head0 + cc) * a.max_parts + part;
         a.part_o[at * a.head_dim + e] = x;
         if (e == 0) {
           a.part_ml[2 * at] = mx;
@@ -480,7 +424,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
         }
       }
     }
-    if (a.part_n && part == 0 && threadIdx.x == 0) a.part_n[row] = n_parts;
+    if (a.part_n && parted && part == 0 && threadIdx.x == 0) a.part_n[slot] = n_parts;
     __syncthreads();  // the fold's memory is the next row's V rows
   }
 }
@@ -488,7 +432,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
 template <typename T, int HDP, bool SPAN>
 hipError_t launch_rows_t(const PoolGeom &g, const ScoredArgs &a, int64_t most_rows, hipStream_t s) {
   const int group = a.n_heads / a.n_kv_heads, head_tiles = (group + 15) / 16;
-  const int64_t wgs = a.n * a.max_parts * a.n_kv_heads * head_tiles;
+  const int64_t wgs = (a.row_items ? a.n_rows : a.n) * a.max_parts * a.n_kv_heads * head_tiles;
   if (wgs * 64 * kRowsWaves >= (int64_t{1} << 32)) return hipErrorInvalidValue;
   const bool mods = a.softcap > 0.f || a.slopes;
   const auto kernel = mods ? scored_rows_kernel<T, HDP, SPAN, true> : scored_rows_kernel<T, HDP, SPAN, false>;

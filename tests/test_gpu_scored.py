@@ -1,13 +1,16 @@
 """Scored attention (capped scores, distance biases, windows, prefixes,
 documents) against the definition in 64 bits over the rows the pool holds.
 
-Tolerances: a score is an f32 sum of head_dim products of Q and K, so it is off
-by at most (head_dim + 16) half-steps of the sum of their magnitudes (16: Q as
-two f16 parts, the scale, the cap and the bias), a tanh by a few half-steps of
-the cap. A weight is then off by as much relatively, twice (numerator and sum),
-the f32 sums over L positions by L + 32 half-steps (32: exp2, the weights as
-two f16 parts, the folds), and f16 / bf16 rows by one f16 rounding per weight
-(2^-11, in numerator and sum) and the rounding of the result to its type.
+Tolerances: a score is an f32 sum of head_dim products of Q and K, with some 16
+roundings more (Q as two f16 parts, the scale, the cap and the bias). Each
+rounds a partial sum by at most half a step, 2^-24 of it; partial sums are at
+most the products' magnitudes together, and six times the root of their squares
+(six sigma of their signs). Roundings are independent: n of them add up to
+6 / sqrt(3) sqrt(n) of one's bound (six sigma of a uniform error) rather than to
+n. A weight is then off by as much relatively, twice (numerator and sum), the
+f32 sums over L positions by L + 32 roundings (32: exp2, the weights as two f16
+parts, the folds), and f16 / bf16 rows by one f16 rounding per weight (2^-11, in
+numerator and sum) and the rounding of the result to its type.
 Small weights are off absolutely: the lo part of a weight is an f16 number, a
 multiple of 2^-24, and a largest weight enters the products as at least 2^6 (8-bit
 pools: as at least 2^6 over the largest scale, times quants of up to 127), so a
@@ -26,6 +29,7 @@ pytestmark = pytest.mark.gpu
 
 BLOCK = 16
 H = 2.0 ** -24  # half a step of f32
+SIGMA = 6 / math.sqrt(3)
 
 
 def held_rows(kv, layer=0):
@@ -105,7 +109,8 @@ def expect(q, held, tables, lens, starts, heads, hd, scale=None, softcap=0.0, sl
                 with np.errstate(invalid="ignore", over="ignore"):
                     s = k[:, a:a + hd] @ qs * scale
                     mag = np.abs(k[:, a:a + hd]) @ np.abs(qs) * abs(scale)
-                    off = (hd + 16) * H * mag
+                    mag = np.minimum(mag, 6 * np.sqrt(k[:, a:a + hd] ** 2 @ qs ** 2) * abs(scale))
+                    off = SIGMA * math.sqrt(hd + 16) * H * mag
                     if softcap:
                         s = softcap * np.tanh(s / softcap)
                         off = off + 16 * H * softcap
@@ -119,7 +124,7 @@ def expect(q, held, tables, lens, starts, heads, hd, scale=None, softcap=0.0, sl
                     out[r, h * hd:(h + 1) * hd] = o
                     mass[r, h * hd:(h + 1) * hd] = m
                     small = 2.0 ** -30 * w.max() * t.size * np.abs(v[:, a:a + hd]).max()
-                    bound[r, h * hd:(h + 1) * hd] = (2 * off.max() + (t.size + 32) * H) * m + small
+                    bound[r, h * hd:(h + 1) * hd] = (2 * off.max() + SIGMA * math.sqrt(t.size + 32) * H) * m + small
     return out, bound, mass
 
 
