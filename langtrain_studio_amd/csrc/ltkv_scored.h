@@ -154,16 +154,31 @@ __device__ __forceinline__ float cell_value(const void *pool, const void *scales
   }
 }
 
-// Quants of q4_0, 8 a dword: a nibble becomes the low mantissa bits of an f16
-// in [1024, 1040) (0x6400 | u), 1032 is subtracted and the scale multiplied,
-// both exactly (the scale's 8 bits).
+// A load at a uniform base plus a 32-bit lane offset. The offset is made opaque
+// where it is used: widened outside of the loop it would be added as 64 bits in
+// vector registers for every load.
+template <typename V>
+__device__ __forceinline__ V load_at(const char *base, uint32_t off) {
+  asm volatile("" : "+v"(off));
+  return *reinterpret_cast<const V *>(base + off);
+}
+
+// Quants of q4_0, 8 a dword: a nibble u becomes the low mantissa bits of an f16
+// in [1024, 1040) (0x6400 | u) and 1032 is subtracted, or the next ones of an f16
+// in [1024, 1280) (1024 + 16 u) that is taken times 1/16 minus 72; then the scale
+// is multiplied. All of it is exact (the scale has 8 bits). The bias sits in a
+// vector register: an and-or takes only one scalar operand.
 __device__ __forceinline__ h8 q4x8_to_h8(uint32_t w, h2 d) {
-  const h2 bias = {(_Float16)1032.f, (_Float16)1032.f};
-  h2 p[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    p[i] = (__builtin_bit_cast(h2, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) - bias) * d;
-  return h8{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
+  uint32_t bias;
+  asm("v_mov_b32 %0, 0x64006400" : "=v"(bias));
+  const h2 off = {(_Float16)-1032.f, (_Float16)-1032.f}, sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f},
+           off16 = {(_Float16)-72.f, (_Float16)-72.f};
+  const uint32_t v = w >> 8;
+  const h2 p0 = (__builtin_bit_cast(h2, (w & 0x000f000fu) | bias) + off) * d;
+  const h2 p1 = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & 0x00f000f0u) | bias), sixteenth, off16) * d;
+  const h2 p2 = (__builtin_bit_cast(h2, (v & 0x000f000fu) | bias) + off) * d;
+  const h2 p3 = __builtin_elementwise_fma(__builtin_bit_cast(h2, (v & 0x00f000f0u) | bias), sixteenth, off16) * d;
+  return h8{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
 }
 
 // hi + lo f16 parts of x: 22 bits together.
@@ -255,22 +270,22 @@ hipError_t by_element(int elem, F &&f) {
 }
 
 
+constexpr int64_t kShortSpan = 8192;
+
 // Tokens per part of a row's visible positions (rounded up to 32-token steps;
 // a multiple of 64): a function of the row's own span, so that a decode
 // query's bits do not depend on its batch.
 __host__ __device__ inline int scored_part_tokens(int64_t span, int fixed) {
   if (fixed > 0) return fixed;
-  return span <= 2048 ? 256 : span <= 8192 ? 512 : 1024;
+  return span <= kShortSpan ? 256 : 512;
 }
 
 // Most parts of spans up to `span` tokens.
 inline int64_t scored_max_parts(int64_t span, int fixed) {
   auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   if (fixed > 0) return up(span, fixed);
-  int64_t parts = up(std::min<int64_t>(span, 2048), 256);
-  if (span > 2048) parts = std::max(parts, up(std::min<int64_t>(span, 8192), 512));
-  if (span > 8192) parts = std::max(parts, up(span, 1024));
-  return parts;
+  const int64_t parts = up(std::min<int64_t>(span, kShortSpan), 256);
+  return span > kShortSpan ? std::max(parts, up(span, 512)) : parts;
 }
 
 // The STEP-position steps over what a row (or rows together) sees: those of the

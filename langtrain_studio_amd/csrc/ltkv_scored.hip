@@ -149,14 +149,31 @@ __global__ void __launch_bounds__(kMergeThreads) scored_merge_kernel(ScoredArgs 
   const int64_t at = (slot * a.n_heads + h) * stride;
   ml += 2 * at;
   o += at * a.head_dim + e;
-  float mx = -INFINITY;
-  for (int p = 0; p < n_parts; ++p) mx = __builtin_fmaxf(mx, ml[2 * p]);
-  const float base = mx == -INFINITY ? 0.f : mx;
-  float l = 0.f, x = 0.f;
-  for (int p = 0; p < n_parts; ++p) {
-    const float f = __builtin_amdgcn_exp2f(ml[2 * p] - base);
-    l = __builtin_fmaf(ml[2 * p + 1], f, l);
-    x = __builtin_fmaf(o[(int64_t)p * a.head_dim], f, x);
+  // eight parts' loads at a time, folded one by one in order
+  float mx = -INFINITY, l = 0.f, x = 0.f;
+  for (int p0 = 0; p0 < n_parts; p0 += 8) {
+    float pm[8], pl[8], po[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int p = p0 + k < n_parts ? p0 + k : n_parts - 1;
+      const f32x2 v = *reinterpret_cast<const f32x2 *>(ml + 2 * p);
+      pm[k] = p0 + k < n_parts ? v.x : -INFINITY;
+      pl[k] = p0 + k < n_parts ? v.y : 0.f;
+      po[k] = p0 + k < n_parts ? o[(int64_t)p * a.head_dim] : 0.f;
+    }
+    float next = mx;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) next = __builtin_fmaxf(next, pm[k]);
+    const float base = next == -INFINITY ? 0.f : next, f = __builtin_amdgcn_exp2f(mx - base);
+    l *= f;
+    x *= f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float g = __builtin_amdgcn_exp2f(pm[k] - base);
+      l = __builtin_fmaf(pl[k], g, l);
+      x = __builtin_fmaf(po[k], g, x);
+    }
+    mx = next;
   }
   row_store(a, row * a.n_heads * a.head_dim + i, l != 0.f ? x / l : 0.f);
 }

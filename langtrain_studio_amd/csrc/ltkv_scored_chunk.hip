@@ -36,7 +36,7 @@ struct Share<_Float16, NC> {
 template <int NC>
 struct Share<Q4, NC> {
   uint32_t x[NC];
-  uint16_t s;
+  uint32_t s;  // (as 32 bits: a 16-bit value would be waited for to be moved)
   __device__ static __forceinline__ int chunk(int part, int j) { return part * NC + j; }
   __device__ __forceinline__ void load(const void *pool, const void *scales, int64_t kv_dim, int32_t blk, int slot,
                                        int part, int64_t head_off) {
@@ -57,7 +57,7 @@ struct Share<Q4, NC> {
     }
   }
   __device__ __forceinline__ h8 get(int j) const {
-    const _Float16 d = __builtin_bit_cast(_Float16, s);
+    const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t)s);
     return q4x8_to_h8(x[j], h2{d, d});
   }
 };
@@ -65,7 +65,7 @@ struct Share<Q4, NC> {
 template <int NC>
 struct Share<int8_t, NC> {
   u32x2 x[NC];
-  uint16_t s;
+  uint32_t s;
   __device__ static __forceinline__ int chunk(int part, int j) { return part * NC + j; }
   __device__ __forceinline__ void load(const void *pool, const void *scales, int64_t kv_dim, int32_t blk, int slot,
                                        int part, int64_t head_off) {
@@ -79,7 +79,7 @@ struct Share<int8_t, NC> {
       x[j + 1] = u32x2{w.z, w.w};
     }
   }
-  __device__ __forceinline__ float scale() const { return (float)__builtin_bit_cast(_Float16, s); }
+  __device__ __forceinline__ float scale() const { return (float)__builtin_bit_cast(_Float16, (uint16_t)s); }
   // chunk j times d (the scale times a power of two), as hi + lo parts
   __device__ __forceinline__ void get2(int j, float d, h8 &hi, h8 &lo) const {
     const h8 q = i8x8_to_h8(x[j]);

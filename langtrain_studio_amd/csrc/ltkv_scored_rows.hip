@@ -7,25 +7,40 @@ namespace ltkv {
 namespace {
 
 constexpr int kRowsWaves = 4;
+constexpr int kAllButVmem = 0x78f;  // sched_barrier: what may move across (not accesses to global memory)
 constexpr int kTopExp = 15;  // q8_0 weights times V scales stay below 2^kTopExp
 
-// K or V of 16 positions as a wave loads them: lane (t, quad) = (lane & 15,
-// lane >> 4) holds NC chunks of 8 elements of position t. Chunk j of a lane is
-// head elements chunk_at(quad, j) ... + 7: a contiguous quarter of the head
-// where that makes loads of 16 bytes (SPAN), else 32 j + 8 quad.
+// K or V of 16 positions (a block) as a wave loads them: lane (t, quad) =
+// (lane & 15, lane >> 4) holds NC chunks of 8 elements of position t. Chunk j of a
+// lane is head elements 8 chunk_of(quad, j) ... + 7: a contiguous quarter of the
+// head where that makes loads of 16 bytes (SPAN), else 32 j + 8 quad. A block's
+// address is uniform over the wave, a lane's place in a block the same for every
+// block (load_at).
+template <int NC, bool SPAN>
+__device__ __forceinline__ int chunk_of(int quad, int j) {
+  return SPAN ? quad * NC + j : 4 * j + quad;
+}
+
 template <typename T, int NC, bool SPAN>
 struct Cells;
 
 template <int NC, bool SPAN>
 struct Cells<_Float16, NC, SPAN> {
   u32x4 x[NC];
-  __device__ __forceinline__ void load(const ScoredArgs &a, const void *pool, const void *, int64_t kv_dim, int32_t blk,
-                                       int t, int quad, int64_t head_off) {
-    const _Float16 *row = static_cast<const _Float16 *>(pool) + ((int64_t)blk * 16 + t) * kv_dim + head_off;
+  struct Place {
+    uint32_t at;
+    int chunks;  // chunks of the lane inside the head
+    __device__ __forceinline__ Place(const ScoredArgs &a, int64_t kv_dim, int64_t head_off, int t, int quad) {
+      at = (uint32_t)((t * kv_dim + head_off + chunk_of<NC, SPAN>(quad, 0) * 8) * 2);
+      chunks = SPAN ? NC : (a.head_dim / 8 - quad + 3) / 4;
+    }
+  };
+  static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 32; }
+  __device__ __forceinline__ void load(const char *pool, const char *, int64_t at, const Place &p) {
+    const char *base = pool + at;
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      const int c = SPAN ? quad * NC + j : 4 * j + quad;
-      if (SPAN || c * 8 < a.head_dim) x[j] = *reinterpret_cast<const u32x4 *>(row + c * 8);
+      if (SPAN || j < p.chunks) x[j] = load_at<u32x4>(base, p.at + j * (SPAN ? 16 : 64));
       else x[j] = u32x4{0, 0, 0, 0};
     }
   }
@@ -36,27 +51,36 @@ template <int NC, bool SPAN>
 struct Cells<Q4, NC, SPAN> {
   static constexpr int NS = SPAN ? (NC + 3) / 4 : NC;  // scales a lane needs
   uint32_t x[NC];
-  uint16_t s[NS];
-  __device__ __forceinline__ void load(const ScoredArgs &a, const void *pool, const void *scales, int64_t kv_dim,
-                                       int32_t blk, int t, int quad, int64_t head_off) {
-    const int64_t tile0 = (int64_t)blk * (kv_dim >> 5);
-    if constexpr (SPAN) {
-      // the quarter lies in one group, or is whole groups (16 bytes each)
-      const int e = (int)head_off + quad * NC * 8;
+  uint32_t s[NS];  // (as 32 bits: a 16-bit value would be waited for to be moved)
+  struct Place {
+    uint32_t at[SPAN ? 1 : NC];  // of quants; scales lie at an eighth of the group's place
+    uint32_t sc[SPAN ? 1 : NC];
+    int chunks;
+    __device__ __forceinline__ Place(const ScoredArgs &a, int64_t, int64_t head_off, int t, int quad) {
+      chunks = SPAN ? NC : (a.head_dim / 8 - quad + 3) / 4;
+#pragma unroll
+      for (int j = 0; j < (SPAN ? 1 : NC); ++j) {
+        const uint32_t e = (uint32_t)head_off + chunk_of<NC, SPAN>(quad, j) * 8, cell = (e >> 5) * 16 + t;
+        at[j] = cell * 16 + ((e & 31) >> 3) * 4;
+        sc[j] = cell * 2;
+      }
+    }
+  };
+  static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 8; }
+  __device__ __forceinline__ void load(const char *pool, const char *scales, int64_t at, const Place &p) {
+    const char *base = pool + at, *sbase = scales + (at >> 3);
+    if constexpr (SPAN) {  // the quarter lies in one group, or is whole groups (16 bytes each)
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        const int64_t at = (tile0 + (e >> 5) + i) * 16 + t;
-        s[i] = static_cast<const uint16_t *>(scales)[at];
-        const uint32_t *p = static_cast<const uint32_t *>(pool) + at * 4 + ((e & 31) >> 3);
-        constexpr int W = NC < 4 ? NC : 4;
-        if constexpr (W == 4) {
-          const u32x4 w = *reinterpret_cast<const u32x4 *>(p);
+        s[i] = load_at<uint16_t>(sbase, p.sc[0] + 32 * i);
+        if constexpr (NC >= 4) {
+          const u32x4 w = load_at<u32x4>(base, p.at[0] + 256 * i);
           x[4 * i] = w.x;
           x[4 * i + 1] = w.y;
           x[4 * i + 2] = w.z;
           x[4 * i + 3] = w.w;
         } else {
-          const u32x2 w = *reinterpret_cast<const u32x2 *>(p);
+          const u32x2 w = load_at<u32x2>(base, p.at[0]);
           x[0] = w.x;
           x[1] = w.y;
         }
@@ -64,20 +88,17 @@ struct Cells<Q4, NC, SPAN> {
     } else {
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
-        const int c = 4 * j + quad;
         x[j] = 0;
         s[j] = 0;
-        if (c * 8 < a.head_dim) {
-          const int e = (int)head_off + c * 8;
-          const int64_t at = (tile0 + (e >> 5)) * 16 + t;
-          x[j] = static_cast<const uint32_t *>(pool)[at * 4 + ((e & 31) >> 3)];
-          s[j] = static_cast<const uint16_t *>(scales)[at];
+        if (j < p.chunks) {
+          x[j] = load_at<uint32_t>(base, p.at[j]);
+          s[j] = load_at<uint16_t>(sbase, p.sc[j]);
         }
       }
     }
   }
   __device__ __forceinline__ h8 get(int j) const {
-    const _Float16 d = __builtin_bit_cast(_Float16, s[SPAN ? j / 4 : j]);
+    const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t)s[SPAN ? j / 4 : j]);
     return q4x8_to_h8(x[j], h2{d, d});
   }
 };
@@ -88,97 +109,211 @@ struct Cells<Q4, NC, SPAN> {
 // positions 4 quad ... + 3.
 template <int NC, bool SPAN>
 struct Cells<int8_t, NC, SPAN> {
+  static_assert(!SPAN, "a product must stay inside a group");
   u32x2 x[NC];
   u32x2 s[NC];
-  __device__ __forceinline__ void load(const ScoredArgs &, const void *pool, const void *scales, int64_t kv_dim,
-                                       int32_t blk, int t, int quad, int64_t head_off) {
-    static_assert(!SPAN, "a product must stay inside a group");
-    const uint8_t *row = static_cast<const uint8_t *>(pool) + ((int64_t)blk * 16 + t) * kv_dim + head_off;
-    const uint16_t *sc =
-        static_cast<const uint16_t *>(scales) + ((int64_t)blk * (kv_dim >> 5) + (head_off >> 5)) * 16 + quad * 4;
+  struct Place {
+    uint32_t at, sc;
+    __device__ __forceinline__ Place(const ScoredArgs &, int64_t kv_dim, int64_t head_off, int t, int quad) {
+      at = (uint32_t)(t * kv_dim + head_off + 8 * quad);
+      sc = (uint32_t)((head_off >> 5) * 32 + quad * 8);
+    }
+  };
+  static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 16; }
+  __device__ __forceinline__ void load(const char *pool, const char *scales, int64_t at, const Place &p) {
+    const char *base = pool + at, *sbase = scales + (at >> 4);
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      x[j] = *reinterpret_cast<const u32x2 *>(row + 32 * j + 8 * quad);
-      s[j] = *reinterpret_cast<const u32x2 *>(sc + 16 * j);
+      x[j] = load_at<u32x2>(base, p.at + 32 * j);
+      s[j] = load_at<u32x2>(sbase, p.sc + 32 * j);
     }
   }
   __device__ __forceinline__ h8 get(int j) const { return i8x8_to_h8(x[j]); }
   __device__ __forceinline__ h4 scale(int j) const { return __builtin_bit_cast(h4, s[j]); }
 };
 
-// A work-group takes one part of one row's visible positions for one kv head:
-// its four waves take 32-position steps in turn. Per step and wave, on 16x16x32
-// products: scores^T = K Q^T (16 positions x the group's query heads as
+// Steps of a part of a row that takes n steps.
+__device__ __forceinline__ int steps_per_part(const ScoredArgs &a, int n) {
+  const int per_part = scored_part_tokens((int64_t)n * 32, a.part_tokens) >> 5;
+  // (never more parts than there is memory for)
+  return (int64_t)per_part * a.max_parts < n ? (n + a.max_parts - 1) / a.max_parts : per_part;
+}
+
+// Parts of a sequence of one row.
+template <bool MODS>
+__device__ __forceinline__ int parts_of(const ScoredArgs &a, int64_t seq) {
+  const int64_t len = a.lens[seq];
+  const int32_t cut = (int32_t)(len < 0 ? 0 : len > a.max_len ? a.max_len : len);
+  int n = (cut + 31) / 32;
+  if constexpr (MODS) n = step_range<32>(row_view(a, SeqRows{seq, 1, cut}, seq, 0)).n;
+  const int per_part = steps_per_part(a, n);
+  return n > per_part ? (n + per_part - 1) / per_part : 1;
+}
+
+// A wave takes a run of parts of one row's visible positions for one kv head
+// (four waves of a work-group: neighbouring kv heads, whose cells lie together).
+// It streams through 32-position steps, the next one in flight, and writes each
+// part's numerators, reference and sum (one part: the output). Per step, on
+// 16x16x32 products: scores^T = K Q^T (16 positions x the group's query heads as
 // columns, twice), weights from the scores in place, numerators^T += V^T W: the
 // score tiles' lane layout (4 quad + r, column) is the operand layout of the
 // second product when its 32 positions are taken as (tile 0: 4 quad ... + 3,
 // tile 1: 4 quad ... + 3), so weights move between no lanes. V is transposed on
 // its way through LDS (ds_read_b64_tr_b16). Q and the weights enter as f16
 // hi + lo pairs: f32 accuracy for twice the matrix-core work, which is idle
-// here otherwise.
-template <typename T, int HDP, bool SPAN, bool MODS>
-__global__ void __launch_bounds__(64 * kRowsWaves)
-scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tiles, int64_t most_rows) {
+// here otherwise. MODS false: plain decode attention, one row per sequence over
+// its whole context.
+// OCC: waves a SIMD that the registers are cut to.
+template <typename T, int HDP, bool SPAN, bool MODS, int OCC>
+__global__ void __launch_bounds__(64 * kRowsWaves, OCC)
+scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tiles, int64_t waves, int64_t share,
+                   int64_t most_rows) {
   constexpr int NC = HDP / 32;     // chunks of 8 elements a lane, products per score tile
   constexpr int ND = HDP / 16;     // 16-element tiles of the numerators
   constexpr int PITCH = HDP * 2 + 32;  // bytes of a V row in LDS: rows of a read start 8 banks apart
   constexpr bool Q8 = std::is_same_v<T, int8_t>;
-  constexpr int RED = HDP + 4;  // floats of a (wave, column) in the final fold: numerators, reference, sum
-  constexpr int V_BYTES = 32 * PITCH, RED_BYTES = 16 * RED * 4;
-  __shared__ __align__(16) char lds[kRowsWaves * (V_BYTES > RED_BYTES ? V_BYTES : RED_BYTES)];
+  __shared__ __align__(16) char lds[kRowsWaves * 32 * PITCH];
 
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
   const int group = a.n_heads / a.n_kv_heads;
-  uint32_t b = blockIdx.x;
+  uint32_t b = blockIdx.x * kRowsWaves + (uint32_t)wave;
+  if ((int64_t)b >= waves) return;
   const int head_tile = (int)(b % (uint32_t)head_tiles);
   b /= (uint32_t)head_tiles;
   const int kvh = (int)(b % (uint32_t)a.n_kv_heads);
   b /= (uint32_t)a.n_kv_heads;
-  const int part = (int)(b % (uint32_t)a.max_parts);
-  const int64_t item = b / (uint32_t)a.max_parts;
-  // an item is a sequence, whose rows are taken one after the other, or a row
-  const int64_t seq = a.row_items ? seq_of_row(a, item) : item;
-  const SeqRows rows = seq_rows(a, seq);
-  if (rows.count > most_rows) return;
-  if (a.row_items && (item < rows.row0 || item >= rows.row0 + rows.count)) return;
-  const int r_begin = a.row_items ? (int)(item - rows.row0) : 0, r_end = a.row_items ? r_begin + 1 : rows.count;
+  // Few parts: a wave for each that a sequence (or row) could have, the last
+  // ones slowest, so that those past the end of shorter contexts come last. Many
+  // (share > 0): every sequence has one row, and wave b of `share` takes the
+  // b-th of as many equal stretches of all parts in sequence order.
+  const uint32_t items = (uint32_t)(MODS && a.row_items ? a.n_rows : a.n);
+  int64_t item = b % items;
+  int p_first = (int)(b / items), p_count = 1;
+  if (share > 0) {
+    auto scan = [&](int64_t i0, int &own) {  // inclusive sums of 64 sequences' parts, from i0 on
+      own = i0 + lane < a.n ? parts_of<MODS>(a, i0 + lane) : 0;
+      int x = own;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int y = __shfl_up(x, off, 64);
+        if (lane >= off) x += y;
+      }
+      return x;
+    };
+    int own, x = scan(0, own);
+    int64_t total = __builtin_amdgcn_readlane(x, 63);
+    for (int64_t i0 = 64; i0 < a.n; i0 += 64) {
+      int rest;
+      total += __builtin_amdgcn_readlane(scan(i0, rest), 63);
+    }
+    const int64_t p0 = total * b / share, p1 = total * (b + 1) / share;
+    if (p0 == p1) return;
+    // the sequence of part p0
+    int64_t before = 0;
+    for (item = 0; item < a.n; item += 64) {
+      if (item > 0) x = scan(item, own);
+      const int sum = __builtin_amdgcn_readlane(x, 63);
+      if (before + sum > p0) {
+        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + x > p0));
+        p_first = (int)(p0 - before) - (__builtin_amdgcn_readlane(x, at) - __builtin_amdgcn_readlane(own, at));
+        item += at;
+        break;
+      }
+      before += sum;
+    }
+    p_count = (int)(p1 - p0);
+  }
   const int cols = min(16, group - head_tile * 16);
   const int head0 = kvh * group + head_tile * 16;
   const bool live = col < cols;
   const int64_t head_off = (int64_t)kvh * a.head_dim;
-  const int32_t *tab = table_of(a.tables, a.table_stride, a.rows, a.table_rows, seq);
-  if (a.rows && part == 0 && wave == 0 && rows.len > 0) {
-    const int32_t r = scalar_read(a.rows, seq);
-    if (r < 0 || r >= a.table_rows) report_fault(a.status, kFaultTable, seq);
-  }
-  char *const my = lds + wave * V_BYTES;
+  char *const my = lds + wave * (32 * PITCH);
+  const typename Cells<T, NC, SPAN>::Place place(a, kv_dim, head_off, col, quad);
 
-  for (int r = r_begin; r < r_end; ++r) {
-    const RowView view = row_view(a, rows, seq, r);
-    const StepRange<32> range = step_range<32>(view);
-    int per_part = scored_part_tokens((int64_t)range.n * 32, a.part_tokens) >> 5;
+  // an item is a sequence, whose rows are taken one after the other, or a row
+  // (MODS false: every sequence has one row)
+  for (int r_next = -1; p_count > 0;) {
+    const int64_t seq = MODS && a.row_items ? seq_of_row(a, item) : item;
+    SeqRows rows = seq_rows(a, seq);
+    if constexpr (!MODS) {
+      rows.row0 = seq;
+      rows.count = 1;
+    }
+    if (MODS && a.row_items) {
+      if (item < rows.row0 || item >= rows.row0 + rows.count) return;
+      r_next = (int)(item - rows.row0);
+    } else {
+      ++r_next;
+    }
+    if (rows.count > most_rows || r_next >= rows.count) return;
+    const int r = r_next;
+    const int32_t *tab = table_of(a.tables, a.table_stride, a.rows, a.table_rows, seq);
+    if (a.rows && p_first == 0 && rows.len > 0) {
+      const int32_t t = scalar_read(a.rows, seq);
+      if (t < 0 || t >= a.table_rows) report_fault(a.status, kFaultTable, seq);
+    }
+    const RowView view = MODS ? row_view(a, rows, seq, r) : RowView{rows.len - 1, 0, 0, 0, rows.len};
+    const StepRange<32> range =
+        MODS ? step_range<32>(view) : StepRange<32>{0, 0, 0, rows.len, 0, (rows.len + 31) / 32};
+    int per_part = steps_per_part(a, range.n);
     // no memory for the parts of rows past the expected most: one part
-    const bool parted = a.row_items || r < a.max_rows;
-    if (!parted) per_part = range.n;
-    else if ((int64_t)per_part * a.max_parts < range.n) per_part = (range.n + a.max_parts - 1) / a.max_parts;
+    const bool parted = !MODS || a.row_items || r < a.max_rows;
+    if (!parted) per_part = max(range.n, 1);
     const int n_parts = range.n > per_part ? (range.n + per_part - 1) / per_part : 1;
-    if (part >= n_parts) continue;
-    const int s_end = min(range.n, (part + 1) * per_part);
-    const int s_first = part * per_part + wave;
-    const int64_t row = rows.row0 + r, slot = a.row_items ? row : seq * a.max_rows + r;
+    const int64_t row = rows.row0 + r, slot = !MODS || a.row_items ? row : seq * a.max_rows + r;
+    if (a.part_n && parted && p_first == 0 && kvh == 0 && head_tile == 0 && lane == 0) a.part_n[slot] = n_parts;
+    int part = p_first;
+    // this item's stretch, and what follows it
+    const int here = min(p_count, n_parts - p_first);
+    if (share > 0) {
+      p_count -= here;
+      p_first = 0;
+      ++item;
+      r_next = -1;
+    } else if (MODS && a.row_items) {
+      p_count = 0;
+    }
+    if (here <= 0) continue;
+    const int s_first = part * per_part, s_end = min(range.n, (part + here) * per_part);
 
-    // block ids of the wave's next 32 steps, two a step, one a lane
-    int entry = 0;
+    // block ids of the next 32 steps, two a step, one a lane
+    int entry = 0, entry_step = s_first;
     auto fill = [&](int s0) {
-      const int s = s0 + kRowsWaves * (lane >> 1);
+      const int s = s0 + (lane >> 1);
       const int32_t t = range.start(s) + 16 * (lane & 1);
       const bool valid = s < s_end && t < range.end(s);
       entry = valid ? tab[t >> 4] : 0;
+      entry_step = s0;
       const bool bad = entry < 0 || entry >= n_blocks;
       if (bad) entry = 0;
       if (__builtin_amdgcn_ballot_w64(bad)) report_fault(a.status, kFaultTable, seq);
     };
+    Cells<T, NC, SPAN> k[2], v[2];
+    int64_t at[2];  // byte offsets of the next step's blocks
+    const int64_t block_bytes = Cells<T, NC, SPAN>::block_bytes(kv_dim);
+    auto find = [&](int s) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        at[u] = (int64_t)(uint32_t)__builtin_amdgcn_readlane(entry, 2 * (s - entry_step) + u) * block_bytes;
+    };
+    auto load = [&](Cells<T, NC, SPAN> (&c)[2], const void *pool, const void *scales) {
+      // not before the last use of what it replaces (the loaded registers would be
+      // copied, and so waited for)
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        c[u].load(static_cast<const char *>(pool), static_cast<const char *>(scales), at[u], place);
+      // V, K, V, K ... in this order everywhere: a wait then leaves the later ones
+      // in flight
+      __builtin_amdgcn_sched_barrier(kAllButVmem);
+    };
+    if (s_first < s_end) {
+      fill(s_first);
+      find(s_first);
+      load(v, a.v_layer, a.v_scale);
+      load(k, a.k_layer, a.k_scale);
+    }
 
     // Q columns, scaled by a power of two so that the head's largest element
     // lies in [2^9, 2^10): any magnitude enters f16 with 22 bits
@@ -189,7 +324,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
       const int64_t at = (row * a.n_heads + head0 + col) * (int64_t)a.head_dim;
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
-        const int e = (SPAN ? quad * NC + j : 4 * j + quad) * 8;
+        const int e = chunk_of<NC, SPAN>(quad, j) * 8;
         load_row8(a, at + e, live && (SPAN || e < a.head_dim), x[j]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) amax = __builtin_fmaxf(amax, __builtin_fabsf(x[j][i]));
@@ -213,69 +348,118 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
     const float slope = MODS && a.slopes && live ? a.slopes[head0 + col] * kLog2e : 0.f;
 
     f32x4 o[ND];
+    float ref, sum, lift, scale_top;
+    auto reset = [&]() {
 #pragma unroll
-    for (int i = 0; i < ND; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float ref = -INFINITY, sum = 0.f;
-    float lift = Q8 ? 0.f : kLift, scale_top = 0.f;  // q8_0: no scale has exceeded scale_top
-
-    Cells<T, NC, SPAN> k[2], v[2];
-    auto load = [&](Cells<T, NC, SPAN> (&c)[2], const void *pool, const void *scales, int i) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        c[u].load(a, pool, scales, kv_dim, __builtin_amdgcn_readlane(entry, 2 * i + u), col, quad, head_off);
+      for (int i = 0; i < ND; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      ref = -INFINITY;
+      sum = 0.f;
+      lift = Q8 ? 0.f : kLift;
+      scale_top = 0.f;  // q8_0: no scale has exceeded it
     };
-    int held = 0;  // step of `entry`'s window
-    if (s_first < s_end) {
-      fill(s_first);
-      load(k, a.k_layer, a.k_scale, 0);
-      load(v, a.v_layer, a.v_scale, 0);
-    }
-    for (int s = s_first; s < s_end; s += kRowsWaves) {
-      const int32_t t0 = range.start(s), t_end = range.end(s);
-      const bool more = s + kRowsWaves < s_end;
-      ++held;
-      if (more && held == 32) {
-        fill(s + kRowsWaves);
-        held = 0;
+    auto flush = [&]() {
+      const float total = rows_reduce<false>(sum);
+      if (!live) return;
+      const int64_t rh = row * a.n_heads + head0 + col;
+      if (n_parts == 1) {
+        const float inv = total != 0.f ? 1.f / total : 0.f;
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+          if (SPAN || 16 * i + 4 * quad < a.head_dim)
+            store_row4(a, rh * a.head_dim + 16 * i + 4 * quad, o[i] * inv);
+        return;
       }
-      // scores
-      f32x4 c[2];
+      const int64_t at = (slot * a.n_heads + head0 + col) * a.max_parts + part;
+      float *dst = a.part_o + at * a.head_dim + 4 * quad;
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+        if (SPAN || 16 * i + 4 * quad < a.head_dim) *reinterpret_cast<f32x4 *>(dst + 16 * i) = o[i];
+      if (quad == 0) {
+        a.part_ml[2 * at] = ref - lift;
+        a.part_ml[2 * at + 1] = total;
+      }
+    };
+
+    auto step = [&](int s) {
+      const int32_t t0 = range.start(s), t_end = range.end(s);
+      // always loaded, so that the loads in flight are counted exactly: past the
+      // end the last step again
+      const int s_next = min(s + 1, s_end - 1);
+      const bool whole = t0 + 32 <= t_end && t0 >= view.first && (t0 >= view.from || t0 + 32 <= view.sink_end);
+      if (s_next - entry_step == 32) fill(s_next);
+      find(s_next);
+      // V into LDS (positions that the row does not see as zeros); the scores are
+      // computed while it settles
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        c[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int32_t t = t0 + 16 * u + col;
+        const bool seen = whole || (view.sees(t) && t < t_end);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          h8 y = v[u].get(j);
+          if constexpr (std::is_same_v<T, _Float16>)
+            if (!seen) y = h8{};
+          *reinterpret_cast<h8 *>(my + (16 * u + col) * PITCH + chunk_of<NC, SPAN>(quad, j) * 16) = y;
+        }
+      }
+      h4 dv[2][Q8 ? NC : 1];
+      if constexpr (Q8) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < NC; ++j) {
+            dv[u][j] = v[u].scale(j);
+            if (!whole)  // a scale of an unseen position may be infinite
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int32_t t = t0 + 16 * u + 4 * quad + i;
+                if (!(view.sees(t) && t < t_end)) dv[u][j][i] = (_Float16)0.f;
+              }
+          }
+      }
+      load(v, a.v_layer, a.v_scale);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+
+      // scores
+      f32x4 c[2], cl[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        c[u] = cl[u] = f32x4{0.f, 0.f, 0.f, 0.f};
         if constexpr (Q8) {
 #pragma unroll
           for (int j = 0; j < NC; ++j) {
-            const h8 x = k[u].get(j);
-            f32x4 g = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qh[j], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-            g = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ql[j], g, 0, 0, 0);
+            const h8 y = k[u].get(j);
+            f32x4 g = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, qh[j], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            g = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ql[j], g, 0, 0, 0);
             const h4 d = k[u].scale(j);
 #pragma unroll
             for (int i = 0; i < 4; ++i) c[u][i] = __builtin_fmaf((float)d[i], g[i], c[u][i]);
           }
-        } else {
+        } else {  // (two chains of dependent products)
 #pragma unroll
           for (int j = 0; j < NC; ++j) {
-            const h8 x = k[u].get(j);
-            c[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qh[j], c[u], 0, 0, 0);
-            c[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ql[j], c[u], 0, 0, 0);
+            const h8 y = k[u].get(j);
+            c[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, qh[j], c[u], 0, 0, 0);
+            cl[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ql[j], cl[u], 0, 0, 0);
           }
         }
       }
-      if (more) load(k, a.k_layer, a.k_scale, held);
-
-      const bool whole = t0 + 32 <= t_end && t0 >= view.first && (t0 >= view.from || t0 + 32 <= view.sink_end);
+      load(k, a.k_layer, a.k_scale);
+      // V^T operands: on their way during the softmax
+      h8 vt[ND];
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+        vt[i] = read_tr2(my + (4 * quad + (col >> 2)) * PITCH + (16 * i + 4 * (col & 3)) * 2, 16 * PITCH);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int32_t t = t0 + 16 * u + 4 * quad + i;
-          float x = c[u][i] * in_scale;
+          float y = (Q8 ? c[u][i] : c[u][i] + cl[u][i]) * in_scale;
           if constexpr (MODS) {
-            if (cap) x = tanh_f32(x) * cap_scale;
-            x = __builtin_fmaf(-slope, (float)abs(view.pos - t), x);
+            if (cap) y = tanh_f32(y) * cap_scale;
+            y = __builtin_fmaf(-slope, (float)abs(view.pos - (t0 + 16 * u + 4 * quad + i)), y);
           }
-          c[u][i] = x;
+          c[u][i] = y;
         }
       if (!whole)
 #pragma unroll
@@ -296,22 +480,12 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
         for (int i = 0; i < ND; ++i) o[i] *= f;
         ref = next;
       }
-      h4 dv[2][Q8 ? NC : 1];
       if constexpr (Q8) {
         h4 most = {};
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int j = 0; j < NC; ++j) {
-            dv[u][j] = v[u].scale(j);
-            if (!whole)  // a scale of an unseen position may be infinite
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int32_t t = t0 + 16 * u + 4 * quad + i;
-                if (!(view.sees(t) && t < t_end)) dv[u][j][i] = (_Float16)0.f;
-              }
-            most = __builtin_elementwise_max(most, dv[u][j]);
-          }
+          for (int j = 0; j < NC; ++j) most = __builtin_elementwise_max(most, dv[u][j]);
         const float top_d = __builtin_fmaxf(__builtin_fmaxf((float)most[0], (float)most[1]),
                                             __builtin_fmaxf((float)most[2], (float)most[3]));
         if (__builtin_amdgcn_ballot_w64(top_d > scale_top)) {
@@ -332,23 +506,6 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
         w[i] = __builtin_amdgcn_exp2f(c[i >> 2][i & 3] - base);
         sum += w[i];
       }
-
-      // V through LDS: positions that the row does not see as zeros
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int32_t t = t0 + 16 * u + col;
-        const bool seen = whole || (view.sees(t) && t < t_end);
-#pragma unroll
-        for (int j = 0; j < NC; ++j) {
-          h8 x = v[u].get(j);
-          if constexpr (std::is_same_v<T, _Float16>)
-            if (!seen) x = h8{};
-          const int e = (SPAN ? quad * NC + j : 4 * j + quad) * 8;
-          *reinterpret_cast<h8 *>(my + (16 * u + col) * PITCH + e * 2) = x;
-        }
-      }
-      if (more) load(v, a.v_layer, a.v_scale, held);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       h8 wh, wl;
       if constexpr (!Q8) {
 #pragma unroll
@@ -358,10 +515,13 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
           wh[i] = hi;
           wl[i] = lo;
         }
-      }
 #pragma unroll
-      for (int i = 0; i < ND; ++i) {
-        if constexpr (Q8) {
+        for (int i = 0; i < ND; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], wh, o[i], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], wl, o[i], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
           if (i % 2 == 0) {  // a group's two tiles share its weights
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -371,72 +531,43 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
               wl[e] = lo;
             }
           }
+          o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], wh, o[i], 0, 0, 0);
+          o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], wl, o[i], 0, 0, 0);
         }
-        const char *p = my + (4 * quad + (col >> 2)) * PITCH + (16 * i + 4 * (col & 3)) * 2;
-        const h8 x = read_tr2(p, 16 * PITCH);
-        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, wh, o[i], 0, 0, 0);
-        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, wl, o[i], 0, 0, 0);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
+    };
 
-    // fold the waves: numerators [column][element], reference and sum
-    sum = rows_reduce<false>(sum);
-    __syncthreads();  // every wave is done with its V rows
-    float *const red = reinterpret_cast<float *>(lds);
-    if (live) {
-      float *dst = red + (wave * 16 + col) * RED;
-#pragma unroll
-      for (int i = 0; i < ND; ++i) *reinterpret_cast<f32x4 *>(dst + 16 * i + 4 * quad) = o[i];
-      if (quad == 0) {
-        dst[HDP] = ref - lift;
-        dst[HDP + 1] = sum;
+    reset();
+    int left = per_part;  // steps until the part ends
+    for (int s = s_first; s < s_end; ++s) {
+      step(s);
+      if (--left == 0 && s + 1 < s_end) {
+        flush();
+        reset();
+        left = per_part;
+        ++part;
       }
     }
-    __syncthreads();
-    for (int i = (int)threadIdx.x; i < cols * HDP; i += 64 * kRowsWaves) {
-      const int cc = i / HDP, e = i - cc * HDP;
-      const float *src = red + cc * RED;
-      float m[kRowsWaves], mx = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kRowsWaves; ++w) {
-        m[w] = src[w * 16 * RED + HDP];
-        mx = __builtin_fmaxf(mx, m[w]);
-      }
-      const float base = mx == -INFINITY ? 0.f : mx;
-      float l = 0.f, x = 0.f;
-#pragma unroll
-      for (int w = 0; w < kRowsWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(m[w] - base);
-        l = __builtin_fmaf(src[w * 16 * RED + HDP + 1], f, l);
-        x = __builtin_fmaf(src[w * 16 * RED + e], f, x);
-      }
-      if (e >= a.head_dim) continue;
-      const int64_t rh = row * a.n_heads + head0 + cc;
-      if (n_parts == 1) {
-        row_store(a, rh * a.head_dim + e, l != 0.f ? x / l : 0.f);
-      } else {
-        const int64_t at = (slot * a.n_heads + head0 + cc) * a.max_parts + part;
-        a.part_o[at * a.head_dim + e] = x;
-        if (e == 0) {
-          a.part_ml[2 * at] = mx;
-          a.part_ml[2 * at + 1] = l;
-        }
-      }
-    }
-    if (a.part_n && parted && part == 0 && threadIdx.x == 0) a.part_n[slot] = n_parts;
-    __syncthreads();  // the fold's memory is the next row's V rows
+    flush();
   }
 }
 
 template <typename T, int HDP, bool SPAN>
 hipError_t launch_rows_t(const PoolGeom &g, const ScoredArgs &a, int64_t most_rows, hipStream_t s) {
   const int group = a.n_heads / a.n_kv_heads, head_tiles = (group + 15) / 16;
-  const int64_t wgs = (a.row_items ? a.n_rows : a.n) * a.max_parts * a.n_kv_heads * head_tiles;
+  constexpr int occ = HDP <= 64 ? 3 : HDP <= 128 ? (std::is_same_v<T, Q4> ? 3 : 2) : 1;
+  // a wave for each possible part, or all parts shared by as many as are resident
+  const int64_t lanes = (int64_t)a.n_kv_heads * head_tiles, slots = std::max<int64_t>(a.cu_count * 4 * occ / lanes, 1);
+  int64_t waves = (a.row_items ? a.n_rows : a.n) * a.max_parts, share = 0;
+  if (waves > slots && !a.row_starts) waves = share = slots;
+  waves *= lanes;
+  const int64_t wgs = (waves + kRowsWaves - 1) / kRowsWaves;
   if (wgs * 64 * kRowsWaves >= (int64_t{1} << 32)) return hipErrorInvalidValue;
-  const bool mods = a.softcap > 0.f || a.slopes;
-  const auto kernel = mods ? scored_rows_kernel<T, HDP, SPAN, true> : scored_rows_kernel<T, HDP, SPAN, false>;
-  kernel<<<(unsigned)wgs, 64 * kRowsWaves, 0, s>>>(a, g.n_blocks, g.kv_dim, head_tiles, most_rows);
+  const bool mods = a.softcap > 0.f || a.slopes || a.window > 0 || a.prefix || a.first || a.row_starts;
+  const auto kernel =
+      mods ? scored_rows_kernel<T, HDP, SPAN, true, occ> : scored_rows_kernel<T, HDP, SPAN, false, occ>;
+  kernel<<<(unsigned)wgs, 64 * kRowsWaves, 0, s>>>(a, g.n_blocks, g.kv_dim, head_tiles, waves, share, most_rows);
   return hipGetLastError();
 }
 
