@@ -327,7 +327,8 @@ LTKV_API int ltkv_append_decode_attention(ltkv_cache *c, size_t layer, size_t n,
  * softcap) where softcap > 0, minus d_slopes[h] * |p - t| for query head h
  * (d_slopes may be null); the output is V weighted by the softmax of the
  * scores over the visible positions, zeros where there are none. Positions a
- * row does not see do not enter its result, whatever they hold.
+ * row does not see do not enter its result, whatever they hold (a row that
+ * sees an infinity or NaN gives values that are not finite).
  * f32 rows are computed to f32 accuracy; f16 and bf16 rows take Q as it is
  * and weights rounded to f16, summed in f32.
  * max_rows: the most rows of one sequence, which chooses the kernels; one with

@@ -8,7 +8,8 @@ namespace {
 
 constexpr int kRowsWaves = 4;
 constexpr int kAllButVmem = 0x78f;  // sched_barrier: what may move across (not accesses to global memory)
-constexpr int kTopExp = 15;  // q8_0 weights times V scales stay below 2^kTopExp
+constexpr int kTopExp = 15;  // f16 operands stay below 2^kTopExp
+constexpr int kNoExp = -10000;
 
 // K or V of 16 positions (a block) as a wave loads them: lane (t, quad) =
 // (lane & 15, lane >> 4) holds NC chunks of 8 elements of position t. Chunk j of a
@@ -132,6 +133,68 @@ struct Cells<int8_t, NC, SPAN> {
   __device__ __forceinline__ h4 scale(int j) const { return __builtin_bit_cast(h4, s[j]); }
 };
 
+// f32 elements enter the products as f16 hi + lo parts of the element times a
+// power of two, which brings the step's largest below 2^kTopExp.
+template <int NC, bool SPAN>
+struct Cells<float, NC, SPAN> {
+  f32x4 x[NC][2];
+  struct Place {
+    uint32_t at;
+    int chunks;
+    __device__ __forceinline__ Place(const ScoredArgs &a, int64_t kv_dim, int64_t head_off, int t, int quad) {
+      at = (uint32_t)((t * kv_dim + head_off + chunk_of<NC, SPAN>(quad, 0) * 8) * 4);
+      chunks = SPAN ? NC : (a.head_dim / 8 - quad + 3) / 4;
+    }
+  };
+  static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 64; }
+  __device__ __forceinline__ void load(const char *pool, const char *, int64_t at, const Place &p) {
+    const char *base = pool + at;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      if (SPAN || j < p.chunks) {
+        x[j][0] = load_at<f32x4>(base, p.at + j * (SPAN ? 32 : 128));
+        x[j][1] = load_at<f32x4>(base, p.at + j * (SPAN ? 32 : 128) + 16);
+      } else {
+        x[j][0] = x[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) x[j][0] = x[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  template <bool FINITE>
+  __device__ __forceinline__ float largest() const {
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float y = __builtin_fabsf(x[j][i >> 2][i & 3]);
+        m = __builtin_fmaxf(m, FINITE && !(y < INFINITY) ? 0.f : y);
+      }
+    return m;
+  }
+  __device__ __forceinline__ void get2(int j, int e, h8 &hi, h8 &lo) const {  // times 2^e
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      _Float16 a, b;
+      split2(__builtin_amdgcn_ldexpf(x[j][i >> 2][i & 3], e), a, b);
+      hi[i] = a;
+      lo[i] = b;
+    }
+  }
+};
+
+// Maximum over the wave, in every lane.
+__device__ __forceinline__ float wave_max(float x) {
+  x = __builtin_fmaxf(x, dpp<0xB1>(x));   // quad_perm [1,0,3,2]
+  x = __builtin_fmaxf(x, dpp<0x4E>(x));   // quad_perm [2,3,0,1]
+  x = __builtin_fmaxf(x, dpp<0x141>(x));  // row_half_mirror
+  x = __builtin_fmaxf(x, dpp<0x140>(x));  // row_mirror
+  return rows_reduce<true>(x);
+}
+
 // Steps of a part of a row that takes n steps.
 __device__ __forceinline__ int steps_per_part(const ScoredArgs &a, int n) {
   const int per_part = scored_part_tokens((int64_t)n * 32, a.part_tokens) >> 5;
@@ -171,8 +234,9 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
   constexpr int NC = HDP / 32;     // chunks of 8 elements a lane, products per score tile
   constexpr int ND = HDP / 16;     // 16-element tiles of the numerators
   constexpr int PITCH = HDP * 2 + 32;  // bytes of a V row in LDS: rows of a read start 8 banks apart
-  constexpr bool Q8 = std::is_same_v<T, int8_t>;
-  __shared__ __align__(16) char lds[kRowsWaves * 32 * PITCH];
+  constexpr bool Q8 = std::is_same_v<T, int8_t>, F32 = std::is_same_v<T, float>;
+  constexpr int V_BYTES = 32 * PITCH * (F32 ? 2 : 1);  // f32: hi parts, then lo parts
+  __shared__ __align__(16) char lds[kRowsWaves * V_BYTES];
 
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
@@ -228,7 +292,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
   const int head0 = kvh * group + head_tile * 16;
   const bool live = col < cols;
   const int64_t head_off = (int64_t)kvh * a.head_dim;
-  char *const my = lds + wave * (32 * PITCH);
+  char *const my = lds + wave * V_BYTES;
   const typename Cells<T, NC, SPAN>::Place place(a, kv_dim, head_off, col, quad);
 
   // an item is a sequence, whose rows are taken one after the other, or a row
@@ -349,6 +413,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
 
     f32x4 o[ND];
     float ref, sum, lift, scale_top;
+    int v_exp;  // f32: numerators are sums of V times 2^-v_exp
     auto reset = [&]() {
 #pragma unroll
       for (int i = 0; i < ND; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -356,8 +421,15 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
       sum = 0.f;
       lift = Q8 ? 0.f : kLift;
       scale_top = 0.f;  // q8_0: no scale has exceeded it
+      v_exp = kNoExp;
     };
     auto flush = [&]() {
+      if constexpr (F32) {
+        const float f = __builtin_amdgcn_ldexpf(1.f, v_exp == kNoExp ? 0 : v_exp / 2);
+        const float g = __builtin_amdgcn_ldexpf(1.f, v_exp == kNoExp ? 0 : v_exp - v_exp / 2);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[i] = o[i] * f * g;
+      }
       const float total = rows_reduce<false>(sum);
       if (!live) return;
       const int64_t rh = row * a.n_heads + head0 + col;
@@ -388,12 +460,57 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
       const bool whole = t0 + 32 <= t_end && t0 >= view.first && (t0 >= view.from || t0 + 32 <= view.sink_end);
       if (s_next - entry_step == 32) fill(s_next);
       find(s_next);
+      // f32: powers of two that bring K and V below 2^kTopExp (positions that the
+      // row does not see count as zeros)
+      int k_exp = 0;
+      if constexpr (F32) {
+        if (!whole)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int32_t t = t0 + 16 * u + col;
+            if (!(view.sees(t) && t < t_end)) {
+              k[u].clear();
+              v[u].clear();
+            }
+          }
+        auto most = [](const Cells<T, NC, SPAN> (&c)[2]) {  // of the finite elements
+          float m = wave_max(__builtin_fmaxf(c[0].template largest<false>(), c[1].template largest<false>()));
+          if (__builtin_amdgcn_readfirstlane(m == INFINITY))
+            m = wave_max(__builtin_fmaxf(c[0].template largest<true>(), c[1].template largest<true>()));
+          return m;
+        };
+        auto exponent = [](float m) {  // m < 2^e
+          return __builtin_amdgcn_readfirstlane(m > 0.f ? __builtin_amdgcn_frexp_expf(m) : 0);
+        };
+        k_exp = exponent(most(k)) - kTopExp;
+        const float m = most(v);
+        const int e = exponent(m) - kTopExp;
+        if (__builtin_amdgcn_readfirstlane(m > 0.f) && e > v_exp) {
+          if (v_exp != kNoExp) {
+            const float f = __builtin_amdgcn_ldexpf(1.f, v_exp - e);
+#pragma unroll
+            for (int i = 0; i < ND; ++i) o[i] *= f;
+          }
+          v_exp = e;
+        }
+      }
       // V into LDS (positions that the row does not see as zeros); the scores are
       // computed while it settles
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int32_t t = t0 + 16 * u + col;
         const bool seen = whole || (view.sees(t) && t < t_end);
+        if constexpr (F32) {
+#pragma unroll
+          for (int j = 0; j < NC; ++j) {
+            h8 hi, lo;
+            v[u].get2(j, v_exp == kNoExp ? 0 : -v_exp, hi, lo);
+            char *p = my + (16 * u + col) * PITCH + chunk_of<NC, SPAN>(quad, j) * 16;
+            *reinterpret_cast<h8 *>(p) = hi;
+            *reinterpret_cast<h8 *>(p + 32 * PITCH) = lo;
+          }
+          continue;
+        } else
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
           h8 y = v[u].get(j);
@@ -435,6 +552,15 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
 #pragma unroll
             for (int i = 0; i < 4; ++i) c[u][i] = __builtin_fmaf((float)d[i], g[i], c[u][i]);
           }
+        } else if constexpr (F32) {
+#pragma unroll
+          for (int j = 0; j < NC; ++j) {
+            h8 hi, lo;
+            k[u].get2(j, -k_exp, hi, lo);
+            c[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qh[j], c[u], 0, 0, 0);
+            cl[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ql[j], cl[u], 0, 0, 0);
+            cl[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qh[j], cl[u], 0, 0, 0);
+          }
         } else {  // (two chains of dependent products)
 #pragma unroll
           for (int j = 0; j < NC; ++j) {
@@ -445,16 +571,19 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
         }
       }
       load(k, a.k_layer, a.k_scale);
-      // V^T operands: on their way during the softmax
-      h8 vt[ND];
+      // V^T operands: on their way during the softmax (f32: too many registers)
+      const char *const my_t = my + (4 * quad + (col >> 2)) * PITCH + 4 * (col & 3) * 2;
+      h8 vt[F32 ? 1 : ND];
+      if constexpr (!F32) {
 #pragma unroll
-      for (int i = 0; i < ND; ++i)
-        vt[i] = read_tr2(my + (4 * quad + (col >> 2)) * PITCH + (16 * i + 4 * (col & 3)) * 2, 16 * PITCH);
+        for (int i = 0; i < ND; ++i) vt[i] = read_tr2(my_t + 32 * i, 16 * PITCH);
+      }
+      const float to_y = F32 ? __builtin_amdgcn_ldexpf(in_scale, k_exp) : in_scale;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float y = (Q8 ? c[u][i] : c[u][i] + cl[u][i]) * in_scale;
+          float y = (Q8 ? c[u][i] : c[u][i] + cl[u][i]) * to_y;
           if constexpr (MODS) {
             if (cap) y = tanh_f32(y) * cap_scale;
             y = __builtin_fmaf(-slope, (float)abs(view.pos - (t0 + 16 * u + 4 * quad + i)), y);
@@ -515,10 +644,20 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
           wh[i] = hi;
           wl[i] = lo;
         }
+        if constexpr (F32) {
 #pragma unroll
-        for (int i = 0; i < ND; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], wh, o[i], 0, 0, 0);
+          for (int i = 0; i < ND; ++i) {
+            const h8 hi = read_tr2(my_t + 32 * i, 16 * PITCH), lo = read_tr2(my_t + 32 * PITCH + 32 * i, 16 * PITCH);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wh, o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wl, o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wh, o[i], 0, 0, 0);
+          }
+        } else {
 #pragma unroll
-        for (int i = 0; i < ND; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], wl, o[i], 0, 0, 0);
+          for (int i = 0; i < ND; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], wh, o[i], 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < ND; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], wl, o[i], 0, 0, 0);
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
@@ -580,15 +719,19 @@ hipError_t launch_rows_hd(const PoolGeom &g, const ScoredArgs &a, int64_t most_r
   if (a.head_dim <= 64) return launch_rows_t<T, 64, false>(g, a, most_rows, s);
   if (a.head_dim <= 96) return launch_rows_t<T, 96, false>(g, a, most_rows, s);
   if (a.head_dim <= 128) return launch_rows_t<T, 128, false>(g, a, most_rows, s);
-  if (a.head_dim <= 192) return launch_rows_t<T, 192, false>(g, a, most_rows, s);
-  return launch_rows_t<T, 256, false>(g, a, most_rows, s);
+  if constexpr (!std::is_same_v<T, float>) {
+    if (a.head_dim <= 192) return launch_rows_t<T, 192, false>(g, a, most_rows, s);
+    return launch_rows_t<T, 256, false>(g, a, most_rows, s);
+  }
+  return hipErrorInvalidValue;
 }
 
 }  // namespace
 
-// q8_0: a head's 32-element products are whole groups, and none is padded.
+// q8_0: a head's 32-element products are whole groups, and none is padded. f32:
+// wider heads would leave no registers for the next step.
 bool scored_rows_supported(int elem, int head_dim) {
-  if (elem == 4 || head_dim % 8 != 0 || head_dim > 256) return false;
+  if (head_dim % 8 != 0 || head_dim > (elem == 4 ? 128 : 256)) return false;
   return elem != 1 || head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 192 ||
          head_dim == 256;
 }
@@ -596,6 +739,7 @@ bool scored_rows_supported(int elem, int head_dim) {
 hipError_t launch_scored_rows(const PoolGeom &g, const ScoredArgs &a, int64_t most_rows, hipStream_t s) {
   if (g.elem == kElemQ4) return launch_rows_hd<Q4>(g, a, most_rows, s);
   if (g.elem == 1) return launch_rows_hd<int8_t>(g, a, most_rows, s);
+  if (g.elem == 4) return launch_rows_hd<float>(g, a, most_rows, s);
   return launch_rows_hd<_Float16>(g, a, most_rows, s);
 }
 
