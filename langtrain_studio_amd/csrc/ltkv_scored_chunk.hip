@@ -19,16 +19,21 @@ constexpr int kChunkTokens = 64;  // positions of a tile
 template <typename T, int NC>
 struct Share;
 
+// A wave stages the 16 positions of one block: its address is uniform, a lane's
+// place in a block always the same (load_at).
 template <int NC>
 struct Share<_Float16, NC> {
   u32x4 x[NC];
   // chunk of the head that x[j] is: 64 consecutive bytes of a position a load
   __device__ static __forceinline__ int chunk(int part, int j) { return part + 4 * j; }
-  __device__ __forceinline__ void load(const void *pool, const void *, int64_t kv_dim, int32_t blk, int slot, int part,
-                                       int64_t head_off) {
-    const _Float16 *row = static_cast<const _Float16 *>(pool) + ((int64_t)blk * 16 + slot) * kv_dim + head_off;
+  static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 32; }
+  static __device__ __forceinline__ uint32_t place(int64_t kv_dim, int64_t head_off, int slot, int part) {
+    return (uint32_t)((slot * kv_dim + head_off + part * 8) * 2);
+  }
+  __device__ __forceinline__ void load(const void *pool, const void *, int64_t at, uint32_t place) {
+    const char *base = static_cast<const char *>(pool) + at;
 #pragma unroll
-    for (int j = 0; j < NC; ++j) x[j] = *reinterpret_cast<const u32x4 *>(row + chunk(part, j) * 8);
+    for (int j = 0; j < NC; ++j) x[j] = load_at<u32x4>(base, place + 64 * j);
   }
   __device__ __forceinline__ h8 get(int j) const { return __builtin_bit_cast(h8, x[j]); }
 };
@@ -38,20 +43,23 @@ struct Share<Q4, NC> {
   uint32_t x[NC];
   uint32_t s;  // (as 32 bits: a 16-bit value would be waited for to be moved)
   __device__ static __forceinline__ int chunk(int part, int j) { return part * NC + j; }
-  __device__ __forceinline__ void load(const void *pool, const void *scales, int64_t kv_dim, int32_t blk, int slot,
-                                       int part, int64_t head_off) {
-    const int e = (int)head_off + part * NC * 8;
-    const int64_t at = ((int64_t)blk * (kv_dim >> 5) + (e >> 5)) * 16 + slot;
-    s = static_cast<const uint16_t *>(scales)[at];
-    const uint32_t *p = static_cast<const uint32_t *>(pool) + at * 4 + ((e & 31) >> 3);
+  static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 8; }
+  // of the quants; the scale lies at an eighth of their group's place
+  static __device__ __forceinline__ uint32_t place(int64_t, int64_t head_off, int slot, int part) {
+    const uint32_t e = (uint32_t)head_off + part * NC * 8;
+    return ((e >> 5) * 16 + slot) * 16 + ((e & 31) >> 3) * 4;
+  }
+  __device__ __forceinline__ void load(const void *pool, const void *scales, int64_t at, uint32_t place) {
+    const char *base = static_cast<const char *>(pool) + at;
+    s = load_at<uint16_t>(static_cast<const char *>(scales) + (at >> 3), (place >> 4) * 2);
     if constexpr (NC == 4) {
-      const u32x4 w = *reinterpret_cast<const u32x4 *>(p);
+      const u32x4 w = load_at<u32x4>(base, place);
       x[0] = w.x;
       x[1] = w.y;
       x[2] = w.z;
       x[3] = w.w;
     } else {
-      const u32x2 w = *reinterpret_cast<const u32x2 *>(p);
+      const u32x2 w = load_at<u32x2>(base, place);
       x[0] = w.x;
       x[1] = w.y;
     }
@@ -67,14 +75,20 @@ struct Share<int8_t, NC> {
   u32x2 x[NC];
   uint32_t s;
   __device__ static __forceinline__ int chunk(int part, int j) { return part * NC + j; }
-  __device__ __forceinline__ void load(const void *pool, const void *scales, int64_t kv_dim, int32_t blk, int slot,
-                                       int part, int64_t head_off) {
-    const int64_t e = head_off + part * NC * 8;
-    s = static_cast<const uint16_t *>(scales)[((int64_t)blk * (kv_dim >> 5) + (e >> 5)) * 16 + slot];
-    const uint8_t *p = static_cast<const uint8_t *>(pool) + ((int64_t)blk * 16 + slot) * kv_dim + e;
+  static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 16; }
+  static __device__ __forceinline__ uint32_t place(int64_t kv_dim, int64_t head_off, int slot, int part) {
+    return (uint32_t)(slot * kv_dim + head_off + part * NC * 8);
+  }
+  static __device__ __forceinline__ uint32_t scale_place(int64_t head_off, int slot, int part) {
+    return (uint32_t)((((head_off + part * NC * 8) >> 5) * 16 + slot) * 2);
+  }
+  __device__ __forceinline__ void load(const void *pool, const void *scales, int64_t at, uint32_t place,
+                                       uint32_t scale_place) {
+    const char *base = static_cast<const char *>(pool) + at;
+    s = load_at<uint16_t>(static_cast<const char *>(scales) + (at >> 4), scale_place);
 #pragma unroll
     for (int j = 0; j < NC; j += 2) {
-      const u32x4 w = *reinterpret_cast<const u32x4 *>(p + 8 * j);
+      const u32x4 w = load_at<u32x4>(base, place + 8 * j);
       x[j] = u32x2{w.x, w.y};
       x[j + 1] = u32x2{w.z, w.w};
     }
@@ -93,13 +107,22 @@ struct Share<int8_t, NC> {
   }
 };
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+// The larger of `most` and the elements' magnitudes, as f16 bits: an infinity or
+// NaN is 0x7c00 or more.
+__device__ __forceinline__ u16x2 larger(u16x2 most, const h8 &x) {
+  const u32x4 u = __builtin_bit_cast(u32x4, x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, u[i] & 0x7fff7fffu));
+  return most;
+}
+
 // True if an element is infinite or NaN.
 __device__ __forceinline__ bool not_finite(const h8 &x) {
-  const u32x4 u = __builtin_bit_cast(u32x4, x);
-  uint32_t bad = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= ((u[i] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
-  return bad != 0;
+  const u16x2 m = larger(u16x2{0, 0}, x);
+  return m.x >= 0x7c00 || m.y >= 0x7c00;
 }
 
 __device__ __forceinline__ h8 finite_or_zero(const h8 &x) {
@@ -139,8 +162,8 @@ struct Bounds {
 
 // A work-group takes 128 columns, which are (row, query head) pairs of one kv
 // head: 128 / group rows; each of its four waves 32 of them. Tiles of 64
-// positions go through LDS as f16 numbers; a wave takes 32 positions at a time
-// on 32x32x16 products: scores^T = K Q^T, weights in place, numerators^T += V^T W
+// positions go through LDS as f16 numbers, on 32x32x16 products (two chains of
+// dependent ones for the scores, one per 32 positions): scores^T = K Q^T, weights in place, numerators^T += V^T W
 // (a lane's scores are positions 8 (r / 4) + 4 (lane / 32) + r % 4 of its column,
 // which is the second product's operand layout when its 16 positions are taken
 // as 4 (lane / 32) ... + 3 and 8 + 4 (lane / 32) ... + 3: no exchange). FULL
@@ -258,7 +281,8 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
       for (int i = 0; i < 8; ++i) amax = __builtin_fmaxf(amax, __builtin_fabsf(x[j][i]));
     }
     amax = halves_reduce<true>(amax);
-    const int up = amax > 0.f && amax < INFINITY ? 10 - __builtin_amdgcn_frexp_expf(amax) : 0;
+    // (at most 100: the scale's share stays a normal number)
+    const int up = amax > 0.f && amax < INFINITY ? min(10 - __builtin_amdgcn_frexp_expf(amax), 100) : 0;
 #pragma unroll
     for (int j = 0; j < NK; ++j)
 #pragma unroll
@@ -274,7 +298,10 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
   const float in_scale = cap ? qscale / a.softcap : qscale * kLog2e;
   const float cap_scale = a.softcap * kLog2e;
   const float slope = a.slopes && live ? a.slopes[head] * kLog2e : 0.f;
-  const bool biased = a.slopes != nullptr;
+  // scores are an affine function of the products (or of the capped rows' c),
+  // which falls with it where its factor is negative
+  const bool affine = !a.slopes && !(FULL && cap) && a.scale != 0.f;
+  const bool falling = affine && (cap || a.scale < 0.f);
 
   f32x16 o[NC];
 #pragma unroll
@@ -286,22 +313,36 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
   const int32_t *tab = table_of(a.tables, a.table_stride, a.rows, a.table_rows, seq);
   const int64_t head_off = (int64_t)kvh * HD;
   const int tok = tid >> 2, part = tid & 3;
-  auto entry_of = [&](int s) {
-    const int32_t t = range.start(s) + tok;
-    int32_t e = s < s_end && t < range.end(s) ? tab[t >> 4] : 0;
+  // The wave's block of a tile, read a tile ahead of its cells (past the end:
+  // block 0, read and masked).
+  auto block_of = [&](int s) {
+    const int32_t t = range.start(s) + 16 * wave;
+    int32_t e = s < s_end && t < range.end(s) ? scalar_read(tab, t >> 4) : 0;
     if (e < 0 || e >= n_blocks) {
       report_fault(a.status, kFaultTable, seq);
       e = 0;
     }
     return e;
   };
+  const int64_t block_bytes = Share<T, NC>::block_bytes(kv_dim);
+  const uint32_t place = Share<T, NC>::place(kv_dim, head_off, tok & 15, part);
+  uint32_t scale_place = 0;
+  if constexpr (Q8) scale_place = Share<T, NC>::scale_place(head_off, tok & 15, part);
   Share<T, NC> ks, vs;
+  auto load = [&](int32_t block) {
+    const int64_t at = (int64_t)(uint32_t)block * block_bytes;
+    if constexpr (Q8) {
+      ks.load(a.k_layer, a.k_scale, at, place, scale_place);
+      vs.load(a.v_layer, a.v_scale, at, place, scale_place);
+    } else {
+      ks.load(a.k_layer, a.k_scale, at, place);
+      vs.load(a.v_layer, a.v_scale, at, place);
+    }
+  };
   int32_t next = 0;
   if (s_begin < s_end) {
-    const int32_t e = entry_of(s_begin);
-    ks.load(a.k_layer, a.k_scale, kv_dim, e, tok & 15, part, head_off);
-    vs.load(a.v_layer, a.v_scale, kv_dim, e, tok & 15, part, head_off);
-    next = entry_of(s_begin + 1);
+    load(block_of(s_begin));
+    next = block_of(s_begin + 1);
   }
 
   for (int s = s_begin; s < s_end; ++s) {
@@ -341,6 +382,7 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
       }
     }
     bool bad = false;
+    u16x2 v_most = {0, 0};
     {
       float dk = 0.f, dv = 0.f;
       if constexpr (Q8) {
@@ -366,12 +408,16 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
         } else {
           *reinterpret_cast<h8 *>(lds_k + tok * K_PITCH + c) = ks.get(j);
           h8 x = vs.get(j);
-          if constexpr (std::is_same_v<T, _Float16>)
-            if (not_finite(x)) {
-              bad = true;
-              x = finite_or_zero(x);
-            }
+          if constexpr (std::is_same_v<T, _Float16>) v_most = larger(v_most, x);
           *reinterpret_cast<h8 *>(lds_v + tok * V_PITCH + c) = x;
+        }
+      }
+      if constexpr (std::is_same_v<T, _Float16>) {
+        bad = v_most.x >= 0x7c00 || v_most.y >= 0x7c00;
+        if (bad) {  // rare: once more, without them
+#pragma unroll
+          for (int j = 0; j < NC; ++j)
+            *reinterpret_cast<h8 *>(lds_v + tok * V_PITCH + Share<T, NC>::chunk(part, j) * 16) = finite_or_zero(vs.get(j));
         }
       }
     }
@@ -380,118 +426,139 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
       if (lane == 0) s_bad[wave] = any_bad;
     }
     if (s + 1 < s_end) {
-      ks.load(a.k_layer, a.k_scale, kv_dim, next, tok & 15, part, head_off);
-      vs.load(a.v_layer, a.v_scale, kv_dim, next, tok & 15, part, head_off);
-      next = entry_of(s + 2);
+      load(next);
+      next = block_of(s + 2);
     }
     lds_barrier();
     bool tile_bad = false;
     if constexpr (!std::is_same_v<T, Q4>) tile_bad = (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) != 0;
 
-#pragma unroll 1
-    for (int u = 0; u < kChunkTokens; u += 32) {
-      const int32_t tb = t0 + u;
-      if (tb >= t_end || wb.none(tb, 32)) continue;
-      f32x16 c = {};
-      const char *kp = lds_k + (u + col) * K_PITCH + 16 * half;
+    if (wb.none(t0, kChunkTokens)) continue;
+    // scores of positions t0 + 32 u + 8 (i / 4) + 4 half + i % 4
+    f32x16 c[2] = {};
+    const char *kp = lds_k + col * K_PITCH + 16 * half;
 #pragma unroll
-      for (int j = 0; j < NK; ++j) {
-        const h8 x = *reinterpret_cast<const h8 *>(kp + 32 * j);
-        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[j], c, 0, 0, 0);
-        if constexpr (FULL) c = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[j], c, 0, 0, 0);
+    for (int j = 0; j < NK; ++j) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const h8 x = *reinterpret_cast<const h8 *>(kp + 32 * u * K_PITCH + 32 * j);
+        c[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[j], c[u], 0, 0, 0);
+        if constexpr (FULL) c[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[j], c[u], 0, 0, 0);
         if constexpr (Q8) {
-          const h8 y = *reinterpret_cast<const h8 *>(kp + K_BYTES + 32 * j);
-          c = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[j], c, 0, 0, 0);
+          const h8 y = *reinterpret_cast<const h8 *>(kp + K_BYTES + 32 * u * K_PITCH + 32 * j);
+          c[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[j], c[u], 0, 0, 0);
         }
       }
-      const float to_x = Q8 ? __builtin_amdgcn_ldexpf(in_scale, k_exp) : in_scale;
+    }
+    const float to_x = Q8 ? __builtin_amdgcn_ldexpf(in_scale, k_exp) : in_scale;
+    const int32_t tl = t0 + 4 * half;
+    // Scores in the log2 domain as m c + m0: the multiplication is left to the
+    // fused one before exp2. Capped rows of 16 bits take c = 1 / (exp(2 x) + 1),
+    // since cap tanh(x) = cap - 2 cap c: five instructions a score.
+    float m = 1.f, m0 = 0.f;
+    if (affine) {
+      m = to_x;
+      if (cap) {
+        const float to_e = to_x * (2.f * kLog2e);
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          c[i >> 4][i & 15] = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(c[i >> 4][i & 15] * to_e) + 1.f);
+        m = -2.f * cap_scale;
+        m0 = cap_scale;
+      }
+    } else {
       if (cap) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float x = c[i] * to_x;
-          if constexpr (FULL) c[i] = tanh_f32(x) * cap_scale;
-          else c[i] = tanh_f16(x) * cap_scale;
+        for (int i = 0; i < 32; ++i) {
+          const float x = c[i >> 4][i & 15] * to_x;
+          if constexpr (FULL) c[i >> 4][i & 15] = tanh_f32(x) * cap_scale;
+          else c[i >> 4][i & 15] = tanh_f16(x) * cap_scale;
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) c[i] *= to_x;
+        for (int i = 0; i < 32; ++i) c[i >> 4][i & 15] *= to_x;
       }
-      const int32_t tl = tb + 4 * half;  // the lane's positions: tl + 8 (i / 4) + i % 4
-      if (biased) {
-        const float d0 = (float)(view.pos - tl);
+      const float d0 = (float)(view.pos - tl);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          c[i] = __builtin_fmaf(-slope, __builtin_fabsf(d0 - (float)(8 * (i / 4) + i % 4)), c[i]);
+      for (int i = 0; i < 32; ++i)
+        c[i >> 4][i & 15] =
+            __builtin_fmaf(-slope, __builtin_fabsf(d0 - (float)(8 * (i / 4) + i % 4)), c[i >> 4][i & 15]);
+    }
+    if (t0 + kChunkTokens > t_end || !wb.all(t0, kChunkTokens)) {
+      const float none = falling ? INFINITY : -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const int32_t t = tl + 8 * (i / 4) + i % 4;
+        if (!(view.sees(t) && t < t_end)) c[i >> 4][i & 15] = none;
       }
-      if (tb + 32 > t_end || !wb.all(tb, 32)) {
+    }
+    float top = c[0][0];
+    if (falling) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int32_t t = tl + 8 * (i / 4) + i % 4;
-          if (!(view.sees(t) && t < t_end)) c[i] = -INFINITY;
+      for (int i = 1; i < 32; ++i) top = __builtin_fminf(top, c[i >> 4][i & 15]);
+    } else {
+#pragma unroll
+      for (int i = 1; i < 32; ++i) top = __builtin_fmaxf(top, c[i >> 4][i & 15]);
+    }
+    top = __builtin_fmaf(top, m, m0);
+    if (__builtin_amdgcn_ballot_w64(top > ref + kSlack)) {
+      const float nr = __builtin_fmaxf(ref, halves_reduce<true>(top));
+      const float f = nr == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - nr);
+      sum *= f;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) o[i] *= f;
+      ref = nr;
+    }
+    const float base = m0 - ((ref == -INFINITY ? 0.f : ref) - kLift);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      c[i >> 4][i & 15] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[i >> 4][i & 15], m, base));
+      sum += c[i >> 4][i & 15];
+    }
+#pragma unroll
+    for (int p = 0; p < kChunkTokens / 16; ++p) {
+      h8 wh, wl;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        _Float16 hi, lo;
+        split2(c[p >> 1][8 * (p & 1) + i], hi, lo);
+        wh[i] = hi;
+        wl[i] = lo;
+      }
+      const char *vp = lds_v + (16 * p + 4 * half + ((lane & 15) >> 2)) * V_PITCH +
+                       (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const h8 x = read_tr2(vp + 64 * i, 8 * V_PITCH);
+        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wh, o[i], 0, 0, 0);
+        if constexpr (FULL) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wl, o[i], 0, 0, 0);
+        if constexpr (V_PLANES == 2) {
+          const h8 y = read_tr2(vp + V_BYTES + 64 * i, 8 * V_PITCH);
+          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, wh, o[i], 0, 0, 0);
         }
       }
-      float top = c[0];
+    }
+    if constexpr (!std::is_same_v<T, Q4>) {
+      if (tile_bad) {
+        // V elements that are infinite or NaN entered as zeros: the rows that
+        // see their positions get them here, the others do not
+        for (int j = 0; j < kChunkTokens; ++j) {
+          const int32_t t = t0 + j;
+          if (t >= t_end) break;
+          int32_t e = scalar_read(tab, t >> 4);
+          if (e < 0 || e >= n_blocks) e = 0;
+          float w = 0.f;
 #pragma unroll
-      for (int i = 1; i < 16; ++i) top = __builtin_fmaxf(top, c[i]);
-      if (__builtin_amdgcn_ballot_w64(top > ref + kSlack)) {
-        const float nr = __builtin_fmaxf(ref, halves_reduce<true>(top));
-        const float f = nr == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - nr);
-        sum *= f;
+          for (int i = 0; i < 32; ++i)  // position j is score i of lane (column, j / 4 % 2)
+            if (i == (j >> 3) * 4 + (j & 3)) w = __shfl(c[i >> 4][i & 15], col + 32 * ((j >> 2) & 1), 64);
+          if (!view.sees(t)) continue;
+          for (int k = 0; k < NC * 16; ++k) {
+            const int64_t d = head_off + 32 * (k / 16) + 8 * (k % 16 / 4) + 4 * half + k % 4;
+            const float x = cell_value<T>(a.v_layer, a.v_scale, (int64_t)e * 16 + (t & 15), kv_dim, d);
+            if (__builtin_fabsf(x) < INFINITY) continue;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) o[i] *= f;
-        ref = nr;
-      }
-      const float base = (ref == -INFINITY ? 0.f : ref) - kLift;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        c[i] = __builtin_amdgcn_exp2f(c[i] - base);
-        sum += c[i];
-      }
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        h8 wh, wl;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          _Float16 hi, lo;
-          split2(c[8 * p + i], hi, lo);
-          wh[i] = hi;
-          wl[i] = lo;
-        }
-        const char *vp = lds_v + (u + 16 * p + 4 * half + ((lane & 15) >> 2)) * V_PITCH +
-                         (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const h8 x = read_tr2(vp + 64 * i, 8 * V_PITCH);
-          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wh, o[i], 0, 0, 0);
-          if constexpr (FULL) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wl, o[i], 0, 0, 0);
-          if constexpr (V_PLANES == 2) {
-            const h8 y = read_tr2(vp + V_BYTES + 64 * i, 8 * V_PITCH);
-            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, wh, o[i], 0, 0, 0);
-          }
-        }
-      }
-      if constexpr (!std::is_same_v<T, Q4>) {
-        if (tile_bad) {
-          // V elements that are infinite or NaN entered as zeros: the rows that
-          // see their positions get them here, the others do not
-          for (int j = 0; j < 32; ++j) {
-            const int32_t t = tb + j;
-            if (t >= t_end) break;
-            int32_t e = tab[t >> 4];
-            if (e < 0 || e >= n_blocks) e = 0;
-            float w = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i)  // position j is element i of lane (column, j / 4 % 2)
-              if (i == (j >> 3) * 4 + (j & 3)) w = __shfl(c[i], col + 32 * ((j >> 2) & 1), 64);
-            if (!view.sees(t)) continue;
-#pragma unroll
-            for (int i = 0; i < NC; ++i)
-#pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                const int64_t d = head_off + 32 * i + 8 * (k / 4) + 4 * half + k % 4;
-                const float x = cell_value<T>(a.v_layer, a.v_scale, (int64_t)e * 16 + (t & 15), kv_dim, d);
-                if (!(__builtin_fabsf(x) < INFINITY)) o[i][k] += w * x;
-              }
+            for (int i = 0; i < NC * 16; ++i)
+              if (i == k) o[i / 16][i % 16] += w * x;
           }
         }
       }

@@ -394,7 +394,8 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
         for (int i = 0; i < 8; ++i) amax = __builtin_fmaxf(amax, __builtin_fabsf(x[j][i]));
       }
       amax = rows_reduce<true>(amax);
-      const int up = amax > 0.f && amax < INFINITY ? 10 - __builtin_amdgcn_frexp_expf(amax) : 0;
+      // (at most 100: the scale's share stays a normal number)
+      const int up = amax > 0.f && amax < INFINITY ? min(10 - __builtin_amdgcn_frexp_expf(amax), 100) : 0;
 #pragma unroll
       for (int j = 0; j < NC; ++j)
 #pragma unroll
