@@ -41,6 +41,7 @@ inline bool scored_chunks_supported(int elem, int head_dim, int group) {
   return elem != 4 && (head_dim == 64 || head_dim == 128) && group <= kChunkColumns;
 }
 inline int chunk_rows(const ScoredArgs &a) { return kChunkColumns / (a.n_heads / a.n_kv_heads); }
+inline int64_t chunk_slots(const ScoredArgs &a) { return a.n_rows / chunk_rows(a) + a.n; }
 hipError_t launch_scored_chunks(const PoolGeom &g, const ScoredArgs &a, int64_t min_rows, hipStream_t s);
 
 namespace {
@@ -100,6 +101,14 @@ __device__ __forceinline__ RowView row_view(const ScoredArgs &a, const SeqRows &
     v.sink_end = v.first < s.len ? v.first + (int32_t)min(a.sinks, (int64_t)(s.len - v.first)) : v.first;
   }
   return v;
+}
+
+// Slots of the chunk kernel's tiles: those of sequence i begin at starts[i] /
+// rows_per_tile + i, which leaves room for all of its tiles whatever its first
+// row's place in a tile.
+__device__ __forceinline__ int64_t first_slot(const ScoredArgs &a, int64_t i, int rows_per_tile) {
+  const int64_t st = a.row_starts[i];
+  return (st < 0 ? 0 : st > a.n_rows ? a.n_rows : st) / rows_per_tile + i;
 }
 
 // Sequence of launch row `row`: the last one whose first row is not behind it.
@@ -270,22 +279,23 @@ hipError_t by_element(int elem, F &&f) {
 }
 
 
-constexpr int64_t kShortSpan = 8192;
-
 // Tokens per part of a row's visible positions (rounded up to 32-token steps;
 // a multiple of 64): a function of the row's own span, so that a decode
 // query's bits do not depend on its batch.
+constexpr int64_t kShortSpan = 2048, kLongSpan = 8192;
 __host__ __device__ inline int scored_part_tokens(int64_t span, int fixed) {
   if (fixed > 0) return fixed;
-  return span <= kShortSpan ? 256 : 512;
+  return span <= kShortSpan ? 128 : span <= kLongSpan ? 256 : 512;
 }
 
 // Most parts of spans up to `span` tokens.
 inline int64_t scored_max_parts(int64_t span, int fixed) {
   auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   if (fixed > 0) return up(span, fixed);
-  const int64_t parts = up(std::min<int64_t>(span, kShortSpan), 256);
-  return span > kShortSpan ? std::max(parts, up(span, 512)) : parts;
+  int64_t parts = up(std::min<int64_t>(span, kShortSpan), 128);
+  if (span > kShortSpan) parts = std::max(parts, up(std::min<int64_t>(span, kLongSpan), 256));
+  if (span > kLongSpan) parts = std::max(parts, up(span, 512));
+  return parts;
 }
 
 // The STEP-position steps over what a row (or rows together) sees: those of the

@@ -113,11 +113,11 @@ __global__ void __launch_bounds__(kAnyThreads) scored_any_kernel(ScoredArgs a, i
 // Rows whose positions were taken in several parts (or splits): their numerators
 // and sums folded in order by their references. A work-group per 256 elements
 // of a row: first the part slots of the rows kernel (ScoredArgs::part_n), then
-// every launch row for the chunk kernel's.
+// the rows of the chunk kernel's split tile slots.
 constexpr int kMergeThreads = 256;
 
 __global__ void __launch_bounds__(kMergeThreads) scored_merge_kernel(ScoredArgs a, int slices, int64_t part_slots,
-                                                                     int64_t min_rows) {
+                                                                     int64_t min_rows, int rows_per_tile) {
   const int64_t item = blockIdx.x / (uint32_t)slices;
   const int i = (int)(blockIdx.x % (uint32_t)slices) * kMergeThreads + (int)threadIdx.x;
   if (i >= a.n_heads * a.head_dim) return;
@@ -137,9 +137,18 @@ __global__ void __launch_bounds__(kMergeThreads) scored_merge_kernel(ScoredArgs 
     o = a.part_o;
     ml = a.part_ml;
   } else {
-    slot = row = item - part_slots;
-    const SeqRows s = seq_rows(a, seq_of_row(a, row));
-    if (row < s.row0 || row >= s.row0 + s.count || s.count <= min_rows) return;
+    slot = item - part_slots;
+    const int64_t tile = slot / rows_per_tile;
+    int64_t seq = 0;  // the last sequence whose tile slots begin at or before this one
+    for (int64_t end = a.n; end - seq > 1;) {
+      const int64_t mid = (seq + end) / 2;
+      if (first_slot(a, mid, rows_per_tile) <= tile) seq = mid;
+      else end = mid;
+    }
+    const SeqRows s = seq_rows(a, seq);
+    const int64_t r = (tile - first_slot(a, seq, rows_per_tile)) * rows_per_tile + slot % rows_per_tile;
+    if (r < 0 || r >= s.count || s.count <= min_rows) return;
+    row = s.row0 + r;
     n_parts = scalar_read(a.chunk_n, slot);
     stride = a.splits;
     o = a.chunk_o;
@@ -278,6 +287,7 @@ ScoredWorkspace scored_workspace(int elem, ScoredArgs &a) {
   a.chunks = k.chunks;
   if (k.chunks && k.rows) a.max_rows = kRowsKernelMax;  // of the sequences that the rows kernel takes
   a.max_parts = a.splits = 1;
+  a.split_slots = 0;
   const int64_t span = span_bound(a);
   int64_t at = 0;
   if (k.rows && (a.max_parts = (int)scored_max_parts(span, a.part_tokens)) > 1) {
@@ -288,15 +298,22 @@ ScoredWorkspace scored_workspace(int elem, ScoredArgs &a) {
     at = (w.part_n_off + slots * 4 + 255) / 256 * 256;
   }
   if (k.chunks) {
-    // as many work-groups as are resident (two a CU), at least 256 positions each
-    const int64_t tiles = (a.n_rows / chunk_rows(a) + 1) * a.n_kv_heads;
-    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({2 * a.cu_count / tiles, span / 256, 32}));
+    // The work-groups that whole rounds of the resident ones (two a CU) leave over
+    // are split over their positions, to fill a round as well (at least 256
+    // positions each): partials cost their traffic only there.
+    const int rows = chunk_rows(a);
+    const int64_t tiles = (a.n_rows + rows - 1) / rows * a.n_kv_heads, resident = 2 * a.cu_count;
+    const int64_t over = tiles % resident;
+    // (a few left over cost less than the merge of their splits)
+    if (over >= resident / 8 || tiles < resident) a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident / over, span / 256, 32}));
     if (a.splits > 1) {
-      const int64_t parts = a.n_rows * a.n_heads * (int64_t)a.splits;
+      // (slots may be empty: a sequence's tiles need not fill its slots)
+      a.split_slots = (int)std::min<int64_t>((over + a.n_kv_heads - 1) / a.n_kv_heads + a.n, chunk_slots(a));
+      const int64_t split_rows = (int64_t)a.split_slots * rows, parts = split_rows * a.n_heads * a.splits;
       w.chunk_o_off = at;
       w.chunk_ml_off = at + parts * a.head_dim * 4;
       w.chunk_n_off = w.chunk_ml_off + parts * 2 * 4;
-      at = w.chunk_n_off + a.n_rows * 4;
+      at = w.chunk_n_off + split_rows * 4;
     }
   }
   w.bytes = at;
@@ -320,11 +337,13 @@ hipError_t launch_scored_attention(const PoolGeom &g, const ScoredArgs &a, hipSt
   if (border > 0)
     if (const hipError_t e = launch_scored_rows(g, a, border, s); e != hipSuccess) return e;
   const int64_t part_slots = border > 0 && a.max_parts > 1 ? (a.row_items ? a.n_rows : a.n * a.max_rows) : 0;
-  const int64_t items = part_slots + (a.splits > 1 ? a.n_rows : 0);
+  const int rows_per_tile = a.chunks ? chunk_rows(a) : 1;
+  const int64_t items = part_slots + (int64_t)a.split_slots * rows_per_tile;
   if (items == 0) return hipSuccess;
   const int slices = (a.n_heads * a.head_dim + kMergeThreads - 1) / kMergeThreads;
   if (items * slices * kMergeThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
-  scored_merge_kernel<<<(unsigned)(items * slices), kMergeThreads, 0, s>>>(a, slices, part_slots, border);
+  scored_merge_kernel<<<(unsigned)(items * slices), kMergeThreads, 0, s>>>(a, slices, part_slots, border,
+                                                                           rows_per_tile);
   return hipGetLastError();
 }
 

@@ -109,19 +109,12 @@ struct Share<int8_t, NC> {
 
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
-// The larger of `most` and the elements' magnitudes, as f16 bits: an infinity or
-// NaN is 0x7c00 or more.
-__device__ __forceinline__ u16x2 larger(u16x2 most, const h8 &x) {
-  const u32x4 u = __builtin_bit_cast(u32x4, x);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, u[i] & 0x7fff7fffu));
-  return most;
-}
-
 // True if an element is infinite or NaN.
 __device__ __forceinline__ bool not_finite(const h8 &x) {
-  const u16x2 m = larger(u16x2{0, 0}, x);
+  const u32x4 u = __builtin_bit_cast(u32x4, x);
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, u[i] & 0x7fff7fffu));
   return m.x >= 0x7c00 || m.y >= 0x7c00;
 }
 
@@ -188,19 +181,19 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int group = a.n_heads / a.n_kv_heads;
-  uint32_t b = blockIdx.x;
-  const int kvh = (int)(b % (uint32_t)a.n_kv_heads);
-  b /= (uint32_t)a.n_kv_heads;
-  const int split = (int)(b % (uint32_t)a.splits);
-  // late slots first: under a causal mask a chunk's last rows see most
-  const int64_t slot = n_slots - 1 - (int64_t)(b / (uint32_t)a.splits);
-
-  // Slots of sequence i begin at starts[i] / rows_per_tile + i: room for all of
-  // its tiles whatever its first row's place in a tile.
-  auto slot0 = [&](int64_t i) {
-    const int64_t st = a.row_starts[i];
-    return (st < 0 ? 0 : st > a.n_rows ? a.n_rows : st) / rows_per_tile + i;
-  };
+  const int kvh = (int)(blockIdx.x % (uint32_t)a.n_kv_heads);
+  const uint32_t b = blockIdx.x / (uint32_t)a.n_kv_heads;
+  // late slots first: under a causal mask a chunk's last rows see most; the
+  // first split_slots slots, which come last, in `splits` work-groups each
+  const uint32_t whole_slots = (uint32_t)(n_slots - a.split_slots);
+  int split = 0, splits = 1;
+  int64_t slot = n_slots - 1 - (int64_t)b;
+  if (b >= whole_slots) {
+    splits = a.splits;
+    split = (int)((b - whole_slots) % (uint32_t)splits);
+    slot = a.split_slots - 1 - (int64_t)((b - whole_slots) / (uint32_t)splits);
+  }
+  auto slot0 = [&](int64_t i) { return first_slot(a, i, rows_per_tile); };
   int64_t seq = 0;
   for (int64_t size = a.n; size > 1;) {  // the last sequence whose slots begin at or before this one
     const int64_t step = (size + 63) / 64, i = seq + lane * step;
@@ -253,8 +246,12 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
     for (int w = 1; w < kChunkWaves; ++w) {
       const Bounds o = s_bounds[w];
       gb.first_min = min(gb.first_min, o.first_min);
+      gb.first_max = max(gb.first_max, o.first_max);
       gb.from_min = min(gb.from_min, o.from_min);
+      gb.from_max = max(gb.from_max, o.from_max);
+      gb.sink_min = min(gb.sink_min, o.sink_min);
       gb.sink_max = max(gb.sink_max, o.sink_max);
+      gb.end_min = min(gb.end_min, o.end_min);
       gb.end_max = max(gb.end_max, o.end_max);
     }
   }
@@ -263,7 +260,7 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
     const RowView all{0, gb.first_min, gb.sink_max, gb.from_min, gb.end_max};
     range = step_range<kChunkTokens>(all);
   }
-  const int per_part = (range.n + a.splits - 1) / a.splits;
+  const int per_part = (range.n + splits - 1) / splits;
   const int n_parts = per_part > 0 ? (range.n + per_part - 1) / per_part : 1;
   if (split >= n_parts) return;
   const int s_begin = split * per_part, s_end = min(range.n, s_begin + per_part);
@@ -381,8 +378,10 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
         v_exp = e;
       }
     }
+    // Infinities and NaN in V may reach only the rows that see them: looked for
+    // where a row of the work-group does not see the whole tile.
+    const bool partial = t0 + kChunkTokens > t_end || !gb.all(t0, kChunkTokens);
     bool bad = false;
-    u16x2 v_most = {0, 0};
     {
       float dk = 0.f, dv = 0.f;
       if constexpr (Q8) {
@@ -398,7 +397,7 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
           *reinterpret_cast<h8 *>(lds_k + tok * K_PITCH + c) = hi;
           *reinterpret_cast<h8 *>(lds_k + K_BYTES + tok * K_PITCH + c) = lo;
           vs.get2(j, dv, hi, lo);
-          if (not_finite(hi)) {
+          if (partial && not_finite(hi)) {
             bad = true;
             hi = h8{};
             lo = h8{};
@@ -407,14 +406,15 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
           if constexpr (V_PLANES == 2) *reinterpret_cast<h8 *>(lds_v + V_BYTES + tok * V_PITCH + c) = lo;
         } else {
           *reinterpret_cast<h8 *>(lds_k + tok * K_PITCH + c) = ks.get(j);
-          h8 x = vs.get(j);
-          if constexpr (std::is_same_v<T, _Float16>) v_most = larger(v_most, x);
-          *reinterpret_cast<h8 *>(lds_v + tok * V_PITCH + c) = x;
+          *reinterpret_cast<h8 *>(lds_v + tok * V_PITCH + c) = vs.get(j);
         }
       }
       if constexpr (std::is_same_v<T, _Float16>) {
-        bad = v_most.x >= 0x7c00 || v_most.y >= 0x7c00;
-        if (bad) {  // rare: once more, without them
+        if (partial) {
+#pragma unroll
+          for (int j = 0; j < NC; ++j) bad = bad || not_finite(vs.get(j));
+        }
+        if (bad) {  // once more, without them
 #pragma unroll
           for (int j = 0; j < NC; ++j)
             *reinterpret_cast<h8 *>(lds_v + tok * V_PITCH + Share<T, NC>::chunk(part, j) * 16) = finite_or_zero(vs.get(j));
@@ -513,7 +513,7 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       c[i >> 4][i & 15] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[i >> 4][i & 15], m, base));
-      sum += c[i >> 4][i & 15];
+      if constexpr (FULL) sum += c[i >> 4][i & 15];
     }
 #pragma unroll
     for (int p = 0; p < kChunkTokens / 16; ++p) {
@@ -524,6 +524,11 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
         split2(c[p >> 1][8 * (p & 1) + i], hi, lo);
         wh[i] = hi;
         wl[i] = lo;
+      }
+      if constexpr (!FULL) {  // the weights as they enter the product, two an instruction
+        const h2 one = {(_Float16)1.f, (_Float16)1.f};
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) sum = __builtin_amdgcn_fdot2(h2{wh[i], wh[i + 1]}, one, sum, false);
       }
       const char *vp = lds_v + (16 * p + 4 * half + ((lane & 15) >> 2)) * V_PITCH +
                        (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
@@ -582,7 +587,7 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
           store_row4(a, rh * HD + 32 * i + 2 * k + 4 * half,
                      f32x4{o[i][k] * inv, o[i][k + 1] * inv, o[i][k + 2] * inv, o[i][k + 3] * inv});
     } else {
-      const int64_t at = rh * a.splits + split;
+      const int64_t at = ((slot * rows_per_tile + rr) * a.n_heads + head) * a.splits + split;
       float *dst = a.chunk_o + at * HD + 4 * half;
 #pragma unroll
       for (int i = 0; i < NC; ++i)
@@ -594,15 +599,16 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
         a.chunk_ml[2 * at + 1] = sum;
       }
     }
-    if (a.chunk_n && split == 0 && half == 0 && kvh == 0 && c128 - rr * group == 0) a.chunk_n[row] = n_parts;
+    if (splits > 1 && split == 0 && half == 0 && kvh == 0 && c128 - rr * group == 0)
+      a.chunk_n[slot * rows_per_tile + rr] = n_parts;
   }
 }
 
 template <typename T, int HD>
 hipError_t launch_chunk_t(const PoolGeom &g, const ScoredArgs &a, int64_t min_rows, hipStream_t s) {
   const int rows_per_tile = chunk_rows(a);
-  const int64_t n_slots = a.n_rows / rows_per_tile + a.n;
-  const int64_t wgs = n_slots * a.splits * a.n_kv_heads;
+  const int64_t n_slots = chunk_slots(a);
+  const int64_t wgs = (n_slots - a.split_slots + (int64_t)a.split_slots * a.splits) * a.n_kv_heads;
   if (wgs * 64 * kChunkWaves >= (int64_t{1} << 32)) return hipErrorInvalidValue;
   const auto kernel =
       a.row_type == LTKV_ROWS_F32 ? scored_chunk_kernel<T, HD, true> : scored_chunk_kernel<T, HD, false>;
