@@ -221,7 +221,7 @@ __device__ __forceinline__ void quantize_store4_q4(const float (&x)[8], int j, u
   float c[8], top = -kLimit, low = kLimit;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    c[i] = x[i] == x[i] ? __builtin_fminf(__builtin_fmaxf(x[i], -kLimit), kLimit) : 0.f;
+    c[i] = x[i] == x[i] ? __builtin_amdgcn_fmed3f(x[i], -kLimit, kLimit) : 0.f;
     top = __builtin_fmaxf(top, c[i]);
     low = __builtin_fminf(low, c[i]);
   }
@@ -233,14 +233,18 @@ __device__ __forceinline__ void quantize_store4_q4(const float (&x)[8], int j, u
   const uint32_t u = __builtin_bit_cast(uint32_t, e);
   const _Float16 dh = (_Float16)__builtin_bit_cast(float, (u + 0x7fffu + ((u >> 16) & 1u)) & 0xffff0000u);
   const float d = (float)dh;
-  uint32_t w = 0;
+  // One division a lane: x * (1 / d) and one step on its exact remainder give
+  // the correctly rounded x / d (every significand of x against the 128 of d
+  // agrees). The nibbles of a half dword add up exactly as a float.
+  const float id = d != 0.f ? 1.f / d : 0.f;
+  float half[2] = {8.f * 0x1111, 8.f * 0x1111};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float r = d != 0.f ? __builtin_rintf(c[i] / d) : 0.f;
-    const int q = (int)__builtin_fminf(__builtin_fmaxf(r, -8.f), 7.f);
-    w |= (uint32_t)(q + 8) << (4 * (i >> 1) + 16 * (i & 1));
+    const float y = c[i] * id, r = __builtin_fmaf(__builtin_fmaf(-y, d, c[i]), id, y);
+    const float q = __builtin_rintf(__builtin_amdgcn_fmed3f(r, -8.f, 7.f));
+    half[i & 1] = __builtin_fmaf(q, (float)(1 << (4 * (i >> 1))), half[i & 1]);
   }
-  reinterpret_cast<uint32_t *>(tile)[j] = w;
+  reinterpret_cast<uint32_t *>(tile)[j] = (uint32_t)half[0] | (uint32_t)half[1] << 16;
   if (j == 0) *ds = d != 0.f ? __builtin_bit_cast(uint16_t, dh) : (uint16_t)0;
 }
 
@@ -265,10 +269,22 @@ write_quant_kernel(int8_t *__restrict__ kpool, int8_t *__restrict__ vpool, uint1
                 const float *__restrict__ k, const float *__restrict__ v, int64_t n, int64_t src_stride,
                 int kv_dim, int64_t n_slots, const int32_t *__restrict__ order, int64_t n_rows) {
   const int e8 = kv_dim >> 3;  // 8-element eighths of a K (or V) row
-  const int64_t gid = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t i = gid / (2 * e8);
+  int64_t i;
+  int u;
+  if constexpr (BITS == 4) {
+    // 16 rows by 16 lanes a work-group: rows of consecutive slots fill whole
+    // lines of the tiles together (one row a wave left 16-byte pieces of lines
+    // to work-groups of different XCDs)
+    const uint32_t across = (uint32_t)(2 * e8 + 15) / 16, rows16 = blockIdx.x / across;
+    i = (int64_t)rows16 * 16 + (threadIdx.x >> 4);
+    u = (int)((blockIdx.x - rows16 * across) * 16 + (threadIdx.x & 15));
+    if (u >= 2 * e8) return;
+  } else {
+    const int64_t gid = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    i = gid / (2 * e8);
+    u = (int)(gid - i * 2 * e8);
+  }
   if (i >= n) return;  // whole 4-lane groups leave together (2 e8 is a multiple of 4)
-  const int u = (int)(gid - i * 2 * e8);
   const int64_t row = order ? order[i] : i;  // write_kernel's order
   if (order && (row < 0 || row >= n_rows)) return;
   const int32_t s = slots[row];
@@ -4308,8 +4324,9 @@ hipError_t launch_write_quant(const PoolGeom &g, void *k_layer, void *v_layer, v
                               int64_t n, int64_t src_stride, hipStream_t s, const int32_t *order,
                               int64_t n_rows) {
   if (n <= 0) return hipSuccess;
-  const int64_t threads = n * (g.kv_dim >> 2);
-  const int64_t blocks = (threads + 255) / 256;
+  const int64_t lanes = g.kv_dim >> 2;  // of a row
+  const int64_t blocks =
+      g.elem == kElemQ4 ? (n + 15) / 16 * ((lanes + 15) / 16) : (n * lanes + 255) / 256;
   const auto kernel = g.elem == kElemQ4 ? write_quant_kernel<4> : write_quant_kernel<8>;
   kernel<<<(unsigned)blocks, 256, 0, s>>>(
       static_cast<int8_t *>(k_layer), static_cast<int8_t *>(v_layer), static_cast<uint16_t *>(k_scale),

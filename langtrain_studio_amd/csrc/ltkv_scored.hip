@@ -216,9 +216,14 @@ gather_values_kernel(const void *__restrict__ kpool, const void *__restrict__ vp
   const void *pool = is_v ? vpool : kpool, *scale = is_v ? vscale : kscale;
   float *dst = (is_v ? vout : kout) + (out_offsets[seq] + start) * kv_dim;
   const int per_row = (int)(kv_dim / VEC);
-  for (int u = (int)threadIdx.x; u < rows * per_row; u += kValuesThreads) {
-    const int slot = u / per_row;
-    const int64_t e = (int64_t)(u - slot * per_row) * VEC, cell = (int64_t)blk * 16 + slot;
+  int slot = (int)threadIdx.x / per_row, unit = (int)threadIdx.x - slot * per_row;
+  const int step = kValuesThreads / per_row, left = kValuesThreads - step * per_row;
+  for (; slot < rows; slot += step, unit += left) {
+    if (unit >= per_row) {
+      unit -= per_row;
+      if (++slot >= rows) break;
+    }
+    const int64_t e = (int64_t)unit * VEC, cell = (int64_t)blk * 16 + slot;
     float x[VEC];
     if constexpr (VEC == 4 && std::is_same_v<T, Q4>) {
       const int64_t at = (((cell >> 4) * (kv_dim >> 5) + (e >> 5)) << 4) + (cell & 15);
@@ -305,7 +310,8 @@ ScoredWorkspace scored_workspace(int elem, ScoredArgs &a) {
     const int64_t tiles = (a.n_rows + rows - 1) / rows * a.n_kv_heads, resident = 2 * a.cu_count;
     const int64_t over = tiles % resident;
     // (a few left over cost less than the merge of their splits)
-    if (over >= resident / 8 || tiles < resident) a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident / over, span / 256, 32}));
+    if (over >= resident / 8 || (over > 0 && tiles < resident))
+      a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident / over, span / 256, 32}));
     if (a.splits > 1) {
       // (slots may be empty: a sequence's tiles need not fill its slots)
       a.split_slots = (int)std::min<int64_t>((over + a.n_kv_heads - 1) / a.n_kv_heads + a.n, chunk_slots(a));
