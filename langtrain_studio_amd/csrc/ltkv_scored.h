@@ -282,7 +282,7 @@ hipError_t by_element(int elem, F &&f) {
 // Tokens per part of a row's visible positions (rounded up to 32-token steps;
 // a multiple of 64): a function of the row's own span, so that a decode
 // query's bits do not depend on its batch.
-constexpr int64_t kShortSpan = 2048, kLongSpan = 8192;
+constexpr int64_t kShortSpan = 1024, kLongSpan = 8192;
 __host__ __device__ inline int scored_part_tokens(int64_t span, int fixed) {
   if (fixed > 0) return fixed;
   return span <= kShortSpan ? 128 : span <= kLongSpan ? 256 : 512;
