@@ -393,15 +393,15 @@ struct ScoredArgs {
   int cu_count;
   int part_tokens;       // 0: the per-length policy of decode partitions
   // Set by scored_workspace: whether the chunk kernel takes sequences, whether
-  // the rows kernel takes rows one by one (not sequences), the most parts of a
+  // the rows kernel takes packs of rows (not sequences), the most parts of a
   // row there, and the chunk kernel's tile slots whose positions are split (the
   // first split_slots) over `splits` work-groups.
-  bool chunks, row_items;
+  bool chunks, packs;
   int max_parts, splits, split_slots;
   // Partials of rows split over their positions: part_o [slot][head][max_parts]
   // [head_dim], part_ml [slot][head][max_parts][2] (reference, sum), part_n
-  // [slot] parts used, a slot per row (row_items) or max_rows per sequence; the
-  // chunk kernel's with one per row of the split tile slots.
+  // [slot] parts used, a slot per row of the pack slots or max_rows per sequence;
+  // the chunk kernel's with one per row of the split tile slots.
   float *part_o, *part_ml;
   int32_t *part_n;
   float *chunk_o, *chunk_ml;

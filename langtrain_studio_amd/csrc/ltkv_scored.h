@@ -41,6 +41,12 @@ inline bool scored_chunks_supported(int elem, int head_dim, int group) {
   return elem != 4 && (head_dim == 64 || head_dim == 128) && group <= kChunkColumns;
 }
 inline int chunk_rows(const ScoredArgs &a) { return kChunkColumns / (a.n_heads / a.n_kv_heads); }
+// Rows that share a wave's 16 columns where the rows kernel takes whole chunks.
+__host__ __device__ inline int pack_rows(const ScoredArgs &a) {
+  const int group = a.n_heads / a.n_kv_heads;
+  return group <= 8 ? 16 / group : 1;
+}
+inline int64_t pack_slots(const ScoredArgs &a) { return a.n_rows / pack_rows(a) + a.n; }
 inline int64_t chunk_slots(const ScoredArgs &a) { return a.n_rows / chunk_rows(a) + a.n; }
 hipError_t launch_scored_chunks(const PoolGeom &g, const ScoredArgs &a, int64_t min_rows, hipStream_t s);
 
@@ -82,7 +88,8 @@ struct RowView {
   int32_t from;      // first position inside the window
   int32_t end;       // positions from here on are not visible
   __device__ __forceinline__ bool sees(int32_t t) const {
-    return t >= first && t < end && (t >= from || t < sink_end);
+    // (no short circuits: a select each, not branches)
+    return (t >= first) & (t < end) & ((t >= from) | (t < sink_end));
   }
 };
 
@@ -103,12 +110,23 @@ __device__ __forceinline__ RowView row_view(const ScoredArgs &a, const SeqRows &
   return v;
 }
 
-// Slots of the chunk kernel's tiles: those of sequence i begin at starts[i] /
+// Slots of the chunk kernel's tiles (and of the rows kernel's packs): those of sequence i begin at starts[i] /
 // rows_per_tile + i, which leaves room for all of its tiles whatever its first
 // row's place in a tile.
 __device__ __forceinline__ int64_t first_slot(const ScoredArgs &a, int64_t i, int rows_per_tile) {
   const int64_t st = a.row_starts[i];
   return (st < 0 ? 0 : st > a.n_rows ? a.n_rows : st) / rows_per_tile + i;
+}
+
+// Sequence of such a slot: the last one whose slots begin at or before it.
+__device__ __forceinline__ int64_t seq_of_slot(const ScoredArgs &a, int64_t slot, int rows_per_tile) {
+  int64_t lo = 0, hi = a.n;
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) / 2;
+    if (first_slot(a, mid, rows_per_tile) <= slot) lo = mid;
+    else hi = mid;
+  }
+  return lo;
 }
 
 // Sequence of launch row `row`: the last one whose first row is not behind it.

@@ -202,6 +202,11 @@ __device__ __forceinline__ int steps_per_part(const ScoredArgs &a, int n) {
   return (int64_t)per_part * a.max_parts < n ? (n + a.max_parts - 1) / a.max_parts : per_part;
 }
 
+// What a launch of the rows kernel takes: plain decode attention, one row per
+// sequence over its whole context; rows of short sequences with any scoring; or
+// packs of consecutive rows of a sequence, which share the columns.
+enum class Take { kDecode, kRows, kPacks };
+
 // Parts of a sequence of one row.
 template <bool MODS>
 __device__ __forceinline__ int parts_of(const ScoredArgs &a, int64_t seq) {
@@ -224,13 +229,15 @@ __device__ __forceinline__ int parts_of(const ScoredArgs &a, int64_t seq) {
 // tile 1: 4 quad ... + 3), so weights move between no lanes. V is transposed on
 // its way through LDS (ds_read_b64_tr_b16). Q and the weights enter as f16
 // hi + lo pairs: f32 accuracy for twice the matrix-core work, which is idle
-// here otherwise. MODS false: plain decode attention, one row per sequence over
-// its whole context.
+// here otherwise. A pack's steps that some row sees in part are taken once for
+// each row, with the other rows' columns masked and unseen values as zeros: no
+// row's values meet another's infinities.
 // OCC: waves a SIMD that the registers are cut to.
-template <typename T, int HDP, bool SPAN, bool MODS, int OCC>
+template <typename T, int HDP, bool SPAN, Take TAKE, int OCC>
 __global__ void __launch_bounds__(64 * kRowsWaves, OCC)
 scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tiles, int64_t waves, int64_t share,
                    int64_t most_rows) {
+  constexpr bool MODS = TAKE != Take::kDecode, PACK = TAKE == Take::kPacks;
   constexpr int NC = HDP / 32;     // chunks of 8 elements a lane, products per score tile
   constexpr int ND = HDP / 16;     // 16-element tiles of the numerators
   constexpr int PITCH = HDP * 2 + 32;  // bytes of a V row in LDS: rows of a read start 8 banks apart
@@ -251,7 +258,8 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
   // ones slowest, so that those past the end of shorter contexts come last. Many
   // (share > 0): every sequence has one row, and wave b of `share` takes the
   // b-th of as many equal stretches of all parts in sequence order.
-  const uint32_t items = (uint32_t)(MODS && a.row_items ? a.n_rows : a.n);
+  const int pack = PACK ? pack_rows(a) : 1;
+  const uint32_t items = (uint32_t)(PACK ? a.n_rows / pack + a.n : a.n);
   int64_t item = b % items;
   int p_first = (int)(b / items), p_count = 1;
   if (share > 0) {
@@ -290,43 +298,65 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
   }
   const int cols = min(16, group - head_tile * 16);
   const int head0 = kvh * group + head_tile * 16;
-  const bool live = col < cols;
+  const int sub = pack > 1 ? col / group : 0;  // the column's row of a pack
+  const int head = head0 + col - sub * group;
   const int64_t head_off = (int64_t)kvh * a.head_dim;
   char *const my = lds + wave * V_BYTES;
   const typename Cells<T, NC, SPAN>::Place place(a, kv_dim, head_off, col, quad);
 
-  // an item is a sequence, whose rows are taken one after the other, or a row
-  // (MODS false: every sequence has one row)
+  // an item is a sequence, whose rows are taken one after the other, or a pack
   for (int r_next = -1; p_count > 0;) {
-    const int64_t seq = MODS && a.row_items ? seq_of_row(a, item) : item;
+    const int64_t seq = PACK ? seq_of_slot(a, item, pack) : item;
     SeqRows rows = seq_rows(a, seq);
     if constexpr (!MODS) {
       rows.row0 = seq;
       rows.count = 1;
     }
-    if (MODS && a.row_items) {
-      if (item < rows.row0 || item >= rows.row0 + rows.count) return;
-      r_next = (int)(item - rows.row0);
-    } else {
-      ++r_next;
-    }
-    if (rows.count > most_rows || r_next >= rows.count) return;
+    if constexpr (PACK) r_next = (int)(item - first_slot(a, seq, pack)) * pack;
+    else ++r_next;
+    if (rows.count > most_rows || r_next < 0 || r_next >= rows.count) return;
     const int r = r_next;
+    const int n_pack = PACK ? min(pack, rows.count - r) : 1;
+    const bool live = PACK && pack > 1 ? sub < n_pack : col < cols;
     const int32_t *tab = table_of(a.tables, a.table_stride, a.rows, a.table_rows, seq);
     if (a.rows && p_first == 0 && rows.len > 0) {
       const int32_t t = scalar_read(a.rows, seq);
       if (t < 0 || t >= a.table_rows) report_fault(a.status, kFaultTable, seq);
     }
-    const RowView view = MODS ? row_view(a, rows, seq, r) : RowView{rows.len - 1, 0, 0, 0, rows.len};
+    // a pack: all that its rows see (seen), and what each of them sees (whole_*)
+    RowView view = MODS ? row_view(a, rows, seq, r) : RowView{rows.len - 1, 0, 0, 0, rows.len};
+    RowView seen = view;
+    int32_t whole_first = view.first, whole_from = view.from, whole_sink_end = view.sink_end, whole_end = view.end;
+    if constexpr (PACK)
+      for (int i = 1; i < n_pack; ++i) {
+        const RowView w = row_view(a, rows, seq, r + i);
+        whole_first = max(whole_first, w.first);
+        whole_from = max(whole_from, w.from);
+        whole_sink_end = min(whole_sink_end, w.sink_end);
+        whole_end = min(whole_end, w.end);
+        if (w.end <= w.first) continue;
+        if (seen.end <= seen.first) {
+          seen = w;
+          continue;
+        }
+        seen.first = min(seen.first, w.first);
+        seen.from = min(seen.from, w.from);
+        seen.sink_end = max(seen.sink_end, w.sink_end);
+        seen.end = max(seen.end, w.end);
+      }
+    const int32_t pos = view.pos + sub;  // of the column's row
     const StepRange<32> range =
-        MODS ? step_range<32>(view) : StepRange<32>{0, 0, 0, rows.len, 0, (rows.len + 31) / 32};
+        MODS ? step_range<32>(seen) : StepRange<32>{0, 0, 0, rows.len, 0, (rows.len + 31) / 32};
     int per_part = steps_per_part(a, range.n);
     // no memory for the parts of rows past the expected most: one part
-    const bool parted = !MODS || a.row_items || r < a.max_rows;
+    const bool parted = !MODS || PACK || r < a.max_rows;
     if (!parted) per_part = max(range.n, 1);
     const int n_parts = range.n > per_part ? (range.n + per_part - 1) / per_part : 1;
-    const int64_t row = rows.row0 + r, slot = !MODS || a.row_items ? row : seq * a.max_rows + r;
-    if (a.part_n && parted && p_first == 0 && kvh == 0 && head_tile == 0 && lane == 0) a.part_n[slot] = n_parts;
+    const int64_t row = rows.row0 + r + sub;  // the column's
+    const int64_t slot = PACK ? item * pack + sub : MODS ? seq * a.max_rows + r : row;
+    if (a.part_n && parted && p_first == 0 && kvh == 0 && head_tile == 0 &&
+        (PACK ? live && quad == 0 && head == 0 : lane == 0))
+      a.part_n[slot] = n_parts;
     int part = p_first;
     // this item's stretch, and what follows it
     const int here = min(p_count, n_parts - p_first);
@@ -335,7 +365,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
       p_first = 0;
       ++item;
       r_next = -1;
-    } else if (MODS && a.row_items) {
+    } else if (PACK) {
       p_count = 0;
     }
     if (here <= 0) continue;
@@ -385,7 +415,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
     float qscale;
     {
       float x[NC][8], amax = 0.f;
-      const int64_t at = (row * a.n_heads + head0 + col) * (int64_t)a.head_dim;
+      const int64_t at = (row * a.n_heads + head) * (int64_t)a.head_dim;
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
         const int e = chunk_of<NC, SPAN>(quad, j) * 8;
@@ -410,7 +440,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
     const bool cap = MODS && a.softcap > 0.f;
     const float in_scale = cap ? qscale / a.softcap : qscale * kLog2e;
     const float cap_scale = a.softcap * kLog2e;
-    const float slope = MODS && a.slopes && live ? a.slopes[head0 + col] * kLog2e : 0.f;
+    const float slope = MODS && a.slopes && live ? a.slopes[head] * kLog2e : 0.f;
 
     f32x4 o[ND];
     float ref, sum, lift, scale_top;
@@ -433,7 +463,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
       }
       const float total = rows_reduce<false>(sum);
       if (!live) return;
-      const int64_t rh = row * a.n_heads + head0 + col;
+      const int64_t rh = row * a.n_heads + head;
       if (n_parts == 1) {
         const float inv = total != 0.f ? 1.f / total : 0.f;
 #pragma unroll
@@ -442,7 +472,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
             store_row4(a, rh * a.head_dim + 16 * i + 4 * quad, o[i] * inv);
         return;
       }
-      const int64_t at = (slot * a.n_heads + head0 + col) * a.max_parts + part;
+      const int64_t at = (slot * a.n_heads + head) * a.max_parts + part;
       float *dst = a.part_o + at * a.head_dim + 4 * quad;
 #pragma unroll
       for (int i = 0; i < ND; ++i)
@@ -453,12 +483,20 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
       }
     };
 
-    auto step = [&](int s) {
+    int turn = 0;  // row of a pack that a step in part is taken for
+    auto step = [&](int s) {  // true: done
       const int32_t t0 = range.start(s), t_end = range.end(s);
+      const bool whole = t0 + 32 <= (PACK ? min(t_end, whole_end) : t_end) && t0 >= whole_first &&
+                         (t0 >= whole_from || t0 + 32 <= whole_sink_end);
+      auto visible = [&](int32_t t) { return MODS ? view.sees(t) & (t < t_end) : t < t_end; };
+      const bool again = PACK && !whole && turn + 1 < n_pack;
+      const bool mine = !PACK || whole || sub == turn;
+      if constexpr (PACK)
+        if (!whole) view = row_view(a, rows, seq, r + turn);
+      turn = again ? turn + 1 : 0;
       // always loaded, so that the loads in flight are counted exactly: past the
       // end the last step again
-      const int s_next = min(s + 1, s_end - 1);
-      const bool whole = t0 + 32 <= t_end && t0 >= view.first && (t0 >= view.from || t0 + 32 <= view.sink_end);
+      const int s_next = again ? s : min(s + 1, s_end - 1);
       if (s_next - entry_step == 32) fill(s_next);
       find(s_next);
       // f32: powers of two that bring K and V below 2^kTopExp (positions that the
@@ -469,7 +507,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int32_t t = t0 + 16 * u + col;
-            if (!(view.sees(t) && t < t_end)) {
+            if (!visible(t)) {
               k[u].clear();
               v[u].clear();
             }
@@ -500,7 +538,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int32_t t = t0 + 16 * u + col;
-        const bool seen = whole || (view.sees(t) && t < t_end);
+        const bool seen = whole || visible(t);
         if constexpr (F32) {
 #pragma unroll
           for (int j = 0; j < NC; ++j) {
@@ -531,7 +569,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int32_t t = t0 + 16 * u + 4 * quad + i;
-                if (!(view.sees(t) && t < t_end)) dv[u][j][i] = (_Float16)0.f;
+                if (!visible(t)) dv[u][j][i] = (_Float16)0.f;
               }
           }
       }
@@ -587,7 +625,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
           float y = (Q8 ? c[u][i] : c[u][i] + cl[u][i]) * to_y;
           if constexpr (MODS) {
             if (cap) y = tanh_f32(y) * cap_scale;
-            y = __builtin_fmaf(-slope, (float)abs(view.pos - (t0 + 16 * u + 4 * quad + i)), y);
+            y = __builtin_fmaf(-slope, (float)abs(pos - (t0 + 16 * u + 4 * quad + i)), y);
           }
           c[u][i] = y;
         }
@@ -597,7 +635,11 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int32_t t = t0 + 16 * u + 4 * quad + i;
-            if (!(view.sees(t) && t < t_end)) c[u][i] = -INFINITY;
+            if constexpr (!MODS) {
+              if (!(t < t_end)) c[u][i] = -INFINITY;
+            } else {
+              c[u][i] = (mine & visible(t)) ? c[u][i] : -INFINITY;
+            }
           }
       float top = __builtin_fmaxf(__builtin_fmaxf(c[0][0], c[0][1]), __builtin_fmaxf(c[0][2], c[0][3]));
       top = __builtin_fmaxf(
@@ -636,6 +678,14 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
         w[i] = __builtin_amdgcn_exp2f(c[i >> 2][i & 3] - base);
         sum += w[i];
       }
+      // a column whose row is not taken keeps its numerators: values that another
+      // row sees may be infinite, and zero weights would not hide that
+      auto keep = [&](f32x4 &to, const f32x4 &x) {
+        if constexpr (!PACK) to = x;
+        else
+#pragma unroll
+          for (int e = 0; e < 4; ++e) to[e] = mine ? x[e] : to[e];
+      };
       h8 wh, wl;
       if constexpr (!Q8) {
 #pragma unroll
@@ -649,9 +699,17 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
 #pragma unroll
           for (int i = 0; i < ND; ++i) {
             const h8 hi = read_tr2(my_t + 32 * i, 16 * PITCH), lo = read_tr2(my_t + 32 * PITCH + 32 * i, 16 * PITCH);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wh, o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wl, o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wh, o[i], 0, 0, 0);
+            f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wh, o[i], 0, 0, 0);
+            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wl, x, 0, 0, 0);
+            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wh, x, 0, 0, 0);
+            keep(o[i], x);
+          }
+        } else if constexpr (PACK) {
+#pragma unroll
+          for (int i = 0; i < ND; ++i) {
+            f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], wh, o[i], 0, 0, 0);
+            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], wl, x, 0, 0, 0);
+            keep(o[i], x);
           }
         } else {
 #pragma unroll
@@ -671,17 +729,24 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
               wl[e] = lo;
             }
           }
-          o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], wh, o[i], 0, 0, 0);
-          o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], wl, o[i], 0, 0, 0);
+          f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], wh, o[i], 0, 0, 0);
+          x = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[i], wl, x, 0, 0, 0);
+          keep(o[i], x);
         }
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      return !again;
     };
 
     reset();
     int left = per_part;  // steps until the part ends
     for (int s = s_first; s < s_end; ++s) {
-      step(s);
+      if constexpr (PACK) {
+        while (!step(s)) {
+        }
+      } else {
+        step(s);
+      }
       if (--left == 0 && s + 1 < s_end) {
         flush();
         reset();
@@ -699,14 +764,15 @@ hipError_t launch_rows_t(const PoolGeom &g, const ScoredArgs &a, int64_t most_ro
   constexpr int occ = HDP <= 64 ? 3 : HDP <= 128 ? (std::is_same_v<T, Q4> ? 3 : 2) : 1;
   // a wave for each possible part, or all parts shared by as many as are resident
   const int64_t lanes = (int64_t)a.n_kv_heads * head_tiles, slots = std::max<int64_t>(a.cu_count * 4 * occ / lanes, 1);
-  int64_t waves = (a.row_items ? a.n_rows : a.n) * a.max_parts, share = 0;
+  int64_t waves = (a.packs ? pack_slots(a) : a.n) * a.max_parts, share = 0;
   if (waves > slots && !a.row_starts) waves = share = slots;
   waves *= lanes;
   const int64_t wgs = (waves + kRowsWaves - 1) / kRowsWaves;
   if (wgs * 64 * kRowsWaves >= (int64_t{1} << 32)) return hipErrorInvalidValue;
   const bool mods = a.softcap > 0.f || a.slopes || a.window > 0 || a.prefix || a.first || a.row_starts;
-  const auto kernel =
-      mods ? scored_rows_kernel<T, HDP, SPAN, true, occ> : scored_rows_kernel<T, HDP, SPAN, false, occ>;
+  const auto kernel = a.packs ? scored_rows_kernel<T, HDP, SPAN, Take::kPacks, occ>
+                      : mods  ? scored_rows_kernel<T, HDP, SPAN, Take::kRows, occ>
+                              : scored_rows_kernel<T, HDP, SPAN, Take::kDecode, occ>;
   kernel<<<(unsigned)wgs, 64 * kRowsWaves, 0, s>>>(a, g.n_blocks, g.kv_dim, head_tiles, waves, share, most_rows);
   return hipGetLastError();
 }
