@@ -301,7 +301,13 @@ ScoredWorkspace scored_workspace(int elem, ScoredArgs &a) {
   a.split_slots = 0;
   const int64_t span = span_bound(a);
   int64_t at = 0;
-  if (k.rows && (a.max_parts = (int)scored_max_parts(span, a.part_tokens)) > 1) {
+  if (k.rows) a.max_parts = (int)scored_max_parts(span, a.part_tokens);
+  // packs are many where a chunk is long: no more parts than fill the chip a few
+  // times (they cost partials)
+  if (a.packs)
+    a.max_parts = (int)std::max<int64_t>(
+        1, std::min<int64_t>(a.max_parts, 32 * a.cu_count / (pack_slots(a) * a.n_kv_heads)));
+  if (a.max_parts > 1) {
     const int64_t slots = a.packs ? pack_slots(a) * pack_rows(a) : a.n * a.max_rows, parts = slots * a.n_heads * (int64_t)a.max_parts;
     w.part_o_off = at;
     w.part_ml_off = at + parts * a.head_dim * 4;
