@@ -9,6 +9,8 @@ import os
 import shlex
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
@@ -35,38 +37,58 @@ COMMON = ["-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wno-un
 VERSION_SCRIPT = os.path.join(CSRC, "ltkv.map")
 
 
-def command(timeline: bool = False) -> list[str]:
-    out = TIMELINE_LIB if timeline else LIB
+def compile_command(source: str, obj: str, timeline: bool) -> list[str]:
     return [HIPCC, f"--offload-arch={ARCH}", *COMMON, *DEVICE_FLAGS, *(["-DLTKV_TIMELINE"] if timeline else []),
-            "-shared", f"-Wl,--version-script={VERSION_SCRIPT}", "-o", out, *SOURCES]
+            "-c", source, "-o", obj]
+
+
+def link_command(objects: list[str], out: str) -> list[str]:
+    return [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", f"-Wl,--version-script={VERSION_SCRIPT}", "-o", out,
+            *objects]
+
+
+def run(cmd: list[str], verbose: bool) -> str:
+    """Runs a compiler command; an error text, or nothing."""
+    if verbose:
+        print("+", " ".join(shlex.quote(c) for c in cmd), flush=True)
+    proc = subprocess.run(cmd, stderr=subprocess.PIPE, stdout=subprocess.DEVNULL, text=True)
+    # hipcc's host pass warns that it does not know the packed-fp32 feature: harmless.
+    noise = ("packed-fp32-ops", "not a recognized feature", "warning: unknown target feature")
+    err = "\n".join(l for l in proc.stderr.splitlines() if not any(n in l for n in noise))
+    if proc.returncode != 0:
+        return f"hipcc failed ({proc.returncode}) for {os.path.basename(cmd[-1])}:\n{err}"
+    if verbose and err.strip():
+        print(err, file=sys.stderr)
+    return ""
 
 
 def build(verbose: bool = True, timeline: bool = True) -> str:
     """Compile every source into libltkv.so (always recompiles), and the
-    profiling build libltkv_timeline.so beside it (in parallel)."""
-    jobs = []
-    for tl in ((False, True) if timeline else (False,)):
-        cmd = command(tl)
-        out = TIMELINE_LIB if tl else LIB
-        if verbose:
-            print("+", " ".join(shlex.quote(c) for c in cmd), flush=True)
-        tmp = out + ".tmp"
-        cmd[cmd.index(out)] = tmp
-        jobs.append((subprocess.Popen(cmd, stderr=subprocess.PIPE, stdout=subprocess.DEVNULL, text=True), tmp, out))
-    # hipcc's host pass warns that it does not know the packed-fp32 feature: harmless.
-    noise = ("packed-fp32-ops", "not a recognized feature", "warning: unknown target feature")
-    failed = []
-    for proc, tmp, out in jobs:
-        stderr = proc.communicate()[1]
-        err = "\n".join(l for l in stderr.splitlines() if not any(n in l for n in noise))
-        if proc.returncode != 0:
-            failed.append(f"hipcc failed ({proc.returncode}) for {os.path.basename(out)}:\n{err}")
-            continue
-        if verbose and err.strip():
-            print(err, file=sys.stderr)
-        os.replace(tmp, out)
-    if failed:
-        raise RuntimeError("\n".join(failed))
+    profiling build libltkv_timeline.so beside it: every source by itself, as
+    many at a time as there are processors (at most 8). Sources without phase
+    stamps serve both libraries."""
+    with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+        objects: dict[bool, list[str]] = {False: [], True: []}
+        jobs = []
+        for source in sorted(SOURCES, key=os.path.getsize, reverse=True):  # the longest first
+            with open(source) as f:
+                stamped = "LTKV_TIMELINE" in f.read()
+            for tl in (False, True) if stamped and timeline else (False,):
+                obj = os.path.join(tmp, os.path.basename(source) + (".timeline.o" if tl else ".o"))
+                jobs.append(pool.submit(run, compile_command(source, obj, tl), verbose))
+                objects[tl].append(obj)
+                if not stamped:
+                    objects[True].append(obj)
+        failed = [e for e in (job.result() for job in jobs) if e]
+        for tl in (False, True) if timeline else (False,):
+            out = TIMELINE_LIB if tl else LIB
+            if not failed and (e := run(link_command(objects[tl], out + ".tmp"), verbose)):
+                failed.append(e)
+        if failed:
+            raise RuntimeError("\n".join(failed))
+        for tl in (False, True) if timeline else (False,):
+            out = TIMELINE_LIB if tl else LIB
+            os.replace(out + ".tmp", out)
     return LIB
 
 
