@@ -1877,6 +1877,9 @@ int ltkv_scored_attention(ltkv_cache *c, size_t layer, size_t n, size_t n_rows, 
   if (table_stride == 0) return fail(LTKV_ERR_ARG, "table_stride must be > 0");
   if (!d_q || !d_tables || !d_lens || !d_out) return fail(LTKV_ERR_ARG, "null device pointer");
   if (((uintptr_t)d_q | (uintptr_t)d_out) % 16 != 0) return fail(LTKV_ERR_ARG, "q and out must be 16-byte aligned");
+  const uintptr_t bytes = n_rows * n_heads * head_dim * (row_type == LTKV_ROWS_F32 ? 4 : 2);
+  if ((uintptr_t)d_q < (uintptr_t)d_out + bytes && (uintptr_t)d_out < (uintptr_t)d_q + bytes)
+    return fail(LTKV_ERR_ARG, "q and out overlap: rows are read after others are written");
   DeviceGuard dg(c->device);
   if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
   const size_t max_len = table_stride >= (size_t)INT32_MAX / LTKV_BLOCK ? (size_t)INT32_MAX : table_stride * LTKV_BLOCK;

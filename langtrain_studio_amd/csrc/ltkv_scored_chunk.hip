@@ -292,7 +292,9 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
     qscale = __builtin_amdgcn_ldexpf(a.scale, -up);
   }
   const bool cap = a.softcap > 0.f;
-  const float in_scale = cap ? qscale / a.softcap : qscale * kLog2e;
+  // (finite for the smallest caps: a score of zero stays zero)
+  const float in_scale =
+      cap ? __builtin_amdgcn_fmed3f(qscale / a.softcap, -1e37f, 1e37f) : qscale * kLog2e;
   const float cap_scale = a.softcap * kLog2e;
   const float slope = a.slopes && live ? a.slopes[head] * kLog2e : 0.f;
   // scores are an affine function of the products (or of the capped rows' c),

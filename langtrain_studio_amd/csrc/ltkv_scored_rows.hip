@@ -438,7 +438,9 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
       qscale = __builtin_amdgcn_ldexpf(a.scale, -up);
     }
     const bool cap = MODS && a.softcap > 0.f;
-    const float in_scale = cap ? qscale / a.softcap : qscale * kLog2e;
+    // (finite for the smallest caps: a score of zero stays zero)
+    const float in_scale =
+        cap ? __builtin_amdgcn_fmed3f(qscale / a.softcap, -1e37f, 1e37f) : qscale * kLog2e;
     const float cap_scale = a.softcap * kLog2e;
     const float slope = MODS && a.slopes && live ? a.slopes[head] * kLog2e : 0.f;
 

@@ -304,3 +304,34 @@ def test_a_sequences_life(gpu, dtype):
             plain, _ = run(kv, q, tables, lens, heads, hd)
             np.testing.assert_array_equal(plain, dec.cpu().numpy())
     assert kv.cow_copies() > 0
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32", "q8_0", "q4_0"])
+@pytest.mark.parametrize("rows", ["f32", "f16"])
+@pytest.mark.parametrize("new", [[1, 1], [40, 33]])
+def test_the_smallest_caps(gpu, dtype, rows, new):
+    """Caps so small that a score over the cap is no number: the weights are
+    equal, also where q.k is exactly zero."""
+    heads, kvh, hd, lens = 8, 2, 64, [300, 50]
+    starts = np.concatenate([[0], np.cumsum(new)])
+    kv, tables = build(kvh * hd, lens, dtype, 47)
+    q = np.random.default_rng(48).standard_normal((starts[-1], heads * hd)).astype(np.float32)
+    q[0] = 0
+    for softcap in (1e-45, 1e-38, 1e-20):
+        got, qr = run(kv, q, tables, lens, heads, hd, rows=rows, starts=starts, max_rows=max(new), softcap=softcap)
+        check(got, expect(np.zeros_like(qr), held_rows(kv), tables, lens, starts, heads, hd), rows)
+
+
+def test_q_and_out_lie_apart(gpu):
+    import torch
+
+    from langtrain_studio_amd import KvError
+
+    heads, kvh, hd = 4, 2, 64
+    kv, tables = build(kvh * hd, [20, 20], "f16", 49)
+    both = torch.zeros((3, heads * hd), device="cuda")
+    t, ld = up(tables, np.int32), up([20, 20], np.int32)
+    for out in (both[:2], both[1:]):
+        with pytest.raises(KvError, match="overlap"):
+            kv.scored_attention(0, both[:2], t, ld, heads, hd, out=out)
+    kv.synchronize()
