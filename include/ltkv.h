@@ -97,7 +97,12 @@ LTKV_API const char *ltkv_last_error(void);
  * not count it): a quarter of one layer's rows, at least 1 and at most 16
  * MiB, from its creation (none if the device has no room left beside the
  * pools); 32 MiB more from the first small launch that it does not suffice
- * for; and a workspace for larger launches, grown on demand. */
+ * for; and a workspace for larger launches, grown on demand. Scored attention
+ * and Q4_0 decodes keep partials that the first does not suffice for in memory
+ * that grows on demand too, but an outgrown piece stays until ltkv_destroy (a
+ * captured launch may still use it), and a call under stream capture that would
+ * have to grow it is refused with LTKV_ERR_ARG: make the call once before
+ * capturing it. */
 LTKV_API int ltkv_create(size_t n_layers, size_t kv_dim, size_t n_tokens, int dtype, int device,
                 ltkv_cache **out);
 LTKV_API void ltkv_destroy(ltkv_cache *c);
@@ -243,7 +248,8 @@ LTKV_API int ltkv_gather_values(ltkv_cache *c, size_t layer, size_t n, const int
  * [n][n_heads*head_dim] f32. Any group size and head_dim <= 1024: head_dim
  * 64 or 128 with groups of 1..8 take the tuned kernels, other f16 shapes with
  * head_dim a multiple of 8 up to 256 a matrix-core kernel of their own, the
- * rest a generic one (one work-group per query head, whole contexts).
+ * rest a generic one (one work-group per query head, whole contexts). Q4_0
+ * pools: any head_dim that is a multiple of 8 up to 256 on the matrix cores.
  * d_lens[i] == 0 yields zeros. A table entry outside the pool is read as
  * block 0 and reported by ltkv_synchronize (the reference panics, kv.rs:147).
  * Q may have any finite magnitude, as the reference's f32 scores allow
@@ -272,7 +278,9 @@ LTKV_API int ltkv_decode_attention(ltkv_cache *c, size_t layer, size_t n, size_t
  * longest context the tables hold (T = table_stride * 16 tokens): 4 up to
  * 4096 tokens, ceil(T / 1024) beyond (or ceil(T / the size fixed with
  * ltkv_set_attention_partition)), doubled on Q8_0 pools whose kv heads
- * pair up with at most 4 query heads each. Every
+ * pair up with at most 4 query heads each; on Q4_0 pools P is (T + 32) / 128 up
+ * to 992 tokens, the larger of 8 and (T + 32) / 256 up to 8160, of 32 and
+ * (T + 32) / 512 beyond, rounded up, and a query takes up to 260 bytes more. Every
  * call on a device shares that device's scratch: calls that overlap on one
  * device (other streams, other threads, caches on the same device) race.
  * No counterpart in the reference: for callers that cannot allocate (code
@@ -331,10 +339,12 @@ LTKV_API int ltkv_append_decode_attention(ltkv_cache *c, size_t layer, size_t n,
  * sees an infinity or NaN gives values that are not finite).
  * f32 rows are computed to f32 accuracy; f16 and bf16 rows take Q as it is
  * and weights rounded to f16, summed in f32.
- * max_rows: the most rows of one sequence, which chooses the kernels; one with
- * more rows is computed all the same. Rows before the first start or behind
+ * max_rows: the most rows of one sequence, which chooses the kernels (one with
+ * more rows is computed all the same): on the matrix cores head_dim that is a
+ * multiple of 8 up to 256 (f32 pools: up to 128; Q8_0: 32, 64, 96, 128, 192,
+ * 256), prompt chunks fastest at head_dim 64 and 128 on pools other than f32. Rows before the first start or behind
  * the last are left as they were. Tables, lengths and faults as
- * ltkv_decode_attention; q and out 16-byte aligned; head_dim up to 1024.
+ * ltkv_decode_attention; q and out 16-byte aligned and apart; head_dim up to 1024.
  * Summation orders depend on the call's shape, not only on a row's own length.
  * No reference counterpart: the reference's models have neither (model.rs:431-475
  * is plain causal attention). */
@@ -350,6 +360,9 @@ LTKV_API int ltkv_scored_attention(ltkv_cache *c, size_t layer, size_t n, size_t
  * four partitions of ceil(len/4) rounded up to 64 tokens (at least 64) up to
  * 4096 tokens, and into 1024-token partitions beyond; on f16 pools (the
  * matrix-core engine) the 1024-token partitions start beyond 2048 tokens.
+ * Q4_0 decodes and scored attention's single tokens take partitions of 128
+ * tokens up to 1024 visible positions (rounded up to steps of 32), of 256 up to
+ * 8192 and of 512 beyond.
  * Either way a query's result depends only on its own inputs, the cache's
  * shape and its engine, never on the rest of the batch. Tuning knob. */
 LTKV_API int ltkv_set_attention_partition(ltkv_cache *c, size_t tokens);

@@ -32,7 +32,8 @@ constexpr int kAnyD = kAnyMaxHeadDim / kAnyThreads;
 // one score a thread, the softmax of the round against the running maximum
 // (exp2 domain), then each thread accumulates up to four output elements over
 // the round's positions. Positions a row does not see are skipped, not
-// multiplied by zero: they may hold infinities or NaN.
+// multiplied by zero: they may hold infinities or NaN. It serves shapes that
+// the matrix-core kernels do not, and is bound by its scalar loads.
 template <typename T>
 __global__ void __launch_bounds__(kAnyThreads) scored_any_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim) {
   __shared__ float sq[kAnyMaxHeadDim];
@@ -195,7 +196,9 @@ __global__ void __launch_bounds__(kMergeThreads) scored_merge_kernel(ScoredArgs 
 
 // Rows of a block as f32 values: a work-group per (table entry, K or V), four
 // elements a thread and 16-byte stores (one element where kv_dim is not a
-// multiple of four), consecutive threads on consecutive elements of a row.
+// multiple of four), consecutive threads on consecutive elements of a row. ~9 500
+// q4_0 rows of 2 x 1024 elements: 18.8 us (89 MB, 4.7 TB/s), bound by the
+// stores; stores past the caches (nontemporal) took 21 us.
 constexpr int kValuesThreads = 256;
 
 template <typename T, int VEC>
@@ -308,7 +311,8 @@ ScoredWorkspace scored_workspace(int elem, ScoredArgs &a) {
     a.max_parts = (int)std::max<int64_t>(
         1, std::min<int64_t>(a.max_parts, 32 * a.cu_count / (pack_slots(a) * a.n_kv_heads)));
   if (a.max_parts > 1) {
-    const int64_t slots = a.packs ? pack_slots(a) * pack_rows(a) : a.n * a.max_rows, parts = slots * a.n_heads * (int64_t)a.max_parts;
+    const int64_t slots = a.packs ? pack_slots(a) * pack_rows(a) : a.n * a.max_rows;
+    const int64_t parts = slots * a.n_heads * (int64_t)a.max_parts;
     w.part_o_off = at;
     w.part_ml_off = at + parts * a.head_dim * 4;
     w.part_n_off = w.part_ml_off + parts * 2 * 4;

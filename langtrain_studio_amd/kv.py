@@ -336,7 +336,8 @@ class KvCache:
         the first `sinks`. prefix (int32 [n]): positions every row of the
         sequence sees. first (int32 [n_rows]): the first position of the row's
         document. max_rows: the most rows of one sequence (a hint; default: as
-        many as there are). Rows of no sequence are left as they were."""
+        many as there are). Rows of no sequence are left as they were (zeros in a
+        new out)."""
         import torch
 
         n = lens.numel()
