@@ -112,19 +112,24 @@ __global__ void __launch_bounds__(kAnyThreads) scored_any_kernel(ScoredArgs a, i
 }
 
 // Rows whose positions were taken in several parts (or splits): their numerators
-// and sums folded in order by their references. A work-group per 256 elements
-// of a row: first the part slots of the rows kernel (ScoredArgs::part_n), then
-// the rows of the chunk kernel's split tile slots.
-// ROWS: only part slots of sequences' rows (two searches less to carry: decode
-// batches' folds 7.9 -> 5.9 us).
+// and sums folded in order by their references. VEC elements of a row a thread:
+// first the part slots of the rows kernel (ScoredArgs::part_n), then the rows of
+// the chunk kernel's split tile slots.
+// ROWS: only part slots of sequences' rows: a thread an element, 16 parts' loads
+// at a time, since latency counts (one context's fold 4.6 us, 5.8 with four
+// elements a thread), and no searches. Else four elements a thread: the splits
+// are many (27 -> 15 us for six chunks of 512 rows).
 constexpr int kMergeThreads = 256;
+constexpr int merge_vec(bool rows) { return rows ? 1 : 4; }
 
 template <bool ROWS>
 __global__ void __launch_bounds__(kMergeThreads) scored_merge_kernel(ScoredArgs a, int slices, int64_t part_slots,
                                                                      int64_t min_rows, int rows_per_tile) {
+  constexpr int VEC = merge_vec(ROWS), AHEAD = ROWS ? 16 : 8;
+  using vec = std::conditional_t<ROWS, float, f32x4>;
   const int64_t item = blockIdx.x / (uint32_t)slices;
-  const int i = (int)(blockIdx.x % (uint32_t)slices) * kMergeThreads + (int)threadIdx.x;
-  if (i >= a.n_heads * a.head_dim) return;
+  const int i = ((int)(blockIdx.x % (uint32_t)slices) * kMergeThreads + (int)threadIdx.x) * VEC;
+  if (i >= a.n_heads * a.head_dim) return;  // (head_dim is a multiple of 8 here)
   const int h = i / a.head_dim, e = i - h * a.head_dim;
   // row of a slot of the tiles (or packs), -1 for slots that no kernel took
   auto slot_row = [&](int64_t slot) -> int64_t {
@@ -165,33 +170,38 @@ __global__ void __launch_bounds__(kMergeThreads) scored_merge_kernel(ScoredArgs 
   const int64_t at = (slot * a.n_heads + h) * stride;
   ml += 2 * at;
   o += at * a.head_dim + e;
-  // eight parts' loads at a time, folded one by one in order
-  float mx = -INFINITY, l = 0.f, x = 0.f;
-  for (int p0 = 0; p0 < n_parts; p0 += 8) {
-    float pm[8], pl[8], po[8];
+  // AHEAD parts' loads at a time, folded one by one in order
+  float mx = -INFINITY, l = 0.f;
+  vec x = {};
+  for (int p0 = 0; p0 < n_parts; p0 += AHEAD) {
+    float pm[AHEAD], pl[AHEAD];
+    vec po[AHEAD];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < AHEAD; ++k) {
       const int p = p0 + k < n_parts ? p0 + k : n_parts - 1;
       const f32x2 v = *reinterpret_cast<const f32x2 *>(ml + 2 * p);
+      po[k] = *reinterpret_cast<const vec *>(o + (int64_t)p * a.head_dim);
       pm[k] = p0 + k < n_parts ? v.x : -INFINITY;
       pl[k] = p0 + k < n_parts ? v.y : 0.f;
-      po[k] = p0 + k < n_parts ? o[(int64_t)p * a.head_dim] : 0.f;
+      if (p0 + k >= n_parts) po[k] = vec{};
     }
     float next = mx;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) next = __builtin_fmaxf(next, pm[k]);
+    for (int k = 0; k < AHEAD; ++k) next = __builtin_fmaxf(next, pm[k]);
     const float base = next == -INFINITY ? 0.f : next, f = __builtin_amdgcn_exp2f(mx - base);
     l *= f;
     x *= f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < AHEAD; ++k) {
       const float g = __builtin_amdgcn_exp2f(pm[k] - base);
       l = __builtin_fmaf(pl[k], g, l);
-      x = __builtin_fmaf(po[k], g, x);
+      x += po[k] * g;
     }
     mx = next;
   }
-  row_store(a, row * a.n_heads * a.head_dim + i, l != 0.f ? x / l : 0.f);
+  x = l != 0.f ? x / l : vec{};
+  if constexpr (ROWS) row_store(a, row * a.n_heads * a.head_dim + i, x);
+  else store_row4(a, row * a.n_heads * a.head_dim + i, x);
 }
 
 // Rows of a block as f32 values: a work-group per (table entry, K or V), four
@@ -362,9 +372,11 @@ hipError_t launch_scored_attention(const PoolGeom &g, const ScoredArgs &a, hipSt
   const int rows_per_tile = a.chunks ? chunk_rows(a) : pack_rows(a);
   const int64_t items = part_slots + (int64_t)a.split_slots * rows_per_tile;
   if (items == 0) return hipSuccess;
-  const int slices = (a.n_heads * a.head_dim + kMergeThreads - 1) / kMergeThreads;
+  const bool rows_only = !a.packs && a.split_slots == 0;
+  const int per_group = kMergeThreads * merge_vec(rows_only);
+  const int slices = (a.n_heads * a.head_dim + per_group - 1) / per_group;
   if (items * slices * kMergeThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
-  const auto merge = a.packs || a.split_slots ? scored_merge_kernel<false> : scored_merge_kernel<true>;
+  const auto merge = rows_only ? scored_merge_kernel<true> : scored_merge_kernel<false>;
   merge<<<(unsigned)(items * slices), kMergeThreads, 0, s>>>(a, slices, part_slots, border, rows_per_tile);
   return hipGetLastError();
 }
