@@ -446,6 +446,7 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
     // scores of positions t0 + 32 u + 8 (i / 4) + 4 half + i % 4
     f32x16 c[2] = {};
     const char *kp = lds_k + col * K_PITCH + 16 * half;
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int j = 0; j < NK; ++j) {
 #pragma unroll
@@ -459,16 +460,15 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
         }
       }
     }
-    const float to_x = Q8 ? __builtin_amdgcn_ldexpf(in_scale, k_exp) : in_scale;
+    __builtin_amdgcn_s_setprio(0);
     const int32_t tl = t0 + 4 * half;
     // Scores in the log2 domain as m c + m0: the multiplication is left to the
     // fused one before exp2. Capped rows of 16 bits take c = 1 / (exp(2 x) + 1),
     // since cap tanh(x) = cap - 2 cap c: five instructions a score.
-    float m = 1.f, m0 = 0.f;
+    float m = Q8 ? __builtin_amdgcn_ldexpf(in_scale, k_exp) : in_scale, m0 = 0.f;
     if (affine) {
-      m = to_x;
       if (cap) {
-        const float to_e = to_x * (2.f * kLog2e);
+        const float to_e = m * (2.f * kLog2e);
 #pragma unroll
         for (int i = 0; i < 32; ++i)
           c[i >> 4][i & 15] = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(c[i >> 4][i & 15] * to_e) + 1.f);
@@ -476,6 +476,8 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
         m0 = cap_scale;
       }
     } else {
+      float to_x = m;  // opaque: the products would be taken before the branch, for both sides
+      asm("" : "+v"(to_x));
       if (cap) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
@@ -492,13 +494,14 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
       for (int i = 0; i < 32; ++i)
         c[i >> 4][i & 15] =
             __builtin_fmaf(-slope, __builtin_fabsf(d0 - (float)(8 * (i / 4) + i % 4)), c[i >> 4][i & 15]);
+      m = 1.f;
     }
     if (t0 + kChunkTokens > t_end || !wb.all(t0, kChunkTokens)) {
       const float none = falling ? INFINITY : -INFINITY;
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         const int32_t t = tl + 8 * (i / 4) + i % 4;
-        if (!(view.sees(t) && t < t_end)) c[i >> 4][i & 15] = none;
+        c[i >> 4][i & 15] = (view.sees(t) & (t < t_end)) ? c[i >> 4][i & 15] : none;
       }
     }
     float top = c[0][0];
@@ -529,10 +532,11 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
       h8 wh, wl;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        _Float16 hi, lo;
-        split2(c[p >> 1][8 * (p & 1) + i], hi, lo);
-        wh[i] = hi;
-        wl[i] = lo;
+        // (an exponential is no product that a conversion could fold: no copy of it
+        // as split2 makes)
+        const float w = c[p >> 1][8 * (p & 1) + i];
+        wh[i] = (_Float16)w;
+        if constexpr (FULL) wl[i] = (_Float16)(w - (float)wh[i]);
       }
       if constexpr (!FULL) {  // the weights as they enter the product, two an instruction
         const h2 one = {(_Float16)1.f, (_Float16)1.f};
