@@ -163,12 +163,13 @@ struct Bounds {
 // (f32 rows): Q and the weights as hi + lo pairs; else Q as it is (times a power
 // of two) and the weights rounded to f16.
 //
-// A prompt of 4096 bf16 rows at 32 / 8 heads of 128 with capped scores takes 218
-// us (137 GFLOP, 631 TFLOP/s): per tile and wave 32 products (~1000 cycles) stand
-// beside ~32 scores a lane of one exp2, one reciprocal and ~9 other vector
-// instructions each, which the two work-groups of a CU only partly overlap. Six
-// chunks of up to 512 f32 rows behind 4-bit contexts at 28 / 4 heads: 200 us
-// (149 GFLOP of hi and lo products, 745 TFLOP/s).
+// A prompt of 4096 bf16 rows at 32 / 8 heads of 128 with capped scores takes 219
+// us (137 GFLOP, 627 TFLOP/s): per tile and wave 32 products (~1000 cycles) stand
+// beside 32 scores a lane of two exp2, one reciprocal and ~5 other vector
+// instructions each, which the two work-groups of a CU only partly overlap (MFMA
+// busy 27%, VALU 48%). Six chunks of up to 512 f32 rows behind 4-bit contexts at
+// 28 / 4 heads: 191 us (149 GFLOP of hi and lo products, 780 TFLOP/s; MFMA busy
+// 44%, VALU 45%).
 template <typename T, int HD, bool FULL>
 __global__ void __launch_bounds__(64 * kChunkWaves, 2)
 scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per_tile, int64_t min_rows,
