@@ -241,7 +241,14 @@ __device__ __forceinline__ float tanh_f32(float x) {
   return ax < 0.35f ? small : __builtin_copysignf(large, x);
 }
 
-// tanh to a few units of f32 in absolute terms, for rows of 16 bits.
+// Largest cap whose tanh may be off by a few units of f32 in absolute terms
+// (tanh_f16, and the chunk kernel's cap - 2 cap / (exp(2 x) + 1)): a score is
+// then off by ~3e-7 times the cap, 8e-5 here, a sixth of what the rounding of a
+// 16-bit row's weight to f16 may cost (2^-11). Larger caps of such rows take
+// f32 rows' way.
+constexpr float kShortCap = 256.f;
+
+// tanh to a few units of f32 in absolute terms.
 __device__ __forceinline__ float tanh_f16(float x) {
   return __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * (2.f * kLog2e)) + 1.f), 1.f);
 }

@@ -160,8 +160,8 @@ struct Bounds {
 // in place, numerators^T += V^T W (a lane's scores are positions 8 (r / 4) + 4 (lane / 32) + r % 4 of its column,
 // which is the second product's operand layout when its 16 positions are taken
 // as 4 (lane / 32) ... + 3 and 8 + 4 (lane / 32) ... + 3: no exchange). FULL
-// (f32 rows): Q and the weights as hi + lo pairs; else Q as it is (times a power
-// of two) and the weights rounded to f16.
+// (f32 rows, and any rows with a cap over kShortCap): Q and the weights as hi +
+// lo pairs; else Q as it is (times a power of two) and the weights rounded to f16.
 //
 // A prompt of 4096 bf16 rows at 32 / 8 heads of 128 with capped scores takes 219
 // us (137 GFLOP, 627 TFLOP/s): per tile and wave 32 products (~1000 cycles) stand
@@ -624,8 +624,10 @@ hipError_t launch_chunk_t(const PoolGeom &g, const ScoredArgs &a, int64_t min_ro
   const int64_t n_slots = chunk_slots(a);
   const int64_t wgs = (n_slots - a.split_slots + (int64_t)a.split_slots * a.splits) * a.n_kv_heads;
   if (wgs * 64 * kChunkWaves >= (int64_t{1} << 32)) return hipErrorInvalidValue;
-  const auto kernel =
-      a.row_type == LTKV_ROWS_F32 ? scored_chunk_kernel<T, HD, true> : scored_chunk_kernel<T, HD, false>;
+  // (a second tanh in the kernel of 16-bit rows took registers that it does not
+  // have: 12 to 22 spilled at head_dim 128)
+  const bool full = a.row_type == LTKV_ROWS_F32 || a.softcap > kShortCap;
+  const auto kernel = full ? scored_chunk_kernel<T, HD, true> : scored_chunk_kernel<T, HD, false>;
   kernel<<<(unsigned)wgs, 64 * kChunkWaves, 0, s>>>(a, g.n_blocks, g.kv_dim, rows_per_tile, min_rows, n_slots);
   return hipGetLastError();
 }

@@ -1,0 +1,66 @@
+"""Capped scores: 16-bit rows, whose caps the chunk kernel takes in a form of its
+own, and caps far above the scores."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from scored_definition import compare, definition
+from test_gpu_scored import build, held_rows, run, slopes_of
+
+pytestmark = pytest.mark.gpu
+
+
+def both(kv, q, tables, lens, starts, heads, hd, rows, max_rows, **how):
+    got, qr = run(kv, q, tables, lens, heads, hd, rows=rows, starts=starts, max_rows=max_rows, **dict(how))
+    compare(got, definition(qr, held_rows(kv), tables, lens, starts, heads, hd, rows=rows, eight=kv.dtype == "q8_0",
+                            **how))
+
+
+@pytest.mark.parametrize("rows", ["f16", "bf16"])
+@pytest.mark.parametrize("dtype", ["f16", "q8_0", "q4_0", "f32"])
+@pytest.mark.parametrize("shape", [(8, 2, 128), (7, 1, 128), (4, 4, 64), (9, 3, 64), (6, 2, 96)])
+def test_chunks_of_16_bit_rows(gpu, shape, dtype, rows):
+    """Ragged chunks beside single tokens: caps alone, with windows, prefixes and
+    documents, and scales of either sign."""
+    heads, kv_heads, hd = shape
+    lens, new = [70, 5, 0, 150, 33, 260], [70, 1, 0, 37, 2, 130]
+    starts = np.concatenate([[0], np.cumsum(new)])
+    kv, tables = build(kv_heads * hd, lens, dtype, 51)
+    q = np.random.default_rng(52).standard_normal((starts[-1], heads * hd)).astype(np.float32) * 3
+    first = np.concatenate([np.arange(n - m, n) // 37 * 37 for n, m in zip(lens, new)]).astype(np.int32)
+    for how in ({"softcap": 5.0}, {"softcap": 30.0}, {"softcap": 256.0}, {"softcap": 5.0, "window": 23, "sinks": 3},
+                {"softcap": 5.0, "prefix": [40, 0, 3, 90, 33, 900]}, {"softcap": 20.0, "first": first},
+                {"softcap": 4.0, "scale": -0.2}, {"scale": -0.2}, {"softcap": 4.0, "scale": 0.0},
+                {"softcap": 5.0, "slopes": slopes_of(heads)}, {"slopes": slopes_of(heads)}, {}):
+        both(kv, q, tables, lens, starts, heads, hd, rows, max(new), **how)
+
+
+@pytest.mark.parametrize("rows", ["f16", "bf16"])
+@pytest.mark.parametrize("dtype", ["f16", "q8_0", "q4_0"])
+def test_split_chunks_of_16_bit_rows(gpu, dtype, rows):
+    """Contexts long enough to be split over their positions."""
+    heads, kv_heads, hd = 8, 2, 128
+    lens, new = [5000, 2049, 3500], [1, 40, 20]
+    starts = np.concatenate([[0], np.cumsum(new)])
+    kv, tables = build(kv_heads * hd, lens, dtype, 53)
+    q = np.random.default_rng(54).standard_normal((starts[-1], heads * hd)).astype(np.float32) * 3
+    for how in ({"softcap": 8.0}, {"softcap": 30.0, "window": 1500, "sinks": 70}, {"softcap": 8.0, "scale": -0.1}):
+        both(kv, q, tables, lens, starts, heads, hd, rows, 40, **how)
+
+
+@pytest.mark.parametrize("rows", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dtype,shape", [("f16", (8, 2, 128)), ("q8_0", (4, 4, 64)), ("q4_0", (9, 3, 64)),
+                                         ("f16", (6, 2, 96)), ("f32", (6, 2, 96)), ("f16", (6, 2, 20))])
+@pytest.mark.parametrize("new", [[1, 1], [60, 33]])
+def test_large_caps(gpu, dtype, shape, new, rows):
+    """A cap far above the scores changes little, and costs no bits."""
+    heads, kv_heads, hd = shape
+    lens = [300, 50]
+    starts = np.concatenate([[0], np.cumsum(new)])
+    kv, tables = build(kv_heads * hd, lens, dtype, 55)
+    q = np.random.default_rng(56).standard_normal((starts[-1], heads * hd)).astype(np.float32) * 3
+    for softcap in (257.0, 1e3, 1e4, 1e5, 1e6, 1e7, 1e12):
+        for slopes in ({}, {"slopes": slopes_of(heads)}):
+            both(kv, q, tables, lens, starts, heads, hd, rows, max(new), softcap=softcap, **slopes)
