@@ -12,10 +12,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kChunkTokens = 64;  // positions of a tile
 
 // A thread's share of a tile on its way from the pool to LDS: a quarter of the
-// head (NC = HD / 32 chunks of 8 elements) of one position, K and V. planes()
-// gives the chunk as f16 numbers: f16 and q4_0 cells are f16 numbers; q8_0
-// cells times a power of two (which keeps the tile's largest scale at the top
-// of f16) as f16 hi + lo pairs.
+// head (NC = HD / 32 chunks of 8 elements) of one position, K and V. get() and
+// get2() give a chunk as f16 numbers: f16 and q4_0 cells are f16 numbers; q8_0
+// cells times a power of two (see TileRange) as f16 hi + lo pairs.
 template <typename T, int NC>
 struct Share;
 
@@ -125,6 +124,50 @@ __device__ __forceinline__ h8 finite_or_zero(const h8 &x) {
   return r;
 }
 
+// Largest of a value over a position's four lanes, in each of them.
+__device__ __forceinline__ float position_max(float x) {
+  x = __builtin_fmaxf(x, dpp<0xB1>(x));     // quad_perm [1,0,3,2]
+  return __builtin_fmaxf(x, dpp<0x4E>(x));  // quad_perm [2,3,0,1]
+}
+
+// The same over a wave's 16 positions, of values that a position's lanes share.
+__device__ __forceinline__ float positions_max(float x) {
+  x = __builtin_fmaxf(x, dpp<0x141>(x));  // row_half_mirror
+  x = __builtin_fmaxf(x, dpp<0x140>(x));  // row_mirror
+  return rows_reduce<true>(x);
+}
+
+// e such that quants of up to 128 times the scale d stay below 2^15 times 2^e.
+__device__ __forceinline__ int scale_exponent(float d) { return d > 0.f ? __builtin_amdgcn_frexp_expf(d) - 8 : 0; }
+
+// K and V of a q8_0 tile enter the products times powers of two. K: one for the
+// tile where every row sees all of it, else one for each position, which the
+// scores are multiplied by. V: one for the tile. A row must not lose bits to a
+// scale that it does not see, so V's power follows the largest scale that some
+// row sees only while that stays within 2^12 of a scale that every row has to do
+// with: the largest one that all of them see, or, where they share no position,
+// the least. (2^12: such a row's V still has f32's bits, since hi + lo parts keep
+// 22 bits down to 2^16 below the largest.) Else it follows that scale, and what
+// then passes the top of f16 is added apart, for the rows that see it
+// (kLeftOut). Positions that no row sees have no part in it. (Against one power
+// for all 64 positions, whoever sees them: chunks of 2 x 1024 f32 rows 180 -> 168
+// us, of bf16 rows 114 -> 122.)
+struct TileRange {
+  float k_top;               // largest scale of K
+  float top, shared, least;  // V's (least: negative, as a maximum)
+  __device__ __forceinline__ void add(const TileRange &o) {
+    k_top = __builtin_fmaxf(k_top, o.k_top);
+    top = __builtin_fmaxf(top, o.top);
+    shared = __builtin_fmaxf(shared, o.shared);
+    least = __builtin_fmaxf(least, o.least);
+  }
+  __device__ __forceinline__ int v_exponent() const {
+    const float base = shared > 0.f ? shared : -least;
+    return __builtin_amdgcn_readfirstlane(scale_exponent(top <= 4096.f * base ? top : 16.f * base));
+  }
+};
+constexpr float kLeftOut = 511.f;  // scales (times the power of two) from here on could pass f16's largest number
+
 // Sum / maximum of a value over lanes l and l ^ 32.
 template <bool MAX>
 __device__ __forceinline__ float halves_reduce(float x) {
@@ -182,8 +225,9 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
   constexpr int K_BYTES = kChunkTokens * K_PITCH, V_BYTES = kChunkTokens * V_PITCH;
   __shared__ __align__(16) char lds[K_PLANES * K_BYTES + V_PLANES * V_BYTES];
   __shared__ Bounds s_bounds[kChunkWaves];
-  __shared__ float s_scale[kChunkWaves][2];  // q8_0: largest K and V scales of the next tile
-  __shared__ uint32_t s_bad[kChunkWaves];    // a V element of the tile is infinite or NaN
+  __shared__ TileRange s_range[kChunkWaves];                     // q8_0: scales of the next tile
+  __shared__ __align__(16) float s_kpow[Q8 ? kChunkTokens : 4];  // q8_0: K of a position entered divided by this
+  __shared__ uint64_t s_bad[kChunkWaves];  // lanes whose share of V is left out (positions 16 wave + lane / 4)
   char *const lds_k = lds, *const lds_v = lds + K_PLANES * K_BYTES;
 
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -262,6 +306,10 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
       gb.end_min = min(gb.end_min, o.end_min);
       gb.end_max = max(gb.end_max, o.end_max);
     }
+    // (the same in every lane: scalar registers)
+    int32_t *const g = reinterpret_cast<int32_t *>(&gb);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof gb / 4); ++i) g[i] = __builtin_amdgcn_readfirstlane(g[i]);
   }
   StepRange<kChunkTokens> range{0, 0, 0, 0, 0, 0};
   if (gb.end_max > 0) {
@@ -354,32 +402,36 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
 
   for (int s = s_begin; s < s_end; ++s) {
     const int32_t t0 = range.start(s), t_end = range.end(s);
-    if constexpr (Q8) {
-      float dk = ks.scale(), dv = vs.scale();
-#pragma unroll
-      for (int off = 32; off >= 1; off >>= 1) {
-        dk = __builtin_fmaxf(dk, __shfl_xor(dk, off, 64));
-        dv = __builtin_fmaxf(dv, __shfl_xor(dv, off, 64));
-      }
-      if (lane == 0) {
-        s_scale[wave][0] = dk;
-        s_scale[wave][1] = dv;
-      }
-    }
-    lds_barrier();  // the last tile has been read
+    // a row of the work-group does not see the whole tile
+    const bool partial = t0 + kChunkTokens > t_end || !gb.all(t0, kChunkTokens);
+    bool inside = false;  // q8_0: some row sees the thread's position
     int k_exp = 0;
     if constexpr (Q8) {
-      float dk = 0.f, dv = 0.f;
-#pragma unroll
-      for (int w = 0; w < kChunkWaves; ++w) {
-        dk = __builtin_fmaxf(dk, s_scale[w][0]);
-        dv = __builtin_fmaxf(dv, s_scale[w][1]);
+      const float d = __builtin_fminf(position_max(vs.scale()), 65504.f);
+      TileRange r;
+      r.k_top = positions_max(__builtin_fminf(position_max(ks.scale()), 65504.f));
+      if (!partial) {
+        inside = true;
+        r.top = r.shared = positions_max(d);
+        r.least = -INFINITY;
+      } else {
+        inside = t0 + tok < t_end && !gb.none(t0 + tok, 1);
+        const bool shared = inside && gb.all(t0 + tok, 1);
+        r.top = positions_max(inside ? d : 0.f);
+        r.shared = positions_max(shared ? d : 0.f);
+        r.least = positions_max(inside && !shared && d > 0.f ? -d : -INFINITY);
       }
-      // quants of up to 128 times the largest scale stay below 2^15
-      k_exp = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(__builtin_fminf(dk, 65504.f))) - 8;
-      if (dk == 0.f) k_exp = 0;
-      const int e = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(__builtin_fminf(dv, 65504.f))) - 8;
-      if (dv > 0.f && e > v_exp) {
+      if (lane == 0) s_range[wave] = r;
+    }
+    lds_barrier();  // the last tile has been read
+    if constexpr (Q8) {
+      TileRange r = s_range[0];
+#pragma unroll
+      for (int w = 1; w < kChunkWaves; ++w) r.add(s_range[w]);
+      if (!partial) k_exp = __builtin_amdgcn_readfirstlane(scale_exponent(r.k_top));
+      const int e = r.v_exponent();
+      // (the numerators are f32 numbers: their power of two may fall as well)
+      if (__builtin_amdgcn_readfirstlane(r.top > 0.f) && (e > v_exp || e < v_exp - 2)) {
         if (v_exp > -1000) {
           const float f = __builtin_amdgcn_ldexpf(1.f, v_exp - e);
 #pragma unroll
@@ -388,16 +440,22 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
         v_exp = e;
       }
     }
-    // Infinities and NaN in V may reach only the rows that see them: looked for
-    // where a row of the work-group does not see the whole tile.
-    const bool partial = t0 + kChunkTokens > t_end || !gb.all(t0, kChunkTokens);
+    // Infinities and NaN in V (and q8_0 elements beyond the tile's power of two)
+    // may reach only the rows that see them: looked for in partial tiles.
     bool bad = false;
     {
       float dk = 0.f, dv = 0.f;
       if constexpr (Q8) {
-        dk = __builtin_amdgcn_ldexpf(ks.scale(), -k_exp);
+        int e = k_exp;
+        if (partial) {
+          e = scale_exponent(__builtin_fminf(position_max(ks.scale()), 65504.f));
+          if (part == 0) s_kpow[tok] = __builtin_amdgcn_ldexpf(1.f, e);
+        }
+        dk = __builtin_amdgcn_ldexpf(ks.scale(), -e);
         dv = __builtin_amdgcn_ldexpf(vs.scale(), -(v_exp > -1000 ? v_exp : 0));
       }
+      const bool left_out = Q8 && partial && !(dv < kLeftOut);
+      bad = left_out && inside;
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
         const int c = Share<T, NC>::chunk(part, j) * 16;
@@ -407,8 +465,7 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
           *reinterpret_cast<h8 *>(lds_k + tok * K_PITCH + c) = hi;
           *reinterpret_cast<h8 *>(lds_k + K_BYTES + tok * K_PITCH + c) = lo;
           vs.get2(j, dv, hi, lo);
-          if (partial && not_finite(hi)) {
-            bad = true;
+          if (left_out) {
             hi = h8{};
             lo = h8{};
           }
@@ -432,17 +489,14 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
       }
     }
     if constexpr (!std::is_same_v<T, Q4>) {
-      const bool any_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
-      if (lane == 0) s_bad[wave] = any_bad;
+      const uint64_t lanes = __builtin_amdgcn_ballot_w64(bad);
+      if (lane == 0) s_bad[wave] = lanes;
     }
     if (s + 1 < s_end) {
       load(next);
       next = block_of(s + 2);
     }
     lds_barrier();
-    bool tile_bad = false;
-    if constexpr (!std::is_same_v<T, Q4>) tile_bad = (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) != 0;
-
     if (wb.none(t0, kChunkTokens)) continue;
     // scores of positions t0 + 32 u + 8 (i / 4) + 4 half + i % 4
     f32x16 c[2] = {};
@@ -462,6 +516,14 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
       }
     }
     __builtin_amdgcn_s_setprio(0);
+    if (Q8 && partial) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const f32x4 f = *reinterpret_cast<const f32x4 *>(s_kpow + 8 * i + 4 * half);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) c[i >> 2][4 * (i & 3) + k] *= f[k];
+      }
+    }
     const int32_t tl = t0 + 4 * half;
     // Scores in the log2 domain as m c + m0: the multiplication is left to the
     // fused one before exp2. Capped rows of 16 bits take c = 1 / (exp(2 x) + 1),
@@ -558,26 +620,46 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
       }
     }
     if constexpr (!std::is_same_v<T, Q4>) {
-      if (tile_bad) {
-        // V elements that are infinite or NaN entered as zeros: the rows that
-        // see their positions get them here, the others do not
+      if (__builtin_amdgcn_readfirstlane((s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) != 0)) {
+        // V elements that are infinite or NaN (q8_0: too large for the tile's
+        // power of two) entered as zeros: the rows that see their positions get
+        // them here, the others do not
         for (int j = 0; j < kChunkTokens; ++j) {
           const int32_t t = t0 + j;
           if (t >= t_end) break;
+          if ((s_bad[j >> 4] >> (4 * (j & 15)) & 15) == 0) continue;
           int32_t e = scalar_read(tab, t >> 4);
           if (e < 0 || e >= n_blocks) e = 0;
+          const int64_t cell = (int64_t)e * 16 + (t & 15);
           float w = 0.f;
 #pragma unroll
           for (int i = 0; i < 32; ++i)  // position j is score i of lane (column, j / 4 % 2)
             if (i == (j >> 3) * 4 + (j & 3)) w = __shfl(c[i >> 4][i & 15], col + 32 * ((j >> 2) & 1), 64);
           if (!view.sees(t)) continue;
-          for (int k = 0; k < NC * 16; ++k) {
-            const int64_t d = head_off + 32 * (k / 16) + 8 * (k % 16 / 4) + 4 * half + k % 4;
-            const float x = cell_value<T>(a.v_layer, a.v_scale, (int64_t)e * 16 + (t & 15), kv_dim, d);
-            if (__builtin_fabsf(x) < INFINITY) continue;
+          if constexpr (Q8) {
 #pragma unroll
-            for (int i = 0; i < NC * 16; ++i)
-              if (i == k) o[i / 16][i % 16] += w * x;
+            for (int i = 0; i < NC; ++i) {  // a tile of the numerators is a group
+              const _Float16 scale = static_cast<const _Float16 *>(
+                  a.v_scale)[scale_index((int32_t)cell, (int)(head_off >> 5) + i, (int)(kv_dim >> 5))];
+              const float d = __builtin_amdgcn_ldexpf((float)scale, -(v_exp > -1000 ? v_exp : 0));
+              if (d < kLeftOut) continue;
+              const char *const row = static_cast<const char *>(a.v_layer) + cell * kv_dim + head_off + 32 * i;
+#pragma unroll
+              for (int k = 0; k < 16; k += 4) {
+                const uint32_t u = load_at<uint32_t>(row + 2 * k, 4 * half);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) o[i][k + b] += w * ((float)((int)(u >> (8 * b) & 255u) - 128) * d);
+              }
+            }
+          } else {
+            for (int k = 0; k < NC * 16; ++k) {
+              const int64_t d = head_off + 32 * (k / 16) + 8 * (k % 16 / 4) + 4 * half + k % 4;
+              const float x = cell_value<T>(a.v_layer, a.v_scale, cell, kv_dim, d);
+              if (__builtin_fabsf(x) < INFINITY) continue;
+#pragma unroll
+              for (int i = 0; i < NC * 16; ++i)
+                if (i == k) o[i / 16][i % 16] += w * x;
+            }
           }
         }
       }
