@@ -456,7 +456,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
 
     f32x4 o[ND];
     float ref, sum, lift, scale_top;
-    int v_exp;  // f32: numerators are sums of V times 2^-v_exp
+    int v_exp;  // f32: numerators are sums of V times 2^-v_exp (a pack: of the column's row)
     auto reset = [&]() {
 #pragma unroll
       for (int i = 0; i < ND; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -513,7 +513,8 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
       find(s_next);
       // f32: powers of two that bring K and V below 2^kTopExp (positions that the
       // row does not see count as zeros)
-      int k_exp = 0;
+      int k_exp = 0, stage_exp = 0;
+      float v_share = 1.f;  // a pack's weights times this: what V entered divided by over the column's 2^v_exp
       if constexpr (F32) {
         if (!whole)
 #pragma unroll
@@ -536,7 +537,21 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
         k_exp = exponent(most(k)) - kTopExp;
         const float m = most(v);
         const int e = exponent(m) - kTopExp;
-        if (__builtin_amdgcn_readfirstlane(m > 0.f) && e > v_exp) {
+        if constexpr (PACK) {
+          // Each row keeps a power of its own: one that follows what another row
+          // sees would cost it its bits.
+          if (__builtin_amdgcn_readfirstlane(m > 0.f)) {
+            stage_exp = e;
+            const int to = mine ? max(v_exp, e) : v_exp;
+            if (__builtin_amdgcn_ballot_w64(to > v_exp)) {
+              const float f = __builtin_amdgcn_ldexpf(1.f, v_exp - to);  // (0 the first time: no numerators yet)
+#pragma unroll
+              for (int i = 0; i < ND; ++i) o[i] *= f;
+              v_exp = to;
+            }
+            v_share = mine ? __builtin_amdgcn_ldexpf(1.f, e - v_exp) : 0.f;
+          }
+        } else if (__builtin_amdgcn_readfirstlane(m > 0.f) && e > v_exp) {
           if (v_exp != kNoExp) {
             const float f = __builtin_amdgcn_ldexpf(1.f, v_exp - e);
 #pragma unroll
@@ -544,6 +559,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
           }
           v_exp = e;
         }
+        if constexpr (!PACK) stage_exp = v_exp == kNoExp ? 0 : v_exp;
       }
       // V into LDS (positions that the row does not see as zeros); the scores are
       // computed while it settles
@@ -555,7 +571,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
 #pragma unroll
           for (int j = 0; j < NC; ++j) {
             h8 hi, lo;
-            v[u].get2(j, v_exp == kNoExp ? 0 : -v_exp, hi, lo);
+            v[u].get2(j, -stage_exp, hi, lo);
             char *p = my + (16 * u + col) * PITCH + chunk_of<NC, SPAN>(quad, j) * 16;
             *reinterpret_cast<h8 *>(p) = hi;
             *reinterpret_cast<h8 *>(p + 32 * PITCH) = lo;
@@ -703,7 +719,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           _Float16 hi, lo;
-          split2(w[i], hi, lo);
+          split2(F32 && PACK ? w[i] * v_share : w[i], hi, lo);
           wh[i] = hi;
           wl[i] = lo;
         }
