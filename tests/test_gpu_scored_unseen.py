@@ -12,8 +12,7 @@ from test_gpu_scored import build, held_rows, run
 pytestmark = pytest.mark.gpu
 
 
-KERNELS = [(dtype, hd) for dtype in ("f16", "q4_0") for hd in (64, 128, 96, 256)]
-KERNELS += [("q8_0", 64), ("q8_0", 128), ("f32", 64), ("f32", 128), ("f32", 96), ("f32", 256)]
+KERNELS = [(dtype, hd) for dtype in ("f16", "f32", "q8_0", "q4_0") for hd in (64, 128, 96, 256)]
 
 
 # lengths as built, lengths of the call, rows, positions with a huge cell, masks
