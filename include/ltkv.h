@@ -332,11 +332,11 @@ LTKV_API int ltkv_append_decode_attention(ltkv_cache *c, size_t layer, size_t n,
  *   t >= d_first[row] (the start of the row's document; d_first may be null);
  *   with window > 0, t > p - window or t - d_first[row] < sinks.
  * The score of a position is s = scale * q.k, capped to softcap * tanh(s /
- * softcap) where softcap > 0, minus d_slopes[h] * |p - t| for query head h
- * (d_slopes may be null); the output is V weighted by the softmax of the
- * scores over the visible positions, zeros where there are none. Positions a
- * row does not see do not enter its result, whatever they hold (a row that
- * sees an infinity or NaN gives values that are not finite).
+ * softcap) where softcap > 0 (caps over 2^96 count as that), minus d_slopes[h] *
+ * |p - t| for query head h (d_slopes may be null); the output is V weighted by
+ * the softmax of the scores over the visible positions, zeros where there are
+ * none. Positions a row does not see do not enter its result, whatever they hold
+ * (a row that sees an infinity or NaN gives values that are not finite).
  * f32 rows are computed to f32 accuracy; f16 and bf16 rows take Q as it is
  * and weights rounded to f16, summed in f32.
  * max_rows: the most rows of one sequence, which chooses the kernels (one with

@@ -1888,7 +1888,7 @@ int ltkv_scored_attention(ltkv_cache *c, size_t layer, size_t n, size_t n_rows, 
   a.row_type = row_type;
   a.row_starts = d_row_starts;
   a.max_rows = d_row_starts ? (int64_t)std::min(max_rows, n_rows) : 1;
-  a.softcap = softcap;
+  a.softcap = std::min(softcap, 0x1p96f);  // (the kernels take it times log2 e)
   a.slopes = d_slopes;
   a.window = (int64_t)std::min<size_t>(window, (size_t)INT32_MAX);
   a.sinks = (int64_t)std::min<size_t>(sinks, (size_t)INT32_MAX);

@@ -217,6 +217,17 @@ __device__ __forceinline__ void split2(float x, _Float16 &hi, _Float16 &lo) {
   lo = (_Float16)(x - (float)hi);
 }
 
+// What the product of a query and a key that entered times powers of two is
+// multiplied by to give a score over the cap (or, without one, a score in log2):
+// factor 2^e, held between 1e-37 and 1e37. Where caps are tiny or the powers far
+// apart it would be infinite or zero, and a product of exactly zero, or a masked
+// position's infinity, times that no number. Products lie between 2^-24 and 2^35,
+// so a score that the limits change is past any cap, or nothing.
+__device__ __forceinline__ float score_factor(float factor, int e) {
+  const float f = __builtin_amdgcn_ldexpf(factor, e);
+  return __builtin_copysignf(__builtin_amdgcn_fmed3f(__builtin_fabsf(f), 1e-37f, 1e37f), f);
+}
+
 // Score references are raised only when a score exceeds them by kSlack (log2),
 // so most steps need no exchange between lanes and no rescaling; weights carry
 // 2^lift, so that the largest (2^(kSlack + lift)) lie near the top of f16 and the

@@ -323,7 +323,7 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
 
   // Q columns (as scored_rows_kernel's)
   h8 qh[NK], ql[FULL ? NK : 1];
-  float qscale;
+  int q_exp;  // Q entered times 2^q_exp
   {
     float x[NK][8], amax = 0.f;
     const int64_t at = (row * a.n_heads + head) * (int64_t)HD;
@@ -334,23 +334,20 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
       for (int i = 0; i < 8; ++i) amax = __builtin_fmaxf(amax, __builtin_fabsf(x[j][i]));
     }
     amax = halves_reduce<true>(amax);
-    // (at most 100: the scale's share stays a normal number)
-    const int up = amax > 0.f && amax < INFINITY ? min(10 - __builtin_amdgcn_frexp_expf(amax), 100) : 0;
+    // (at most 100: a smaller row's scores are nothing beside their rounding)
+    q_exp = amax > 0.f && amax < INFINITY ? min(10 - __builtin_amdgcn_frexp_expf(amax), 100) : 0;
 #pragma unroll
     for (int j = 0; j < NK; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         _Float16 hi, lo;
-        split2(__builtin_amdgcn_ldexpf(x[j][i], up), hi, lo);
+        split2(__builtin_amdgcn_ldexpf(x[j][i], q_exp), hi, lo);
         qh[j][i] = hi;
         if constexpr (FULL) ql[j][i] = lo;
       }
-    qscale = __builtin_amdgcn_ldexpf(a.scale, -up);
   }
   const bool cap = a.softcap > 0.f;
-  // (finite for the smallest caps: a score of zero stays zero)
-  const float in_scale =
-      cap ? __builtin_amdgcn_fmed3f(qscale / a.softcap, -1e37f, 1e37f) : qscale * kLog2e;
+  const float factor = cap ? a.scale / a.softcap : a.scale * kLog2e, in_scale = score_factor(factor, -q_exp);
   const float cap_scale = a.softcap * kLog2e;
   const float slope = a.slopes && live ? a.slopes[head] * kLog2e : 0.f;
   // scores are an affine function of the products (or of the capped rows' c),
@@ -528,7 +525,7 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
     // Scores in the log2 domain as m c + m0: the multiplication is left to the
     // fused one before exp2. Capped rows of 16 bits take c = 1 / (exp(2 x) + 1),
     // since cap tanh(x) = cap - 2 cap c: five instructions a score.
-    float m = Q8 ? __builtin_amdgcn_ldexpf(in_scale, k_exp) : in_scale, m0 = 0.f;
+    float m = Q8 ? score_factor(factor, k_exp - q_exp) : in_scale, m0 = 0.f;
     if (affine) {
       if (cap) {
         const float to_e = m * (2.f * kLog2e);

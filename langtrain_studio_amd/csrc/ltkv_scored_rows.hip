@@ -422,7 +422,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
     // Q columns, scaled by a power of two so that the head's largest element
     // lies in [2^9, 2^10): any magnitude enters f16 with 22 bits
     h8 qh[NC], ql[NC];
-    float qscale;
+    int q_exp;  // Q entered times 2^q_exp
     {
       float x[NC][8], amax = 0.f;
       const int64_t at = (row * a.n_heads + head) * (int64_t)a.head_dim;
@@ -434,23 +434,20 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
         for (int i = 0; i < 8; ++i) amax = __builtin_fmaxf(amax, __builtin_fabsf(x[j][i]));
       }
       amax = rows_reduce<true>(amax);
-      // (at most 100: the scale's share stays a normal number)
-      const int up = amax > 0.f && amax < INFINITY ? min(10 - __builtin_amdgcn_frexp_expf(amax), 100) : 0;
+      // (at most 100: a smaller row's scores are nothing beside their rounding)
+      q_exp = amax > 0.f && amax < INFINITY ? min(10 - __builtin_amdgcn_frexp_expf(amax), 100) : 0;
 #pragma unroll
       for (int j = 0; j < NC; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           _Float16 hi, lo;
-          split2(__builtin_amdgcn_ldexpf(x[j][i], up), hi, lo);
+          split2(__builtin_amdgcn_ldexpf(x[j][i], q_exp), hi, lo);
           qh[j][i] = hi;
           ql[j][i] = lo;
         }
-      qscale = __builtin_amdgcn_ldexpf(a.scale, -up);
     }
     const bool cap = MODS && a.softcap > 0.f;
-    // (finite for the smallest caps: a score of zero stays zero)
-    const float in_scale =
-        cap ? __builtin_amdgcn_fmed3f(qscale / a.softcap, -1e37f, 1e37f) : qscale * kLog2e;
+    const float factor = cap ? a.scale / a.softcap : a.scale * kLog2e, in_scale = score_factor(factor, -q_exp);
     const float cap_scale = a.softcap * kLog2e;
     const float slope = MODS && a.slopes && live ? a.slopes[head] * kLog2e : 0.f;
 
@@ -645,7 +642,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
 #pragma unroll
         for (int i = 0; i < ND; ++i) vt[i] = read_tr2(my_t + 32 * i, 16 * PITCH);
       }
-      const float to_y = F32 ? __builtin_amdgcn_ldexpf(in_scale, k_exp) : in_scale;
+      const float to_y = F32 ? score_factor(factor, k_exp - q_exp) : in_scale;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll

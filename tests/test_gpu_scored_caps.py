@@ -1,5 +1,6 @@
 """Capped scores: 16-bit rows, whose caps the chunk kernel takes in a form of its
-own, and caps far above the scores."""
+own, caps from the smallest to the largest, and scores whose factor is near the
+ends of f32."""
 
 from __future__ import annotations
 
@@ -61,6 +62,47 @@ def test_large_caps(gpu, dtype, shape, new, rows):
     starts = np.concatenate([[0], np.cumsum(new)])
     kv, tables = build(kv_heads * hd, lens, dtype, 55)
     q = np.random.default_rng(56).standard_normal((starts[-1], heads * hd)).astype(np.float32) * 3
-    for softcap in (257.0, 1e3, 1e4, 1e5, 1e6, 1e7, 1e12):
+    for softcap in (257.0, 1e3, 1e4, 1e5, 1e6, 1e7, 1e12, 1e25, 3e38):
         for slopes in ({}, {"slopes": slopes_of(heads)}):
             both(kv, q, tables, lens, starts, heads, hd, rows, max(new), softcap=softcap, **slopes)
+
+
+@pytest.mark.parametrize("rows", ["f32", "f16"])
+@pytest.mark.parametrize("dtype,size", [("f32", 1e8), ("q8_0", 1e6), ("f16", 1e4), ("q4_0", 1e4)])
+@pytest.mark.parametrize("shape", [(8, 2, 64), (6, 2, 96)])
+@pytest.mark.parametrize("new", [[1, 1], [40, 33]])
+def test_the_smallest_caps_of_large_rows(gpu, dtype, size, shape, new, rows):
+    """Scores over caps so small are no numbers, and some are exactly zero."""
+    heads, kv_heads, hd = shape
+    lens = [300, 50]
+    starts = np.concatenate([[0], np.cumsum(new)])
+
+    def large(i, k, v):
+        k *= np.float32(size)
+        k[::7] = 0
+
+    kv, tables = build(kv_heads * hd, lens, dtype, 57, edit=large)
+    q = np.random.default_rng(58).standard_normal((starts[-1], heads * hd)).astype(np.float32)
+    q[0] = 0
+    for softcap in (1e-45, 1e-38, 1e-30):
+        # (the weights are equal: a capped score is at most the cap)
+        got, qr = run(kv, q, tables, lens, heads, hd, rows=rows, starts=starts, max_rows=max(new), softcap=softcap)
+        compare(got, definition(np.zeros_like(qr), held_rows(kv), tables, lens, starts, heads, hd, rows=rows,
+                                eight=dtype == "q8_0"))
+
+
+@pytest.mark.parametrize("rows", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype", ["f16", "q8_0", "q4_0", "f32"])
+@pytest.mark.parametrize("shape", [(8, 2, 64), (6, 2, 96)])
+@pytest.mark.parametrize("new", [[1, 1], [40, 33]])
+def test_factors_near_the_ends_of_f32(gpu, dtype, shape, new, rows):
+    """Scales and queries whose product is below or near the top of f32's range."""
+    heads, kv_heads, hd = shape
+    lens = [300, 50]
+    starts = np.concatenate([[0], np.cumsum(new)])
+    kv, tables = build(kv_heads * hd, lens, dtype, 59)
+    q = np.random.default_rng(60).standard_normal((starts[-1], heads * hd)).astype(np.float32)
+    for size, scale in ((1e-30, 1e-25), (1.0, 1e-38), (1e-30, -1e-25), (1e-25, 1e24), (1e30, 1e-31)):
+        for softcap in (0.0, 7.0):
+            both(kv, (q * np.float32(size)).astype(np.float32), tables, lens, starts, heads, hd, rows, max(new),
+                 scale=scale, softcap=softcap)
