@@ -85,11 +85,15 @@ __global__ void __launch_bounds__(kAnyThreads) scored_any_kernel(ScoredArgs a, i
     const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
     const float alpha = __builtin_amdgcn_exp2f(m - ref);
     const float p = seen ? __builtin_amdgcn_exp2f(sc - ref) : 0.f;
-    sp[t] = seen ? p : -1.f;
-    l = l * alpha + block_reduce<false>(p, red);
+    const float sum = l * alpha + block_reduce<false>(p, red);
+    // o: the average over the positions so far, no larger than their V
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;  // (a NaN sum stays one)
+    sp[t] = seen ? p * inv : -1.f;
+    const float keep = l * alpha * inv;
+    l = sum;
     m = mn;
 #pragma unroll
-    for (int k = 0; k < kAnyD; ++k) o[k] *= alpha;
+    for (int k = 0; k < kAnyD; ++k) o[k] *= keep;
     __syncthreads();
     for (int j = 0; j < n_tok; ++j) {
       const float pj = sp[j];
@@ -103,11 +107,10 @@ __global__ void __launch_bounds__(kAnyThreads) scored_any_kernel(ScoredArgs a, i
     }
     __syncthreads();  // sblk and sp are rewritten next round
   }
-  const float inv = l != 0.f ? 1.f / l : 0.f;  // (a NaN sum stays one)
 #pragma unroll
   for (int k = 0; k < kAnyD; ++k) {
     const int d = t + kAnyThreads * k;
-    if (d < a.head_dim) row_store(a, qh + d, o[k] * inv);
+    if (d < a.head_dim) row_store(a, qh + d, o[k]);
   }
 }
 

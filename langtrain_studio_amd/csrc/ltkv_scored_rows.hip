@@ -464,17 +464,25 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
       v_exp = kNoExp;
     };
     auto flush = [&]() {
-      if constexpr (F32) {
-        const float f = __builtin_amdgcn_ldexpf(1.f, v_exp == kNoExp ? 0 : v_exp / 2);
-        const float g = __builtin_amdgcn_ldexpf(1.f, v_exp == kNoExp ? 0 : v_exp - v_exp / 2);
-#pragma unroll
-        for (int i = 0; i < ND; ++i) o[i] = o[i] * f * g;
-      }
-      const float total = rows_reduce<false>(sum);
+      float total = rows_reduce<false>(sum);
       if (!live) return;
       const int64_t rh = row * a.n_heads + head;
+      float inv = n_parts == 1 ? total != 0.f ? 1.f / total : 0.f : 1.f;
+      int lower = 0;
+      if constexpr (F32) {
+        // Numerators are up to 2^23 and more times their V: of values near f32's
+        // largest they are divided first (one part), or lowered with their sum, as
+        // weights of a reference that much higher.
+        const int e = v_exp == kNoExp ? 0 : v_exp;
+        if (n_parts > 1 && e > 60) lower = 40;
+        total = __builtin_amdgcn_ldexpf(total, -lower);
+        const float f = __builtin_amdgcn_ldexpf(1.f, (e - lower) / 2);
+        const float g = __builtin_amdgcn_ldexpf(1.f, e - lower - (e - lower) / 2);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[i] = o[i] * inv * f * g;
+        inv = 1.f;
+      }
       if (n_parts == 1) {
-        const float inv = total != 0.f ? 1.f / total : 0.f;
 #pragma unroll
         for (int i = 0; i < ND; ++i)
           if (SPAN || 16 * i + 4 * quad < a.head_dim)
@@ -487,7 +495,7 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
       for (int i = 0; i < ND; ++i)
         if (SPAN || 16 * i + 4 * quad < a.head_dim) *reinterpret_cast<f32x4 *>(dst + 16 * i) = o[i];
       if (quad == 0) {
-        a.part_ml[2 * at] = ref - lift;
+        a.part_ml[2 * at] = ref - lift + (float)lower;
         a.part_ml[2 * at + 1] = total;
       }
     };
