@@ -91,6 +91,11 @@ struct RowView {
     // (no short circuits: a select each, not branches)
     return (t >= first) & (t < end) & ((t >= from) | (t < sink_end));
   }
+  // any of the positions of the block that begins at t
+  __device__ __forceinline__ bool sees_of_block(int32_t t) const {
+    const int32_t lo = max(t, first), hi = min(t + 16, end);
+    return hi > lo && (hi > from || lo < sink_end);
+  }
 };
 
 __device__ __forceinline__ RowView row_view(const ScoredArgs &a, const SeqRows &s, int64_t seq, int32_t r) {

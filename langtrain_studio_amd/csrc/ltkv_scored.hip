@@ -52,9 +52,11 @@ __global__ void __launch_bounds__(kAnyThreads) scored_any_kernel(ScoredArgs a, i
   for (int d = t; d < a.head_dim; d += kAnyThreads) sq[d] = row_load(a, qh + d);
   const int32_t *tab = table_of(a.tables, a.table_stride, a.rows, a.table_rows, seq);
   if (t < 64) {
-    check_table(tab, view.first >> 4, (min(view.sink_end, view.end) + 15) >> 4, n_blocks, a.rows, a.table_rows, seq,
-                a.status);
-    check_table(tab, view.from >> 4, (view.end + 15) >> 4, n_blocks, a.rows, a.table_rows, seq, a.status);
+    const int32_t sinks = min(view.sink_end, view.end);
+    if (sinks > view.first)
+      check_table(tab, view.first >> 4, (sinks + 15) >> 4, n_blocks, a.rows, a.table_rows, seq, a.status);
+    if (view.end > view.from)
+      check_table(tab, view.from >> 4, (view.end + 15) >> 4, n_blocks, a.rows, a.table_rows, seq, a.status);
   }
   const float slope = a.slopes ? a.slopes[h] : 0.f;
   float m = -INFINITY, l = 0.f, o[kAnyD];

@@ -321,6 +321,18 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
   if (split >= n_parts) return;
   const int s_begin = split * per_part, s_end = min(range.n, s_begin + per_part);
 
+  // Table entries outside the pool are reported where some row sees a position of
+  // their block (between the rows' ranges may lie blocks that none of them sees):
+  // once, in front of the loop, which only reads block 0 in their place. The first
+  // come with Q.
+  const int32_t *tab = table_of(a.tables, a.table_stride, a.rows, a.table_rows, seq);
+  auto entry_of = [&](int32_t i) {  // i counts blocks from step s_begin on
+    if (i >= 4 * (s_end - s_begin)) return 0;
+    const int32_t t = range.start(s_begin + i / 4) + 16 * (i % 4);
+    return t < range.end(s_begin + i / 4) ? tab[t >> 4] : 0;
+  };
+  int32_t entry = entry_of(tid);
+
   // Q columns (as scored_rows_kernel's)
   h8 qh[NK], ql[FULL ? NK : 1];
   int q_exp;  // Q entered times 2^q_exp
@@ -362,19 +374,22 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
   int v_exp = -1000;  // q8_0: V enters the products times 2^-v_exp
 
   // staging
-  const int32_t *tab = table_of(a.tables, a.table_stride, a.rows, a.table_rows, seq);
   const int64_t head_off = (int64_t)kvh * HD;
   const int tok = tid >> 2, part = tid & 3;
+  for (int32_t i = tid; i < 4 * (s_end - s_begin); entry = entry_of(i += 64 * kChunkWaves)) {
+    if ((uint32_t)entry < (uint32_t)n_blocks) continue;
+    const int32_t t = range.start(s_begin + i / 4) + 16 * (i % 4);
+    bool needed = false;
+    for (int32_t r = 0; r < rows_per_tile && r0 + r < rows.count; ++r)
+      needed |= row_view(a, rows, seq, r0 + r).sees_of_block(t);
+    if (needed) report_fault(a.status, kFaultTable, seq);
+  }
   // The wave's block of a tile, read a tile ahead of its cells (past the end:
   // block 0, read and masked).
   auto block_of = [&](int s) {
     const int32_t t = range.start(s) + 16 * wave;
     int32_t e = s < s_end && t < range.end(s) ? scalar_read(tab, t >> 4) : 0;
-    if (e < 0 || e >= n_blocks) {
-      report_fault(a.status, kFaultTable, seq);
-      e = 0;
-    }
-    return e;
+    return (uint32_t)e < (uint32_t)n_blocks ? e : 0;
   };
   const int64_t block_bytes = Share<T, NC>::block_bytes(kv_dim);
   const uint32_t place = Share<T, NC>::place(kv_dim, head_off, tok & 15, part);

@@ -389,8 +389,14 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
       const bool valid = s < s_end && t < range.end(s);
       entry = valid ? tab[t >> 4] : 0;
       entry_step = s0;
-      const bool bad = entry < 0 || entry >= n_blocks;
+      bool bad = entry < 0 || entry >= n_blocks;
       if (bad) entry = 0;
+      if constexpr (PACK)
+        if (__builtin_amdgcn_ballot_w64(bad)) {  // (between the rows' ranges may lie blocks that none of them sees)
+          bool needed = false;
+          for (int i = 0; i < n_pack; ++i) needed |= row_view(a, rows, seq, r + i).sees_of_block(t);
+          bad &= needed;
+        }
       if (__builtin_amdgcn_ballot_w64(bad)) report_fault(a.status, kFaultTable, seq);
     };
     Cells<T, NC, SPAN> k[2], v[2];
