@@ -355,7 +355,7 @@ class KvCache:
         elif row_starts.numel() != n + 1:
             raise ValueError("row_starts must have one entry per sequence and one more")
         if out is None:
-            out = torch.zeros_like(q) if row_starts is not None else torch.empty_like(q)
+            out = self._zeros_like(q) if row_starts is not None else torch.empty_like(q)
         elif out.shape != q.shape:
             raise ValueError("out must match q")
         if scale is None:
@@ -377,6 +377,21 @@ class KvCache:
             _dev_ptr(q, q.dtype, "q", self.device), _dev_ptr(tables, torch.int32, "tables", self.device),
             tables.shape[1], _dev_ptr(lens, torch.int32, "lens", self.device),
             given(row_starts, torch.int32, "row_starts", n + 1), _dev_ptr(out, q.dtype, "out", self.device)))
+        return out
+
+    def _zeros_like(self, t):
+        """Zeros cleared on the cache's stream, in order with its launches, whatever
+        the current stream is."""
+        import torch
+
+        if not t.is_cuda or t.get_device() != self.device:
+            return torch.zeros_like(t)  # (the call refuses t)
+        current = torch.cuda.current_stream(self.device)
+        if current.cuda_stream == self._stream:
+            return torch.zeros_like(t)
+        with torch.cuda.stream(torch.cuda.ExternalStream(self._stream, device=self.device)):
+            out = torch.zeros_like(t)
+        out.record_stream(current)  # the caller's: the memory is not reused under its work
         return out
 
     def decode_attention(self, layer: int, q, tables, lens, n_heads: int, head_dim: int,
