@@ -1655,9 +1655,9 @@ ltkv::ScoredArgs scored_args(ltkv_cache *c, size_t layer, size_t n, size_t n_row
   return a;
 }
 
-// Launches it, its partials in the cache's memory, or with use_scratch in the
+// Sets up its partials: in the cache's memory, or with use_scratch in the
 // device's static scratch (which allocates nothing).
-int scored_attention(ltkv_cache *c, ltkv::ScoredArgs &a, bool use_scratch = false) {
+int scored_memory(ltkv_cache *c, ltkv::ScoredArgs &a, bool use_scratch) {
   const ltkv::ScoredWorkspace ws = ltkv::scored_workspace((int)c->elem, a);
   if (use_scratch && (size_t)ws.bytes > ltkv::kScratchBytes)
     return fail(LTKV_ERR_ARG,
@@ -1679,6 +1679,11 @@ int scored_attention(ltkv_cache *c, ltkv::ScoredArgs &a, bool use_scratch = fals
       a.chunk_n = (int32_t *)(base + ws.chunk_n_off);
     }
   }
+  return LTKV_OK;
+}
+
+int scored_attention(ltkv_cache *c, ltkv::ScoredArgs &a, bool use_scratch = false) {
+  if (int rc = scored_memory(c, a, use_scratch)) return rc;
   const hipError_t e = ltkv::launch_scored_attention(head_geom(c, (size_t)a.head_dim), a, c->stream);
   if (e == hipErrorInvalidValue) return fail(LTKV_ERR_ARG, "attention grid too large for one launch");
   if (e != hipSuccess) return hip_fail(e, "attention launch");
@@ -1821,7 +1826,15 @@ int ltkv_append_decode_attention(ltkv_cache *c, size_t layer, size_t n, size_t n
   if (((uintptr_t)d_k | (uintptr_t)d_v) % 16 != 0) return fail(LTKV_ERR_ARG, "K/V rows must be 16-byte aligned");
   if (!ltkv::attention_tuned((int)c->elem, (int)head_dim, (int)group) || c->attn_engine == LTKV_ENGINE_VALU) {
     // fused on the tuned shapes, except by the vector-ALU kernels on f16
-    // pools: otherwise append, then attention, as two launches
+    // pools: otherwise append, then attention, as two launches (q4_0: with memory
+    // for the second before the first, so that a refused call appends nothing)
+    if (c->q4()) {
+      DeviceGuard dg(c->device);
+      if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
+      ltkv::ScoredArgs a = scored_args(c, layer, n, n, n_heads, head_dim, scale, d_q, d_tables, table_stride,
+                                       table_stride * LTKV_BLOCK, d_lens, d_out);
+      if (int rc = scored_memory(c, a, false)) return rc;
+    }
     if (int rc = ltkv_write(c, layer, n, d_slot_mapping, d_k, d_v, src_stride)) return rc;
     return ltkv_decode_attention(c, layer, n, n_heads, head_dim, scale, d_q, d_tables, table_stride,
                                  d_lens, d_out);
