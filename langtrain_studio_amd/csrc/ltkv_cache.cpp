@@ -45,6 +45,7 @@ int fail(int code, const char *fmt, ...) {
 }
 
 int hip_fail(hipError_t e, const char *what) {
+  (void)hipGetLastError();  // (else the next launch would report it again)
   return fail(LTKV_ERR_HIP, "HIP error in %s: %s", what, hipGetErrorString(e));
 }
 
@@ -495,14 +496,21 @@ int kept_memory(ltkv_cache *c, size_t bytes, uint8_t **base) {
                   "attention needs %zu bytes of partials, which a stream capture cannot allocate: make the call once "
                   "before capturing it",
                   bytes);
-    const size_t size = std::max(bytes, 2 * c->kept_bytes);
+    size_t size = std::max(bytes, 2 * c->kept_bytes);
     try {
       c->kept.reserve(c->kept.size() + 1);
     } catch (const std::bad_alloc &) {
       return fail(LTKV_ERR_ARG, "out of host memory");
     }
     uint8_t *p = nullptr;
-    HIP_TRY(hipMalloc((void **)&p, size), "hipMalloc(partials)");
+    if (size > bytes && hipMalloc((void **)&p, size) != hipSuccess) {  // no room for twice: what is needed
+      (void)hipGetLastError();
+      p = nullptr;
+    }
+    if (!p) {
+      size = bytes;
+      HIP_TRY(hipMalloc((void **)&p, size), "hipMalloc(partials)");
+    }
     c->kept.push_back(p);
     c->kept_bytes = size;
   }

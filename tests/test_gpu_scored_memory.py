@@ -1,5 +1,5 @@
-"""Memory and streams of scored attention and 4-bit decodes: outputs made by the
-call, refused calls."""
+"""Memory and streams of scored attention and 4-bit decodes: growth beside a full
+device, refused calls, outputs made by the call."""
 
 from __future__ import annotations
 
@@ -7,15 +7,25 @@ import numpy as np
 import pytest
 
 from scored_definition import compare, definition
-from test_gpu_scored import build, held_rows, run
+from test_gpu_scored import BLOCK, build, held_rows, run
 
 pytestmark = pytest.mark.gpu
+
+MIB = 1 << 20
 
 
 def up(a, dtype):
     import torch
 
     return torch.from_numpy(np.ascontiguousarray(a, dtype)).cuda()
+
+
+def free_bytes():
+    import torch
+
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    return torch.cuda.mem_get_info()[0]
 
 
 def test_new_outputs_on_the_caches_stream(gpu):
@@ -75,3 +85,54 @@ def test_a_refused_append_writes_nothing(gpu):
     kv.synchronize()
     compare(out.cpu().numpy(), definition(q.cpu().numpy(), held_rows(kv), t.cpu().numpy(), [x + 1 for x in lens],
                                           list(range(n + 1)), heads, hd))
+
+
+def test_partials_grow_beside_a_full_device(gpu):
+    """Twice the old size does not fit, what the call needs does; a call whose
+    partials do not fit is refused, and the next one runs."""
+    import torch
+
+    from langtrain_studio_amd import KvError
+
+    heads, kvh, hd, stride = 32, 8, 128, 8192
+    kv, tables = build(kvh * hd, [1], "q4_0", 73)
+    # 257 parts of up to 131 072 positions a sequence: 32 x 257 x 130 floats
+    need = {n: n * (32 * 257 * 130 * 4 + 4) for n in (192, 256)}
+    q = torch.randn((256, heads * hd), device="cuda")
+    t = torch.full((256, stride), -1, dtype=torch.int32, device="cuda")
+    t[:, 0] = int(tables[0, 0])
+    ld = torch.ones(256, dtype=torch.int32, device="cuda")
+    out = torch.empty_like(q)
+    q2, t2, ld2 = (x.repeat(2, *[1] * (x.dim() - 1)) for x in (q, t, ld))  # twice the sequences: too many
+    want = kv.decode_attention(0, q[:1], t[:1, :1].contiguous(), ld[:1], heads, hd)
+    # room for the first call's partials, then for the second's and 300 MiB, not for twice the first's
+    room = need[192] + need[256] + 300 * MIB
+    assert need[256] + 300 * MIB < 2 * need[192]
+    ballast = []
+    try:
+        for size in (free_bytes() // MIB * 3 // 4, 4096, 64):  # MiB a piece, until the device is full
+            try:
+                while len(ballast) < 256:
+                    ballast.append(torch.empty(size * MIB, dtype=torch.uint8, device="cuda"))
+            except torch.OutOfMemoryError:
+                torch.cuda.empty_cache()
+            if size == 4096:
+                ballast.pop()  # (in small pieces, some of which are given back)
+                torch.cuda.empty_cache()
+        pieces = -(-room // (64 * MIB))
+        assert len(ballast) < 256 and ballast[-pieces].numel() == 64 * MIB
+        del ballast[-pieces:]
+        torch.cuda.empty_cache()
+        kv.decode_attention(0, q[:192], t[:192], ld[:192], heads, hd, out=out[:192])
+        kv.synchronize()
+        with pytest.raises(KvError, match="out of memory"):
+            kv.decode_attention(0, q2, t2, ld2, heads, hd, out=q2)
+        kv.decode_attention(0, q, t, ld, heads, hd, out=out)
+        kv.synchronize()
+    finally:
+        ballast.clear()
+        torch.cuda.empty_cache()
+    assert torch.equal(out[0], want[0])
+    v = held_rows(kv)[1][int(tables[0, 0]) * BLOCK].reshape(kvh, 1, hd).repeat(heads // kvh, axis=1).reshape(-1)
+    np.testing.assert_allclose(out.cpu().numpy(), np.tile(v, (256, 1)), rtol=1e-6)
+    kv.close()
