@@ -401,7 +401,7 @@ struct ScoredArgs {
   // Partials of rows split over their positions: part_o [slot][head][max_parts]
   // [head_dim], part_ml [slot][head][max_parts][2] (reference, sum), part_n
   // [slot] parts used, a slot per row of the pack slots or max_rows per sequence;
-  // the chunk kernel's with one per row of the split tile slots.
+  // the chunk kernel's likewise by the call's rows (as far as split tile slots reach).
   float *part_o, *part_ml;
   int32_t *part_n;
   float *chunk_o, *chunk_ml;

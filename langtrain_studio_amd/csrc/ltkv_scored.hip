@@ -118,8 +118,8 @@ __global__ void __launch_bounds__(kAnyThreads) scored_any_kernel(ScoredArgs a, i
 
 // Rows whose positions were taken in several parts (or splits): their numerators
 // and sums folded in order by their references. VEC elements of a row a thread:
-// first the part slots of the rows kernel (ScoredArgs::part_n), then the rows of
-// the chunk kernel's split tile slots.
+// first the part slots of the rows kernel (ScoredArgs::part_n), then the rows
+// that the chunk kernel's split tile slots may hold.
 // ROWS: only part slots of sequences' rows: a thread an element, 16 parts' loads
 // at a time, since latency counts (one context's fold 4.6 us, 5.8 with four
 // elements a thread), and no searches. Else four elements a thread: the splits
@@ -136,12 +136,12 @@ __global__ void __launch_bounds__(kMergeThreads) scored_merge_kernel(ScoredArgs 
   const int i = ((int)(blockIdx.x % (uint32_t)slices) * kMergeThreads + (int)threadIdx.x) * VEC;
   if (i >= a.n_heads * a.head_dim) return;  // (head_dim is a multiple of 8 here)
   const int h = i / a.head_dim, e = i - h * a.head_dim;
-  // row of a slot of the tiles (or packs), -1 for slots that no kernel took
+  // row of a slot of the packs, -1 for slots without one
   auto slot_row = [&](int64_t slot) -> int64_t {
-    const int64_t tile = slot / rows_per_tile, seq = seq_of_slot(a, tile, rows_per_tile);
+    const int64_t pack = slot / rows_per_tile, seq = seq_of_slot(a, pack, rows_per_tile);
     const SeqRows s = seq_rows(a, seq);
-    const int64_t r = (tile - first_slot(a, seq, rows_per_tile)) * rows_per_tile + slot % rows_per_tile;
-    return r < 0 || r >= s.count || (!a.packs && s.count <= min_rows) ? -1 : s.row0 + r;
+    const int64_t r = (pack - first_slot(a, seq, rows_per_tile)) * rows_per_tile + slot % rows_per_tile;
+    return r < 0 || r >= s.count ? -1 : s.row0 + r;
   };
   int64_t row, slot;
   int n_parts, stride;
@@ -163,10 +163,14 @@ __global__ void __launch_bounds__(kMergeThreads) scored_merge_kernel(ScoredArgs 
     o = a.part_o;
     ml = a.part_ml;
   } else {
-    slot = item - part_slots;
-    row = slot_row(slot);
-    if (row < 0) return;
-    n_parts = scalar_read(a.chunk_n, slot);
+    slot = row = item - part_slots;
+    const int64_t seq = seq_of_row(a, row);
+    const SeqRows s = seq_rows(a, seq);
+    const int64_t r = row - s.row0;
+    if (r < 0 || r >= s.count || s.count <= min_rows ||
+        first_slot(a, seq, rows_per_tile) + r / rows_per_tile >= a.split_slots)
+      return;
+    n_parts = scalar_read(a.chunk_n, row);
     stride = a.splits;
     o = a.chunk_o;
     ml = a.chunk_ml;
@@ -283,6 +287,12 @@ gather_values_kernel(const void *__restrict__ kpool, const void *__restrict__ vp
 
 namespace {
 
+// Rows from the first on among which those of the split tile slots are: row r is
+// in slot r / (rows of a tile) - 1 or a later one.
+int64_t split_rows(const ScoredArgs &a) {
+  return a.split_slots > 0 ? std::min<int64_t>(a.n_rows, (int64_t)(a.split_slots + 1) * chunk_rows(a)) : 0;
+}
+
 // Most positions that the steps of a row cover.
 int64_t span_bound(const ScoredArgs &a) {
   int64_t span = a.max_len;
@@ -320,6 +330,14 @@ ScoredWorkspace scored_workspace(int elem, ScoredArgs &a) {
   const int64_t span = span_bound(a);
   int64_t at = 0;
   if (k.rows) a.max_parts = (int)scored_max_parts(span, a.part_tokens);
+  // Rows with starts: no more parts a sequence than 128 waves a CU make in all, or
+  // eight. Tables may be far wider than the contexts: 64 rows beside 255 single
+  // tokens on tables of 131 072 positions, 32 / 8 heads of 128, took 526 000 waves,
+  // most of them empty, and 2.2 GB of partials (677 us); so 33 000 and 136 MB (119
+  // us; with half as many 104, but 540 instead of 364 where one of the sequences
+  // has 60 000 positions and the others 200).
+  if (a.row_starts && !a.packs)
+    a.max_parts = (int)std::min<int64_t>(a.max_parts, std::max<int64_t>(8, 128 * a.cu_count / (a.n * a.n_kv_heads)));
   // packs are many where a chunk is long: no more parts than fill the chip a few
   // times (they cost partials)
   if (a.packs)
@@ -346,11 +364,11 @@ ScoredWorkspace scored_workspace(int elem, ScoredArgs &a) {
     if (a.splits > 1) {
       // (slots may be empty: a sequence's tiles need not fill its slots)
       a.split_slots = (int)std::min<int64_t>((over + a.n_kv_heads - 1) / a.n_kv_heads + a.n, chunk_slots(a));
-      const int64_t split_rows = (int64_t)a.split_slots * rows, parts = split_rows * a.n_heads * a.splits;
+      const int64_t parts = split_rows(a) * a.n_heads * a.splits;
       w.chunk_o_off = at;
       w.chunk_ml_off = at + parts * a.head_dim * 4;
       w.chunk_n_off = w.chunk_ml_off + parts * 2 * 4;
-      at = w.chunk_n_off + split_rows * 4;
+      at = w.chunk_n_off + split_rows(a) * 4;
     }
   }
   w.bytes = at;
@@ -375,7 +393,7 @@ hipError_t launch_scored_attention(const PoolGeom &g, const ScoredArgs &a, hipSt
     if (const hipError_t e = launch_scored_rows(g, a, border, s); e != hipSuccess) return e;
   const int64_t part_slots = border > 0 && a.max_parts > 1 ? (a.packs ? pack_slots(a) * pack_rows(a) : a.n * a.max_rows) : 0;
   const int rows_per_tile = a.chunks ? chunk_rows(a) : pack_rows(a);
-  const int64_t items = part_slots + (int64_t)a.split_slots * rows_per_tile;
+  const int64_t items = part_slots + split_rows(a);
   if (items == 0) return hipSuccess;
   const bool rows_only = !a.packs && a.split_slots == 0;
   const int per_group = kMergeThreads * merge_vec(rows_only);

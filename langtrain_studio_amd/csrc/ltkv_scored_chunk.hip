@@ -695,7 +695,7 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
           store_row4(a, rh * HD + 32 * i + 2 * k + 4 * half,
                      f32x4{o[i][k] * inv, o[i][k + 1] * inv, o[i][k + 2] * inv, o[i][k + 3] * inv});
     } else {
-      const int64_t at = ((slot * rows_per_tile + rr) * a.n_heads + head) * a.splits + split;
+      const int64_t at = rh * a.splits + split;
       float *dst = a.chunk_o + at * HD + 4 * half;
 #pragma unroll
       for (int i = 0; i < NC; ++i)
@@ -708,7 +708,7 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
       }
     }
     if (splits > 1 && split == 0 && half == 0 && kvh == 0 && c128 - rr * group == 0)
-      a.chunk_n[slot * rows_per_tile + rr] = n_parts;
+      a.chunk_n[row] = n_parts;
   }
 }
 

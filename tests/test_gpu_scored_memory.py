@@ -1,5 +1,5 @@
-"""Memory and streams of scored attention and 4-bit decodes: growth beside a full
-device, refused calls, outputs made by the call."""
+"""Memory and streams of scored attention and 4-bit decodes: partials of wide
+tables, growth beside a full device, refused calls, outputs made by the call."""
 
 from __future__ import annotations
 
@@ -18,6 +18,12 @@ def up(a, dtype):
     import torch
 
     return torch.from_numpy(np.ascontiguousarray(a, dtype)).cuda()
+
+
+def wide(tables, stride):
+    t = np.full((tables.shape[0], stride), -1, np.int32)
+    t[:, :tables.shape[1]] = tables
+    return t
 
 
 def free_bytes():
@@ -135,4 +141,27 @@ def test_partials_grow_beside_a_full_device(gpu):
     assert torch.equal(out[0], want[0])
     v = held_rows(kv)[1][int(tables[0, 0]) * BLOCK].reshape(kvh, 1, hd).repeat(heads // kvh, axis=1).reshape(-1)
     np.testing.assert_allclose(out.cpu().numpy(), np.tile(v, (256, 1)), rtol=1e-6)
+    kv.close()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "q4_0"])
+def test_partials_of_wide_tables_beside_chunks(gpu, dtype):
+    """A chunk beside 255 single tokens on tables of 131 072 positions: partials
+    follow what the launch can use, not the tables' width."""
+    import torch
+
+    heads, kvh, hd = 32, 8, 128
+    lens, new = [300] + [1 + i * 7 % 400 for i in range(255)], [64] + [1] * 255
+    lens[9], lens[200] = 5000, 2100
+    starts = np.concatenate([[0], np.cumsum(new)])
+    kv, tables = build(kvh * hd, lens, dtype, 74)
+    q = np.random.default_rng(75).standard_normal((starts[-1], heads * hd)).astype(np.float32)
+    run(kv, q[:1], tables[:1], [1], heads, hd)
+    qd, t, ld, sd = up(q, np.float32), up(wide(tables, 8192), np.int32), up(lens, np.int32), up(starts, np.int32)
+    out = torch.empty_like(qd)
+    before = free_bytes()
+    kv.scored_attention(0, qd, t, ld, heads, hd, row_starts=sd, max_rows=64, out=out)
+    kv.synchronize()
+    assert before - free_bytes() < 256 * MIB
+    compare(out.cpu().numpy(), definition(q, held_rows(kv), tables, lens, starts, heads, hd))
     kv.close()
