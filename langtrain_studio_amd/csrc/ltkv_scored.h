@@ -94,7 +94,7 @@ struct RowView {
   // any of the positions of the block that begins at t
   __device__ __forceinline__ bool sees_of_block(int32_t t) const {
     const int32_t lo = max(t, first), hi = min(t + 16, end);
-    return hi > lo && (hi > from || lo < sink_end);
+    return (hi > lo) & ((hi > from) | (lo < sink_end));
   }
 };
 

@@ -185,14 +185,15 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// The least and largest of what the rows of a wave (or work-group) see.
+// The least and largest of what the rows of a wave (or work-group) see. (No short
+// circuits, as in RowView::sees.)
 struct Bounds {
   int32_t first_min, first_max, from_min, from_max, sink_min, sink_max, end_min, end_max;
   __device__ __forceinline__ bool none(int32_t t, int32_t n) const {  // of positions [t, t + n)
-    return t >= end_max || t + n <= first_min || (t + n <= from_min && t >= sink_max);
+    return (t >= end_max) | (t + n <= first_min) | ((t + n <= from_min) & (t >= sink_max));
   }
   __device__ __forceinline__ bool all(int32_t t, int32_t n) const {
-    return t >= first_max && t + n <= end_min && (t >= from_max || t + n <= sink_min);
+    return (t >= first_max) & (t + n <= end_min) & ((t >= from_max) | (t + n <= sink_min));
   }
 };
 
@@ -427,11 +428,11 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
         r.top = r.shared = positions_max(d);
         r.least = -INFINITY;
       } else {
-        inside = t0 + tok < t_end && !gb.none(t0 + tok, 1);
-        const bool shared = inside && gb.all(t0 + tok, 1);
+        inside = (t0 + tok < t_end) & !gb.none(t0 + tok, 1);
+        const bool shared = inside & gb.all(t0 + tok, 1);
         r.top = positions_max(inside ? d : 0.f);
         r.shared = positions_max(shared ? d : 0.f);
-        r.least = positions_max(inside && !shared && d > 0.f ? -d : -INFINITY);
+        r.least = positions_max((inside & !shared & (d > 0.f)) ? -d : -INFINITY);
       }
       if (lane == 0) s_range[wave] = r;
     }
@@ -466,8 +467,8 @@ scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per
         dk = __builtin_amdgcn_ldexpf(ks.scale(), -e);
         dv = __builtin_amdgcn_ldexpf(vs.scale(), -(v_exp > -1000 ? v_exp : 0));
       }
-      const bool left_out = Q8 && partial && !(dv < kLeftOut);
-      bad = left_out && inside;
+      const bool left_out = Q8 & partial & !(dv < kLeftOut);
+      bad = left_out & inside;
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
         const int c = Share<T, NC>::chunk(part, j) * 16;

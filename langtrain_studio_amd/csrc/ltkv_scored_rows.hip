@@ -699,12 +699,12 @@ scored_rows_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int head_tile
           for (int j = 0; j < NC; ++j) most = __builtin_elementwise_max(most, dv[u][j]);
         const float top_d = __builtin_fmaxf(__builtin_fmaxf((float)most[0], (float)most[1]),
                                             __builtin_fmaxf((float)most[2], (float)most[3]));
-        if (__builtin_amdgcn_ballot_w64(top_d > scale_top && mine)) {
+        if (__builtin_amdgcn_ballot_w64((top_d > scale_top) & mine)) {
           const float d = __builtin_fminf(rows_reduce<true>(top_d), 65504.f);  // the same in every column
           const int ex = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(d));
           // (a pack: only of the rows that see the scale, and not met a larger one)
           const float to_top = __builtin_amdgcn_ldexpf(1.f, ex);
-          const bool raise = !PACK || (mine && to_top > scale_top);
+          const bool raise = !PACK | (mine & (to_top > scale_top));
           const float next = raise ? (float)(kTopExp - ex) - kSlack : lift, f = __builtin_amdgcn_exp2f(next - lift);
           sum *= f;
 #pragma unroll
