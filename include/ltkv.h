@@ -335,16 +335,22 @@ LTKV_API int ltkv_append_decode_attention(ltkv_cache *c, size_t layer, size_t n,
  * softcap) where softcap > 0 (caps over 2^96 count as that), minus d_slopes[h] *
  * |p - t| for query head h (d_slopes may be null); the output is V weighted by
  * the softmax of the scores over the visible positions, zeros where there are
- * none. Positions a row does not see do not enter its result, whatever they hold
- * (a row that sees an infinity or NaN gives values that are not finite).
- * f32 rows are computed to f32 accuracy; f16 and bf16 rows take Q as it is
- * and weights rounded to f16, summed in f32.
+ * none, also for a row that would stand before position 0 (p < 0). Positions a
+ * row does not see do not enter its result, whatever they hold; what a row that
+ * sees an infinity or NaN gives is not specified.
+ * f32 rows are computed to f32 accuracy; f16 and bf16 rows take Q as it is and
+ * weights rounded to f16, summed in f32 (chunks on Q8_0 pools: V rounded to f16
+ * too). Values of f32 and Q8_0 pools enter the products as f16 pairs times a
+ * power of two that a row's positions share: an element of V, or of K within 32
+ * to 64 positions, keeps 22 bits down to 2^16 below the largest that the row sees,
+ * and fewer below that.
  * max_rows: the most rows of one sequence, which chooses the kernels (one with
  * more rows is computed all the same): on the matrix cores head_dim that is a
  * multiple of 8 up to 256 (f32 pools: up to 128; Q8_0: 32, 64, 96, 128, 192,
- * 256), prompt chunks fastest at head_dim 64 and 128 on pools other than f32. Rows before the first start or behind
- * the last are left as they were. Tables, lengths and faults as
- * ltkv_decode_attention; q and out 16-byte aligned and apart; head_dim up to 1024.
+ * 256), prompt chunks fastest at head_dim 64 and 128 on pools other than f32.
+ * Rows before the first start or behind the last are left as they were. Tables,
+ * lengths and faults as ltkv_decode_attention (entries of blocks that no row sees
+ * may hold anything); q and out 16-byte aligned and apart; head_dim up to 1024.
  * Summation orders depend on the call's shape, not only on a row's own length.
  * No reference counterpart: the reference's models have neither (model.rs:431-475
  * is plain causal attention). */

@@ -123,7 +123,8 @@ __global__ void __launch_bounds__(kAnyThreads) scored_any_kernel(ScoredArgs a, i
 // ROWS: only part slots of sequences' rows: a thread an element, 16 parts' loads
 // at a time, since latency counts (one context's fold 4.6 us, 5.8 with four
 // elements a thread), and no searches. Else four elements a thread: the splits
-// are many (27 -> 15 us for six chunks of 512 rows).
+// are many (27 -> 15 us for six chunks of 512 rows, 9.4 by the call's rows instead
+// of the tiles').
 constexpr int kMergeThreads = 256;
 constexpr int merge_vec(bool rows) { return rows ? 1 : 4; }
 

@@ -201,19 +201,22 @@ struct Bounds {
 // head: 128 / group rows; each of its four waves 32 of them. Tiles of 64
 // positions go through LDS as f16 numbers, on 32x32x16 products (two chains of
 // dependent ones for the scores, one per 32 positions): scores^T = K Q^T, weights
-// in place, numerators^T += V^T W (a lane's scores are positions 8 (r / 4) + 4 (lane / 32) + r % 4 of its column,
-// which is the second product's operand layout when its 16 positions are taken
-// as 4 (lane / 32) ... + 3 and 8 + 4 (lane / 32) ... + 3: no exchange). FULL
+// in place, numerators^T += V^T W (a lane's scores are positions 8 (r / 4) + 4
+// (lane / 32) + r % 4 of its column, which is the second product's operand layout
+// when its 16 positions are taken as 4 (lane / 32) ... + 3 and 8 + 4 (lane / 32)
+// ... + 3: no exchange). FULL
 // (f32 rows, and any rows with a cap over kShortCap): Q and the weights as hi +
-// lo pairs; else Q as it is (times a power of two) and the weights rounded to f16.
+// lo pairs; else Q as it is (times a power of two), the weights rounded to f16, and
+// V of q8_0 pools by its hi parts alone (one f16 rounding, as the weights': a third
+// of the products less).
 //
-// A prompt of 4096 bf16 rows at 32 / 8 heads of 128 with capped scores takes 219
-// us (137 GFLOP, 627 TFLOP/s): per tile and wave 32 products (~1000 cycles) stand
+// A prompt of 4096 bf16 rows at 32 / 8 heads of 128 with capped scores takes 224
+// us (137 GFLOP, 615 TFLOP/s): per tile and wave 32 products (~1000 cycles) stand
 // beside 32 scores a lane of two exp2, one reciprocal and ~5 other vector
 // instructions each, which the two work-groups of a CU only partly overlap (MFMA
 // busy 27%, VALU 48%). Six chunks of up to 512 f32 rows behind 4-bit contexts at
-// 28 / 4 heads: 191 us (149 GFLOP of hi and lo products, 780 TFLOP/s; MFMA busy
-// 44%, VALU 45%).
+// 28 / 4 heads: 188 us with their merge (149 GFLOP of hi and lo products, 790
+// TFLOP/s; MFMA busy 44%, VALU 45%).
 template <typename T, int HD, bool FULL>
 __global__ void __launch_bounds__(64 * kChunkWaves, 2)
 scored_chunk_kernel(ScoredArgs a, int64_t n_blocks, int64_t kv_dim, int rows_per_tile, int64_t min_rows,

@@ -134,7 +134,8 @@ struct Cells<int8_t, NC, SPAN> {
 };
 
 // f32 elements enter the products as f16 hi + lo parts of the element times a
-// power of two, which brings the step's largest below 2^kTopExp.
+// power of two, which brings the step's largest below 2^kTopExp (22 bits down to
+// 2^16 below it, fewer for smaller elements).
 template <int NC, bool SPAN>
 struct Cells<float, NC, SPAN> {
   f32x4 x[NC][2];
@@ -231,7 +232,7 @@ __device__ __forceinline__ int parts_of(const ScoredArgs &a, int64_t seq) {
 // hi + lo pairs: f32 accuracy for twice the matrix-core work, which is idle
 // here otherwise. A pack's steps that some row sees in part are taken once for
 // each row, with the other rows' columns masked and unseen values as zeros: no
-// row's values meet another's infinities.
+// row's values meet another's infinities, or its powers of two.
 // OCC: waves a SIMD that the registers are cut to.
 //
 // Bound by the vector ALU: a step of 32 q4_0 positions of 128 elements is ~300
