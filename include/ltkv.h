@@ -329,7 +329,8 @@ LTKV_API int ltkv_append_decode_attention(ltkv_cache *c, size_t layer, size_t n,
  * d_row_starts every sequence has one row, and n_rows is n. A row sees the
  * positions t < lens[i] with
  *   t <= p, or t < d_prefix[i] (a bidirectional prefix; d_prefix may be null);
- *   t >= d_first[row] (the start of the row's document; d_first may be null);
+ *   t >= d_first[row] (the start of the row's document, negative ones count as
+ *   0; d_first may be null);
  *   with window > 0, t > p - window or t - d_first[row] < sinks.
  * The score of a position is s = scale * q.k, capped to softcap * tanh(s /
  * softcap) where softcap > 0 (caps over 2^96 count as that), minus d_slopes[h] *

@@ -150,8 +150,8 @@ __device__ __forceinline__ int scale_exponent(float d) { return d > 0.f ? __buil
 // 22 bits down to 2^16 below the largest.) Else it follows that scale, and what
 // then passes the top of f16 is added apart, for the rows that see it
 // (kLeftOut). Positions that no row sees have no part in it. (Against one power
-// for all 64 positions, whoever sees them: chunks of 2 x 1024 f32 rows 178 -> 172
-// us, of bf16 rows 111 -> 126.)
+// for all 64 positions, whoever sees them: chunks of 2 x 1024 f32 rows 176 -> 171
+// us, of bf16 rows 110 -> 126.)
 struct TileRange {
   float k_top;               // largest scale of K
   float top, shared, least;  // V's (least: negative, as a maximum)
