@@ -389,7 +389,10 @@ class KvCache:
         current = torch.cuda.current_stream(self.device)
         if current.cuda_stream == self._stream:
             return torch.zeros_like(t)
-        with torch.cuda.stream(torch.cuda.ExternalStream(self._stream, device=self.device)):
+        own = torch.cuda.default_stream(self.device)  # (the null stream; ExternalStream(0) is a new one)
+        if self._stream:
+            own = torch.cuda.ExternalStream(self._stream, device=self.device)
+        with torch.cuda.stream(own):
             out = torch.zeros_like(t)
         out.record_stream(current)  # the caller's: the memory is not reused under its work
         return out

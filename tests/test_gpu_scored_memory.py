@@ -34,23 +34,26 @@ def free_bytes():
     return torch.cuda.mem_get_info()[0]
 
 
-def test_new_outputs_on_the_caches_stream(gpu):
+@pytest.mark.parametrize("own_stream", [True, False])
+def test_new_outputs_on_the_caches_stream(gpu, own_stream):
     """The rows of no sequence in a new output are cleared before the call writes
-    the others, whatever the current stream is busy with."""
+    the others, whatever the current stream is busy with (a cache without a stream
+    of its own: on the null stream)."""
     import torch
 
     heads, kvh, hd, lens, new = 8, 2, 64, [300, 50], [40, 33]
     starts = np.concatenate([[0], np.cumsum(new)])
-    side = torch.cuda.Stream()
-    kv, tables = build(kvh * hd, lens, "f16", 71, stream=side)
+    kv, tables = build(kvh * hd, lens, "f16", 71, stream=torch.cuda.Stream() if own_stream else None)
     kv.synchronize()
     q = torch.randn((80, heads * hd), device="cuda")
     t, ld, sd = up(tables, np.int32), up(lens, np.int32), up(starts, np.int32)
     a = torch.randn((8192, 8192), device="cuda").half()
     torch.cuda.synchronize()
-    for _ in range(40):  # some 40 ms before the current stream gets to anything else
-        a = a @ a
-    got = kv.scored_attention(0, q, t, ld, heads, hd, row_starts=sd, max_rows=40)
+    current = torch.cuda.current_stream() if own_stream else torch.cuda.Stream()
+    with torch.cuda.stream(current):
+        for _ in range(40):  # some 40 ms before the current stream gets to anything else
+            a = a @ a
+        got = kv.scored_attention(0, q, t, ld, heads, hd, row_starts=sd, max_rows=40)
     torch.cuda.synchronize()
     got = got.cpu().numpy()
     assert (got[73:] == 0).all()
