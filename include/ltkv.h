@@ -194,6 +194,12 @@ LTKV_API int ltkv_write_ordered(ltkv_cache *c, size_t layer, size_t n, const int
                        const float *d_k, const float *d_v, size_t src_stride, size_t m,
                        const int32_t *d_order);
 
+/* Types of the rows of a call: Q and output of scored and tree attention, and K,
+ * V and Q of ltkv_write_rope_rows. */
+#define LTKV_ROWS_F32 0
+#define LTKV_ROWS_F16 1
+#define LTKV_ROWS_BF16 2
+
 /* RoPE of Model::rope (model.rs:291-308) with the table of model.rs:263-265:
  * inv_freq[i] = base^(-2i / rope_dim), angle = pos * inv_freq[i], cos/sin by
  * the host libm (as the reference), pairs (2i, 2i+1) or, with neox, (i, i +
@@ -211,6 +217,51 @@ LTKV_API int ltkv_rope_init(ltkv_cache *c, float base, size_t rope_dim, size_t h
 LTKV_API int ltkv_write_rope(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_slot_mapping,
                     const int32_t *d_positions, const float *d_k, const float *d_v, size_t src_stride,
                     float *d_q, size_t q_stride, size_t n_heads);
+
+/* Scalings of rotary positions for contexts longer than a model was trained on
+ * (ltkv_rope_init_scaled). With f_i = base^(-2i / rope_dim), pair i turns per
+ * position by
+ *   PLAIN   f_i;
+ *   LINEAR  f_i / factor (positions squeezed into the trained range);
+ *   NTK     f_i with base * factor^(rope_dim / (rope_dim - 2)) as base;
+ *   YARN    a blend of f_i / factor and f_i by how often the pair turns within
+ *           `original` positions: f_i where that is `high` times or more, f_i /
+ *           factor at `low` times or less, linear in i between (its ends rounded
+ *           outward to whole pairs); cosines and sines times 1 + 0.1 ln(factor);
+ *   LLAMA3  the same blend, linear in the number of turns between `low` and
+ *           `high`. */
+#define LTKV_ROPE_PLAIN 0
+#define LTKV_ROPE_LINEAR 1
+#define LTKV_ROPE_NTK 2
+#define LTKV_ROPE_YARN 3
+#define LTKV_ROPE_LLAMA3 4
+
+/* ltkv_rope_init with scaled frequencies and 64-bit angles: the table holds the
+ * f32 values of cos and sin (pos * frequency, all in 64 bits) times the
+ * magnitude. factor: of every scaling but PLAIN; original, low and high: of YARN
+ * (usually low 1, high 32) and LLAMA3 (low 1, high 4), ignored by the others.
+ * divisors (host, [rope_dim / 2], or null): each pair's frequency is divided by
+ * its own as well. magnitude: of cosines and sines, 0 for the scaling's own.
+ * Replaces the cache's table for ltkv_write_rope and ltkv_write_rope_rows once
+ * the stream is done with it; a captured append still names the old one. Not
+ * under stream capture. No reference counterpart (its positions are unscaled,
+ * model.rs:263-265). */
+LTKV_API int ltkv_rope_init_scaled(ltkv_cache *c, float base, size_t rope_dim, size_t head_dim, int neox,
+                                   size_t max_positions, int scaling, float factor, size_t original,
+                                   float low, float high, const float *divisors, float magnitude);
+
+/* ltkv_write_rope for rows of row_type (LTKV_ROWS_*; K, V and Q alike, strides in
+ * elements): K rotated in f32 (each product and sum rounded, as there) and
+ * stored as ltkv_write stores f32 rows; V stored so; Q, when d_q is not null,
+ * rotated into d_q_out and rounded to row_type. d_q_out may be d_q with the same
+ * stride, or rows apart from q, k and v (columns of one [q | k | v] buffer are). A
+ * token with a position outside the table is skipped, Q too; one with a negative
+ * or out-of-range cell rotates Q only. Row pointers 16-byte aligned, strides
+ * whole 16-byte pieces, head_dim up to 512. No two rows may have one cell. */
+LTKV_API int ltkv_write_rope_rows(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_slot_mapping,
+                                  const int32_t *d_positions, int row_type, const void *d_k, const void *d_v,
+                                  size_t src_stride, const void *d_q, size_t q_stride, size_t n_heads,
+                                  void *d_q_out, size_t q_out_stride);
 
 /* Kernel 2, block copy: the copy-on-write body of kv.rs:99-110 (all layers,
  * K and V) for n pairs d_pairs[2i] = src block, d_pairs[2i+1] = dst block.
@@ -316,11 +367,6 @@ LTKV_API int ltkv_append_decode_attention(ltkv_cache *c, size_t layer, size_t n,
 
 /* ---- scored attention -------------------------------------------------- */
 
-/* Types of the rows of a scored attention call (its Q and output). */
-#define LTKV_ROWS_F32 0
-#define LTKV_ROWS_F16 1
-#define LTKV_ROWS_BF16 2
-
 /* Attention with capped scores, distance biases and masks, over single tokens
  * and prompt chunks alike. Sequence i (of n) has the rows [d_row_starts[i],
  * d_row_starts[i+1]) of d_q and d_out ([n_rows][n_heads*head_dim] of row_type),
@@ -361,6 +407,91 @@ LTKV_API int ltkv_scored_attention(ltkv_cache *c, size_t layer, size_t n, size_t
                                    const int32_t *d_prefix, const int32_t *d_first, int row_type,
                                    const void *d_q, const int32_t *d_tables, size_t table_stride,
                                    const int32_t *d_lens, const int32_t *d_row_starts, void *d_out);
+
+/* ---- trees of drafted tokens ------------------------------------------- */
+/* A step that checks drafted tokens: ltkv_step_layout lays it out on the device
+ * from the requests' lengths; per layer ltkv_write_rope_rows (or ltkv_write)
+ * stores the drafts' rows and ltkv_tree_attention attends; ltkv_accept_tree keeps
+ * the path that the model agrees with. No reference counterpart (its engine
+ * decodes a token at a time, scheduler.rs:356-450). */
+
+/* Attention of drafted rows over the cache. Sequence i (of n) has the rows
+ * [d_row_starts[i], d_row_starts[i+1]) of d_q and d_out ([n_rows][n_heads *
+ * head_dim] of row_type), whose K and V are its last cells: row j of m is the cell
+ * at position C + j of its d_lens[i] positions, C = lens[i] - m its context. (Write
+ * this step's K and V first.) A row sees
+ *   the context's positions t < C, with window > 0 only t > p - window for the
+ *   row's position p = d_positions[row] (at least C; needed with a window only:
+ *   for a tree it is C plus the row's depth);
+ *   the rows' cells C + j for which bit j % 32 of word j / 32 of its mask is set
+ *   (d_masks [n_rows][mask_words]; rows past the words are not seen; the window
+ *   does not bound these). Without d_masks a row sees the rows up to its own, as
+ *   in a prompt chunk.
+ * The score of a position is scale * q.k, capped to softcap * tanh(s / softcap)
+ * where softcap > 0 (caps over 2^96 count as that); the output is V weighted by the
+ * softmax of the scores over what the row sees, zeros where that is nothing.
+ * Positions a row does not see do not enter its result, whatever they hold; what
+ * a row that sees an infinity or NaN gives is not specified (it is not finite
+ * where a visible V is not).
+ * f32 rows are computed to f32 accuracy, f16 and bf16 rows with weights (and V of
+ * f32 and Q8_0 pools) rounded to f16, summed in f32. Elements of f32 and Q8_0 pools
+ * keep 22 bits down to 2^16 below the largest of their row's head.
+ * max_rows: the most rows of one sequence, which sizes the tiles (one with more is
+ * computed all the same). head_dim a multiple of 8 up to 256 and groups of up to
+ * 64 run on the matrix cores, others on a generic kernel; head_dim up to 1024. Rows
+ * of no sequence are left as they were. Tables, lengths and faults as
+ * ltkv_decode_attention (entries of blocks that no row sees may hold anything); q
+ * and out 16-byte aligned and apart. Summation orders depend on the call's shape.
+ * Calls under stream capture need their partials allocated: make the call once
+ * before capturing it. */
+LTKV_API int ltkv_tree_attention(ltkv_cache *c, size_t layer, size_t n, size_t n_rows, size_t max_rows,
+                                 size_t n_heads, size_t head_dim, float scale, float softcap, size_t window,
+                                 const int32_t *d_positions, const int32_t *d_masks, size_t mask_words,
+                                 int row_type, const void *d_q, const int32_t *d_tables, size_t table_stride,
+                                 const int32_t *d_lens, const int32_t *d_row_starts, void *d_out);
+
+/* The arrays of a step, on the device, from its requests' lengths: request i holds
+ * d_lens[i] tokens of the sequence in row d_rows[i] of the resident tables (-1: no
+ * request, without tokens) and gets d_counts[i] new ones (null: one each), whose
+ * cells are claimed (ltkv_append_batch). Outputs:
+ *   d_row_starts [n + 1]: request i has tokens [d_row_starts[i], d_row_starts[i+1]);
+ *   d_new_lens [n]: lens + counts;
+ *   d_tables [n][table_stride]: block tables of these lengths, -1 behind them;
+ *   d_slot_mapping, d_positions [n_tokens]: each token's cell (-1 without one, as
+ *   ltkv_slot_mapping) and position, both -1 behind the last token;
+ *   with d_parents [n_tokens] (each token's parent among its request's tokens, one
+ *   before it; anything else, as -1, makes a root): positions are lens plus the
+ *   token's depth in its tree, and d_masks [n_tokens][mask_words] gets the bits of
+ *   the token and its ancestors, for ltkv_tree_attention (zeros behind the last
+ *   token; tokens from 32 * mask_words of a request on have no bit).
+ * Tokens beyond n_tokens are left out of their request; that, tokens without a
+ * block and tables narrower than a length are reported by ltkv_synchronize
+ * (LTKV_ERR_RANGE). Inputs and outputs may not overlap. Pending table changes are
+ * uploaded first; refused under stream capture (lay the step out before, capture
+ * its layers). */
+LTKV_API int ltkv_step_layout(ltkv_cache *c, size_t n, const int32_t *d_rows, const int32_t *d_lens,
+                              const int32_t *d_counts, size_t n_tokens, size_t table_stride,
+                              const int32_t *d_parents, size_t mask_words, int32_t *d_row_starts,
+                              int32_t *d_new_lens, int32_t *d_tables, int32_t *d_slot_mapping,
+                              int32_t *d_positions, int32_t *d_masks);
+
+/* Keeps what the model agrees with of every request's drafted tree, in all layers.
+ * Request i's rows lie as in ltkv_tree_attention (d_lens with the drafts); its
+ * token j has parent d_parents[j] (before it), token d_tokens[j], and the model
+ * chose d_targets[j] behind it. Token 0 is kept; from a kept token the lowest
+ * child whose token is the kept one's target is kept next, until there is none.
+ * The K and V rows of the kept tokens move together, the k-th to position C + k;
+ * cells behind them hold what they held. Outputs: d_accepted [n] how many were
+ * kept (0 without rows), d_path [n_rows] the kept tokens in order, -1 behind them
+ * and in rows of no request; d_next [n] the last one's target (-1 without rows);
+ * d_new_lens [n] the length after it (truncate the sequences to it). Blocks shared
+ * with other sequences must have been copied, as appending the drafts does. A
+ * table entry outside the pool moves nothing and is reported by ltkv_synchronize.
+ * Inputs and outputs may not overlap. */
+LTKV_API int ltkv_accept_tree(ltkv_cache *c, size_t n, size_t n_rows, const int32_t *d_tables,
+                              size_t table_stride, const int32_t *d_lens, const int32_t *d_row_starts,
+                              const int32_t *d_parents, const int32_t *d_tokens, const int32_t *d_targets,
+                              int32_t *d_accepted, int32_t *d_path, int32_t *d_next, int32_t *d_new_lens);
 
 /* Tokens per context partition of the decode attention split (multiple of
  * 64), or 0 (the default) for the per-query policy: a query is split into
@@ -512,7 +643,8 @@ LTKV_API int ltkv_write_row(ltkv_cache *c, size_t layer, uint32_t block, uint32_
  *   LTKV_ERR_RANGE  a block-table entry outside the pool was read by attention
  *                   (which used block 0 in its place) or by gather (which copied
  *                   nothing for it), or a resident-table row outside the tables
- *                   came with a nonzero length;
+ *                   came with a nonzero length; or a request of ltkv_step_layout
+ *                   had more tokens than its blocks, the tables or arrays hold;
  *   LTKV_ERR_ARG    a fused append + attention cell (ltkv_append_decode_attention)
  *                   was not position lens[i] - 1 of query i's table.
  * ltkv_last_error() names the query (or gathered sequence). */

@@ -35,6 +35,11 @@ pub mod ffi {
     pub const LTKV_ROWS_F32: c_int = 0;
     pub const LTKV_ROWS_F16: c_int = 1;
     pub const LTKV_ROWS_BF16: c_int = 2;
+    pub const LTKV_ROPE_PLAIN: c_int = 0;
+    pub const LTKV_ROPE_LINEAR: c_int = 1;
+    pub const LTKV_ROPE_NTK: c_int = 2;
+    pub const LTKV_ROPE_YARN: c_int = 3;
+    pub const LTKV_ROPE_LLAMA3: c_int = 4;
     pub const LTKV_PLAN_SHARED_PREFIX: c_uint = 1;
     pub const LTKV_PLAN_F16_PRODUCTS: c_uint = 2;
     pub const LTKV_NOALLOC_SCRATCH_BYTES: usize = 32 << 20;
@@ -86,6 +91,13 @@ pub mod ffi {
         pub fn ltkv_write_rope(c: *mut ltkv_cache, layer: usize, n: usize, d_slot_mapping: *const i32,
                                d_positions: *const i32, d_k: *const f32, d_v: *const f32, src_stride: usize,
                                d_q: *mut f32, q_stride: usize, n_heads: usize) -> c_int;
+        pub fn ltkv_rope_init_scaled(c: *mut ltkv_cache, base: f32, rope_dim: usize, head_dim: usize, neox: c_int,
+                                     max_positions: usize, scaling: c_int, factor: f32, original: usize, low: f32,
+                                     high: f32, divisors: *const f32, magnitude: f32) -> c_int;
+        pub fn ltkv_write_rope_rows(c: *mut ltkv_cache, layer: usize, n: usize, d_slot_mapping: *const i32,
+                                    d_positions: *const i32, row_type: c_int, d_k: *const c_void, d_v: *const c_void,
+                                    src_stride: usize, d_q: *const c_void, q_stride: usize, n_heads: usize,
+                                    d_q_out: *mut c_void, q_out_stride: usize) -> c_int;
         pub fn ltkv_copy_blocks(c: *mut ltkv_cache, n: usize, d_pairs: *const i32) -> c_int;
         pub fn ltkv_gather(c: *mut ltkv_cache, layer: usize, n: usize, d_tables: *const i32, table_stride: usize,
                            d_lens: *const i32, d_out_offsets: *const i64, d_k_out: *mut c_void,
@@ -110,6 +122,23 @@ pub mod ffi {
                                      d_first: *const i32, row_type: c_int, d_q: *const c_void,
                                      d_tables: *const i32, table_stride: usize, d_lens: *const i32,
                                      d_row_starts: *const i32, d_out: *mut c_void) -> c_int;
+
+        // trees of drafted tokens
+        pub fn ltkv_tree_attention(c: *mut ltkv_cache, layer: usize, n: usize, n_rows: usize, max_rows: usize,
+                                   n_heads: usize, head_dim: usize, scale: f32, softcap: f32, window: usize,
+                                   d_positions: *const i32, d_masks: *const i32, mask_words: usize, row_type: c_int,
+                                   d_q: *const c_void, d_tables: *const i32, table_stride: usize,
+                                   d_lens: *const i32, d_row_starts: *const i32, d_out: *mut c_void) -> c_int;
+        pub fn ltkv_step_layout(c: *mut ltkv_cache, n: usize, d_rows: *const i32, d_lens: *const i32,
+                                d_counts: *const i32, n_tokens: usize, table_stride: usize, d_parents: *const i32,
+                                mask_words: usize, d_row_starts: *mut i32, d_new_lens: *mut i32, d_tables: *mut i32,
+                                d_slot_mapping: *mut i32, d_positions: *mut i32, d_masks: *mut i32) -> c_int;
+        pub fn ltkv_accept_tree(c: *mut ltkv_cache, n: usize, n_rows: usize, d_tables: *const i32,
+                                table_stride: usize, d_lens: *const i32, d_row_starts: *const i32,
+                                d_parents: *const i32, d_tokens: *const i32, d_targets: *const i32,
+                                d_accepted: *mut i32, d_path: *mut i32, d_next: *mut i32,
+                                d_new_lens: *mut i32) -> c_int;
+
         pub fn ltkv_set_attention_partition(c: *mut ltkv_cache, tokens: usize) -> c_int;
         pub fn ltkv_set_attention_engine(c: *mut ltkv_cache, engine: c_int) -> c_int;
 
@@ -155,12 +184,35 @@ pub enum Dtype {
     Q4_0,
 }
 
-/// Type of the rows (Q and output) of `KvCache::scored_attention`.
+/// Type of the rows of `KvCache::scored_attention`, `tree_attention` (Q and output)
+/// and `write_rope_rows` (K, V and Q).
 #[derive(Clone, Copy, Debug, PartialEq, Eq)]
 pub enum RowType {
     F32,
     F16,
     BF16,
+}
+
+impl RowType {
+    fn code(self) -> c_int {
+        match self {
+            RowType::F32 => LTKV_ROWS_F32,
+            RowType::F16 => LTKV_ROWS_F16,
+            RowType::BF16 => LTKV_ROWS_BF16,
+        }
+    }
+}
+
+/// How `KvCache::rope_init_scaled` scales positions: `kind` is an `LTKV_ROPE_*`
+/// code, `magnitude` 0 means the kind's own.
+#[derive(Clone, Copy, Debug)]
+pub struct RopeScaling {
+    pub kind: c_int,
+    pub factor: f32,
+    pub original: usize,
+    pub low: f32,
+    pub high: f32,
+    pub magnitude: f32,
 }
 
 /// What `KvCache::scored_attention` does to scores and which positions a row
@@ -476,6 +528,27 @@ impl KvCache {
                               n_heads))
     }
 
+    /// `rope_init` with scaled frequencies and 64-bit angles; `divisors` is empty or
+    /// has one entry per pair.
+    pub fn rope_init_scaled(&mut self, base: f32, rope_dim: usize, head_dim: usize, neox: bool, max_positions: usize,
+                            how: &RopeScaling, divisors: &[f32]) -> anyhow::Result<()> {
+        anyhow::ensure!(divisors.is_empty() || divisors.len() == rope_dim / 2, "divisors need one entry per pair");
+        let d = if divisors.is_empty() { std::ptr::null() } else { divisors.as_ptr() };
+        check(unsafe {
+            ltkv_rope_init_scaled(self.raw, base, rope_dim, head_dim, neox as c_int, max_positions, how.kind, how.factor,
+                                  how.original, how.low, how.high, d, how.magnitude)
+        })
+    }
+
+    /// `write_rope` for rows of any type, Q (may be null) rotated into `d_q_out`.
+    pub unsafe fn write_rope_rows(&mut self, layer: usize, n: usize, d_slot_mapping: *const i32,
+                                  d_positions: *const i32, rows: RowType, d_k: *const c_void, d_v: *const c_void,
+                                  src_stride: usize, d_q: *const c_void, q_stride: usize, n_heads: usize,
+                                  d_q_out: *mut c_void, q_out_stride: usize) -> anyhow::Result<()> {
+        check(ltkv_write_rope_rows(self.raw, layer, n, d_slot_mapping, d_positions, rows.code(), d_k, d_v, src_stride,
+                                   d_q, q_stride, n_heads, d_q_out, q_out_stride))
+    }
+
     /// Kernel 2 (the copy-on-write body of kv.rs:99-110) for device (src, dst) pairs.
     pub unsafe fn copy_blocks(&mut self, n: usize, d_pairs: *const i32) -> anyhow::Result<()> {
         check(ltkv_copy_blocks(self.raw, n, d_pairs))
@@ -502,14 +575,43 @@ impl KvCache {
                                    head_dim: usize, how: &Scoring, rows: RowType, d_q: *const c_void,
                                    d_tables: *const i32, table_stride: usize, d_lens: *const i32,
                                    d_row_starts: *const i32, d_out: *mut c_void) -> anyhow::Result<()> {
-        let row_type = match rows {
-            RowType::F32 => LTKV_ROWS_F32,
-            RowType::F16 => LTKV_ROWS_F16,
-            RowType::BF16 => LTKV_ROWS_BF16,
-        };
+        let row_type = rows.code();
         check(ltkv_scored_attention(self.raw, layer, n, n_rows, max_rows, n_heads, head_dim, how.scale, how.softcap,
                                     how.d_slopes, how.window, how.sinks, how.d_prefix, how.d_first, row_type, d_q,
                                     d_tables, table_stride, d_lens, d_row_starts, d_out))
+    }
+
+    /// Attention of drafted rows: sequence i has rows
+    /// d_row_starts[i]..d_row_starts[i+1] of n_rows, at most about max_rows each;
+    /// d_masks and d_positions may be null (`ltkv_tree_attention`).
+    pub unsafe fn tree_attention(&mut self, layer: usize, n: usize, n_rows: usize, max_rows: usize, n_heads: usize,
+                                 head_dim: usize, scale: f32, softcap: f32, window: usize, d_positions: *const i32,
+                                 d_masks: *const i32, mask_words: usize, rows: RowType, d_q: *const c_void,
+                                 d_tables: *const i32, table_stride: usize, d_lens: *const i32,
+                                 d_row_starts: *const i32, d_out: *mut c_void) -> anyhow::Result<()> {
+        check(ltkv_tree_attention(self.raw, layer, n, n_rows, max_rows, n_heads, head_dim, scale, softcap, window,
+                                  d_positions, d_masks, mask_words, rows.code(), d_q, d_tables, table_stride, d_lens,
+                                  d_row_starts, d_out))
+    }
+
+    /// A step's arrays from its requests' lengths (`ltkv_step_layout`).
+    pub unsafe fn step_layout(&mut self, n: usize, d_rows: *const i32, d_lens: *const i32, d_counts: *const i32,
+                              n_tokens: usize, table_stride: usize, d_parents: *const i32, mask_words: usize,
+                              d_row_starts: *mut i32, d_new_lens: *mut i32, d_tables: *mut i32,
+                              d_slot_mapping: *mut i32, d_positions: *mut i32,
+                              d_masks: *mut i32) -> anyhow::Result<()> {
+        check(ltkv_step_layout(self.raw, n, d_rows, d_lens, d_counts, n_tokens, table_stride, d_parents, mask_words,
+                               d_row_starts, d_new_lens, d_tables, d_slot_mapping, d_positions, d_masks))
+    }
+
+    /// Keeps the path of every drafted tree that the model agrees with
+    /// (`ltkv_accept_tree`); truncate the sequences to d_new_lens.
+    pub unsafe fn accept_tree(&mut self, n: usize, n_rows: usize, d_tables: *const i32, table_stride: usize,
+                              d_lens: *const i32, d_row_starts: *const i32, d_parents: *const i32,
+                              d_tokens: *const i32, d_targets: *const i32, d_accepted: *mut i32, d_path: *mut i32,
+                              d_next: *mut i32, d_new_lens: *mut i32) -> anyhow::Result<()> {
+        check(ltkv_accept_tree(self.raw, n, n_rows, d_tables, table_stride, d_lens, d_row_starts, d_parents, d_tokens,
+                               d_targets, d_accepted, d_path, d_next, d_new_lens))
     }
 
     /// Kernel 4 (the attention closure of model.rs:431-475).

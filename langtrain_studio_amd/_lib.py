@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libltkv.so"
 OK, ERR_FULL, ERR_NONCONTIG, ERR_RANGE, ERR_HIP, ERR_ARG = 0, 1, 2, 3, 4, 5
 F16, F32, Q8_0, Q4_0 = 0, 1, 2, 3
 ROWS_F32, ROWS_F16, ROWS_BF16 = 0, 1, 2
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN, ROPE_LLAMA3 = 0, 1, 2, 3, 4
 PLAN_SHARED_PREFIX, PLAN_F16_PRODUCTS = 1, 2
 ENGINE_AUTO, ENGINE_VALU = 0, 1
 NO_DEVICE = -1
@@ -50,6 +51,8 @@ SIGNATURES = {
     "ltkv_write_ordered": (_int, [_vp, _sz, _sz, _vp, _vp, _vp, _sz, _sz, _vp]),
     "ltkv_rope_init": (_int, [_vp, _f32, _sz, _sz, _int, _sz]),
     "ltkv_write_rope": (_int, [_vp, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _sz]),
+    "ltkv_rope_init_scaled": (_int, [_vp, _f32, _sz, _sz, _int, _sz, _int, _f32, _sz, _f32, _f32, _vp, _f32]),
+    "ltkv_write_rope_rows": (_int, [_vp, _sz, _sz, _vp, _vp, _int, _vp, _vp, _sz, _vp, _sz, _sz, _vp, _sz]),
     "ltkv_copy_blocks": (_int, [_vp, _sz, _vp]),
     "ltkv_gather": (_int, [_vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp]),
     "ltkv_gather_values": (_int, [_vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp]),
@@ -59,6 +62,10 @@ SIGNATURES = {
                                             _sz, _vp]),
     "ltkv_scored_attention": (_int, [_vp, _sz, _sz, _sz, _sz, _sz, _sz, _f32, _f32, _vp, _sz, _sz, _vp, _vp, _int,
                                      _vp, _vp, _sz, _vp, _vp, _vp]),
+    "ltkv_tree_attention": (_int, [_vp, _sz, _sz, _sz, _sz, _sz, _sz, _f32, _f32, _sz, _vp, _vp, _sz, _int, _vp, _vp,
+                                   _sz, _vp, _vp, _vp]),
+    "ltkv_step_layout": (_int, [_vp, _sz, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ltkv_accept_tree": (_int, [_vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "ltkv_set_attention_partition": (_int, [_vp, _sz]),
     "ltkv_set_attention_engine": (_int, [_vp, _int]),
     "ltkv_plan_attention": (_int, [_vp, _sz, _vp, _vp, _sz, _sz, _u32]),

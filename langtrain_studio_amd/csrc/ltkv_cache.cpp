@@ -415,8 +415,11 @@ int take_status(ltkv_cache *c) {
                 "a device op read a block-table entry outside the pool (query or sequence %d); it read "
                 "block 0 in its place (attention) or copied nothing (gather)",
                 st[1]);
-  return fail(LTKV_ERR_ARG,
-              "fused append + attention: the cell of query %d is not position len - 1 of its table", st[1]);
+  if (st[0] & 2)
+    return fail(LTKV_ERR_ARG,
+                "fused append + attention: the cell of query %d is not position len - 1 of its table", st[1]);
+  return fail(LTKV_ERR_RANGE,
+              "step layout: request %d has more tokens than its blocks, the tables or the token arrays hold", st[1]);
 }
 
 int check_attention_shape(const ltkv_cache *c, size_t n_heads, size_t head_dim, size_t *group) {
@@ -1507,6 +1510,168 @@ int ltkv_write_rope(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_slot
   return LTKV_OK;
 }
 
+namespace {
+
+// Angle that a position adds to pair i of rope_dim dimensions, and the rotation's
+// magnitude, under a scaling of positions (ltkv_rope_init_scaled). In 64 bits.
+void rope_frequencies(std::vector<double> &f, double base, size_t rope_dim, int scaling, double factor, double original,
+                      double low, double high, double *magnitude) {
+  const double pi = 3.14159265358979323846, d = (double)rope_dim;
+  if (scaling == LTKV_ROPE_NTK) base = base * std::pow(factor, d / (d - 2.0));
+  f.resize(rope_dim / 2);
+  for (size_t i = 0; i < f.size(); ++i) f[i] = std::pow(base, -2.0 * (double)i / d);
+  *magnitude = 1.0;
+  if (scaling == LTKV_ROPE_LINEAR) {
+    for (double &x : f) x = x / factor;
+  } else if (scaling == LTKV_ROPE_LLAMA3) {
+    for (double &x : f) {
+      const double turns = original * x / (2.0 * pi);
+      const double blend = std::min(std::max((turns - low) / (high - low), 0.0), 1.0);
+      x = x / factor * (1.0 - blend) + x * blend;
+    }
+  } else if (scaling == LTKV_ROPE_YARN) {
+    auto pair = [&](double turns) { return d * std::log(original / (turns * 2.0 * pi)) / (2.0 * std::log(base)); };
+    const double lo = std::max(std::floor(pair(high)), 0.0), hi = std::min(std::ceil(pair(low)), d - 1.0);
+    for (size_t i = 0; i < f.size(); ++i) {
+      const double blend = std::min(std::max(((double)i - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
+      f[i] = f[i] / factor * blend + f[i] * (1.0 - blend);
+    }
+    *magnitude = 0.1 * std::log(factor) + 1.0;
+  }
+}
+
+}  // namespace
+
+int ltkv_rope_init_scaled(ltkv_cache *c, float base, size_t rope_dim, size_t head_dim, int neox, size_t max_positions,
+                          int scaling, float factor, size_t original, float low, float high, const float *divisors,
+                          float magnitude) {
+  if (!c) return fail(LTKV_ERR_ARG, "cache is null");
+  if (c->device == LTKV_NO_DEVICE) return no_device();
+  if (head_dim == 0 || head_dim % 8 != 0 || c->kv_dim % head_dim != 0)
+    return fail(LTKV_ERR_ARG, "head_dim %zu must be a multiple of 8 dividing kv_dim %zu", head_dim, c->kv_dim);
+  if (rope_dim == 0 || rope_dim % 8 != 0 || rope_dim > head_dim)
+    return fail(LTKV_ERR_ARG, "rope_dim %zu must be a multiple of 8 and at most head_dim", rope_dim);
+  if (max_positions == 0 || max_positions > (size_t)INT32_MAX / 2 ||
+      max_positions > ((size_t{1} << 32) - 256) / (rope_dim / 2))
+    return fail(LTKV_ERR_ARG, "max_positions out of range");
+  if (!(base > 0.f) || std::isinf(base)) return fail(LTKV_ERR_ARG, "rope base must be positive");
+  if (scaling < LTKV_ROPE_PLAIN || scaling > LTKV_ROPE_LLAMA3) return fail(LTKV_ERR_ARG, "unknown rope scaling %d", scaling);
+  if (scaling != LTKV_ROPE_PLAIN && (!(factor > 0.f) || std::isinf(factor)))
+    return fail(LTKV_ERR_ARG, "a rope scaling's factor must be positive");
+  if (scaling == LTKV_ROPE_YARN || scaling == LTKV_ROPE_LLAMA3) {
+    if (original == 0) return fail(LTKV_ERR_ARG, "this rope scaling needs the original context length");
+    if (!(low > 0.f) || !(high > low) || std::isinf(high))
+      return fail(LTKV_ERR_ARG, "this rope scaling needs 0 < low < high");
+  }
+  if (scaling == LTKV_ROPE_YARN && !(base > 1.f)) return fail(LTKV_ERR_ARG, "this rope scaling needs a base over 1");
+  if (!(magnitude >= 0.f) || std::isinf(magnitude))
+    return fail(LTKV_ERR_ARG, "magnitude must be positive, or 0 for the scaling's own");
+  std::vector<double> f;
+  double own = 1.0;
+  try {
+    rope_frequencies(f, base, rope_dim, scaling, factor, (double)original, low, high, &own);
+  } catch (const std::bad_alloc &) {
+    return fail(LTKV_ERR_ARG, "out of host memory");
+  }
+  if (divisors) {
+    for (size_t i = 0; i < f.size(); ++i) {
+      if (!(divisors[i] > 0.f) || std::isinf(divisors[i])) return fail(LTKV_ERR_ARG, "rope divisors must be positive");
+      f[i] /= (double)divisors[i];
+    }
+  }
+  DeviceGuard dg(c->device);
+  if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
+  if (capturing(c)) return fail(LTKV_ERR_ARG, "a rope table cannot be made under stream capture");
+  // The new table first: a failure leaves the old one in use.
+  float *table = nullptr;
+  double *d_f = nullptr;
+  const size_t half = rope_dim / 2;
+  HIP_TRY(hipMalloc((void **)&table, max_positions * half * 2 * sizeof(float)), "hipMalloc(rope table)");
+  hipError_t e = hipMalloc((void **)&d_f, half * sizeof(double));
+  if (e == hipSuccess) e = hipMemcpy(d_f, f.data(), half * sizeof(double), hipMemcpyHostToDevice);
+  if (e == hipSuccess)
+    e = ltkv::launch_rope_table(d_f, magnitude > 0.f ? magnitude : (float)own, (int)half, (int64_t)max_positions, table,
+                                c->stream);
+  // (enqueued appends may still read the old table, the launch the frequencies)
+  if (e == hipSuccess) e = c->stream ? hipStreamSynchronize(c->stream) : hipDeviceSynchronize();
+  (void)hipFree(d_f);
+  if (e != hipSuccess) {
+    (void)hipFree(table);
+    return hip_fail(e, "rope table");
+  }
+  if (c->rope) (void)hipFree(c->rope);
+  c->rope = table;
+  c->rope_geom.table = table;
+  c->rope_geom.max_pos = (int)max_positions;
+  c->rope_geom.rope_dim = (int)rope_dim;
+  c->rope_geom.head_dim = (int)head_dim;
+  c->rope_geom.neox = neox ? 1 : 0;
+  return LTKV_OK;
+}
+
+int ltkv_write_rope_rows(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_slot_mapping,
+                         const int32_t *d_positions, int row_type, const void *d_k, const void *d_v, size_t src_stride,
+                         const void *d_q, size_t q_stride, size_t n_heads, void *d_q_out, size_t q_out_stride) {
+  if (!c) return fail(LTKV_ERR_ARG, "cache is null");
+  if (c->device == LTKV_NO_DEVICE) return no_device();
+  if (!c->rope) return fail(LTKV_ERR_ARG, "no RoPE table (ltkv_rope_init, ltkv_rope_init_scaled)");
+  if (layer >= c->n_layers) return fail(LTKV_ERR_RANGE, "layer %zu out of range (%zu)", layer, c->n_layers);
+  if (row_type != LTKV_ROWS_F32 && row_type != LTKV_ROWS_F16 && row_type != LTKV_ROWS_BF16)
+    return fail(LTKV_ERR_ARG, "unknown row type %d", row_type);
+  const size_t hd = (size_t)c->rope_geom.head_dim, size = row_type == LTKV_ROWS_F32 ? 4 : 2, unit = 16 / size;
+  if (hd > (size_t)ltkv::kRopeRowsMaxHeadDim)
+    return fail(LTKV_ERR_ARG, "head_dim %zu: at most %d", hd, ltkv::kRopeRowsMaxHeadDim);
+  if (c->quantised() && hd % 32 != 0)
+    return fail(LTKV_ERR_ARG, "the Q8_0 and Q4_0 RoPE appends need head_dim a multiple of 32 (whole scale groups per head)");
+  if (n == 0) return LTKV_OK;
+  if (!d_slot_mapping || !d_positions || !d_k || !d_v) return fail(LTKV_ERR_ARG, "null device pointer");
+  if ((d_q != nullptr) != (d_q_out != nullptr)) return fail(LTKV_ERR_ARG, "q and its output come together");
+  // (row lengths whose bytes fit a pointer's range)
+  const size_t most = (size_t{1} << 40);
+  if (n > (size_t)INT32_MAX || src_stride > most || q_stride > most || q_out_stride > most || n_heads > most / hd)
+    return fail(LTKV_ERR_ARG, "too many rows for one launch");
+  if (src_stride < c->kv_dim || src_stride % unit != 0)
+    return fail(LTKV_ERR_ARG, "src_stride must be >= kv_dim and whole 16-byte pieces");
+  if (d_q && (n_heads == 0 || q_stride < n_heads * hd || q_out_stride < n_heads * hd || q_stride % unit != 0 ||
+              q_out_stride % unit != 0))
+    return fail(LTKV_ERR_ARG, "q strides must be >= n_heads * head_dim and whole 16-byte pieces");
+  if (((uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_q | (uintptr_t)d_q_out) % 16 != 0)
+    return fail(LTKV_ERR_ARG, "K/V/Q rows must be 16-byte aligned");
+  if (d_q && !(d_q == d_q_out && q_stride == q_out_stride)) {  // in place, or apart
+    // (rows of one buffer may interleave: q as columns of a wider output is refused too)
+    const uintptr_t in = (uintptr_t)d_q, out = (uintptr_t)d_q_out;
+    const size_t in_bytes = ((n - 1) * q_stride + n_heads * hd) * size;
+    const size_t out_bytes = ((n - 1) * q_out_stride + n_heads * hd) * size;
+    if (in < out + out_bytes && out < in + in_bytes)
+      return fail(LTKV_ERR_ARG, "q and its output overlap: they are the same rows or apart");
+  }
+  if (d_q) {  // K and V rows are read while Q's are written
+    const uintptr_t out = (uintptr_t)d_q_out;
+    const size_t out_bytes = ((n - 1) * q_out_stride + n_heads * hd) * size;
+    const size_t src_bytes = ((n - 1) * src_stride + c->kv_dim) * size;
+    for (const void *src : {d_k, d_v}) {
+      const uintptr_t in = (uintptr_t)src;
+      if (!(in < out + out_bytes && out < in + src_bytes)) continue;
+      // columns of one buffer ([q | k | v] rows): apart if a row's columns are
+      const bool columns = src_stride == q_out_stride;
+      const size_t row = q_out_stride * size;
+      const size_t at = columns ? (in >= out ? (in - out) % row : (row - (out - in) % row) % row) : 0;
+      if (!columns || at < n_heads * hd * size || at + c->kv_dim * size > row)
+        return fail(LTKV_ERR_ARG, "q's output overlaps the rows of K or V");
+    }
+  }
+  ltkv::RopeRows a{d_slot_mapping, d_positions, row_type, d_k, d_v, d_q, d_q_out, (int64_t)n, (int64_t)src_stride,
+                   (int64_t)q_stride, (int64_t)q_out_stride, d_q ? (int)n_heads : 0};
+  if (d_q && n_heads > (size_t)INT32_MAX / 2 - c->kv_dim) return fail(LTKV_ERR_ARG, "too many heads");
+  DeviceGuard dg(c->device);
+  if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
+  const hipError_t e = ltkv::launch_write_rope_rows(c->geom, c->k_layer(layer), c->v_layer(layer), c->k_scales(layer),
+                                                    c->v_scales(layer), a, c->rope_geom, c->stream);
+  if (e == hipErrorInvalidValue) return fail(LTKV_ERR_ARG, "too many rows for one launch");
+  if (e != hipSuccess) return hip_fail(e, "write_rope_rows launch");
+  return LTKV_OK;
+}
+
 int ltkv_copy_blocks(ltkv_cache *c, size_t n, const int32_t *d_pairs) {
   if (!c) return fail(LTKV_ERR_ARG, "cache is null");
   if (c->device == LTKV_NO_DEVICE) return no_device();
@@ -1916,6 +2081,188 @@ int ltkv_scored_attention(ltkv_cache *c, size_t layer, size_t n, size_t n_rows, 
   a.prefix = d_prefix;
   a.first = d_first;
   return scored_attention(c, a);
+}
+
+namespace {
+
+// Whether two device arrays share bytes.
+bool overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
+  return a && b && (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
+}
+
+}  // namespace
+
+int ltkv_tree_attention(ltkv_cache *c, size_t layer, size_t n, size_t n_rows, size_t max_rows, size_t n_heads,
+                        size_t head_dim, float scale, float softcap, size_t window, const int32_t *d_positions,
+                        const int32_t *d_masks, size_t mask_words, int row_type, const void *d_q,
+                        const int32_t *d_tables, size_t table_stride, const int32_t *d_lens,
+                        const int32_t *d_row_starts, void *d_out) {
+  if (!c) return fail(LTKV_ERR_ARG, "cache is null");
+  if (c->device == LTKV_NO_DEVICE) return no_device();
+  if (layer >= c->n_layers) return fail(LTKV_ERR_RANGE, "layer %zu out of range (%zu)", layer, c->n_layers);
+  size_t group = 0;
+  if (int rc = check_attention_shape(c, n_heads, head_dim, &group)) return rc;
+  if (row_type != LTKV_ROWS_F32 && row_type != LTKV_ROWS_F16 && row_type != LTKV_ROWS_BF16)
+    return fail(LTKV_ERR_ARG, "unknown row type %d", row_type);
+  if (!(softcap >= 0.f) || std::isinf(softcap)) return fail(LTKV_ERR_ARG, "softcap must be 0 (none) or positive");
+  if (!std::isfinite(scale)) return fail(LTKV_ERR_ARG, "scale must be finite");
+  if (n_rows > (size_t)INT32_MAX / 2 || n > (size_t)INT32_MAX / 2)
+    return fail(LTKV_ERR_ARG, "%zu rows of %zu sequences are too many for one call", n_rows, n);
+  if (n == 0 || n_rows == 0) return LTKV_OK;
+  if (max_rows == 0) return fail(LTKV_ERR_ARG, "max_rows must be > 0");
+  if (table_stride == 0) return fail(LTKV_ERR_ARG, "table_stride must be > 0");
+  if (!d_q || !d_tables || !d_lens || !d_row_starts || !d_out) return fail(LTKV_ERR_ARG, "null device pointer");
+  if (window > 0 && !d_positions) return fail(LTKV_ERR_ARG, "a window needs the rows' positions");
+  if (d_masks && (mask_words == 0 || mask_words > (size_t)INT32_MAX / 32))
+    return fail(LTKV_ERR_ARG, "masks need 1 to 2^26 words a row");
+  if (((uintptr_t)d_q | (uintptr_t)d_out) % 16 != 0) return fail(LTKV_ERR_ARG, "q and out must be 16-byte aligned");
+  const size_t bytes = n_rows * n_heads * head_dim * (row_type == LTKV_ROWS_F32 ? 4 : 2);
+  if (overlap(d_q, bytes, d_out, bytes))
+    return fail(LTKV_ERR_ARG, "q and out overlap: rows are read after others are written");
+  DeviceGuard dg(c->device);
+  if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
+  const size_t max_len = table_stride >= (size_t)INT32_MAX / LTKV_BLOCK ? (size_t)INT32_MAX : table_stride * LTKV_BLOCK;
+  ltkv::TreeArgs a{};
+  static_cast<ltkv::ScoredArgs &>(a) =
+      scored_args(c, layer, n, n_rows, n_heads, head_dim, scale, d_q, d_tables, table_stride, max_len, d_lens, d_out);
+  a.row_type = row_type;
+  a.row_starts = d_row_starts;
+  a.max_rows = (int64_t)std::min(max_rows, n_rows);
+  a.softcap = std::min(softcap, 0x1p96f);  // (the kernels take it times log2 e)
+  a.window = (int64_t)std::min<size_t>(window, (size_t)INT32_MAX);
+  a.positions = d_positions;
+  a.masks = d_masks;
+  a.mask_words = d_masks ? (int64_t)mask_words : 0;
+  const int64_t need = ltkv::tree_workspace((int)c->elem, a);
+  if (need > 0) {
+    uint8_t *base = nullptr;
+    if (int rc = kept_memory(c, (size_t)need, &base)) return rc;
+    ltkv::tree_partials(a, base);
+  }
+  const hipError_t e = ltkv::launch_tree_attention(head_geom(c, head_dim), a, c->stream);
+  if (e == hipErrorInvalidValue) return fail(LTKV_ERR_ARG, "attention grid too large for one launch");
+  if (e != hipSuccess) return hip_fail(e, "attention launch");
+  return LTKV_OK;
+}
+
+int ltkv_step_layout(ltkv_cache *c, size_t n, const int32_t *d_rows, const int32_t *d_lens, const int32_t *d_counts,
+                     size_t n_tokens, size_t table_stride, const int32_t *d_parents, size_t mask_words,
+                     int32_t *d_row_starts, int32_t *d_new_lens, int32_t *d_tables, int32_t *d_slot_mapping,
+                     int32_t *d_positions, int32_t *d_masks) {
+  if (!c) return fail(LTKV_ERR_ARG, "cache is null");
+  if (c->device == LTKV_NO_DEVICE) return no_device();
+  if (n == 0) return LTKV_OK;
+  if (n > (size_t{1} << 20) || n_tokens > (size_t)INT32_MAX / 2 || table_stride > (size_t)INT32_MAX / LTKV_BLOCK ||
+      mask_words > (size_t)INT32_MAX / 32)
+    return fail(LTKV_ERR_ARG, "%zu requests of %zu tokens are too many for one step", n, n_tokens);
+  if (table_stride == 0) return fail(LTKV_ERR_ARG, "table_stride must be > 0");
+  if (!d_rows || !d_lens || !d_row_starts || !d_new_lens || !d_tables)
+    return fail(LTKV_ERR_ARG, "null device pointer");
+  if (n_tokens > 0 && (!d_slot_mapping || !d_positions)) return fail(LTKV_ERR_ARG, "null device pointer");
+  if ((d_parents != nullptr) != (d_masks != nullptr) || (d_parents && mask_words == 0))
+    return fail(LTKV_ERR_ARG, "parents and masks (of at least one word) come together");
+  const size_t word = sizeof(int32_t);
+  const std::pair<const void *, size_t> in[] = {{d_rows, n * word}, {d_lens, n * word}, {d_counts, n * word},
+                                                {d_parents, n_tokens * word}};
+  const std::pair<const void *, size_t> out[] = {{d_row_starts, (n + 1) * word},
+                                                 {d_new_lens, n * word},
+                                                 {d_tables, n * table_stride * word},
+                                                 {d_slot_mapping, n_tokens * word},
+                                                 {d_positions, n_tokens * word},
+                                                 {d_masks, n_tokens * mask_words * word}};
+  for (const auto &o : out) {
+    for (const auto &i : in)
+      if (overlap(i.first, i.second, o.first, o.second))
+        return fail(LTKV_ERR_ARG, "inputs and outputs overlap: they are read after others are written");
+    for (const auto &p : out)
+      if (&p != &o && overlap(p.first, p.second, o.first, o.second)) return fail(LTKV_ERR_ARG, "outputs overlap");
+  }
+  DeviceGuard dg(c->device);
+  if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
+  // (a replay would take the tables of the capture's moment, whose memory may move)
+  if (capturing(c))
+    return fail(LTKV_ERR_ARG, "a step cannot be laid out under stream capture: lay it out before, capture its layers");
+  if (int rc = sync_tables(c)) return rc;
+  ltkv::LayoutArgs a{};
+  a.tables = c->d_rt;
+  a.counts = c->d_rt_nb;
+  a.width = (int64_t)c->rt_width;
+  a.n_table_rows = (int64_t)c->rt_rows;
+  a.rows = d_rows;
+  a.lens = d_lens;
+  a.news = d_counts;
+  a.parents = d_parents;
+  a.n = (int64_t)n;
+  a.n_tokens = (int64_t)n_tokens;
+  a.stride = (int64_t)table_stride;
+  a.mask_words = (int64_t)mask_words;
+  a.row_starts = d_row_starts;
+  a.new_lens = d_new_lens;
+  a.out_tables = d_tables;
+  a.slots = d_slot_mapping;
+  a.positions = d_positions;
+  a.masks = d_masks;
+  a.status = c->d_status;
+  const hipError_t e = ltkv::launch_step_layout(a, c->stream);
+  if (e == hipErrorInvalidValue) return fail(LTKV_ERR_ARG, "too many requests for one launch");
+  if (e != hipSuccess) return hip_fail(e, "step layout launch");
+  return LTKV_OK;
+}
+
+int ltkv_accept_tree(ltkv_cache *c, size_t n, size_t n_rows, const int32_t *d_tables, size_t table_stride,
+                     const int32_t *d_lens, const int32_t *d_row_starts, const int32_t *d_parents,
+                     const int32_t *d_tokens, const int32_t *d_targets, int32_t *d_accepted, int32_t *d_path,
+                     int32_t *d_next, int32_t *d_new_lens) {
+  if (!c) return fail(LTKV_ERR_ARG, "cache is null");
+  if (c->device == LTKV_NO_DEVICE) return no_device();
+  if (n_rows > (size_t)INT32_MAX / 2 || n > (size_t{1} << 24) || table_stride > (size_t)INT32_MAX)
+    return fail(LTKV_ERR_ARG, "%zu rows of %zu sequences are too many for one call", n_rows, n);
+  if (n == 0) return LTKV_OK;
+  if (table_stride == 0) return fail(LTKV_ERR_ARG, "table_stride must be > 0");
+  if (!d_tables || !d_lens || !d_row_starts || !d_accepted || !d_next || !d_new_lens)
+    return fail(LTKV_ERR_ARG, "null device pointer");
+  if (n_rows > 0 && (!d_parents || !d_tokens || !d_targets || !d_path)) return fail(LTKV_ERR_ARG, "null device pointer");
+  const size_t word = sizeof(int32_t);
+  const std::pair<const void *, size_t> in[] = {{d_tables, n * table_stride * word}, {d_lens, n * word},
+                                                {d_row_starts, (n + 1) * word},      {d_parents, n_rows * word},
+                                                {d_tokens, n_rows * word},           {d_targets, n_rows * word}};
+  const std::pair<const void *, size_t> out[] = {
+      {d_accepted, n * word}, {d_path, n_rows * word}, {d_next, n * word}, {d_new_lens, n * word}};
+  for (const auto &o : out) {
+    for (const auto &i : in)
+      if (overlap(i.first, i.second, o.first, o.second))
+        return fail(LTKV_ERR_ARG, "inputs and outputs overlap: they are read after others are written");
+    for (const auto &p : out)
+      if (&p != &o && overlap(p.first, p.second, o.first, o.second)) return fail(LTKV_ERR_ARG, "outputs overlap");
+  }
+  DeviceGuard dg(c->device);
+  if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
+  ltkv::AcceptArgs a{};
+  a.k = c->k;
+  a.v = c->v;
+  a.k_scale = c->ks;
+  a.v_scale = c->vs;
+  a.layer_bytes = (int64_t)c->layer_bytes();
+  a.layer_scales = (int64_t)(c->quantised() ? c->layer_scales() : 0);
+  a.n_layers = (int64_t)c->n_layers;
+  a.tables = d_tables;
+  a.table_stride = (int64_t)table_stride;
+  a.lens = d_lens;
+  a.row_starts = d_row_starts;
+  a.parents = d_parents;
+  a.tokens = d_tokens;
+  a.targets = d_targets;
+  a.n = (int64_t)n;
+  a.n_rows = (int64_t)n_rows;
+  a.accepted = d_accepted;
+  a.path = d_path;
+  a.next = d_next;
+  a.new_lens = d_new_lens;
+  a.status = c->d_status;
+  const hipError_t e = ltkv::launch_accept_tree(c->geom, a, c->stream);
+  if (e == hipErrorInvalidValue) return fail(LTKV_ERR_ARG, "%zu sequences of %zu layers are too many for one launch", n, c->n_layers);
+  if (e != hipSuccess) return hip_fail(e, "accept launch");
+  return LTKV_OK;
 }
 
 int ltkv_seq_rows(const ltkv_cache *c, size_t n, const uint32_t *seqs, int32_t *rows) {

@@ -422,6 +422,70 @@ hipError_t launch_gather_values(const PoolGeom &g, const void *k_layer, const vo
                                 const int32_t *lens, const int64_t *out_offsets, int64_t n, float *k_out,
                                 float *v_out, int32_t *status, hipStream_t s);
 
+// ---- steps with drafted tokens (ltkv_steps.hip, ltkv_tree.hip) --------------
+
+// Table of the scaled rotary frequencies: cos and sin of pos * inv_freq[i], taken
+// in 64 bits, times `magnitude`, as f32 pairs [max_pos][half].
+hipError_t launch_rope_table(const double *inv_freq, float magnitude, int half, int64_t max_pos, float *table,
+                             hipStream_t s);
+
+// Kernel 1 with RoPE for rows of any type: K rotated into its cell, V appended, Q
+// (optional, [n][q_stride] with n_heads heads) rotated into q_out.
+struct RopeRows {
+  const int32_t *slots, *positions;
+  int row_type;  // LTKV_ROWS_*
+  const void *k, *v, *q;
+  void *q_out;
+  int64_t n, src_stride, q_stride, out_stride;
+  int n_heads;
+};
+constexpr int kRopeRowsMaxHeadDim = 512;  // a head's 8-element slices lie in one wave
+hipError_t launch_write_rope_rows(const PoolGeom &g, void *k_layer, void *v_layer, void *k_scale, void *v_scale,
+                                  const RopeRows &a, const RopeGeom &r, hipStream_t s);
+
+// A step's arrays from its requests' lengths (ltkv_step_layout).
+struct LayoutArgs {
+  const int32_t *tables, *counts;  // resident tables and their lengths in blocks
+  int64_t width, n_table_rows;
+  const int32_t *rows, *lens, *news;  // per request; news nullptr: one token each
+  const int32_t *parents;             // [n_tokens], or nullptr
+  int64_t n, n_tokens, stride, mask_words;
+  int32_t *row_starts, *new_lens, *out_tables, *slots, *positions, *masks;
+  int32_t *status;
+};
+hipError_t launch_step_layout(const LayoutArgs &a, hipStream_t s);
+
+// The accepted path of drafted trees and the move of its rows (ltkv_accept_tree).
+struct AcceptArgs {
+  void *k, *v, *k_scale, *v_scale;  // whole pools
+  int64_t layer_bytes, layer_scales;  // bytes of a layer of a pool, entries of a layer of a scale pool
+  int64_t n_layers;
+  const int32_t *tables;
+  int64_t table_stride;
+  const int32_t *lens, *row_starts, *parents, *tokens, *targets;
+  int64_t n, n_rows;
+  int32_t *accepted, *path, *next, *new_lens;
+  int32_t *status;
+};
+hipError_t launch_accept_tree(const PoolGeom &g, const AcceptArgs &a, hipStream_t s);
+
+// Rows of drafted trees over a cache (ltkv_tree_attention): ScoredArgs without
+// slopes, sinks, prefixes and documents. Row j of a sequence's m rows is the cell
+// at position len - m + j; the rows' masks say which of these cells they see.
+struct TreeArgs : ScoredArgs {
+  const int32_t *positions;  // [n_rows], or nullptr (no window)
+  const int32_t *masks;      // [n_rows][mask_words], or nullptr: a row sees the rows up to its own
+  int64_t mask_words;
+  // Set by tree_workspace: rows of a work-group's tile and work-groups of the
+  // launch (0: the generic kernel).
+  int rows_per_tile, groups;
+  // Averages of the tiles that several work-groups share: part_o [slot][column]
+  // [head_dim], part_ml [slot][column][2] (reference, sum), two slots a work-group.
+};
+int64_t tree_workspace(int elem, TreeArgs &a);  // bytes of its partials
+void tree_partials(TreeArgs &a, uint8_t *base);
+hipError_t launch_tree_attention(const PoolGeom &g, const TreeArgs &a, hipStream_t s);
+
 // Scratch of the allocation-free decode attention: a static device array of
 // kScratchBytes on every device the library runs on. scratch_address gives
 // its address on `device`, which must be the current device on the first

@@ -1,4 +1,4 @@
-// What the kernels of scored attention share.
+// What the kernels of scored and tree attention share.
 //
 // Scored attention (ltkv_scored_attention): row r of a sequence with m rows and
 // L positions stands at position p = L - m + r and sees the positions t with
@@ -51,6 +51,8 @@ inline int64_t chunk_slots(const ScoredArgs &a) { return a.n_rows / chunk_rows(a
 hipError_t launch_scored_chunks(const PoolGeom &g, const ScoredArgs &a, int64_t min_rows, hipStream_t s);
 
 namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 struct Q4 {};  // element tag of q4_0 pools
 
@@ -151,13 +153,6 @@ __device__ __forceinline__ float row_load(const ScoredArgs &a, int64_t i) {
   const uint16_t u = static_cast<const uint16_t *>(a.q)[i];
   return a.row_type == LTKV_ROWS_F16 ? (float)__builtin_bit_cast(_Float16, u)
                                      : __builtin_bit_cast(float, (uint32_t)u << 16);
-}
-
-// f32 -> bf16, nearest even (NaN stays NaN).
-__device__ __forceinline__ uint16_t bf16_bits(float x) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
 }
 
 __device__ __forceinline__ void row_store(const ScoredArgs &a, int64_t i, float x) {
@@ -309,6 +304,40 @@ __device__ __forceinline__ void store_row4(const ScoredArgs &a, int64_t i, const
 __device__ __forceinline__ h8 read_tr2(const char *p, int step) {
   const h4 x = __builtin_bit_cast(h4, lds_read_tr(p)), y = __builtin_bit_cast(h4, lds_read_tr(p + step));
   return h8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+}
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+// True if an element is infinite or NaN.
+__device__ __forceinline__ bool not_finite(const h8 &x) {
+  const u32x4 u = __builtin_bit_cast(u32x4, x);
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, u[i] & 0x7fff7fffu));
+  return m.x >= 0x7c00 || m.y >= 0x7c00;
+}
+
+// Largest of a value over a position's four lanes, in each of them.
+__device__ __forceinline__ float position_max(float x) {
+  x = __builtin_fmaxf(x, dpp<0xB1>(x));     // quad_perm [1,0,3,2]
+  return __builtin_fmaxf(x, dpp<0x4E>(x));  // quad_perm [2,3,0,1]
+}
+
+// Sum / maximum of a value over lanes l and l ^ 32.
+template <bool MAX>
+__device__ __forceinline__ float halves_reduce(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const float p = __builtin_bit_cast(float, (uint32_t)b[0]), q = __builtin_bit_cast(float, (uint32_t)b[1]);
+  return MAX ? __builtin_fmaxf(p, q) : p + q;
+}
+
+// Work-group barrier that orders LDS only: loads from global memory stay in
+// flight across it.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 template <typename F>

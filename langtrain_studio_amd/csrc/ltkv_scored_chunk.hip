@@ -7,8 +7,6 @@
 namespace ltkv {
 namespace {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
 constexpr int kChunkTokens = 64;  // positions of a tile
 
 // A thread's share of a tile on its way from the pool to LDS: a quarter of the
@@ -106,28 +104,11 @@ struct Share<int8_t, NC> {
   }
 };
 
-typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-
-// True if an element is infinite or NaN.
-__device__ __forceinline__ bool not_finite(const h8 &x) {
-  const u32x4 u = __builtin_bit_cast(u32x4, x);
-  u16x2 m = {0, 0};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, u[i] & 0x7fff7fffu));
-  return m.x >= 0x7c00 || m.y >= 0x7c00;
-}
-
 __device__ __forceinline__ h8 finite_or_zero(const h8 &x) {
   h8 r;
 #pragma unroll
   for (int i = 0; i < 8; ++i) r[i] = __builtin_fabsf((float)x[i]) <= 65504.f ? x[i] : (_Float16)0.f;
   return r;
-}
-
-// Largest of a value over a position's four lanes, in each of them.
-__device__ __forceinline__ float position_max(float x) {
-  x = __builtin_fmaxf(x, dpp<0xB1>(x));     // quad_perm [1,0,3,2]
-  return __builtin_fmaxf(x, dpp<0x4E>(x));  // quad_perm [2,3,0,1]
 }
 
 // The same over a wave's 16 positions, of values that a position's lanes share.
@@ -167,23 +148,6 @@ struct TileRange {
   }
 };
 constexpr float kLeftOut = 511.f;  // scales (times the power of two) from here on could pass f16's largest number
-
-// Sum / maximum of a value over lanes l and l ^ 32.
-template <bool MAX>
-__device__ __forceinline__ float halves_reduce(float x) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  const float p = __builtin_bit_cast(float, (uint32_t)b[0]), q = __builtin_bit_cast(float, (uint32_t)b[1]);
-  return MAX ? __builtin_fmaxf(p, q) : p + q;
-}
-
-// Work-group barrier that orders LDS only: loads from global memory stay in
-// flight across it.
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
 
 // The least and largest of what the rows of a wave (or work-group) see. (No short
 // circuits, as in RowView::sees.)

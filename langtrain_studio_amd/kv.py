@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
 
@@ -72,6 +72,26 @@ def _dev_ptr(t, dtype, name: str, device: int) -> int:
     return t.data_ptr()
 
 
+class StepLayout(NamedTuple):
+    """The device arrays of a step (KvCache.step_layout), int32."""
+
+    row_starts: "object"    # [n + 1]: request i has tokens row_starts[i]..row_starts[i+1]
+    lens: "object"          # [n]: lengths, the step's tokens included
+    tables: "object"        # [n][stride]: block tables, -1 behind their ends
+    slot_mapping: "object"  # [n_tokens]: each token's cell, -1 behind the last token
+    positions: "object"     # [n_tokens]: each token's position, -1 behind the last token
+    masks: "object" = None  # [n_tokens][words]: a drafted token's ancestors and itself
+
+
+class AcceptedTree(NamedTuple):
+    """What KvCache.accept_tree kept, int32 on the device."""
+
+    accepted: "object"  # [n]: tokens kept
+    path: "object"      # [n_rows]: the kept tokens of each request in order, -1 behind them
+    next: "object"      # [n]: the token behind the last kept one
+    lens: "object"      # [n]: lengths after it
+
+
 class KvCache:
     """kv.rs KvCache with its pools in HBM.
 
@@ -99,6 +119,7 @@ class KvCache:
         self.n_blocks = self._lib.ltkv_n_blocks(h)
         self._kv_dim = self._lib.ltkv_kv_dim(h)
         self._plan_shape = None
+        self._rope_dims = 0  # head_dim of the RoPE table
         self._stream = 0
         if stream is not None:
             self.set_stream(stream)
@@ -259,6 +280,7 @@ class KvCache:
         """RoPE table of Model::rope (model.rs:263-265, 291-308) for write_rope."""
         _check(self._lib.ltkv_rope_init(self._h, float(base), rope_dim, head_dim, 1 if neox else 0,
                                         max_positions))
+        self._rope_dims = head_dim
 
     def write_rope(self, layer: int, slot_mapping, positions, k, v, q=None, n_heads: int = 0) -> None:
         """Kernel 1 with RoPE (model.rs:414-429): k rotated into its cell, v appended,
@@ -280,6 +302,91 @@ class KvCache:
             _dev_ptr(positions, torch.int32, "positions", self.device),
             _dev_ptr(k, torch.float32, "k", self.device), _dev_ptr(v, torch.float32, "v", self.device),
             k.shape[1], qp, qs, n_heads))
+
+    def rope_init_scaled(self, base: float, rope_dim: int, head_dim: int, neox: bool, max_positions: int,
+                         kind: str = "none", factor: float = 1.0, original: int = 0, low: Optional[float] = None,
+                         high: Optional[float] = None, divisors=None, magnitude: Optional[float] = None) -> None:
+        """rope_init with frequencies scaled for long contexts
+        (ltkv_rope_init_scaled): kind "none", "linear", "ntk", "yarn" or "llama3" by
+        `factor`; yarn and llama3 keep the frequencies of pairs that turn `high`
+        (32; 4) times within `original` positions and scale those that turn up to
+        `low` (1) times. divisors: one per pair. magnitude: of the cosines and
+        sines (default: the kind's own)."""
+        kinds = {"none": (_lib.ROPE_PLAIN, 1.0, 1.0), "linear": (_lib.ROPE_LINEAR, 1.0, 1.0),
+                 "ntk": (_lib.ROPE_NTK, 1.0, 1.0), "yarn": (_lib.ROPE_YARN, 1.0, 32.0),
+                 "llama3": (_lib.ROPE_LLAMA3, 1.0, 4.0)}
+        if kind not in kinds:
+            raise ValueError(f"kind must be one of {sorted(kinds)}")
+        if rope_dim < 0 or head_dim < 0 or max_positions < 0 or original < 0:
+            raise ValueError("rope_dim, head_dim, max_positions and original must not be negative")
+        if magnitude is not None and not magnitude > 0:
+            raise ValueError("magnitude must be positive")
+        code, lo, hi = kinds[kind]
+        if divisors is not None:
+            divisors = np.ascontiguousarray(divisors, dtype=np.float32).reshape(-1)
+            if divisors.size != rope_dim // 2:
+                raise ValueError("divisors must have rope_dim / 2 entries")
+        _check(self._lib.ltkv_rope_init_scaled(
+            self._h, float(base), rope_dim, head_dim, 1 if neox else 0, max_positions, code, float(factor), original,
+            float(lo if low is None else low), float(hi if high is None else high),
+            None if divisors is None else _np_ptr(divisors), 0.0 if magnitude is None else float(magnitude)))
+        self._rope_dims = head_dim
+
+    def write_rope_rows(self, layer: int, slot_mapping, positions, k, v, q=None, n_heads: int = 0, out=None):
+        """write_rope for f32, f16 or bf16 rows: k rotated into its cell, v
+        appended, and q ([n][n_heads*head_dim], optional) rotated into out, which
+        is returned (default: a new tensor; out=q rotates in place). Rows may be
+        columns of a wider tensor (unit stride within a row)."""
+        import torch
+
+        n = slot_mapping.numel()
+        types = self._row_types()
+        if k.dtype not in types:
+            raise TypeError(f"k must be float32, float16 or bfloat16, got {k.dtype}")
+        if k.dim() != 2 or k.shape != v.shape or k.shape[0] != n or k.shape[1] != self.kv_dim:
+            raise ValueError("k and v must be [n][kv_dim] and match slot_mapping")
+        if positions.numel() != n:
+            raise ValueError("positions must match slot_mapping")
+
+        def rows(t, name):
+            if t.dtype is not k.dtype:
+                raise TypeError(f"{name} must be {k.dtype}, got {t.dtype}")
+            if not t.is_cuda or t.get_device() != self.device:
+                raise ValueError(f"{name} must be on the cache's device")
+            if t.shape[0] > 0 and t.stride(1) != 1 or t.stride(0) < 0:
+                raise ValueError(f"{name} must have rows of unit stride")
+            return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else -(-max(t.shape[1], 1) // 8) * 8
+
+        kp, ks = rows(k, "k")
+        vp, vs = rows(v, "v")
+        if ks != vs:
+            raise ValueError("k and v must have the same row stride")
+        qp = op = None
+        qs = os = 0
+        if q is not None:
+            if q.dim() != 2 or q.shape[0] != n:
+                raise ValueError("q must be [n][n_heads*head_dim]")
+            if out is None:
+                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            elif out.shape != q.shape:
+                raise ValueError("out must match q")
+            qp, qs = rows(q, "q")
+            op, os = rows(out, "out")
+            if n_heads < 0 or (self._rope_dims and n_heads * self._rope_dims != q.shape[1]):
+                raise ValueError("q must be [n][n_heads*head_dim]")
+        elif out is not None:
+            raise ValueError("out without q")
+        _check(self._lib.ltkv_write_rope_rows(
+            self._h, layer, n, _dev_ptr(slot_mapping, torch.int32, "slot_mapping", self.device),
+            _dev_ptr(positions, torch.int32, "positions", self.device), types[k.dtype], kp, vp, ks, qp, qs, n_heads,
+            op, os))
+        return out
+
+    @staticmethod
+    def _row_types() -> dict:
+        import torch
+
+        return {torch.float32: _lib.ROWS_F32, torch.float16: _lib.ROWS_F16, torch.bfloat16: _lib.ROWS_BF16}
 
     def copy_blocks(self, pairs) -> None:
         """Kernel 2: copy block pairs[i,0] -> pairs[i,1] (all layers, K and V)."""
@@ -341,7 +448,7 @@ class KvCache:
         import torch
 
         n = lens.numel()
-        types = {torch.float32: _lib.ROWS_F32, torch.float16: _lib.ROWS_F16, torch.bfloat16: _lib.ROWS_BF16}
+        types = self._row_types()
         if q.dim() != 2 or q.shape[1] != n_heads * head_dim:
             raise ValueError("q must be [n_rows][n_heads*head_dim]")
         if q.dtype not in types:
@@ -377,6 +484,137 @@ class KvCache:
             _dev_ptr(q, q.dtype, "q", self.device), _dev_ptr(tables, torch.int32, "tables", self.device),
             tables.shape[1], _dev_ptr(lens, torch.int32, "lens", self.device),
             given(row_starts, torch.int32, "row_starts", n + 1), _dev_ptr(out, q.dtype, "out", self.device)))
+        return out
+
+    def tree_attention(self, layer: int, q, tables, lens, n_heads: int, head_dim: int, row_starts, positions=None,
+                       masks=None, max_rows: Optional[int] = None, scale: Optional[float] = None,
+                       softcap: float = 0.0, window: int = 0, out=None):
+        """Attention of drafted rows over the cache (ltkv_tree_attention):
+        sequence i has rows row_starts[i]..row_starts[i+1] of q
+        ([n_rows][n_heads*head_dim], f32, f16 or bf16), the last cells of its
+        lens[i] positions. A row sees the context in front of them (with window >
+        0: less than that many positions back from positions[row], int32
+        [n_rows]) and the rows whose bits its masks (int32 [n_rows][words]) hold;
+        without masks the rows up to its own. softcap > 0: scores become softcap
+        * tanh(score / softcap). max_rows: the most rows of one sequence (a hint;
+        default: as many as there are). Rows of no sequence are left as they were
+        (zeros in a new out)."""
+        import torch
+
+        n = lens.numel()
+        types = self._row_types()
+        if q.dim() != 2 or q.shape[1] != n_heads * head_dim:
+            raise ValueError("q must be [n_rows][n_heads*head_dim]")
+        if q.dtype not in types:
+            raise TypeError(f"q must be float32, float16 or bfloat16, got {q.dtype}")
+        if tables.dim() != 2 or tables.shape[0] != n:
+            raise ValueError("tables must be [n][stride]")
+        n_rows = q.shape[0]
+        if row_starts.numel() != n + 1:
+            raise ValueError("row_starts must have one entry per sequence and one more")
+        words = 0
+        if masks is not None:
+            if masks.dim() != 2 or masks.shape[0] != n_rows or masks.shape[1] == 0:
+                raise ValueError("masks must be [n_rows][words], of at least one word")
+            words = masks.shape[1]
+        if positions is not None and positions.numel() != n_rows:
+            raise ValueError("positions must have one entry per row")
+        if window < 0 or (max_rows is not None and max_rows < 0):
+            raise ValueError("window and max_rows must not be negative")
+        if out is None:
+            out = self._zeros_like(q)
+        elif out.shape != q.shape:
+            raise ValueError("out must match q")
+        if scale is None:
+            scale = 1.0 / math.sqrt(head_dim)  # model.rs:402
+        _check(self._lib.ltkv_tree_attention(
+            self._h, layer, n, n_rows, n_rows if max_rows is None else max_rows, n_heads, head_dim, float(scale),
+            float(softcap), window,
+            None if positions is None else _dev_ptr(positions, torch.int32, "positions", self.device),
+            None if masks is None else _dev_ptr(masks, torch.int32, "masks", self.device), words, types[q.dtype],
+            _dev_ptr(q, q.dtype, "q", self.device), _dev_ptr(tables, torch.int32, "tables", self.device),
+            tables.shape[1], _dev_ptr(lens, torch.int32, "lens", self.device),
+            _dev_ptr(row_starts, torch.int32, "row_starts", self.device), _dev_ptr(out, q.dtype, "out", self.device)))
+        return out
+
+    def step_layout(self, rows, lens, counts, n_tokens: int, table_stride: int, parents=None, mask_words: int = 0,
+                    out: Optional[StepLayout] = None) -> StepLayout:
+        """The arrays of a step from its requests' lengths, on the device
+        (ltkv_step_layout): request i holds lens[i] tokens of the sequence in
+        resident table row rows[i] (seq_rows; -1: no request) and gets counts[i]
+        new ones (None: one each), whose cells are claimed. parents ([n_tokens]):
+        each token's parent among its request's (-1: a root), for positions by
+        depth and the masks of tree_attention. All int32 device tensors; out: the
+        arrays of an earlier call to fill again."""
+        import torch
+
+        n = rows.numel()
+        if n_tokens < 0 or table_stride < 0 or mask_words < 0:
+            raise ValueError("n_tokens, table_stride and mask_words must not be negative")
+        if lens.numel() != n or (counts is not None and counts.numel() != n):
+            raise ValueError("rows, lens and counts must have equal length")
+        if parents is not None and parents.numel() != n_tokens:
+            raise ValueError("parents must have n_tokens entries")
+
+        def new(*shape):
+            return torch.empty(shape, dtype=torch.int32, device=rows.device)
+
+        shapes = [(n + 1,), (n,), (n, table_stride), (n_tokens,), (n_tokens,),
+                  (n_tokens, mask_words) if parents is not None else None]
+        if out is None:
+            out = StepLayout(*(None if s is None else new(*s) for s in shapes))
+        for name, t, s in zip(StepLayout._fields, out, shapes):
+            if (t is None) != (s is None) or (t is not None and tuple(t.shape) != s):
+                raise ValueError(f"out.{name} must have shape {s}")
+        if n == 0:  # nothing to lay out: every token is behind the last one
+            out.row_starts.zero_()
+            for t in (out.slot_mapping, out.positions):
+                t.fill_(-1)
+            if out.masks is not None:
+                out.masks.zero_()
+            return out
+
+        def ptr(t, name):
+            return None if t is None else _dev_ptr(t, torch.int32, name, self.device)
+
+        _check(self._lib.ltkv_step_layout(
+            self._h, n, ptr(rows, "rows"), ptr(lens, "lens"), ptr(counts, "counts"), n_tokens, table_stride,
+            ptr(parents, "parents"), mask_words if parents is not None else 0,
+            *(ptr(t, f"out.{name}") for name, t in zip(StepLayout._fields, out))))
+        return out
+
+    def accept_tree(self, tables, lens, row_starts, parents, tokens, targets,
+                    out: Optional[AcceptedTree] = None) -> AcceptedTree:
+        """Keeps what the model agrees with of every request's drafted tree
+        (ltkv_accept_tree), in all layers: rows as in tree_attention; token j of a
+        request has parent parents[j] and the model chose targets[j] behind it.
+        Token 0 is kept, then from each kept token the lowest child that is its
+        target; their K and V rows move together behind the context. All int32
+        device tensors; truncate the sequences to the lens returned."""
+        import torch
+
+        n, n_rows = lens.numel(), tokens.numel()
+        if tables.dim() != 2 or tables.shape[0] != n:
+            raise ValueError("tables must be [n][stride]")
+        if row_starts.numel() != n + 1:
+            raise ValueError("row_starts must have one entry per sequence and one more")
+        if parents.numel() != n_rows or targets.numel() != n_rows:
+            raise ValueError("parents, tokens and targets must have equal length")
+        sizes = (n, n_rows, n, n)
+        if out is None:
+            out = AcceptedTree(*(torch.empty((s,), dtype=torch.int32, device=lens.device) for s in sizes))
+        for name, t, s in zip(AcceptedTree._fields, out, sizes):
+            if t.numel() != s:
+                raise ValueError(f"out.{name} must have {s} entries")
+        if n == 0:
+            out.path.fill_(-1)
+            return out
+        args = dict(tables=tables, lens=lens, row_starts=row_starts, parents=parents, tokens=tokens, targets=targets,
+                    **{f"out.{name}": t for name, t in zip(AcceptedTree._fields, out)})
+        p = {name: _dev_ptr(t, torch.int32, name, self.device) for name, t in args.items()}
+        _check(self._lib.ltkv_accept_tree(
+            self._h, n, n_rows, p["tables"], tables.shape[1], p["lens"], p["row_starts"], p["parents"], p["tokens"],
+            p["targets"], p["out.accepted"], p["out.path"], p["out.next"], p["out.lens"]))
         return out
 
     def _zeros_like(self, t):

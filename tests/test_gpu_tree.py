@@ -1,0 +1,287 @@
+"""Attention of drafted trees (tree_attention) against its definition in 64 bits
+over the rows the pool holds (tree_definition, with its tolerances)."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from test_gpu_scored import BLOCK, build, held_rows
+from tree_definition import ancestors, compare, definition, depths, random_tree, visible, words_of
+
+pytestmark = pytest.mark.gpu
+
+
+def up(a, dtype, dev=None):
+    import torch
+
+    return torch.from_numpy(np.ascontiguousarray(a, dtype)).to(dev or torch.device("cuda", 0))
+
+
+def types():
+    import torch
+
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+class Trees:
+    """Sequences of a cache with drafted rows behind their contexts."""
+
+    def __init__(self, shape, dtype, ctx, new, seed, branch=0.4, roots=0.1, words=None, causal=False, stream=None,
+                 edit=None, gain=1.5, rows="f32"):
+        heads, kvh, hd = shape
+        self.heads, self.hd = heads, hd
+        self.lens = [c + m for c, m in zip(ctx, new)]
+        self.kv, self.tables = build(kvh * hd, self.lens, dtype, seed, stream=stream, edit=edit)
+        rng = np.random.default_rng(seed + 1)
+        self.starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        self.parents = [random_tree(rng, m, branch, roots) for m in new]
+        self.words = words or (max([1] + new) + 31) // 32
+        drafted = [np.tril(np.ones((m, m), bool)) if causal else ancestors(p) for m, p in zip(new, self.parents)]
+        for d in drafted:  # rows past the words are not seen
+            if not causal:
+                d[:, 32 * self.words:] = False
+        self.drafted = drafted
+        self.masks = None if causal else np.concatenate(
+            [words_of(d, self.words) for d in drafted] + [np.zeros((0, self.words), np.int32)])
+        deep = [np.arange(m) if causal else depths(p) for m, p in zip(new, self.parents)]
+        self.positions = np.concatenate([c + d for c, d in zip(ctx, deep)] + [np.zeros(0)]).astype(np.int32)
+        self.rows = rows
+        q = (rng.standard_normal((int(self.starts[-1]), heads * hd)) * gain).astype(np.float32)
+        self.q = up(q, np.float32).to(types()[rows])
+        self.new = new
+
+    def args(self):
+        return (self.q, up(self.tables, np.int32), up(self.lens, np.int32), self.heads, self.hd,
+                up(self.starts, np.int32))
+
+    def run(self, out=None, **how):
+        got = self.kv.tree_attention(0, *self.args(), positions=up(self.positions, np.int32),
+                                     masks=None if self.masks is None else up(self.masks, np.int32), out=out, **how)
+        self.kv.synchronize()
+        return got.float().cpu().numpy()
+
+    def want(self, window=0, **how):
+        sees, row = [], 0
+        for length, d in zip(self.lens, self.drafted):
+            sees.append(visible(length, d, window, self.positions[row:row + d.shape[0]]))
+            row += d.shape[0]
+        return definition(self.q.float().cpu().numpy(), held_rows(self.kv), self.tables, self.lens, self.starts,
+                          self.heads, self.hd, sees, rows=self.rows, eight=self.kv.dtype in ("q8_0", "f32"), **how)
+
+    def check(self, window=0, softcap=0.0, **how):
+        got = self.run(window=window, softcap=softcap, **how)
+        compare(got, self.want(window=window, softcap=softcap))
+
+
+# (heads, kv heads, head_dim): common widths and groups, and ones outside them
+SHAPES = [(8, 2, 128), (7, 1, 128), (4, 4, 64), (9, 3, 64), (16, 1, 64), (6, 2, 96), (20, 4, 80), (2, 2, 256),
+          (3, 1, 40), (3, 1, 20), (2, 1, 320), (65, 1, 32)]
+HOW = {"plain": {}, "cap": {"softcap": 5.0}, "window": {"window": 23}, "both": {"softcap": 8.0, "window": 100}}
+
+
+def shape_dtype():
+    for shape in SHAPES:
+        for dtype in ("f16", "f32", "q8_0", "q4_0"):
+            if dtype in ("q8_0", "q4_0") and shape[1] * shape[2] % 32:
+                continue
+            yield shape, dtype
+
+
+@pytest.mark.parametrize("how", HOW)
+@pytest.mark.parametrize("shape,dtype", list(shape_dtype()))
+def test_shapes(gpu, shape, dtype, how):
+    """Trees of one to a few rows behind contexts of zero, one, block and tile borders."""
+    Trees(shape, dtype, [0, 1, 15, 16, 63, 64, 130, 500], [1, 3, 1, 8, 2, 5, 0, 7], 1).check(**HOW[how])
+
+
+@pytest.mark.parametrize("rows", ["f16", "bf16"])
+@pytest.mark.parametrize("how", ["plain", "both"])
+@pytest.mark.parametrize("dtype", ["f16", "f32", "q8_0", "q4_0"])
+@pytest.mark.parametrize("shape", [(8, 2, 128), (9, 3, 64), (6, 2, 96)])
+def test_row_types(gpu, shape, dtype, how, rows):
+    Trees(shape, dtype, [0, 40, 300, 129], [4, 20, 9, 33], 2, rows=rows).check(**HOW[how])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "q8_0"])
+@pytest.mark.parametrize("new", [[64, 31, 65], [130, 1, 200], [333, 0, 17]])
+def test_wide_trees(gpu, dtype, new):
+    """More rows than a tile, masks of several words."""
+    Trees((8, 2, 64), dtype, [100, 0, 17], new, 3).check()
+
+
+def test_rows_past_the_mask_words_are_not_seen(gpu):
+    Trees((4, 1, 64), "f16", [30, 0], [50, 40], 4, words=1).check()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32", "q4_0"])
+def test_without_masks_as_prompt_chunks(gpu, dtype):
+    """Rows up to their own: the definition, and scored attention's result."""
+    t = Trees((8, 2, 128), dtype, [50, 0, 200], [33, 20, 1], 5, causal=True)
+    t.check()
+    scored = t.kv.scored_attention(0, t.q, *t.args()[1:5], row_starts=t.args()[5])
+    t.kv.synchronize()
+    compare(scored.float().cpu().numpy(), t.want())
+
+
+def test_long_contexts(gpu):
+    """Many parts a tree, ragged over the batch."""
+    Trees((8, 2, 128), "f16", [20000, 3, 7777, 12000], [12, 30, 1, 16], 6).check()
+    Trees((7, 1, 128), "q8_0", [16384, 100], [9, 40], 7, rows="bf16").check(window=5000)
+
+
+def test_many_sequences(gpu):
+    """More sequences than a work-group has threads, some without rows."""
+    rng = np.random.default_rng(8)
+    ctx = [int(x) for x in rng.integers(0, 90, 700)]
+    new = [int(x) for x in rng.integers(0, 5, 700)]
+    Trees((4, 2, 64), "f16", ctx, new, 8).check()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32", "q8_0", "q4_0"])
+@pytest.mark.parametrize("shape", [(8, 2, 128), (3, 1, 20 + 12)])
+def test_rows_that_see_nothing(gpu, shape, dtype):
+    """No context and an empty mask, or a window that ends before the context's
+    end: zeros, beside rows that see something."""
+    t = Trees(shape, dtype, [0, 20, 0], [3, 4, 1], 9)
+    t.masks[:] = 0
+    t.masks[1] = 1  # the second row of the first tree sees its first one
+    for d, n in zip(t.drafted, (0, 1, 2)):
+        d[:] = False
+    t.drafted[0][1, 0] = True
+    t.positions[3:7] = [20, 10 ** 6, 2 ** 31 - 1, 0]  # far rows see none of the context
+    t.check(window=7)
+    got = t.run(window=7)
+    assert (got[[0, 2, 4, 5, 7]] == 0).all() and (got[[1, 3, 6]] != 0).any(axis=1).all()
+
+
+@pytest.mark.parametrize("value", [np.inf, np.nan, -np.inf, 3e38])
+@pytest.mark.parametrize("rows", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype", ["f16", "f32", "q8_0", "q4_0"])
+@pytest.mark.parametrize("shape", [(8, 2, 128), (6, 2, 96), (3, 1, 32)])
+def test_what_a_row_does_not_see(gpu, shape, dtype, rows, value):
+    """Infinities, NaN and huge values in a sibling's K and V, in context cells
+    in front of every window and behind the last position stay out of the rows
+    that do not see them; rows that see an infinity are not specified."""
+    ctx, new = [70, 5], [6, 4]
+
+    def edit(i, k, v):
+        if i == 0:
+            for x in (k, v):
+                x[[3, 40, ctx[0] + 2], ::3] = value  # (3 and 40: outside the windows)
+        else:
+            v[ctx[1] + 1, 1::2] = value
+
+    with np.errstate(over="ignore", invalid="ignore"):
+        t = Trees(shape, dtype, ctx, new, 10, edit=edit, rows=rows)
+        # row 2 of the first tree and row 1 of the second have no other row below them
+        for d, bad in zip(t.drafted, (2, 1)):
+            d[:, bad] = False
+        t.masks = np.concatenate([words_of(d, t.words) for d in t.drafted])
+        t.check(window=20)
+
+
+def test_extreme_magnitudes_of_f32_and_8_bit_pools(gpu):
+    """A tiny sequence beside siblings that are 2^60 (8-bit: 2^16) larger, and
+    values near the largest f32: rows keep their bits."""
+    for dtype, big in (("f32", 2.0 ** 60), ("q8_0", 2.0 ** 16)):
+        def edit(i, k, v):
+            v[-1] *= np.float32(big)
+            k *= np.float32(1e-3)
+
+        t = Trees((4, 2, 64), dtype, [40, 3], [3, 2], 11, edit=edit)
+        for d in t.drafted:
+            d[:, -1] = False
+        t.masks = np.concatenate([words_of(d, t.words) for d in t.drafted])
+        t.check()
+
+    def huge(i, k, v):
+        v *= np.float32(2.0 ** 125)
+        k *= np.float32(2.0 ** -100)
+
+    t = Trees((4, 2, 64), "f32", [200, 3], [3, 2], 12, edit=huge)
+    t.q *= 2.0 ** 100
+    t.check()
+
+
+def test_short_lengths_and_rows_of_no_sequence(gpu):
+    """Fewer positions than rows; rows outside every sequence stay as they were;
+    lengths over the tables are cut."""
+    import torch
+
+    t = Trees((4, 2, 64), "f16", [0, 30], [4, 3], 13)
+    out = torch.full_like(t.q, 7.0)
+    starts = up([0, 4, 6], np.int32)
+    lens = up([2, 33], np.int32)  # rows 0 and 1 of the first stand before position 0
+    got = t.kv.tree_attention(0, t.q, up(t.tables, np.int32), lens, 4, 64, starts, out=out)
+    t.kv.synchronize()
+    got = got.cpu().numpy()
+    assert (got[6] == 7).all(), "a row of no sequence was written"
+    assert (got[:2] == 0).all(), "rows before position 0 see nothing"
+    drafted = [np.tril(np.ones((4, 4), bool)), np.tril(np.ones((2, 2), bool))]
+    sees = [visible(n, d) for n, d in zip([2, 33], drafted)]
+    want = definition(t.q.cpu().numpy(), held_rows(t.kv), t.tables, [2, 33], [0, 4, 6], 4, 64, sees)
+    compare(got[:6], tuple(x[:6] for x in want))
+
+
+@pytest.mark.parametrize("shape", [(8, 2, 128), (3, 1, 20)])
+def test_bad_table_entries(gpu, shape):
+    """An entry outside the pool is read as block 0 and reported, unless no row
+    sees its block."""
+    from langtrain_studio_amd import KvError
+
+    t = Trees(shape, "f16", [100, 40], [3, 2], 14)
+    seen, unseen = t.tables.copy(), t.tables.copy()
+    seen[0, 2] = 10 ** 6
+    unseen[0, :4] = -5
+    t.tables = seen
+    with pytest.raises(KvError, match="block-table entry"):
+        t.run()
+    t.kv.synchronize()  # taken once
+    t.tables = unseen
+    got = t.run(window=20)
+    t.tables = np.maximum(unseen, 0)
+    np.testing.assert_array_equal(got, t.run(window=20))
+
+
+def test_refusals(gpu):
+    import torch
+
+    from langtrain_studio_amd import KvError
+
+    t = Trees((4, 2, 64), "f16", [10], [3], 15)
+    q, tables, lens, heads, hd, starts = t.args()
+    masks = up(t.masks, np.int32)
+    call = t.kv.tree_attention
+    with pytest.raises(ValueError, match="heads"):
+        call(0, q[:, :-1], tables, lens, heads, hd, starts)
+    with pytest.raises(TypeError, match="q must be"):
+        call(0, q.double(), tables, lens, heads, hd, starts)
+    with pytest.raises(ValueError, match="row_starts"):
+        call(0, q, tables, lens, heads, hd, starts[:-1])
+    with pytest.raises(ValueError, match="masks"):
+        call(0, q, tables, lens, heads, hd, starts, masks=masks[:-1])
+    with pytest.raises(TypeError, match="masks must be"):
+        call(0, q, tables, lens, heads, hd, starts, masks=masks.long())
+    with pytest.raises(ValueError, match="positions"):
+        call(0, q, tables, lens, heads, hd, starts, positions=lens)
+    with pytest.raises(ValueError, match="negative"):
+        call(0, q, tables, lens, heads, hd, starts, window=-1)
+    with pytest.raises(KvError, match="window needs"):
+        call(0, q, tables, lens, heads, hd, starts, window=4)
+    with pytest.raises(ValueError, match="one word"):
+        call(0, q, tables, lens, heads, hd, starts, masks=masks[:, :0].contiguous())
+    with pytest.raises(KvError, match="max_rows"):
+        call(0, q, tables, lens, heads, hd, starts, max_rows=0)
+    with pytest.raises(KvError, match="overlap"):
+        call(0, q, tables, lens, heads, hd, starts, out=q)
+    with pytest.raises(KvError, match="softcap"):
+        call(0, q, tables, lens, heads, hd, starts, softcap=float("nan"))
+    with pytest.raises(KvError, match="scale"):
+        call(0, q, tables, lens, heads, hd, starts, scale=float("inf"))
+    with pytest.raises(KvError, match="layer"):
+        call(1, q, tables, lens, heads, hd, starts)
+    with pytest.raises(KvError, match="multiple of n_kv_heads"):
+        call(0, q[:, :192].contiguous(), tables, lens, 3, 64, starts)
+    empty = call(0, q[:0], tables, lens, heads, hd, torch.zeros_like(starts))
+    assert empty.shape == (0, heads * hd)
