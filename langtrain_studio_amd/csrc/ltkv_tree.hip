@@ -1,5 +1,7 @@
 // gfx950 (MI355X, CDNA4) kernels of attention for trees of drafted tokens.
 //
+//   tree_tile_kernel   tiles of rows against tiles of positions, on the matrix cores
+//   tree_merge_kernel  fold of the tiles that several work-groups share
 //   tree_any_kernel    any shape
 //
 // Row j of a sequence with m rows and L positions (context C = L - m) is the cell
@@ -149,24 +151,775 @@ __global__ void __launch_bounds__(kAnyThreads) tree_any_kernel(TreeArgs a, int64
   }
 }
 
-}  // namespace
+// ---- the tile kernel ----------------------------------------------------------
+//
+// Its work is laid out as one line of steps: sequence by sequence, of each the kv
+// heads, of each the tiles of rows (rows_per_tile rows by the group's query heads
+// are the columns of a work-group), of each the steps of 64 positions. Every
+// work-group takes an equal share of the line, wherever that begins and ends, so
+// that a ragged batch, one long context and a short step all load the chip evenly,
+// and a table wider than its contexts costs nothing. A tile that lies in several
+// shares leaves an average per share, which tree_merge_kernel folds.
+constexpr int kTreeWaves = 4, kTreeThreads = 64 * kTreeWaves;
+constexpr int kTreeTokens = 64;  // positions of a step
 
-int64_t tree_workspace(int elem, TreeArgs &a) {
-  (void)elem;
-  a.rows_per_tile = a.groups = 0;
-  return 0;
+struct TreeSeq {
+  SeqRows rows;
+  int32_t ctx;    // below 0 where the rows outnumber the positions
+  int32_t first;  // position of the first step
+  int32_t steps, tiles;
+};
+
+__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int64_t i) {
+  TreeSeq s;
+  s.rows = seq_rows(a, i);
+  s.ctx = s.rows.len - s.rows.count;
+  // no row sees a position in front of the window of the context's end
+  s.first = a.window > 0 ? (int32_t)max((int64_t)s.ctx - a.window + 1, (int64_t)0) & ~15 : 0;
+  s.steps = max((s.rows.len - s.first + kTreeTokens - 1) / kTreeTokens, 1);  // (rows that see nothing: zeros)
+  s.tiles = (s.rows.count + a.rows_per_tile - 1) / a.rows_per_tile;
+  return s;
 }
 
-void tree_partials(TreeArgs &, uint8_t *) {}
+__device__ __forceinline__ int64_t tree_steps(const TreeArgs &a, int64_t i) {
+  const TreeSeq s = tree_seq(a, i);
+  return (int64_t)s.steps * s.tiles * a.n_kv_heads;
+}
+
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return ((int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) |
+         (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+}
+
+// What a position's K and V hold as products' operands: f16 and q4_0 cells are f16
+// numbers; q8_0 and f32 cells enter as f16 hi + lo pairs (22 bits) times a power of
+// two of the position's own, so that no row loses bits to a position that it does
+// not see.
+template <typename T>
+constexpr bool kPairs = std::is_same_v<T, int8_t> || std::is_same_v<T, float>;
+
+// A thread's share of a step on its way from the pool to LDS: a quarter of the
+// head (NC chunks of 8 elements) of one position, K or V; a wave takes the 16
+// positions of one block, whose address is uniform. EXACT: head_dim is HD; else
+// elements past head_dim are zeros and a chunk brings its own scale (a head may
+// begin inside a group of 32).
+template <typename T, int HD, bool EXACT>
+struct Cells;
+
+template <int HD, bool EXACT>
+struct Cells<_Float16, HD, EXACT> {
+  static constexpr int NC = HD / 32;
+  u32x4 x[NC];
+  __device__ static __forceinline__ int chunk(int part, int j) { return part + 4 * j; }
+  static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 32; }
+  __device__ __forceinline__ void load(const void *pool, const void *, int64_t at, int64_t kv_dim, uint32_t head_off,
+                                       int slot, int part, int head_dim) {
+    const char *base = static_cast<const char *>(pool) + at;
+    const uint32_t place = (uint32_t)((slot * (uint32_t)kv_dim + head_off + part * 8) * 2);
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      if (EXACT || chunk(part, j) * 8 < head_dim) x[j] = load_at<u32x4>(base, place + 64 * j);
+      else x[j] = u32x4{0, 0, 0, 0};
+    }
+  }
+  __device__ __forceinline__ h8 get(int j) const { return __builtin_bit_cast(h8, x[j]); }
+  __device__ __forceinline__ bool bad() const {
+    bool b = false;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) b |= not_finite(get(j));
+    return b;
+  }
+};
+
+template <int HD, bool EXACT>
+struct Cells<Q4, HD, EXACT> {
+  static constexpr int NC = HD / 32, NS = EXACT ? 1 : NC;
+  uint32_t x[NC];
+  uint32_t s[NS];  // (as 32 bits: a 16-bit value would be waited for to be moved)
+  __device__ static __forceinline__ int chunk(int part, int j) { return EXACT ? part * NC + j : part + 4 * j; }
+  static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 8; }
+  __device__ __forceinline__ void load(const void *pool, const void *scales, int64_t at, int64_t, uint32_t head_off,
+                                       int slot, int part, int head_dim) {
+    const char *base = static_cast<const char *>(pool) + at, *sbase = static_cast<const char *>(scales) + (at >> 3);
+    if constexpr (EXACT) {
+      static_assert(NC == 2 || NC == 4, "a thread's chunks lie in one group");
+      const uint32_t e = head_off + part * NC * 8, place = ((e >> 5) * 16 + slot) * 16 + ((e & 31) >> 3) * 4;
+      s[0] = load_at<uint16_t>(sbase, (place >> 4) * 2);
+      if constexpr (NC == 4) {
+        const u32x4 w = load_at<u32x4>(base, place);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = w[j];
+      } else {
+        const u32x2 w = load_at<u32x2>(base, place);
+        x[0] = w.x;
+        x[1] = w.y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        x[j] = 0;
+        s[j] = 0;
+        if (chunk(part, j) * 8 >= head_dim) continue;
+        const uint32_t e = head_off + chunk(part, j) * 8, tile = (e >> 5) * 16 + slot;
+        x[j] = load_at<uint32_t>(base, tile * 16 + ((e & 31) >> 3) * 4);
+        s[j] = load_at<uint16_t>(sbase, tile * 2);
+      }
+    }
+  }
+  __device__ __forceinline__ h8 get(int j) const {
+    const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t)s[EXACT ? 0 : j]);
+    return q4x8_to_h8(x[j], h2{d, d});
+  }
+  __device__ __forceinline__ bool bad() const { return false; }
+};
+
+template <int HD, bool EXACT>
+struct Cells<int8_t, HD, EXACT> {
+  static constexpr int NC = HD / 32, NS = EXACT ? 1 : NC;
+  u32x2 x[NC];
+  uint32_t s[NS];
+  __device__ static __forceinline__ int chunk(int part, int j) { return EXACT ? part * NC + j : part + 4 * j; }
+  static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 16; }
+  __device__ __forceinline__ void load(const void *pool, const void *scales, int64_t at, int64_t kv_dim,
+                                       uint32_t head_off, int slot, int part, int head_dim) {
+    const char *base = static_cast<const char *>(pool) + at, *sbase = static_cast<const char *>(scales) + (at >> 4);
+    const uint32_t row = slot * (uint32_t)kv_dim;
+    if constexpr (EXACT) {
+      static_assert(NC == 2 || NC == 4, "a thread's chunks lie in one group");
+      const uint32_t e = head_off + part * NC * 8;
+      s[0] = load_at<uint16_t>(sbase, ((e >> 5) * 16 + slot) * 2);
+#pragma unroll
+      for (int j = 0; j < NC; j += 2) {
+        const u32x4 w = load_at<u32x4>(base, row + e + 8 * j);
+        x[j] = u32x2{w.x, w.y};
+        x[j + 1] = u32x2{w.z, w.w};
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        x[j] = u32x2{0x80808080u, 0x80808080u};  // (quants are stored offset by 128)
+        s[j] = 0;
+        if (chunk(part, j) * 8 >= head_dim) continue;
+        const uint32_t e = head_off + chunk(part, j) * 8;
+        x[j] = load_at<u32x2>(base, row + e);
+        s[j] = load_at<uint16_t>(sbase, ((e >> 5) * 16 + slot) * 2);
+      }
+    }
+  }
+  __device__ __forceinline__ float scale(int j) const {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)s[EXACT ? 0 : j]);
+  }
+  // e such that elements times 2^-e stay below 2^15
+  __device__ __forceinline__ int exponent() const {
+    float d = 0.f;
+#pragma unroll
+    for (int j = 0; j < NS; ++j) d = __builtin_fmaxf(d, scale(j));
+    d = __builtin_fminf(position_max(d), 65504.f);
+    return d > 0.f ? __builtin_amdgcn_frexp_expf(d) - 8 : -32;
+  }
+  __device__ __forceinline__ void pair(int j, int e, h8 &hi, h8 &lo) const {
+    const h8 q = i8x8_to_h8(x[j]);
+    const float d = __builtin_amdgcn_ldexpf(scale(j), -e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      _Float16 a, b;
+      split2((float)q[i] * d, a, b);
+      hi[i] = a;
+      lo[i] = b;
+    }
+  }
+  __device__ __forceinline__ bool bad() const {
+    bool b = false;
+#pragma unroll
+    for (int j = 0; j < NS; ++j) b |= !(scale(j) <= 65504.f);
+    return b;
+  }
+};
+
+template <int HD, bool EXACT>
+struct Cells<float, HD, EXACT> {
+  static constexpr int NC = HD / 32;
+  u32x4 x[2 * NC];
+  __device__ static __forceinline__ int chunk(int part, int j) { return part + 4 * j; }
+  static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 64; }
+  __device__ __forceinline__ void load(const void *pool, const void *, int64_t at, int64_t kv_dim, uint32_t head_off,
+                                       int slot, int part, int head_dim) {
+    const char *base = static_cast<const char *>(pool) + at;
+    const uint32_t place = (uint32_t)((slot * (uint32_t)kv_dim + head_off + part * 8) * 4);
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (EXACT || chunk(part, j) * 8 < head_dim) x[2 * j + i] = load_at<u32x4>(base, place + 128 * j + 16 * i);
+        else x[2 * j + i] = u32x4{0, 0, 0, 0};
+      }
+    }
+  }
+  __device__ __forceinline__ uint32_t top_bits() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 2 * NC; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = max(m, x[j][i] & 0x7fffffffu);
+    return m;
+  }
+  // (at least -100: smaller values are nothing beside their products' rounding)
+  __device__ __forceinline__ int exponent() const {
+    const float m = position_max(__builtin_bit_cast(float, min(top_bits(), 0x7f7fffffu)));
+    return m > 0.f ? max(__builtin_amdgcn_frexp_expf(m) - 15, -100) : -100;
+  }
+  __device__ __forceinline__ void pair(int j, int e, h8 &hi, h8 &lo) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      _Float16 a, b;
+      const uint32_t u = x[2 * j + (i >> 2)][i & 3];
+      split2(__builtin_amdgcn_ldexpf(__builtin_bit_cast(float, u), -e), a, b);
+      hi[i] = a;
+      lo[i] = b;
+    }
+  }
+  __device__ __forceinline__ bool bad() const { return top_bits() >= 0x7f800000u; }
+};
+
+// WC waves share a step's columns, 32 each; 4 / WC waves its positions. Steps go
+// through LDS as f16 numbers, on 32x32x16 products: scores^T = K Q^T, weights in
+// place, numerators^T += V^T W (a lane's scores are positions 8 (r / 4) + 4 (lane /
+// 32) + r % 4 of its column, which is the second product's operand layout when its
+// 16 positions are taken as 4 (lane / 32) ... + 3 and 8 + 4 (lane / 32) ... + 3: no
+// exchange). FULL (f32 rows, and any rows with a cap over kShortCap): Q and the
+// weights as hi + lo pairs; else Q as it is (times a power of two), the weights and V
+// rounded to f16.
+// Of pairs (kPairs) the scores are multiplied by their position's power of two, and
+// so are the weights, whose column then has a reference of its own (`top_o`): the
+// largest weight times V, not the largest weight, lies near the top of f16.
+template <typename T, int HD, bool EXACT, bool FULL, int WC>
+__global__ void __launch_bounds__(kTreeThreads, HD > 128 ? 1 : 2)
+tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
+  constexpr int NC = HD / 32, NK = HD / 16, WP = kTreeWaves / WC, U = 2 / WP;
+  constexpr bool PAIRS = kPairs<T>;
+  constexpr int K_PLANES = PAIRS ? 2 : 1, V_PLANES = PAIRS && FULL ? 2 : 1;
+  constexpr int K_PITCH = HD * 2 + 16;  // rows 4 banks apart: 16-byte reads of 16 rows without conflicts
+  constexpr int V_PITCH = HD * 2 + 64;  // rows 16 banks apart, for the transposing reads
+  constexpr int K_BYTES = kTreeTokens * K_PITCH, V_BYTES = kTreeTokens * V_PITCH;
+  constexpr int STEP_BYTES = K_PLANES * K_BYTES + V_PLANES * V_BYTES;
+  constexpr int FOLD = NC * 16 + 4;  // floats that a lane hands over where waves share columns
+  static_assert(WP == 1 || (kTreeWaves - WC) * 64 * FOLD * 4 <= STEP_BYTES, "the fold fits the step's memory");
+  __shared__ __align__(16) char lds[STEP_BYTES];
+  __shared__ __align__(16) float s_kpow[PAIRS ? kTreeTokens : 4], s_vpow[PAIRS ? kTreeTokens : 4];
+  __shared__ uint64_t s_bad[kTreeWaves];  // lanes whose share of V is left out (positions 16 wave + lane / 4)
+  __shared__ int64_t s_begin[kTreeThreads + 1];
+  __shared__ int64_t s_sum[kTreeWaves];
+  __shared__ int64_t s_found[2];
+  __shared__ int32_t s_from[kTreeWaves];
+  char *const lds_k = lds, *const lds_v = lds + K_PLANES * K_BYTES;
+
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int cw = wave % WC, pw = wave / WC;
+  const int col = lane & 31, half = lane >> 5;
+  const int group = a.n_heads / a.n_kv_heads;
+
+  // the line: a thread's sequences [i0, i1) begin at s_begin[tid]
+  const int64_t each = (a.n + kTreeThreads - 1) / kTreeThreads;
+  const int64_t i0 = min((int64_t)tid * each, a.n), i1 = min(i0 + each, a.n);
+  {
+    int64_t sum = 0;
+    for (int64_t i = i0; i < i1; ++i) sum += tree_steps(a, i);
+    int64_t upto = sum;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t y = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += y;
+    }
+    if (lane == 63) s_sum[wave] = upto;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) upto += s_sum[w];
+    s_begin[tid] = upto - sum;
+    if (tid == kTreeThreads - 1) s_begin[kTreeThreads] = upto;
+    __syncthreads();
+  }
+  const int64_t total = uniform64(s_begin[kTreeThreads]);
+  const uint32_t groups = gridDim.x;  // a multiple of 8: neighbours on the line share an XCD's L2
+  const int64_t per = (total + groups - 1) / groups;
+  const int64_t share = (int64_t)(blockIdx.x & 7) * (groups >> 3) + (blockIdx.x >> 3);
+  int64_t at = share * per;
+  const int64_t end = min(total, at + per);
+
+  while (at < end) {
+    __syncthreads();  // s_found, and the step's memory, have been read
+    if (s_begin[tid] <= at && at < s_begin[tid + 1]) {
+      int64_t begin = s_begin[tid];
+      for (int64_t i = i0; i < i1; ++i) {
+        const int64_t next = begin + tree_steps(a, i);
+        if (at < next) {
+          s_found[0] = i;
+          s_found[1] = begin;
+          break;
+        }
+        begin = next;
+      }
+    }
+    __syncthreads();
+    const int64_t seq = uniform64(s_found[0]), off = at - uniform64(s_found[1]);
+    const TreeSeq ts = tree_seq(a, seq);
+    const SeqRows rows = ts.rows;
+    const int64_t unit = off / ts.steps;
+    const int s_first = (int)(off - unit * ts.steps);
+    const int s_last = (int)min((int64_t)ts.steps, s_first + (end - at));
+    const int kvh = (int)(unit / ts.tiles), tile = (int)(unit - (int64_t)kvh * ts.tiles);
+    const int32_t r0 = tile * a.rows_per_tile;
+    at += s_last - s_first;
+
+    // the lane's column
+    const int c = cw * 32 + col, rr = c / group;
+    const bool live = rr < a.rows_per_tile && r0 + rr < rows.count;
+    const int head = kvh * group + c - rr * group;
+    const int64_t row = rows.row0 + r0 + (live ? rr : 0);
+    TreeView view = tree_view(a, rows, r0 + (live ? rr : 0));
+    view.ctx = ts.ctx;
+    const bool wave_live = __builtin_amdgcn_ballot_w64(live) != 0;
+    int32_t from_max = 0;  // positions in front of it some row does not see
+    if (a.window > 0) {
+      from_max = live ? view.from : 0;
+#pragma unroll
+      for (int x = 16; x >= 1; x >>= 1) from_max = max(from_max, __shfl_xor(from_max, x, 64));
+      if (lane == 0) s_from[wave] = from_max;
+      __syncthreads();
+      from_max = __builtin_amdgcn_readfirstlane(max(max(s_from[0], s_from[1]), max(s_from[2], s_from[3])));
+    }
+
+    const int32_t *tab = table_of(a.tables, a.table_stride, nullptr, 0, seq);
+    // Table entries outside the pool are reported where a row sees a position of
+    // their block; the steps read block 0 in their place.
+    for (int32_t t = ts.first + kTreeTokens * s_first + 16 * tid; t < min(rows.len, ts.first + kTreeTokens * s_last);
+         t += 16 * kTreeThreads) {
+      if ((uint32_t)tab[t >> 4] < (uint32_t)n_blocks) continue;
+      bool needed = false;
+      for (int32_t r = 0; r < a.rows_per_tile && r0 + r < rows.count; ++r) {
+        TreeView v = tree_view(a, rows, r0 + r);
+        v.ctx = ts.ctx;
+        needed |= (v.sees32(t) & 0xffffu) != 0;
+      }
+      if (needed) report_fault(a.status, kFaultTable, seq);
+    }
+
+    // Q columns, times a power of two and the scale's sign
+    h8 qh[NK], ql[FULL ? NK : 1];
+    int q_exp;
+    {
+      float x[NK][8], amax = 0.f;
+      const int64_t q0 = (row * a.n_heads + head) * (int64_t)a.head_dim;
+#pragma unroll
+      for (int j = 0; j < NK; ++j) {
+        load_row8(a, q0 + 16 * j + 8 * half, live && (EXACT || 16 * j + 8 * half < a.head_dim), x[j]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = __builtin_fmaxf(amax, __builtin_fabsf(x[j][i]));
+      }
+      amax = halves_reduce<true>(amax);
+      // (at most 100: a smaller row's scores are nothing beside their rounding)
+      q_exp = amax > 0.f && amax < INFINITY ? min(10 - __builtin_amdgcn_frexp_expf(amax), 100) : 0;
+#pragma unroll
+      for (int j = 0; j < NK; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float y = __builtin_amdgcn_ldexpf(x[j][i], q_exp);
+          _Float16 hi, lo;
+          split2(a.scale < 0.f ? -y : y, hi, lo);
+          qh[j][i] = hi;
+          if constexpr (FULL) ql[j][i] = lo;
+        }
+    }
+    const bool cap = a.softcap > 0.f;
+    const float scale = __builtin_fabsf(a.scale);
+    const float in_scale = score_factor(cap ? scale / a.softcap : scale * kLog2e, -q_exp);
+    const float cap_scale = a.softcap * kLog2e;
+
+    f32x16 o[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) o[i] = f32x16{};
+    float ref = -INFINITY, sum = 0.f;      // weights are 2^(score - ref + kLift)
+    float top_o = -INFINITY, to_o = 0.f;   // pairs: numerators are taken times 2^(ref - top_o) = to_o
+    bool poisoned = false;                 // the column sees an infinity or NaN in V
+
+    const int tok = tid >> 2, part = tid & 3;
+    auto block_of = [&](int s) {  // the wave's block of a step (past the end: block 0, read and masked)
+      const int32_t t = ts.first + kTreeTokens * s + 16 * wave;
+      const int32_t e = s < s_last && t < rows.len ? scalar_read(tab, t >> 4) : 0;
+      return (uint32_t)e < (uint32_t)n_blocks ? e : 0;
+    };
+    const int64_t block_bytes = Cells<T, HD, EXACT>::block_bytes(kv_dim);
+    const uint32_t head_off = (uint32_t)(kvh * a.head_dim);
+    Cells<T, HD, EXACT> ks, vs;
+    auto load = [&](int32_t block) {
+      const int64_t b = (int64_t)(uint32_t)block * block_bytes;
+      ks.load(a.k_layer, a.k_scale, b, kv_dim, head_off, tok & 15, part, a.head_dim);
+      vs.load(a.v_layer, a.v_scale, b, kv_dim, head_off, tok & 15, part, a.head_dim);
+    };
+    int32_t next = block_of(s_first + 1);
+    load(block_of(s_first));
+
+    for (int s = s_first; s < s_last; ++s) {
+      const int32_t t0 = ts.first + kTreeTokens * s;
+      const bool partial = t0 + kTreeTokens > ts.ctx || t0 < from_max;  // some row does not see all of it
+      lds_barrier();  // the last step has been read
+      bool bad = false;
+      if (partial) bad = vs.bad();
+      if constexpr (PAIRS) {
+        const int ek = ks.exponent(), ev = vs.exponent();
+        if (part == 0) {
+          s_kpow[tok] = __builtin_amdgcn_ldexpf(1.f, ek);
+          s_vpow[tok] = __builtin_amdgcn_ldexpf(1.f, ev);
+        }
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          const int x = Cells<T, HD, EXACT>::chunk(part, j) * 16;
+          h8 hi, lo;
+          ks.pair(j, ek, hi, lo);
+          *reinterpret_cast<h8 *>(lds_k + tok * K_PITCH + x) = hi;
+          *reinterpret_cast<h8 *>(lds_k + K_BYTES + tok * K_PITCH + x) = lo;
+          vs.pair(j, ev, hi, lo);
+          *reinterpret_cast<h8 *>(lds_v + tok * V_PITCH + x) = bad ? h8{} : hi;
+          if constexpr (V_PLANES == 2) *reinterpret_cast<h8 *>(lds_v + V_BYTES + tok * V_PITCH + x) = bad ? h8{} : lo;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          const int x = Cells<T, HD, EXACT>::chunk(part, j) * 16;
+          *reinterpret_cast<h8 *>(lds_k + tok * K_PITCH + x) = ks.get(j);
+          *reinterpret_cast<h8 *>(lds_v + tok * V_PITCH + x) = bad ? h8{} : vs.get(j);
+        }
+      }
+      const uint64_t bad_lanes = __builtin_amdgcn_ballot_w64(bad);
+      if (lane == 0) s_bad[wave] = bad_lanes;
+      if (s + 1 < s_last) {
+        load(next);
+        next = block_of(s + 2);
+      }
+      lds_barrier();
+      if (!wave_live) continue;
+
+      // scores of positions t0 + 32 (pw U + u) + 8 (i / 4) + 4 half + i % 4
+      f32x16 sc[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) sc[u] = f32x16{};
+      const char *kp = lds_k + (32 * pw * U + col) * K_PITCH + 16 * half;
+#pragma unroll
+      for (int j = 0; j < NK; ++j) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const h8 x = *reinterpret_cast<const h8 *>(kp + 32 * u * K_PITCH + 32 * j);
+          sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[j], sc[u], 0, 0, 0);
+          if constexpr (FULL) sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[j], sc[u], 0, 0, 0);
+          if constexpr (PAIRS) {
+            const h8 y = *reinterpret_cast<const h8 *>(kp + K_BYTES + 32 * u * K_PITCH + 32 * j);
+            sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[j], sc[u], 0, 0, 0);
+          }
+        }
+      }
+      float m = in_scale;  // scores are m sc
+      if constexpr (PAIRS) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const f32x4 f = *reinterpret_cast<const f32x4 *>(s_kpow + 32 * (pw * U + u) + 2 * i + 4 * half);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sc[u][i + k] *= __builtin_fminf(f[k] * in_scale, 1e37f);
+          }
+        m = 1.f;
+      }
+      if (cap) {
+        float to_x = m;  // opaque: the products would be taken before the branch, for both sides
+        asm("" : "+v"(to_x));
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float x = sc[u][i] * to_x;
+            sc[u][i] = (FULL ? tanh_f32(x) : tanh_f16(x)) * cap_scale;
+          }
+        m = 1.f;
+      }
+      if (partial) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t seen = live ? view.sees32(t0 + 32 * (pw * U + u)) : 0u, mine = seen >> (4 * half);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            sc[u][i] = mine >> (8 * (i / 4) + i % 4) & 1 ? sc[u][i] : -INFINITY;
+          // the infinities and NaN of V entered as zeros
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint64_t lanes = s_bad[2 * (pw * U + u) + w];
+            if (__builtin_amdgcn_readfirstlane(lanes != 0))
+              for (int p = 0; p < 16; ++p)
+                poisoned |= (lanes >> (4 * p) & 15) != 0 && (seen >> (16 * w + p) & 1);
+          }
+        }
+      }
+      float top = sc[0][0];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, sc[u][i]);
+      top *= m;
+      if (__builtin_amdgcn_ballot_w64(top > ref + kSlack)) {
+        const float nr = __builtin_fmaxf(ref, halves_reduce<true>(top));
+        const float f = nr == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - nr);
+        sum *= f;
+        if constexpr (PAIRS) {
+          if (top_o > -INFINITY) to_o = __builtin_fminf(__builtin_amdgcn_exp2f(nr - top_o), 3e38f);
+        } else {
+#pragma unroll
+          for (int i = 0; i < NC; ++i) o[i] *= f;
+        }
+        ref = nr;
+      }
+      const float base = kLift - (ref == -INFINITY ? 0.f : ref);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          sc[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], m, base));
+          if constexpr (FULL || PAIRS) sum += sc[u][i];
+        }
+      if constexpr (PAIRS) {
+        float most = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const f32x4 f = *reinterpret_cast<const f32x4 *>(s_vpow + 32 * (pw * U + u) + 2 * i + 4 * half);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              sc[u][i + k] *= f[k];
+              most = __builtin_fmaxf(most, sc[u][i + k]);
+            }
+          }
+        // (kLift + kSlack: the largest weights times V stay below 2^14)
+        const bool first = top_o == -INFINITY && most > 0.f;
+        if (__builtin_amdgcn_ballot_w64(first || most * to_o > 16384.f)) {
+          const float z = halves_reduce<true>(__builtin_amdgcn_logf(most)) + ref - kLift;
+          const float nt = __builtin_fmaxf(top_o, z);
+          const float f = top_o > -INFINITY ? __builtin_amdgcn_exp2f(top_o - nt) : 1.f;
+#pragma unroll
+          for (int i = 0; i < NC; ++i) o[i] *= f;
+          top_o = nt;
+          if (nt > -INFINITY) to_o = __builtin_fminf(__builtin_amdgcn_exp2f(ref - nt), 3e38f);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[u][i] *= to_o;
+      }
+#pragma unroll
+      for (int p = 0; p < 2 * U; ++p) {  // 16 positions each
+        h8 wh, wl;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          _Float16 hi, lo;
+          split2(sc[p >> 1][8 * (p & 1) + i], hi, lo);
+          wh[i] = hi;
+          if constexpr (FULL) wl[i] = lo;
+        }
+        if constexpr (!FULL && !PAIRS) {  // the weights as they enter the product, two an instruction
+          const h2 one = {(_Float16)1.f, (_Float16)1.f};
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) sum = __builtin_amdgcn_fdot2(h2{wh[i], wh[i + 1]}, one, sum, false);
+        }
+        const char *vp = lds_v + (32 * pw * U + 16 * p + 4 * half + ((lane & 15) >> 2)) * V_PITCH +
+                         (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const h8 x = read_tr2(vp + 64 * i, 8 * V_PITCH);
+          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wh, o[i], 0, 0, 0);
+          if constexpr (FULL) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wl, o[i], 0, 0, 0);
+          if constexpr (V_PLANES == 2) {
+            const h8 y = read_tr2(vp + V_BYTES + 64 * i, 8 * V_PITCH);
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, wh, o[i], 0, 0, 0);
+          }
+        }
+      }
+    }
+
+    // the column's average
+    sum = halves_reduce<false>(sum);
+    if (poisoned) sum = __builtin_nanf("");
+    if constexpr (WP > 1) {
+      __syncthreads();  // the last step has been read
+      float *const fold = reinterpret_cast<float *>(lds) + (wave - WC) * 64 * FOLD + lane;
+      if (pw > 0) {
+#pragma unroll
+        for (int i = 0; i < NC * 16; ++i) fold[64 * i] = o[i >> 4][i & 15];
+        fold[64 * (NC * 16)] = ref;
+        fold[64 * (NC * 16 + 1)] = sum;
+        fold[64 * (NC * 16 + 2)] = top_o;
+      }
+      __syncthreads();
+      if (pw > 0) continue;
+#pragma unroll
+      for (int w = 1; w < WP; ++w) {
+        const float *const other = reinterpret_cast<const float *>(lds) + (w * WC + cw - WC) * 64 * FOLD + lane;
+        const float ref2 = other[64 * (NC * 16)], sum2 = other[64 * (NC * 16 + 1)], top2 = other[64 * (NC * 16 + 2)];
+        const float nr = __builtin_fmaxf(ref, ref2), r = nr == -INFINITY ? 0.f : nr;
+        float f = __builtin_amdgcn_exp2f(ref - r), g = __builtin_amdgcn_exp2f(ref2 - r);
+        sum = sum * f + sum2 * g;
+        ref = nr;
+        if constexpr (PAIRS) {
+          const float nt = __builtin_fmaxf(top_o, top2), t = nt == -INFINITY ? 0.f : nt;
+          f = __builtin_amdgcn_exp2f(top_o - t);
+          g = __builtin_amdgcn_exp2f(top2 - t);
+          top_o = nt;
+        }
+#pragma unroll
+        for (int i = 0; i < NC * 16; ++i) o[i >> 4][i & 15] = o[i >> 4][i & 15] * f + other[64 * i] * g;
+      }
+    }
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;  // (a NaN sum stays one)
+    const float back = PAIRS && top_o > -INFINITY ? __builtin_amdgcn_exp2f(top_o - ref) : 1.f;
+    const bool whole = s_first == 0 && s_last == ts.steps;
+    // (a share's last tile may go on in the next one, its first come from the last)
+    const int64_t slot = 2 * share + (s_first == 0 ? 1 : 0);
+    const int64_t column = slot * (a.rows_per_tile * group) + c;
+    const int64_t out0 = (row * a.n_heads + head) * (int64_t)a.head_dim;
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; k += 4) {
+        const int d = 32 * i + 2 * k + 4 * half;
+        if (!live || (!EXACT && d >= a.head_dim)) continue;
+        f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = o[i][k + e] * inv * back;
+        if (whole) store_row4(a, out0 + d, x);
+        else *reinterpret_cast<f32x4 *>(a.part_o + column * a.head_dim + d) = x;
+      }
+    if (live && !whole && half == 0) {
+      a.part_ml[2 * column] = ref;
+      a.part_ml[2 * column + 1] = sum;
+    }
+  }
+}
+
+// A work-group a (row, kv head) whose tile lies in several shares: their averages,
+// weighted by their sums against the largest reference, in order. It finds the
+// tile's place on the line by itself.
+__global__ void __launch_bounds__(kTreeThreads) tree_merge_kernel(TreeArgs a) {
+  __shared__ int64_t red[2][kTreeWaves];
+  const int tid = (int)threadIdx.x;
+  const int kvh = (int)(blockIdx.x % (uint32_t)a.n_kv_heads);
+  const int64_t row = blockIdx.x / (uint32_t)a.n_kv_heads;
+  const int64_t seq = seq_of_row(a, row);
+  int64_t total = 0, before = 0;
+  for (int64_t i = tid; i < a.n; i += kTreeThreads) {
+    const int64_t x = tree_steps(a, i);
+    total += x;
+    if (i < seq) before += x;
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    total += __shfl_xor(total, off, 64);
+    before += __shfl_xor(before, off, 64);
+  }
+  if ((tid & 63) == 0) {
+    red[0][tid >> 6] = total;
+    red[1][tid >> 6] = before;
+  }
+  __syncthreads();
+  total = red[0][0] + red[0][1] + red[0][2] + red[0][3];
+  before = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+  const TreeSeq s = tree_seq(a, seq);
+  const int64_t r = row - s.rows.row0;
+  if (r < 0 || r >= s.rows.count) return;
+  const int64_t per = (total + a.groups - 1) / a.groups;
+  const int tile = (int)(r / a.rows_per_tile);
+  const int64_t begin = before + ((int64_t)kvh * s.tiles + tile) * s.steps;
+  const int64_t w0 = begin / per, w1 = (begin + s.steps - 1) / per;
+  if (w0 == w1) return;  // written whole
+  const int group = a.n_heads / a.n_kv_heads, columns = a.rows_per_tile * group;
+  const int64_t column0 = (r - (int64_t)tile * a.rows_per_tile) * group;
+  for (int e = tid * 4; e < group * a.head_dim; e += kTreeThreads * 4) {
+    const int g = e / a.head_dim, d = e - g * a.head_dim;
+    float mx = -INFINITY, l = 0.f;
+    f32x4 x = {};
+    for (int64_t w = w0; w <= w1; ++w) {
+      const int64_t column = (2 * w + (w == w0 ? 1 : 0)) * columns + column0 + g;
+      const f32x2 ml = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * column);
+      const f32x4 o = *reinterpret_cast<const f32x4 *>(a.part_o + column * a.head_dim + d);
+      const float next = __builtin_fmaxf(mx, ml.x), ref = next == -INFINITY ? 0.f : next;
+      const float kept = l * __builtin_amdgcn_exp2f(mx - ref), p = ml.y * __builtin_amdgcn_exp2f(ml.x - ref);
+      l = kept + p;
+      const float inv = l != 0.f ? 1.f / l : 0.f;  // (x stays an average, no larger than its V)
+      x = x * (kept * inv) + o * (p * inv);
+      mx = next;
+    }
+    store_row4(a, (row * a.n_heads + (int64_t)kvh * group) * a.head_dim + e, x);
+  }
+}
+
+bool tree_tiles_supported(const TreeArgs &a) {
+  const int group = a.n_heads / a.n_kv_heads;
+  return a.head_dim % 8 == 0 && a.head_dim <= 256 && group <= 64;
+}
+
+// Waves that share a step's columns: two where a tile has up to 64 (the other two
+// take half of the positions), else four.
+int tile_waves(const TreeArgs &a) {
+  return a.head_dim <= 128 && (int64_t)a.rows_per_tile * (a.n_heads / a.n_kv_heads) <= 64 ? 2 : 4;
+}
+
+template <typename T, int HD, bool EXACT, int WC>
+hipError_t launch_tiles(const PoolGeom &g, const TreeArgs &a, hipStream_t s) {
+  const bool full = a.row_type == LTKV_ROWS_F32 || a.softcap > kShortCap;
+  const auto kernel = full ? tree_tile_kernel<T, HD, EXACT, true, WC> : tree_tile_kernel<T, HD, EXACT, false, WC>;
+  kernel<<<(unsigned)a.groups, kTreeThreads, 0, s>>>(a, g.n_blocks, g.kv_dim);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_tiles_of(const PoolGeom &g, const TreeArgs &a, hipStream_t s) {
+  const bool two = tile_waves(a) == 2;
+  if (a.head_dim > 128) return launch_tiles<T, 256, false, 4>(g, a, s);
+  if (a.head_dim == 64) return two ? launch_tiles<T, 64, true, 2>(g, a, s) : launch_tiles<T, 64, true, 4>(g, a, s);
+  if (a.head_dim == 128) return two ? launch_tiles<T, 128, true, 2>(g, a, s) : launch_tiles<T, 128, true, 4>(g, a, s);
+  return two ? launch_tiles<T, 128, false, 2>(g, a, s) : launch_tiles<T, 128, false, 4>(g, a, s);
+}
+
+}  // namespace
+
+int64_t tree_workspace(int, TreeArgs &a) {
+  a.rows_per_tile = a.groups = 0;
+  if (!tree_tiles_supported(a) || a.max_len == 0) return 0;  // (max_len 0: a cache without blocks)
+  const int group = a.n_heads / a.n_kv_heads;
+  a.rows_per_tile = (int)std::min<int64_t>(a.max_rows, 32 * kTreeWaves / group);
+  // two work-groups a CU, or as many as there can be steps
+  const int64_t tiles = a.n_rows / a.rows_per_tile + a.n;
+  const int64_t steps = tiles * a.n_kv_heads * std::max<int64_t>((a.max_len + kTreeTokens - 1) / kTreeTokens, 1);
+  a.groups = (int)((std::min<int64_t>(2 * a.cu_count, steps) + 7) / 8 * 8);
+  return 2 * (int64_t)a.groups * a.rows_per_tile * group * (a.head_dim + 2) * 4;
+}
+
+void tree_partials(TreeArgs &a, uint8_t *base) {
+  a.part_o = reinterpret_cast<float *>(base);
+  a.part_ml = a.part_o + 2 * (int64_t)a.groups * a.rows_per_tile * (a.n_heads / a.n_kv_heads) * a.head_dim;
+}
 
 hipError_t launch_tree_attention(const PoolGeom &g, const TreeArgs &a, hipStream_t s) {
   if (a.n <= 0 || a.n_rows <= 0) return hipSuccess;
-  const int64_t grid = a.n_rows * a.n_heads;
-  if (grid * kAnyThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
-  return by_element(g.elem, [&](auto tag) {
-    tree_any_kernel<decltype(tag)><<<(unsigned)grid, kAnyThreads, 0, s>>>(a, g.n_blocks, g.kv_dim);
-    return hipGetLastError();
-  });
+  if (a.groups == 0) {
+    const int64_t grid = a.n_rows * a.n_heads;
+    if (grid * kAnyThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
+    return by_element(g.elem, [&](auto tag) {
+      tree_any_kernel<decltype(tag)><<<(unsigned)grid, kAnyThreads, 0, s>>>(a, g.n_blocks, g.kv_dim);
+      return hipGetLastError();
+    });
+  }
+  const int64_t merges = a.n_rows * a.n_kv_heads;
+  if (merges * kTreeThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
+  if (const hipError_t e = by_element(g.elem, [&](auto tag) { return launch_tiles_of<decltype(tag)>(g, a, s); });
+      e != hipSuccess)
+    return e;
+  tree_merge_kernel<<<(unsigned)merges, kTreeThreads, 0, s>>>(a);
+  return hipGetLastError();
 }
 
 }  // namespace ltkv
