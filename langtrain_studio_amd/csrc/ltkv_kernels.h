@@ -480,7 +480,10 @@ struct TreeArgs : ScoredArgs {
   // launch (0: the generic kernel).
   int rows_per_tile, groups;
   // Averages of the tiles that several work-groups share: part_o [slot][column]
-  // [head_dim], part_ml [slot][column][2] (reference, sum), two slots a work-group.
+  // [head_dim], part_ml [slot][column][2] (reference, sum), two slots a work-group;
+  // ends [work-group][4] names the tile that ends in a work-group's share and began
+  // in an earlier one: (first row or -1, rows, kv head, share that it began in).
+  int64_t *ends;
 };
 int64_t tree_workspace(int elem, TreeArgs &a);  // bytes of its partials
 void tree_partials(TreeArgs &a, uint8_t *base);

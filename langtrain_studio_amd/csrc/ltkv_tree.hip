@@ -317,16 +317,15 @@ struct Cells<int8_t, HD, EXACT> {
     d = __builtin_fminf(position_max(d), 65504.f);
     return d > 0.f ? __builtin_amdgcn_frexp_expf(d) - 8 : -32;
   }
+  // q d as hi + lo parts in packed f16: q has 8 bits and d 11, so what the rounding
+  // of the product leaves is an f16 number, which the fused multiply-add gives exactly
+  // (d times a power of two is one too, down to 2^-22 of the largest scale)
   __device__ __forceinline__ void pair(int j, int e, h8 &hi, h8 &lo) const {
     const h8 q = i8x8_to_h8(x[j]);
-    const float d = __builtin_amdgcn_ldexpf(scale(j), -e);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      _Float16 a, b;
-      split2((float)q[i] * d, a, b);
-      hi[i] = a;
-      lo[i] = b;
-    }
+    const _Float16 d = (_Float16)__builtin_amdgcn_ldexpf(scale(j), -e);
+    const h8 d8 = {d, d, d, d, d, d, d, d};
+    hi = q * d8;
+    lo = __builtin_elementwise_fma(q, d8, -hi);
   }
   __device__ __forceinline__ bool bad() const {
     bool b = false;
@@ -443,6 +442,7 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   const int64_t share = (int64_t)(blockIdx.x & 7) * (groups >> 3) + (blockIdx.x >> 3);
   int64_t at = share * per;
   const int64_t end = min(total, at + per);
+  if (tid == 0) a.ends[4 * share] = -1;
 
   while (at < end) {
     __syncthreads();  // s_found, and the step's memory, have been read
@@ -467,6 +467,13 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
     const int s_last = (int)min((int64_t)ts.steps, s_first + (end - at));
     const int kvh = (int)(unit / ts.tiles), tile = (int)(unit - (int64_t)kvh * ts.tiles);
     const int32_t r0 = tile * a.rows_per_tile;
+    if (tid == 0 && s_first > 0 && s_last == ts.steps) {
+      int64_t *const e = a.ends + 4 * share;
+      e[0] = rows.row0 + r0;
+      e[1] = min(a.rows_per_tile, rows.count - r0);
+      e[2] = kvh;
+      e[3] = (at - s_first) / per;
+    }
     at += s_last - s_first;
 
     // the lane's column
@@ -713,13 +720,24 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
       }
 #pragma unroll
       for (int p = 0; p < 2 * U; ++p) {  // 16 positions each
+        // hi parts of pairs by truncation (two an instruction; the lo parts take what
+        // is left), alone to nearest
         h8 wh, wl;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          _Float16 hi, lo;
-          split2(sc[p >> 1][8 * (p & 1) + i], hi, lo);
-          wh[i] = hi;
-          if constexpr (FULL) wl[i] = lo;
+        for (int i = 0; i < 8; i += 2) {
+          const float x = sc[p >> 1][8 * (p & 1) + i], y = sc[p >> 1][8 * (p & 1) + i + 1];
+          if constexpr (FULL) {
+            const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x, y));
+            const h2 lo = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi.x, -1.f, x),
+                                                                           __builtin_fmaf((float)hi.y, -1.f, y)));
+            wh[i] = hi.x;
+            wh[i + 1] = hi.y;
+            wl[i] = lo.x;
+            wl[i + 1] = lo.y;
+          } else {
+            wh[i] = (_Float16)x;
+            wh[i + 1] = (_Float16)y;
+          }
         }
         if constexpr (!FULL && !PAIRS) {  // the weights as they enter the product, two an instruction
           const h2 one = {(_Float16)1.f, (_Float16)1.f};
@@ -800,60 +818,44 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   }
 }
 
-// A work-group a (row, kv head) whose tile lies in several shares: their averages,
-// weighted by their sums against the largest reference, in order. It finds the
-// tile's place on the line by itself.
-__global__ void __launch_bounds__(kTreeThreads) tree_merge_kernel(TreeArgs a) {
-  __shared__ int64_t red[2][kTreeWaves];
-  const int tid = (int)threadIdx.x;
-  const int kvh = (int)(blockIdx.x % (uint32_t)a.n_kv_heads);
-  const int64_t row = blockIdx.x / (uint32_t)a.n_kv_heads;
-  const int64_t seq = seq_of_row(a, row);
-  int64_t total = 0, before = 0;
-  for (int64_t i = tid; i < a.n; i += kTreeThreads) {
-    const int64_t x = tree_steps(a, i);
-    total += x;
-    if (i < seq) before += x;
-  }
+// A work-group a slice of a tile that lies in several shares: their averages,
+// weighted by their sums against the largest reference, in order, four parts' loads
+// at a time.
+__global__ void __launch_bounds__(kTreeThreads) tree_merge_kernel(TreeArgs a, int slices) {
+  const int64_t share = blockIdx.x / (uint32_t)slices;
+  const int64_t *const e = a.ends + 4 * share;
+  const int64_t row0 = e[0];
+  if (row0 < 0) return;
+  const int rows = (int)e[1], kvh = (int)e[2], group = a.n_heads / a.n_kv_heads;
+  const int64_t first = e[3], columns = (int64_t)a.rows_per_tile * group;
+  const int x0 = ((int)(blockIdx.x % (uint32_t)slices) * kTreeThreads + (int)threadIdx.x) * 4;
+  const int c = x0 / a.head_dim, d = x0 - c * a.head_dim;
+  if (c >= rows * group) return;
+  constexpr int AHEAD = 4;
+  float mx = -INFINITY, l = 0.f;
+  f32x4 x = {};
+  for (int64_t w = first; w <= share; w += AHEAD) {
+    f32x2 ml[AHEAD];
+    f32x4 o[AHEAD];
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    total += __shfl_xor(total, off, 64);
-    before += __shfl_xor(before, off, 64);
-  }
-  if ((tid & 63) == 0) {
-    red[0][tid >> 6] = total;
-    red[1][tid >> 6] = before;
-  }
-  __syncthreads();
-  total = red[0][0] + red[0][1] + red[0][2] + red[0][3];
-  before = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-  const TreeSeq s = tree_seq(a, seq);
-  const int64_t r = row - s.rows.row0;
-  if (r < 0 || r >= s.rows.count) return;
-  const int64_t per = (total + a.groups - 1) / a.groups;
-  const int tile = (int)(r / a.rows_per_tile);
-  const int64_t begin = before + ((int64_t)kvh * s.tiles + tile) * s.steps;
-  const int64_t w0 = begin / per, w1 = (begin + s.steps - 1) / per;
-  if (w0 == w1) return;  // written whole
-  const int group = a.n_heads / a.n_kv_heads, columns = a.rows_per_tile * group;
-  const int64_t column0 = (r - (int64_t)tile * a.rows_per_tile) * group;
-  for (int e = tid * 4; e < group * a.head_dim; e += kTreeThreads * 4) {
-    const int g = e / a.head_dim, d = e - g * a.head_dim;
-    float mx = -INFINITY, l = 0.f;
-    f32x4 x = {};
-    for (int64_t w = w0; w <= w1; ++w) {
-      const int64_t column = (2 * w + (w == w0 ? 1 : 0)) * columns + column0 + g;
-      const f32x2 ml = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * column);
-      const f32x4 o = *reinterpret_cast<const f32x4 *>(a.part_o + column * a.head_dim + d);
-      const float next = __builtin_fmaxf(mx, ml.x), ref = next == -INFINITY ? 0.f : next;
-      const float kept = l * __builtin_amdgcn_exp2f(mx - ref), p = ml.y * __builtin_amdgcn_exp2f(ml.x - ref);
+    for (int k = 0; k < AHEAD; ++k) {
+      const int64_t v = min(w + k, share), column = (2 * v + (v == first ? 1 : 0)) * columns + c;
+      ml[k] = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * column);
+      o[k] = *reinterpret_cast<const f32x4 *>(a.part_o + column * a.head_dim + d);
+      if (w + k > share) ml[k] = f32x2{-INFINITY, 0.f};
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const float next = __builtin_fmaxf(mx, ml[k].x), ref = next == -INFINITY ? 0.f : next;
+      const float kept = l * __builtin_amdgcn_exp2f(mx - ref), p = ml[k].y * __builtin_amdgcn_exp2f(ml[k].x - ref);
       l = kept + p;
       const float inv = l != 0.f ? 1.f / l : 0.f;  // (x stays an average, no larger than its V)
-      x = x * (kept * inv) + o * (p * inv);
+      x = x * (kept * inv) + o[k] * (p * inv);
       mx = next;
     }
-    store_row4(a, (row * a.n_heads + (int64_t)kvh * group) * a.head_dim + e, x);
   }
+  const int rr = c / group;
+  store_row4(a, ((row0 + rr) * a.n_heads + (int64_t)kvh * group + (c - rr * group)) * a.head_dim + d, x);
 }
 
 bool tree_tiles_supported(const TreeArgs &a) {
@@ -895,11 +897,12 @@ int64_t tree_workspace(int, TreeArgs &a) {
   const int64_t tiles = a.n_rows / a.rows_per_tile + a.n;
   const int64_t steps = tiles * a.n_kv_heads * std::max<int64_t>((a.max_len + kTreeTokens - 1) / kTreeTokens, 1);
   a.groups = (int)((std::min<int64_t>(2 * a.cu_count, steps) + 7) / 8 * 8);
-  return 2 * (int64_t)a.groups * a.rows_per_tile * group * (a.head_dim + 2) * 4;
+  return 2 * (int64_t)a.groups * a.rows_per_tile * group * (a.head_dim + 2) * 4 + (int64_t)a.groups * 4 * 8;
 }
 
 void tree_partials(TreeArgs &a, uint8_t *base) {
-  a.part_o = reinterpret_cast<float *>(base);
+  a.ends = reinterpret_cast<int64_t *>(base);
+  a.part_o = reinterpret_cast<float *>(base + (int64_t)a.groups * 4 * 8);
   a.part_ml = a.part_o + 2 * (int64_t)a.groups * a.rows_per_tile * (a.n_heads / a.n_kv_heads) * a.head_dim;
 }
 
@@ -913,12 +916,12 @@ hipError_t launch_tree_attention(const PoolGeom &g, const TreeArgs &a, hipStream
       return hipGetLastError();
     });
   }
-  const int64_t merges = a.n_rows * a.n_kv_heads;
-  if (merges * kTreeThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
   if (const hipError_t e = by_element(g.elem, [&](auto tag) { return launch_tiles_of<decltype(tag)>(g, a, s); });
       e != hipSuccess)
     return e;
-  tree_merge_kernel<<<(unsigned)merges, kTreeThreads, 0, s>>>(a);
+  const int columns = a.rows_per_tile * (a.n_heads / a.n_kv_heads);
+  const int slices = (columns * a.head_dim + 4 * kTreeThreads - 1) / (4 * kTreeThreads);
+  tree_merge_kernel<<<(unsigned)(a.groups * slices), kTreeThreads, 0, s>>>(a, slices);
   return hipGetLastError();
 }
 
