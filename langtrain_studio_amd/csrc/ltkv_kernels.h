@@ -476,13 +476,13 @@ struct TreeArgs : ScoredArgs {
   const int32_t *positions;  // [n_rows], or nullptr (no window)
   const int32_t *masks;      // [n_rows][mask_words], or nullptr: a row sees the rows up to its own
   int64_t mask_words;
-  // Set by tree_workspace: rows of a work-group's tile and work-groups of the
-  // launch (0: the generic kernel).
-  int rows_per_tile, groups;
-  // Averages of the tiles that several work-groups share: part_o [slot][column]
+  // Set by tree_workspace: rows of a work-group's tile and shares of the line of
+  // steps, a work-group a share and kv head (0: the generic kernel).
+  int rows_per_tile, shares;
+  // Averages of the tiles that lie in several shares: part_o [slot][column]
   // [head_dim], part_ml [slot][column][2] (reference, sum), two slots a work-group;
   // ends [work-group][4] names the tile that ends in a work-group's share and began
-  // in an earlier one: (first row or -1, rows, kv head, share that it began in).
+  // in an earlier one: (first row or -1, rows, share that it began in).
   int64_t *ends;
 };
 int64_t tree_workspace(int elem, TreeArgs &a);  // bytes of its partials

@@ -153,13 +153,14 @@ __global__ void __launch_bounds__(kAnyThreads) tree_any_kernel(TreeArgs a, int64
 
 // ---- the tile kernel ----------------------------------------------------------
 //
-// Its work is laid out as one line of steps: sequence by sequence, of each the kv
-// heads, of each the tiles of rows (rows_per_tile rows by the group's query heads
-// are the columns of a work-group), of each the steps of 64 positions. Every
-// work-group takes an equal share of the line, wherever that begins and ends, so
-// that a ragged batch, one long context and a short step all load the chip evenly,
-// and a table wider than its contexts costs nothing. A tile that lies in several
-// shares leaves an average per share, which tree_merge_kernel folds.
+// Its work is laid out as one line of steps: sequence by sequence, of each the tiles
+// of rows (rows_per_tile rows by the group's query heads are the columns of a
+// work-group), of each the steps of 64 positions. The line is cut into equal
+// shares, wherever they begin and end, so that a ragged batch, one long context and
+// a short step all load the chip evenly, and a table wider than its contexts costs
+// nothing. A share has a work-group for each kv head, next to each other on one XCD:
+// they read whole pool rows together. A tile that lies in several shares leaves an
+// average per share, which tree_merge_kernel folds.
 constexpr int kTreeWaves = 4, kTreeThreads = 64 * kTreeWaves;
 constexpr int kTreeTokens = 64;  // positions of a step
 
@@ -183,7 +184,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int64_t i) {
 
 __device__ __forceinline__ int64_t tree_steps(const TreeArgs &a, int64_t i) {
   const TreeSeq s = tree_seq(a, i);
-  return (int64_t)s.steps * s.tiles * a.n_kv_heads;
+  return (int64_t)s.steps * s.tiles;
 }
 
 __device__ __forceinline__ int64_t uniform64(int64_t x) {
@@ -198,59 +199,101 @@ __device__ __forceinline__ int64_t uniform64(int64_t x) {
 template <typename T>
 constexpr bool kPairs = std::is_same_v<T, int8_t> || std::is_same_v<T, float>;
 
-// A thread's share of a step on its way from the pool to LDS: a quarter of the
-// head (NC chunks of 8 elements) of one position, K or V; a wave takes the 16
-// positions of one block, whose address is uniform. EXACT: head_dim is HD; else
-// elements past head_dim are zeros and a chunk brings its own scale (a head may
-// begin inside a group of 32).
-template <typename T, int HD, bool EXACT>
+// A load at a uniform base plus a 32-bit lane offset (see load_at). NT: past the
+// caches, for rows that one work-group reads alone; each line in one instruction, else
+// it is fetched twice.
+template <bool NT, typename V>
+__device__ __forceinline__ V pool_load(const char *base, uint32_t off) {
+  if constexpr (!NT) return load_at<V>(base, off);
+  asm volatile("" : "+v"(off));
+  return __builtin_nontemporal_load(reinterpret_cast<const V *>(base + off));
+}
+
+// Largest of a value over aligned groups of N lanes (a power of two), in each of them.
+template <int N>
+__device__ __forceinline__ float lanes_max(float x) {
+  if constexpr (N > 1) x = __builtin_fmaxf(x, dpp<0xB1>(x));    // quad_perm [1,0,3,2]
+  if constexpr (N > 2) x = __builtin_fmaxf(x, dpp<0x4E>(x));    // quad_perm [2,3,0,1]
+  if constexpr (N > 4) x = __builtin_fmaxf(x, dpp<0x141>(x));   // row_half_mirror
+  if constexpr (N > 8) x = __builtin_fmaxf(x, dpp<0x140>(x));   // row_mirror
+  if constexpr (N > 16) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t p = a[0], q = a[1];
+    x = __builtin_fmaxf(__builtin_bit_cast(float, p), __builtin_bit_cast(float, q));
+  }
+  if constexpr (N > 32) x = halves_reduce<true>(x);
+  return x;
+}
+
+// A wave's share of a step on its way from the pool to LDS: K or V of the 16
+// positions of one block, whose address is uniform. A load takes whole rows of the
+// head, ROW lanes each, 64 / ROW rows an instruction: with 64 bytes of 16 rows an
+// instruction, lines were fetched in two pieces (64 trees of up to 16 rows, f16: the
+// loads alone 197 us; so, past the caches, 160). EXACT: head_dim is HD, 64 or 128; else
+// elements past head_dim are zeros, and 8-bit and 4-bit chunks of 8 bring a scale
+// each (a head may begin inside a group of 32).
+// put() writes the positions' rows in LDS; `bad` has a bit for each load whose V
+// enters as zeros (bad()). Types of pairs give each position's power of two too.
+template <typename T, int HD, bool EXACT, bool NT>
 struct Cells;
 
-template <int HD, bool EXACT>
-struct Cells<_Float16, HD, EXACT> {
-  static constexpr int NC = HD / 32;
-  u32x4 x[NC];
-  __device__ static __forceinline__ int chunk(int part, int j) { return part + 4 * j; }
+template <int HD, bool EXACT, bool NT>
+struct Cells<_Float16, HD, EXACT, NT> {
+  static constexpr int ROW = HD / 8, ROWS = 64 / ROW, N = 16 / ROWS;
+  u32x4 x[N];
   static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 32; }
+  static __device__ __forceinline__ int row(int lane, int j) { return lane / ROW + ROWS * j; }
   __device__ __forceinline__ void load(const void *pool, const void *, int64_t at, int64_t kv_dim, uint32_t head_off,
-                                       int slot, int part, int head_dim) {
+                                       int lane, int head_dim) {
     const char *base = static_cast<const char *>(pool) + at;
-    const uint32_t place = (uint32_t)((slot * (uint32_t)kv_dim + head_off + part * 8) * 2);
+    const uint32_t e = lane % ROW * 8, place = ((lane / ROW) * (uint32_t)kv_dim + head_off + e) * 2;
 #pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      if (EXACT || chunk(part, j) * 8 < head_dim) x[j] = load_at<u32x4>(base, place + 64 * j);
+    for (int j = 0; j < N; ++j) {
+      if (EXACT || (int)e < head_dim) x[j] = pool_load<NT, u32x4>(base, place + (uint32_t)(2 * ROWS * j) * (uint32_t)kv_dim);
       else x[j] = u32x4{0, 0, 0, 0};
     }
   }
-  __device__ __forceinline__ h8 get(int j) const { return __builtin_bit_cast(h8, x[j]); }
-  __device__ __forceinline__ bool bad() const {
-    bool b = false;
+  __device__ __forceinline__ uint32_t bad() const {
+    uint32_t b = 0;
 #pragma unroll
-    for (int j = 0; j < NC; ++j) b |= not_finite(get(j));
+    for (int j = 0; j < N; ++j) b |= not_finite(__builtin_bit_cast(h8, x[j])) ? 1u << j : 0u;
     return b;
+  }
+  __device__ __forceinline__ void put(char *lds, int pitch, int lane, uint32_t bad) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      *reinterpret_cast<u32x4 *>(lds + row(lane, j) * pitch + lane % ROW * 16) =
+          bad >> j & 1 ? u32x4{0, 0, 0, 0} : x[j];
   }
 };
 
-template <int HD, bool EXACT>
-struct Cells<Q4, HD, EXACT> {
-  static constexpr int NC = HD / 32, NS = EXACT ? 1 : NC;
+template <int HD, bool EXACT, bool NT>
+struct Cells<Q4, HD, EXACT, NT> {
+  // a lane takes a quarter of one position's head: of a head of whole groups, the
+  // lanes of a load take a contiguous piece of the block's tiles
+  static constexpr int ROW = 4, ROWS = 16, N = 1, NC = HD / 32, NS = EXACT ? 1 : NC;
   uint32_t x[NC];
   uint32_t s[NS];  // (as 32 bits: a 16-bit value would be waited for to be moved)
-  __device__ static __forceinline__ int chunk(int part, int j) { return EXACT ? part * NC + j : part + 4 * j; }
   static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 8; }
+  static __device__ __forceinline__ int row(int lane, int) { return lane >> 2; }
+  static __device__ __forceinline__ int chunk(int lane, int j) {
+    return EXACT ? (lane & 3) * NC + j : (lane & 3) + 4 * j;
+  }
   __device__ __forceinline__ void load(const void *pool, const void *scales, int64_t at, int64_t, uint32_t head_off,
-                                       int slot, int part, int head_dim) {
+                                       int lane, int head_dim) {
     const char *base = static_cast<const char *>(pool) + at, *sbase = static_cast<const char *>(scales) + (at >> 3);
+    const uint32_t slot = lane >> 2;
     if constexpr (EXACT) {
-      static_assert(NC == 2 || NC == 4, "a thread's chunks lie in one group");
-      const uint32_t e = head_off + part * NC * 8, place = ((e >> 5) * 16 + slot) * 16 + ((e & 31) >> 3) * 4;
+      static_assert(NC == 2 || NC == 4, "a lane's chunks lie in one group");
+      const uint32_t e = head_off + chunk(lane, 0) * 8, place = ((e >> 5) * 16 + slot) * 16 + ((e & 31) >> 3) * 4;
       s[0] = load_at<uint16_t>(sbase, (place >> 4) * 2);
       if constexpr (NC == 4) {
-        const u32x4 w = load_at<u32x4>(base, place);
+        const u32x4 w = pool_load<NT, u32x4>(base, place);
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = w[j];
       } else {
-        const u32x2 w = load_at<u32x2>(base, place);
+        const u32x2 w = pool_load<NT, u32x2>(base, place);
         x[0] = w.x;
         x[1] = w.y;
       }
@@ -259,125 +302,131 @@ struct Cells<Q4, HD, EXACT> {
       for (int j = 0; j < NC; ++j) {
         x[j] = 0;
         s[j] = 0;
-        if (chunk(part, j) * 8 >= head_dim) continue;
-        const uint32_t e = head_off + chunk(part, j) * 8, tile = (e >> 5) * 16 + slot;
+        if (chunk(lane, j) * 8 >= head_dim) continue;
+        const uint32_t e = head_off + chunk(lane, j) * 8, tile = (e >> 5) * 16 + slot;
         x[j] = load_at<uint32_t>(base, tile * 16 + ((e & 31) >> 3) * 4);
         s[j] = load_at<uint16_t>(sbase, tile * 2);
       }
     }
   }
-  __device__ __forceinline__ h8 get(int j) const {
-    const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t)s[EXACT ? 0 : j]);
-    return q4x8_to_h8(x[j], h2{d, d});
+  __device__ __forceinline__ uint32_t bad() const { return 0; }
+  __device__ __forceinline__ void put(char *lds, int pitch, int lane, uint32_t) const {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t)s[EXACT ? 0 : j]);
+      *reinterpret_cast<h8 *>(lds + row(lane, 0) * pitch + chunk(lane, j) * 16) = q4x8_to_h8(x[j], h2{d, d});
+    }
   }
-  __device__ __forceinline__ bool bad() const { return false; }
 };
 
-template <int HD, bool EXACT>
-struct Cells<int8_t, HD, EXACT> {
-  static constexpr int NC = HD / 32, NS = EXACT ? 1 : NC;
-  u32x2 x[NC];
-  uint32_t s[NS];
-  __device__ static __forceinline__ int chunk(int part, int j) { return EXACT ? part * NC + j : part + 4 * j; }
+template <int HD, bool EXACT, bool NT>
+struct Cells<int8_t, HD, EXACT, NT> {
+  static constexpr int E = EXACT ? 16 : 8;  // elements a load and lane
+  static constexpr int ROW = HD / E, ROWS = 64 / ROW, N = 16 / ROWS;
+  typedef std::conditional_t<EXACT, u32x4, u32x2> Quants;
+  Quants x[N];
+  uint32_t s[N];
   static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 16; }
+  static __device__ __forceinline__ int row(int lane, int j) { return lane / ROW + ROWS * j; }
   __device__ __forceinline__ void load(const void *pool, const void *scales, int64_t at, int64_t kv_dim,
-                                       uint32_t head_off, int slot, int part, int head_dim) {
+                                       uint32_t head_off, int lane, int head_dim) {
     const char *base = static_cast<const char *>(pool) + at, *sbase = static_cast<const char *>(scales) + (at >> 4);
-    const uint32_t row = slot * (uint32_t)kv_dim;
-    if constexpr (EXACT) {
-      static_assert(NC == 2 || NC == 4, "a thread's chunks lie in one group");
-      const uint32_t e = head_off + part * NC * 8;
-      s[0] = load_at<uint16_t>(sbase, ((e >> 5) * 16 + slot) * 2);
+    const uint32_t e = head_off + lane % ROW * E, place = lane / ROW * (uint32_t)kv_dim + e;
 #pragma unroll
-      for (int j = 0; j < NC; j += 2) {
-        const u32x4 w = load_at<u32x4>(base, row + e + 8 * j);
-        x[j] = u32x2{w.x, w.y};
-        x[j + 1] = u32x2{w.z, w.w};
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        x[j] = u32x2{0x80808080u, 0x80808080u};  // (quants are stored offset by 128)
+    for (int j = 0; j < N; ++j) {
+      if (EXACT || lane % ROW * E < head_dim) {
+        s[j] = load_at<uint16_t>(sbase, ((e >> 5) * 16 + row(lane, j)) * 2);
+        x[j] = pool_load<NT, Quants>(base, place + (uint32_t)(ROWS * j) * (uint32_t)kv_dim);
+      } else {
         s[j] = 0;
-        if (chunk(part, j) * 8 >= head_dim) continue;
-        const uint32_t e = head_off + chunk(part, j) * 8;
-        x[j] = load_at<u32x2>(base, row + e);
-        s[j] = load_at<uint16_t>(sbase, ((e >> 5) * 16 + slot) * 2);
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i) x[j][i] = 0x80808080u;  // (quants are stored offset by 128)
       }
     }
   }
   __device__ __forceinline__ float scale(int j) const {
-    return (float)__builtin_bit_cast(_Float16, (uint16_t)s[EXACT ? 0 : j]);
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)s[j]);
   }
-  // e such that elements times 2^-e stay below 2^15
-  __device__ __forceinline__ int exponent() const {
-    float d = 0.f;
+  __device__ __forceinline__ uint32_t bad() const {
+    uint32_t b = 0;
 #pragma unroll
-    for (int j = 0; j < NS; ++j) d = __builtin_fmaxf(d, scale(j));
-    d = __builtin_fminf(position_max(d), 65504.f);
-    return d > 0.f ? __builtin_amdgcn_frexp_expf(d) - 8 : -32;
-  }
-  // q d as hi + lo parts in packed f16: q has 8 bits and d 11, so what the rounding
-  // of the product leaves is an f16 number, which the fused multiply-add gives exactly
-  // (d times a power of two is one too, down to 2^-22 of the largest scale)
-  __device__ __forceinline__ void pair(int j, int e, h8 &hi, h8 &lo) const {
-    const h8 q = i8x8_to_h8(x[j]);
-    const _Float16 d = (_Float16)__builtin_amdgcn_ldexpf(scale(j), -e);
-    const h8 d8 = {d, d, d, d, d, d, d, d};
-    hi = q * d8;
-    lo = __builtin_elementwise_fma(q, d8, -hi);
-  }
-  __device__ __forceinline__ bool bad() const {
-    bool b = false;
-#pragma unroll
-    for (int j = 0; j < NS; ++j) b |= !(scale(j) <= 65504.f);
+    for (int j = 0; j < N; ++j) b |= scale(j) <= 65504.f ? 0u : 1u << j;
     return b;
   }
-};
-
-template <int HD, bool EXACT>
-struct Cells<float, HD, EXACT> {
-  static constexpr int NC = HD / 32;
-  u32x4 x[2 * NC];
-  __device__ static __forceinline__ int chunk(int part, int j) { return part + 4 * j; }
-  static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 64; }
-  __device__ __forceinline__ void load(const void *pool, const void *, int64_t at, int64_t kv_dim, uint32_t head_off,
-                                       int slot, int part, int head_dim) {
-    const char *base = static_cast<const char *>(pool) + at;
-    const uint32_t place = (uint32_t)((slot * (uint32_t)kv_dim + head_off + part * 8) * 4);
+  // Elements times 2^-e stay below 2^15. q d as hi + lo parts in packed f16: q has 8
+  // bits and d 11, so what the rounding of the product leaves is an f16 number, which
+  // the fused multiply-add gives exactly (d times a power of two is one too, down to
+  // 2^-22 of the largest scale).
+  template <int PLANES>
+  __device__ __forceinline__ void put(char *lds, int plane, int pitch, int lane, uint32_t bad, float *pow) const {
 #pragma unroll
-    for (int j = 0; j < NC; ++j) {
+    for (int j = 0; j < N; ++j) {
+      const float d0 = scale(j), top = lanes_max<ROW>(__builtin_fminf(d0, 65504.f));
+      const int e = top > 0.f ? __builtin_amdgcn_frexp_expf(top) - 8 : -32;
+      const _Float16 d = bad >> j & 1 ? (_Float16)0.f : (_Float16)__builtin_amdgcn_ldexpf(d0, -e);
+      const h8 d8 = {d, d, d, d, d, d, d, d};
+      if (lane % ROW == 0) pow[row(lane, j)] = __builtin_amdgcn_ldexpf(1.f, e);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (EXACT || chunk(part, j) * 8 < head_dim) x[2 * j + i] = load_at<u32x4>(base, place + 128 * j + 16 * i);
-        else x[2 * j + i] = u32x4{0, 0, 0, 0};
+      for (int i = 0; i < E / 8; ++i) {
+        const h8 q = i8x8_to_h8(u32x2{x[j][2 * i], x[j][2 * i + 1]}), hi = q * d8;
+        char *const to = lds + row(lane, j) * pitch + lane % ROW * (2 * E) + 16 * i;
+        *reinterpret_cast<h8 *>(to) = hi;
+        if constexpr (PLANES == 2) *reinterpret_cast<h8 *>(to + plane) = __builtin_elementwise_fma(q, d8, -hi);
       }
     }
   }
-  __device__ __forceinline__ uint32_t top_bits() const {
-    uint32_t m = 0;
+};
+
+template <int HD, bool EXACT, bool NT>
+struct Cells<float, HD, EXACT, NT> {
+  static constexpr int ROW = HD / 4, ROWS = 64 / ROW, N = 16 / ROWS;
+  u32x4 x[N];
+  static __device__ __forceinline__ int64_t block_bytes(int64_t kv_dim) { return kv_dim * 64; }
+  static __device__ __forceinline__ int row(int lane, int j) { return lane / ROW + ROWS * j; }
+  __device__ __forceinline__ void load(const void *pool, const void *, int64_t at, int64_t kv_dim, uint32_t head_off,
+                                       int lane, int head_dim) {
+    const char *base = static_cast<const char *>(pool) + at;
+    const uint32_t e = lane % ROW * 4, place = ((lane / ROW) * (uint32_t)kv_dim + head_off + e) * 4;
 #pragma unroll
-    for (int j = 0; j < 2 * NC; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) m = max(m, x[j][i] & 0x7fffffffu);
-    return m;
-  }
-  // (at least -100: smaller values are nothing beside their products' rounding)
-  __device__ __forceinline__ int exponent() const {
-    const float m = position_max(__builtin_bit_cast(float, min(top_bits(), 0x7f7fffffu)));
-    return m > 0.f ? max(__builtin_amdgcn_frexp_expf(m) - 15, -100) : -100;
-  }
-  __device__ __forceinline__ void pair(int j, int e, h8 &hi, h8 &lo) const {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      _Float16 a, b;
-      const uint32_t u = x[2 * j + (i >> 2)][i & 3];
-      split2(__builtin_amdgcn_ldexpf(__builtin_bit_cast(float, u), -e), a, b);
-      hi[i] = a;
-      lo[i] = b;
+    for (int j = 0; j < N; ++j) {
+      if (EXACT || (int)e < head_dim) x[j] = pool_load<NT, u32x4>(base, place + (uint32_t)(4 * ROWS * j) * (uint32_t)kv_dim);
+      else x[j] = u32x4{0, 0, 0, 0};
     }
   }
-  __device__ __forceinline__ bool bad() const { return top_bits() >= 0x7f800000u; }
+  __device__ __forceinline__ uint32_t top_bits(int j) const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, x[j][i] & 0x7fffffffu);
+    return m;
+  }
+  __device__ __forceinline__ uint32_t bad() const {
+    uint32_t b = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) b |= top_bits(j) >= 0x7f800000u ? 1u << j : 0u;
+    return b;
+  }
+  // (powers of at least 2^-100: smaller values are nothing beside their products' rounding)
+  template <int PLANES>
+  __device__ __forceinline__ void put(char *lds, int plane, int pitch, int lane, uint32_t bad, float *pow) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float top = lanes_max<ROW>(__builtin_bit_cast(float, min(top_bits(j), 0x7f7fffffu)));
+      const int e = top > 0.f ? max(__builtin_amdgcn_frexp_expf(top) - 15, -100) : -100;
+      if (lane % ROW == 0) pow[row(lane, j)] = __builtin_amdgcn_ldexpf(1.f, e);
+      h4 hi, lo;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        _Float16 a, b;
+        const uint32_t u = bad >> j & 1 ? 0u : x[j][i];
+        split2(__builtin_amdgcn_ldexpf(__builtin_bit_cast(float, u), -e), a, b);
+        hi[i] = a;
+        lo[i] = b;
+      }
+      char *const to = lds + row(lane, j) * pitch + lane % ROW * 8;
+      *reinterpret_cast<h4 *>(to) = hi;
+      if constexpr (PLANES == 2) *reinterpret_cast<h4 *>(to + plane) = lo;
+    }
+  }
 };
 
 // WC waves share a step's columns, 32 each; 4 / WC waves its positions. Steps go
@@ -402,10 +451,16 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   constexpr int K_BYTES = kTreeTokens * K_PITCH, V_BYTES = kTreeTokens * V_PITCH;
   constexpr int STEP_BYTES = K_PLANES * K_BYTES + V_PLANES * V_BYTES;
   constexpr int FOLD = NC * 16 + 4;  // floats that a lane hands over where waves share columns
+  // Few columns (WC 2) are bound by the pool's bytes: two steps ahead of the products,
+  // in registers that Q leaves free in LDS.
+  constexpr int AHEAD = WC == 2 && !PAIRS ? 2 : 1;
+  constexpr bool Q_LDS = AHEAD == 2 && HD > 64;
+  constexpr int Q_BYTES = Q_LDS ? 32 * WC * K_PITCH : 16;
   static_assert(WP == 1 || (kTreeWaves - WC) * 64 * FOLD * 4 <= STEP_BYTES, "the fold fits the step's memory");
   __shared__ __align__(16) char lds[STEP_BYTES];
+  __shared__ __align__(16) char lds_q[(FULL ? 2 : 1) * Q_BYTES];
   __shared__ __align__(16) float s_kpow[PAIRS ? kTreeTokens : 4], s_vpow[PAIRS ? kTreeTokens : 4];
-  __shared__ uint64_t s_bad[kTreeWaves];  // lanes whose share of V is left out (positions 16 wave + lane / 4)
+  __shared__ uint32_t s_bad[kTreeWaves];  // bit p: V of position 16 wave + p has an infinity or NaN
   __shared__ int64_t s_begin[kTreeThreads + 1];
   __shared__ int64_t s_sum[kTreeWaves];
   __shared__ int64_t s_found[2];
@@ -437,12 +492,15 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
     __syncthreads();
   }
   const int64_t total = uniform64(s_begin[kTreeThreads]);
-  const uint32_t groups = gridDim.x;  // a multiple of 8: neighbours on the line share an XCD's L2
-  const int64_t per = (total + groups - 1) / groups;
-  const int64_t share = (int64_t)(blockIdx.x & 7) * (groups >> 3) + (blockIdx.x >> 3);
+  const int64_t per = (total + a.shares - 1) / a.shares;
+  // (shares: a multiple of 8; neighbours on the line lie on one XCD too, of eight)
+  const uint32_t place = blockIdx.x >> 3;
+  const int kvh = (int)(place % (uint32_t)a.n_kv_heads);
+  const int64_t share = (int64_t)(blockIdx.x & 7) * (a.shares >> 3) + place / (uint32_t)a.n_kv_heads;
+  const int64_t me = share * a.n_kv_heads + kvh;
   int64_t at = share * per;
   const int64_t end = min(total, at + per);
-  if (tid == 0) a.ends[4 * share] = -1;
+  if (tid == 0) a.ends[4 * me] = -1;
 
   while (at < end) {
     __syncthreads();  // s_found, and the step's memory, have been read
@@ -462,17 +520,15 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
     const int64_t seq = uniform64(s_found[0]), off = at - uniform64(s_found[1]);
     const TreeSeq ts = tree_seq(a, seq);
     const SeqRows rows = ts.rows;
-    const int64_t unit = off / ts.steps;
-    const int s_first = (int)(off - unit * ts.steps);
+    const int tile = (int)(off / ts.steps);
+    const int s_first = (int)(off - (int64_t)tile * ts.steps);
     const int s_last = (int)min((int64_t)ts.steps, s_first + (end - at));
-    const int kvh = (int)(unit / ts.tiles), tile = (int)(unit - (int64_t)kvh * ts.tiles);
     const int32_t r0 = tile * a.rows_per_tile;
     if (tid == 0 && s_first > 0 && s_last == ts.steps) {
-      int64_t *const e = a.ends + 4 * share;
+      int64_t *const e = a.ends + 4 * me;
       e[0] = rows.row0 + r0;
       e[1] = min(a.rows_per_tile, rows.count - r0);
-      e[2] = kvh;
-      e[3] = (at - s_first) / per;
+      e[2] = (at - s_first) / per;
     }
     at += s_last - s_first;
 
@@ -510,7 +566,8 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
     }
 
     // Q columns, times a power of two and the scale's sign
-    h8 qh[NK], ql[FULL ? NK : 1];
+    h8 qh[Q_LDS ? 1 : NK], ql[FULL && !Q_LDS ? NK : 1];
+    char *const qp = lds_q + (Q_LDS ? (32 * cw + col) * K_PITCH + 16 * half : 0);
     int q_exp;
     {
       float x[NK][8], amax = 0.f;
@@ -525,15 +582,24 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
       // (at most 100: a smaller row's scores are nothing beside their rounding)
       q_exp = amax > 0.f && amax < INFINITY ? min(10 - __builtin_amdgcn_frexp_expf(amax), 100) : 0;
 #pragma unroll
-      for (int j = 0; j < NK; ++j)
+      for (int j = 0; j < NK; ++j) {
+        h8 hi8, lo8;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float y = __builtin_amdgcn_ldexpf(x[j][i], q_exp);
           _Float16 hi, lo;
           split2(a.scale < 0.f ? -y : y, hi, lo);
-          qh[j][i] = hi;
-          if constexpr (FULL) ql[j][i] = lo;
+          hi8[i] = hi;
+          lo8[i] = lo;
         }
+        if constexpr (Q_LDS) {  // (waves of the same columns write the same; the loop's barriers come first)
+          *reinterpret_cast<h8 *>(qp + 32 * j) = hi8;
+          if constexpr (FULL) *reinterpret_cast<h8 *>(qp + Q_BYTES + 32 * j) = lo8;
+        } else {
+          qh[j] = hi8;
+          if constexpr (FULL) ql[j] = lo8;
+        }
+      }
     }
     const bool cap = a.softcap > 0.f;
     const float scale = __builtin_fabsf(a.scale);
@@ -547,62 +613,56 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
     float top_o = -INFINITY, to_o = 0.f;   // pairs: numerators are taken times 2^(ref - top_o) = to_o
     bool poisoned = false;                 // the column sees an infinity or NaN in V
 
-    const int tok = tid >> 2, part = tid & 3;
     auto block_of = [&](int s) {  // the wave's block of a step (past the end: block 0, read and masked)
       const int32_t t = ts.first + kTreeTokens * s + 16 * wave;
       const int32_t e = s < s_last && t < rows.len ? scalar_read(tab, t >> 4) : 0;
       return (uint32_t)e < (uint32_t)n_blocks ? e : 0;
     };
-    const int64_t block_bytes = Cells<T, HD, EXACT>::block_bytes(kv_dim);
     const uint32_t head_off = (uint32_t)(kvh * a.head_dim);
-    Cells<T, HD, EXACT> ks, vs;
-    auto load = [&](int32_t block) {
-      const int64_t b = (int64_t)(uint32_t)block * block_bytes;
-      ks.load(a.k_layer, a.k_scale, b, kv_dim, head_off, tok & 15, part, a.head_dim);
-      vs.load(a.v_layer, a.v_scale, b, kv_dim, head_off, tok & 15, part, a.head_dim);
+    // (rows of one tile are read by one work-group alone)
+    typedef Cells<T, HD, EXACT, WC == 2> Rows;
+    struct Step {
+      Rows k, v;
     };
-    int32_t next = block_of(s_first + 1);
-    load(block_of(s_first));
+    Step steps[AHEAD];
+    auto load = [&](Step &x, int32_t block) {
+      const int64_t b = (int64_t)(uint32_t)block * Rows::block_bytes(kv_dim);
+      x.k.load(a.k_layer, a.k_scale, b, kv_dim, head_off, lane, a.head_dim);
+      x.v.load(a.v_layer, a.v_scale, b, kv_dim, head_off, lane, a.head_dim);
+    };
+    int32_t next = block_of(s_first + AHEAD);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) load(steps[k], block_of(s_first + k));
 
-    for (int s = s_first; s < s_last; ++s) {
+    auto step = [&](Step &cells, int s) __attribute__((always_inline)) {
       const int32_t t0 = ts.first + kTreeTokens * s;
       const bool partial = t0 + kTreeTokens > ts.ctx || t0 < from_max;  // some row does not see all of it
       lds_barrier();  // the last step has been read
-      bool bad = false;
-      if (partial) bad = vs.bad();
+      uint32_t bad = 0, bad_rows = 0;  // infinities and NaN of V may reach only the rows that see them
+      if (partial) {
+        bad = cells.v.bad();
+        if (__builtin_amdgcn_ballot_w64(bad != 0)) {
+#pragma unroll
+          for (int j = 0; j < Rows::N; ++j) {
+            const uint64_t lanes = __builtin_amdgcn_ballot_w64(bad >> j & 1);
+            for (int r = 0; r < Rows::ROWS; ++r)
+              if (lanes >> (r * Rows::ROW) & (~0ull >> (64 - Rows::ROW))) bad_rows |= 1u << (r + Rows::ROWS * j);
+          }
+        }
+      }
       if constexpr (PAIRS) {
-        const int ek = ks.exponent(), ev = vs.exponent();
-        if (part == 0) {
-          s_kpow[tok] = __builtin_amdgcn_ldexpf(1.f, ek);
-          s_vpow[tok] = __builtin_amdgcn_ldexpf(1.f, ev);
-        }
-#pragma unroll
-        for (int j = 0; j < NC; ++j) {
-          const int x = Cells<T, HD, EXACT>::chunk(part, j) * 16;
-          h8 hi, lo;
-          ks.pair(j, ek, hi, lo);
-          *reinterpret_cast<h8 *>(lds_k + tok * K_PITCH + x) = hi;
-          *reinterpret_cast<h8 *>(lds_k + K_BYTES + tok * K_PITCH + x) = lo;
-          vs.pair(j, ev, hi, lo);
-          *reinterpret_cast<h8 *>(lds_v + tok * V_PITCH + x) = bad ? h8{} : hi;
-          if constexpr (V_PLANES == 2) *reinterpret_cast<h8 *>(lds_v + V_BYTES + tok * V_PITCH + x) = bad ? h8{} : lo;
-        }
+        cells.k.template put<2>(lds_k + 16 * wave * K_PITCH, K_BYTES, K_PITCH, lane, 0, s_kpow + 16 * wave);
+        cells.v.template put<V_PLANES>(lds_v + 16 * wave * V_PITCH, V_BYTES, V_PITCH, lane, bad, s_vpow + 16 * wave);
       } else {
-#pragma unroll
-        for (int j = 0; j < NC; ++j) {
-          const int x = Cells<T, HD, EXACT>::chunk(part, j) * 16;
-          *reinterpret_cast<h8 *>(lds_k + tok * K_PITCH + x) = ks.get(j);
-          *reinterpret_cast<h8 *>(lds_v + tok * V_PITCH + x) = bad ? h8{} : vs.get(j);
-        }
+        cells.k.put(lds_k + 16 * wave * K_PITCH, K_PITCH, lane, 0);
+        cells.v.put(lds_v + 16 * wave * V_PITCH, V_PITCH, lane, bad);
       }
-      const uint64_t bad_lanes = __builtin_amdgcn_ballot_w64(bad);
-      if (lane == 0) s_bad[wave] = bad_lanes;
-      if (s + 1 < s_last) {
-        load(next);
-        next = block_of(s + 2);
-      }
+      if (lane == 0) s_bad[wave] = bad_rows;
+      // (without a condition: it would have the loads of all steps waited for)
+      load(cells, next);
+      next = block_of(s + AHEAD + 1);
       lds_barrier();
-      if (!wave_live) continue;
+      if (!wave_live) return;
 
       // scores of positions t0 + 32 (pw U + u) + 8 (i / 4) + 4 half + i % 4
       f32x16 sc[U];
@@ -611,14 +671,22 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
       const char *kp = lds_k + (32 * pw * U + col) * K_PITCH + 16 * half;
 #pragma unroll
       for (int j = 0; j < NK; ++j) {
+        h8 qhi, qlo;
+        if constexpr (Q_LDS) {
+          qhi = *reinterpret_cast<const h8 *>(qp + 32 * j);
+          if constexpr (FULL) qlo = *reinterpret_cast<const h8 *>(qp + Q_BYTES + 32 * j);
+        } else {
+          qhi = qh[j];
+          if constexpr (FULL) qlo = ql[j];
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const h8 x = *reinterpret_cast<const h8 *>(kp + 32 * u * K_PITCH + 32 * j);
-          sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[j], sc[u], 0, 0, 0);
-          if constexpr (FULL) sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[j], sc[u], 0, 0, 0);
+          sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qhi, sc[u], 0, 0, 0);
+          if constexpr (FULL) sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qlo, sc[u], 0, 0, 0);
           if constexpr (PAIRS) {
             const h8 y = *reinterpret_cast<const h8 *>(kp + K_BYTES + 32 * u * K_PITCH + 32 * j);
-            sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[j], sc[u], 0, 0, 0);
+            sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qhi, sc[u], 0, 0, 0);
           }
         }
       }
@@ -654,13 +722,7 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
           for (int i = 0; i < 16; ++i)
             sc[u][i] = mine >> (8 * (i / 4) + i % 4) & 1 ? sc[u][i] : -INFINITY;
           // the infinities and NaN of V entered as zeros
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const uint64_t lanes = s_bad[2 * (pw * U + u) + w];
-            if (__builtin_amdgcn_readfirstlane(lanes != 0))
-              for (int p = 0; p < 16; ++p)
-                poisoned |= (lanes >> (4 * p) & 15) != 0 && (seen >> (16 * w + p) & 1);
-          }
+          poisoned |= (seen & (s_bad[2 * (pw * U + u)] | s_bad[2 * (pw * U + u) + 1] << 16)) != 0;
         }
       }
       float top = sc[0][0];
@@ -757,6 +819,11 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
           }
         }
       }
+    };
+    for (int s = s_first; s < s_last; s += AHEAD) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (s + k < s_last) step(steps[k], s + k);
     }
 
     // the column's average
@@ -796,7 +863,7 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
     const float back = PAIRS && top_o > -INFINITY ? __builtin_amdgcn_exp2f(top_o - ref) : 1.f;
     const bool whole = s_first == 0 && s_last == ts.steps;
     // (a share's last tile may go on in the next one, its first come from the last)
-    const int64_t slot = 2 * share + (s_first == 0 ? 1 : 0);
+    const int64_t slot = 2 * me + (s_first == 0 ? 1 : 0);
     const int64_t column = slot * (a.rows_per_tile * group) + c;
     const int64_t out0 = (row * a.n_heads + head) * (int64_t)a.head_dim;
 #pragma unroll
@@ -822,12 +889,12 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
 // weighted by their sums against the largest reference, in order, four parts' loads
 // at a time.
 __global__ void __launch_bounds__(kTreeThreads) tree_merge_kernel(TreeArgs a, int slices) {
-  const int64_t share = blockIdx.x / (uint32_t)slices;
-  const int64_t *const e = a.ends + 4 * share;
+  const int64_t me = blockIdx.x / (uint32_t)slices, share = me / a.n_kv_heads;
+  const int64_t *const e = a.ends + 4 * me;
   const int64_t row0 = e[0];
   if (row0 < 0) return;
-  const int rows = (int)e[1], kvh = (int)e[2], group = a.n_heads / a.n_kv_heads;
-  const int64_t first = e[3], columns = (int64_t)a.rows_per_tile * group;
+  const int rows = (int)e[1], kvh = (int)(me - share * a.n_kv_heads), group = a.n_heads / a.n_kv_heads;
+  const int64_t first = e[2], columns = (int64_t)a.rows_per_tile * group;
   const int x0 = ((int)(blockIdx.x % (uint32_t)slices) * kTreeThreads + (int)threadIdx.x) * 4;
   const int c = x0 / a.head_dim, d = x0 - c * a.head_dim;
   if (c >= rows * group) return;
@@ -839,7 +906,8 @@ __global__ void __launch_bounds__(kTreeThreads) tree_merge_kernel(TreeArgs a, in
     f32x4 o[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      const int64_t v = min(w + k, share), column = (2 * v + (v == first ? 1 : 0)) * columns + c;
+      const int64_t v = min(w + k, share);
+      const int64_t column = (2 * (v * a.n_kv_heads + kvh) + (v == first ? 1 : 0)) * columns + c;
       ml[k] = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * column);
       o[k] = *reinterpret_cast<const f32x4 *>(a.part_o + column * a.head_dim + d);
       if (w + k > share) ml[k] = f32x2{-INFINITY, 0.f};
@@ -873,7 +941,7 @@ template <typename T, int HD, bool EXACT, int WC>
 hipError_t launch_tiles(const PoolGeom &g, const TreeArgs &a, hipStream_t s) {
   const bool full = a.row_type == LTKV_ROWS_F32 || a.softcap > kShortCap;
   const auto kernel = full ? tree_tile_kernel<T, HD, EXACT, true, WC> : tree_tile_kernel<T, HD, EXACT, false, WC>;
-  kernel<<<(unsigned)a.groups, kTreeThreads, 0, s>>>(a, g.n_blocks, g.kv_dim);
+  kernel<<<(unsigned)(a.shares * a.n_kv_heads), kTreeThreads, 0, s>>>(a, g.n_blocks, g.kv_dim);
   return hipGetLastError();
 }
 
@@ -889,26 +957,29 @@ hipError_t launch_tiles_of(const PoolGeom &g, const TreeArgs &a, hipStream_t s) 
 }  // namespace
 
 int64_t tree_workspace(int, TreeArgs &a) {
-  a.rows_per_tile = a.groups = 0;
+  a.rows_per_tile = a.shares = 0;
   if (!tree_tiles_supported(a) || a.max_len == 0) return 0;  // (max_len 0: a cache without blocks)
   const int group = a.n_heads / a.n_kv_heads;
   a.rows_per_tile = (int)std::min<int64_t>(a.max_rows, 32 * kTreeWaves / group);
   // two work-groups a CU, or as many as there can be steps
   const int64_t tiles = a.n_rows / a.rows_per_tile + a.n;
-  const int64_t steps = tiles * a.n_kv_heads * std::max<int64_t>((a.max_len + kTreeTokens - 1) / kTreeTokens, 1);
-  a.groups = (int)((std::min<int64_t>(2 * a.cu_count, steps) + 7) / 8 * 8);
-  return 2 * (int64_t)a.groups * a.rows_per_tile * group * (a.head_dim + 2) * 4 + (int64_t)a.groups * 4 * 8;
+  const int64_t steps = tiles * std::max<int64_t>((a.max_len + kTreeTokens - 1) / kTreeTokens, 1);
+  const int64_t resident = std::max<int64_t>(2 * a.cu_count / a.n_kv_heads / 8 * 8, 8);
+  a.shares = (int)std::min<int64_t>(resident, (steps + 7) / 8 * 8);
+  const int64_t groups = (int64_t)a.shares * a.n_kv_heads;
+  return 2 * groups * a.rows_per_tile * group * (a.head_dim + 2) * 4 + groups * 4 * 8;
 }
 
 void tree_partials(TreeArgs &a, uint8_t *base) {
   a.ends = reinterpret_cast<int64_t *>(base);
-  a.part_o = reinterpret_cast<float *>(base + (int64_t)a.groups * 4 * 8);
-  a.part_ml = a.part_o + 2 * (int64_t)a.groups * a.rows_per_tile * (a.n_heads / a.n_kv_heads) * a.head_dim;
+  const int64_t groups = (int64_t)a.shares * a.n_kv_heads;
+  a.part_o = reinterpret_cast<float *>(base + groups * 4 * 8);
+  a.part_ml = a.part_o + 2 * groups * a.rows_per_tile * (a.n_heads / a.n_kv_heads) * a.head_dim;
 }
 
 hipError_t launch_tree_attention(const PoolGeom &g, const TreeArgs &a, hipStream_t s) {
   if (a.n <= 0 || a.n_rows <= 0) return hipSuccess;
-  if (a.groups == 0) {
+  if (a.shares == 0) {
     const int64_t grid = a.n_rows * a.n_heads;
     if (grid * kAnyThreads >= (int64_t{1} << 32)) return hipErrorInvalidValue;
     return by_element(g.elem, [&](auto tag) {
@@ -921,7 +992,7 @@ hipError_t launch_tree_attention(const PoolGeom &g, const TreeArgs &a, hipStream
     return e;
   const int columns = a.rows_per_tile * (a.n_heads / a.n_kv_heads);
   const int slices = (columns * a.head_dim + 4 * kTreeThreads - 1) / (4 * kTreeThreads);
-  tree_merge_kernel<<<(unsigned)(a.groups * slices), kTreeThreads, 0, s>>>(a, slices);
+  tree_merge_kernel<<<(unsigned)(a.shares * a.n_kv_heads * slices), kTreeThreads, 0, s>>>(a, slices);
   return hipGetLastError();
 }
 
