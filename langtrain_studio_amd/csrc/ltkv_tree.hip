@@ -163,6 +163,8 @@ __global__ void __launch_bounds__(kAnyThreads) tree_any_kernel(TreeArgs a, int64
 // average per share, which tree_merge_kernel folds.
 constexpr int kTreeWaves = 4, kTreeThreads = 64 * kTreeWaves;
 constexpr int kTreeTokens = 64;  // positions of a step
+// Instruction classes of sched_group_barrier: LDS reads, matrix products.
+constexpr int kSchedReads = 0x100, kSchedProducts = 0x8;
 
 struct TreeSeq {
   SeqRows rows;
@@ -357,8 +359,10 @@ struct Cells<int8_t, HD, EXACT, NT> {
   // bits and d 11, so what the rounding of the product leaves is an f16 number, which
   // the fused multiply-add gives exactly (d times a power of two is one too, down to
   // 2^-22 of the largest scale).
+  // Returns the largest power of the lane's positions.
   template <int PLANES>
-  __device__ __forceinline__ void put(char *lds, int plane, int pitch, int lane, uint32_t bad, float *pow) const {
+  __device__ __forceinline__ float put(char *lds, int plane, int pitch, int lane, uint32_t bad, float *pow) const {
+    float most = 0.f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const float d0 = scale(j), top = lanes_max<ROW>(__builtin_fminf(d0, 65504.f));
@@ -366,6 +370,7 @@ struct Cells<int8_t, HD, EXACT, NT> {
       const _Float16 d = bad >> j & 1 ? (_Float16)0.f : (_Float16)__builtin_amdgcn_ldexpf(d0, -e);
       const h8 d8 = {d, d, d, d, d, d, d, d};
       if (lane % ROW == 0) pow[row(lane, j)] = __builtin_amdgcn_ldexpf(1.f, e);
+      most = __builtin_fmaxf(most, __builtin_amdgcn_ldexpf(1.f, e));
 #pragma unroll
       for (int i = 0; i < E / 8; ++i) {
         const h8 q = i8x8_to_h8(u32x2{x[j][2 * i], x[j][2 * i + 1]}), hi = q * d8;
@@ -374,6 +379,7 @@ struct Cells<int8_t, HD, EXACT, NT> {
         if constexpr (PLANES == 2) *reinterpret_cast<h8 *>(to + plane) = __builtin_elementwise_fma(q, d8, -hi);
       }
     }
+    return most;
   }
 };
 
@@ -407,7 +413,7 @@ struct Cells<float, HD, EXACT, NT> {
   }
   // (powers of at least 2^-100: smaller values are nothing beside their products' rounding)
   template <int PLANES>
-  __device__ __forceinline__ void put(char *lds, int plane, int pitch, int lane, uint32_t bad, float *pow) const {
+  __device__ __forceinline__ float put(char *lds, int plane, int pitch, int lane, uint32_t bad, float *pow) const {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const float top = lanes_max<ROW>(__builtin_bit_cast(float, min(top_bits(j), 0x7f7fffffu)));
@@ -426,6 +432,7 @@ struct Cells<float, HD, EXACT, NT> {
       *reinterpret_cast<h4 *>(to) = hi;
       if constexpr (PLANES == 2) *reinterpret_cast<h4 *>(to + plane) = lo;
     }
+    return 0.f;
   }
 };
 
@@ -438,13 +445,15 @@ struct Cells<float, HD, EXACT, NT> {
 // weights as hi + lo pairs; else Q as it is (times a power of two), the weights and V
 // rounded to f16.
 // Of pairs (kPairs) the scores are multiplied by their position's power of two, and
-// so are the weights, whose column then has a reference of its own (`top_o`): the
-// largest weight times V, not the largest weight, lies near the top of f16.
+// so are the weights. f32 pools: a column's numerators have a reference of their own
+// (`top_o`): the largest weight times V, not the largest weight, lies near the top of
+// f16. 8-bit pools, whose powers lie between 2^-32 and 2^8: weights carry the inverse
+// of the largest power that the column has seen (`v_exp`), one instruction a score.
 template <typename T, int HD, bool EXACT, bool FULL, int WC>
 __global__ void __launch_bounds__(kTreeThreads, HD > 128 ? 1 : 2)
 tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   constexpr int NC = HD / 32, NK = HD / 16, WP = kTreeWaves / WC, U = 2 / WP;
-  constexpr bool PAIRS = kPairs<T>;
+  constexpr bool PAIRS = kPairs<T>, BYTES = std::is_same_v<T, int8_t>, WIDE = PAIRS && !BYTES;
   constexpr int K_PLANES = PAIRS ? 2 : 1, V_PLANES = PAIRS && FULL ? 2 : 1;
   constexpr int K_PITCH = HD * 2 + 16;  // rows 4 banks apart: 16-byte reads of 16 rows without conflicts
   constexpr int V_PITCH = HD * 2 + 64;  // rows 16 banks apart, for the transposing reads
@@ -464,7 +473,9 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   __shared__ int64_t s_begin[kTreeThreads + 1];
   __shared__ int64_t s_sum[kTreeWaves];
   __shared__ int64_t s_found[2];
+  __shared__ TreeSeq s_seq;
   __shared__ int32_t s_from[kTreeWaves];
+  __shared__ float s_top[kTreeWaves];  // 8-bit pools: the largest power of a wave's positions' V
   char *const lds_k = lds, *const lds_v = lds + K_PLANES * K_BYTES;
 
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -507,10 +518,12 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
     if (s_begin[tid] <= at && at < s_begin[tid + 1]) {
       int64_t begin = s_begin[tid];
       for (int64_t i = i0; i < i1; ++i) {
-        const int64_t next = begin + tree_steps(a, i);
+        const TreeSeq x = tree_seq(a, i);
+        const int64_t next = begin + (int64_t)x.steps * x.tiles;
         if (at < next) {
           s_found[0] = i;
           s_found[1] = begin;
+          s_seq = x;
           break;
         }
         begin = next;
@@ -518,7 +531,14 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
     }
     __syncthreads();
     const int64_t seq = uniform64(s_found[0]), off = at - uniform64(s_found[1]);
-    const TreeSeq ts = tree_seq(a, seq);
+    TreeSeq ts;
+    ts.rows.row0 = uniform64(s_seq.rows.row0);
+    ts.rows.count = __builtin_amdgcn_readfirstlane(s_seq.rows.count);
+    ts.rows.len = __builtin_amdgcn_readfirstlane(s_seq.rows.len);
+    ts.ctx = __builtin_amdgcn_readfirstlane(s_seq.ctx);
+    ts.first = __builtin_amdgcn_readfirstlane(s_seq.first);
+    ts.steps = __builtin_amdgcn_readfirstlane(s_seq.steps);
+    ts.tiles = __builtin_amdgcn_readfirstlane(s_seq.tiles);
     const SeqRows rows = ts.rows;
     const int tile = (int)(off / ts.steps);
     const int s_first = (int)(off - (int64_t)tile * ts.steps);
@@ -531,6 +551,29 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
       e[2] = (at - s_first) / per;
     }
     at += s_last - s_first;
+
+    // the first steps, on their way while Q is laid out
+    const int32_t *tab = table_of(a.tables, a.table_stride, nullptr, 0, seq);
+    auto block_of = [&](int s) {  // the wave's block of a step (past the end: block 0, read and masked)
+      const int32_t t = ts.first + kTreeTokens * s + 16 * wave;
+      const int32_t e = s < s_last && t < rows.len ? scalar_read(tab, t >> 4) : 0;
+      return (uint32_t)e < (uint32_t)n_blocks ? e : 0;
+    };
+    const uint32_t head_off = (uint32_t)(kvh * a.head_dim);
+    // (rows of one tile are read by one work-group alone)
+    typedef Cells<T, HD, EXACT, WC == 2> Rows;
+    struct Step {
+      Rows k, v;
+    };
+    Step steps[AHEAD];
+    auto load = [&](Step &x, int32_t block) {
+      const int64_t b = (int64_t)(uint32_t)block * Rows::block_bytes(kv_dim);
+      x.k.load(a.k_layer, a.k_scale, b, kv_dim, head_off, lane, a.head_dim);
+      x.v.load(a.v_layer, a.v_scale, b, kv_dim, head_off, lane, a.head_dim);
+    };
+    int32_t next = block_of(s_first + AHEAD);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) load(steps[k], block_of(s_first + k));
 
     // the lane's column
     const int c = cw * 32 + col, rr = c / group;
@@ -550,7 +593,6 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
       from_max = __builtin_amdgcn_readfirstlane(max(max(s_from[0], s_from[1]), max(s_from[2], s_from[3])));
     }
 
-    const int32_t *tab = table_of(a.tables, a.table_stride, nullptr, 0, seq);
     // Table entries outside the pool are reported where a row sees a position of
     // their block; the steps read block 0 in their place.
     for (int32_t t = ts.first + kTreeTokens * s_first + 16 * tid; t < min(rows.len, ts.first + kTreeTokens * s_last);
@@ -611,28 +653,8 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
     for (int i = 0; i < NC; ++i) o[i] = f32x16{};
     float ref = -INFINITY, sum = 0.f;      // weights are 2^(score - ref + kLift)
     float top_o = -INFINITY, to_o = 0.f;   // pairs: numerators are taken times 2^(ref - top_o) = to_o
+    float v_exp = -1000.f;                 // 8-bit pools: weights and sums are taken times 2^-v_exp
     bool poisoned = false;                 // the column sees an infinity or NaN in V
-
-    auto block_of = [&](int s) {  // the wave's block of a step (past the end: block 0, read and masked)
-      const int32_t t = ts.first + kTreeTokens * s + 16 * wave;
-      const int32_t e = s < s_last && t < rows.len ? scalar_read(tab, t >> 4) : 0;
-      return (uint32_t)e < (uint32_t)n_blocks ? e : 0;
-    };
-    const uint32_t head_off = (uint32_t)(kvh * a.head_dim);
-    // (rows of one tile are read by one work-group alone)
-    typedef Cells<T, HD, EXACT, WC == 2> Rows;
-    struct Step {
-      Rows k, v;
-    };
-    Step steps[AHEAD];
-    auto load = [&](Step &x, int32_t block) {
-      const int64_t b = (int64_t)(uint32_t)block * Rows::block_bytes(kv_dim);
-      x.k.load(a.k_layer, a.k_scale, b, kv_dim, head_off, lane, a.head_dim);
-      x.v.load(a.v_layer, a.v_scale, b, kv_dim, head_off, lane, a.head_dim);
-    };
-    int32_t next = block_of(s_first + AHEAD);
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k) load(steps[k], block_of(s_first + k));
 
     auto step = [&](Step &cells, int s) __attribute__((always_inline)) {
       const int32_t t0 = ts.first + kTreeTokens * s;
@@ -652,7 +674,12 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
       }
       if constexpr (PAIRS) {
         cells.k.template put<2>(lds_k + 16 * wave * K_PITCH, K_BYTES, K_PITCH, lane, 0, s_kpow + 16 * wave);
-        cells.v.template put<V_PLANES>(lds_v + 16 * wave * V_PITCH, V_BYTES, V_PITCH, lane, bad, s_vpow + 16 * wave);
+        const float v_top =
+            cells.v.template put<V_PLANES>(lds_v + 16 * wave * V_PITCH, V_BYTES, V_PITCH, lane, bad, s_vpow + 16 * wave);
+        if constexpr (BYTES) {
+          const float x = lanes_max<64>(v_top);
+          if (lane == 0) s_top[wave] = x;
+        }
       } else {
         cells.k.put(lds_k + 16 * wave * K_PITCH, K_PITCH, lane, 0);
         cells.v.put(lds_v + 16 * wave * V_PITCH, V_PITCH, lane, bad);
@@ -690,6 +717,17 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
           }
         }
       }
+      {  // operands two products ahead
+        constexpr int READS = U * (PAIRS ? 2 : 1) + (Q_LDS ? (FULL ? 2 : 1) : 0);
+        constexpr int PRODUCTS = U * (1 + (FULL ? 1 : 0) + (PAIRS ? 1 : 0));
+        __builtin_amdgcn_sched_group_barrier(kSchedReads, 2 * READS, 0);
+#pragma unroll
+        for (int j = 0; j < NK - 2; ++j) {
+          __builtin_amdgcn_sched_group_barrier(kSchedProducts, PRODUCTS, 0);
+          __builtin_amdgcn_sched_group_barrier(kSchedReads, READS, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kSchedProducts, 2 * PRODUCTS, 0);
+      }
       float m = in_scale;  // scores are m sc
       if constexpr (PAIRS) {
 #pragma unroll
@@ -698,9 +736,9 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
           for (int i = 0; i < 16; i += 4) {
             const f32x4 f = *reinterpret_cast<const f32x4 *>(s_kpow + 32 * (pw * U + u) + 2 * i + 4 * half);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) sc[u][i + k] *= __builtin_fminf(f[k] * in_scale, 1e37f);
+            for (int k = 0; k < 4; ++k) sc[u][i + k] *= BYTES ? f[k] : __builtin_fminf(f[k] * in_scale, 1e37f);
           }
-        m = 1.f;
+        if constexpr (WIDE) m = 1.f;
       }
       if (cap) {
         float to_x = m;  // opaque: the products would be taken before the branch, for both sides
@@ -714,6 +752,7 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
           }
         m = 1.f;
       }
+      float most_v = 0.f;  // 8-bit pools: the largest power of the positions that the column sees
       if (partial) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -721,8 +760,29 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             sc[u][i] = mine >> (8 * (i / 4) + i % 4) & 1 ? sc[u][i] : -INFINITY;
+          if constexpr (BYTES) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              const f32x4 f = *reinterpret_cast<const f32x4 *>(s_vpow + 32 * (pw * U + u) + 2 * i + 4 * half);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                most_v = __builtin_fmaxf(most_v, mine >> (2 * i + k) & 1 ? f[k] : 0.f);
+            }
+          }
           // the infinities and NaN of V entered as zeros
           poisoned |= (seen & (s_bad[2 * (pw * U + u)] | s_bad[2 * (pw * U + u) + 1] << 16)) != 0;
+        }
+      }
+      if constexpr (BYTES) {
+        most_v = partial ? halves_reduce<true>(most_v)
+                         : __builtin_fmaxf(__builtin_fmaxf(s_top[0], s_top[1]), __builtin_fmaxf(s_top[2], s_top[3]));
+        const float e = most_v > 0.f ? (float)(__builtin_amdgcn_frexp_expf(most_v) - 1) : -1000.f;
+        if (__builtin_amdgcn_ballot_w64(e > v_exp)) {
+          const float ne = __builtin_fmaxf(e, v_exp), f = __builtin_amdgcn_exp2f(v_exp - ne);
+          sum *= f;
+#pragma unroll
+          for (int i = 0; i < NC; ++i) o[i] *= f;
+          v_exp = ne;
         }
       }
       float top = sc[0][0];
@@ -735,7 +795,7 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
         const float nr = __builtin_fmaxf(ref, halves_reduce<true>(top));
         const float f = nr == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - nr);
         sum *= f;
-        if constexpr (PAIRS) {
+        if constexpr (WIDE) {
           if (top_o > -INFINITY) to_o = __builtin_fminf(__builtin_amdgcn_exp2f(nr - top_o), 3e38f);
         } else {
 #pragma unroll
@@ -743,7 +803,7 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
         }
         ref = nr;
       }
-      const float base = kLift - (ref == -INFINITY ? 0.f : ref);
+      const float base = kLift - (ref == -INFINITY ? 0.f : ref) - (BYTES ? v_exp : 0.f);
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -751,7 +811,17 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
           sc[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], m, base));
           if constexpr (FULL || PAIRS) sum += sc[u][i];
         }
-      if constexpr (PAIRS) {
+      if constexpr (BYTES) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const f32x4 f = *reinterpret_cast<const f32x4 *>(s_vpow + 32 * (pw * U + u) + 2 * i + 4 * half);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sc[u][i + k] *= f[k];
+          }
+      }
+      if constexpr (WIDE) {
         float most = 0.f;
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -828,6 +898,7 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
 
     // the column's average
     sum = halves_reduce<false>(sum);
+    if constexpr (BYTES) ref += v_exp;  // (a column that has seen nothing: -inf)
     if (poisoned) sum = __builtin_nanf("");
     if constexpr (WP > 1) {
       __syncthreads();  // the last step has been read
@@ -849,7 +920,7 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
         float f = __builtin_amdgcn_exp2f(ref - r), g = __builtin_amdgcn_exp2f(ref2 - r);
         sum = sum * f + sum2 * g;
         ref = nr;
-        if constexpr (PAIRS) {
+        if constexpr (WIDE) {
           const float nt = __builtin_fmaxf(top_o, top2), t = nt == -INFINITY ? 0.f : nt;
           f = __builtin_amdgcn_exp2f(top_o - t);
           g = __builtin_amdgcn_exp2f(top2 - t);
@@ -860,7 +931,7 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
       }
     }
     const float inv = sum != 0.f ? 1.f / sum : 0.f;  // (a NaN sum stays one)
-    const float back = PAIRS && top_o > -INFINITY ? __builtin_amdgcn_exp2f(top_o - ref) : 1.f;
+    const float back = WIDE && top_o > -INFINITY ? __builtin_amdgcn_exp2f(top_o - ref) : 1.f;
     const bool whole = s_first == 0 && s_last == ts.steps;
     // (a share's last tile may go on in the next one, its first come from the last)
     const int64_t slot = 2 * me + (s_first == 0 ? 1 : 0);
