@@ -481,9 +481,9 @@ struct TreeArgs : ScoredArgs {
   int rows_per_tile, shares;
   // Averages of the tiles that lie in several shares: part_o [slot][column]
   // [head_dim], part_ml [slot][column][2] (reference, sum), two slots a work-group;
-  // ends [work-group][4] names the tile that ends in a work-group's share and began
-  // in an earlier one: (first row or -1, rows, share that it began in).
-  int64_t *ends;
+  // ends [work-group][2][4] names the tile that began in an earlier share and the one
+  // that goes on in a later: (first row or -1, rows, its first share, its last).
+  int32_t *ends;
 };
 int64_t tree_workspace(int elem, TreeArgs &a);  // bytes of its partials
 void tree_partials(TreeArgs &a, uint8_t *base);

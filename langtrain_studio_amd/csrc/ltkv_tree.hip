@@ -31,9 +31,10 @@ struct TreeView {
       const int32_t j = t - ctx;  // first drafted row of the word (below 0: later bits)
       uint32_t drafted;
       if (mask) {
-        const int32_t w = j >> 5;  // (floor)
-        const uint32_t a = w >= 0 && w < words ? (uint32_t)mask[w] : 0u;
-        const uint32_t b = w + 1 < words ? (uint32_t)mask[w + 1] : 0u;
+        // (both words loaded in any case: conditions would wait for one after the other)
+        const int32_t w = j >> 5, last = (int32_t)words - 1;  // (floor)
+        const uint32_t x = (uint32_t)mask[min(max(w, 0), last)], y = (uint32_t)mask[min(max(w + 1, 0), last)];
+        const uint32_t a = w >= 0 && w <= last ? x : 0u, b = w + 1 <= last ? y : 0u;
         drafted = (uint32_t)((((uint64_t)b << 32) | a) >> (j & 31));
       } else {
         drafted = low_bits(min(max(row + 1 - j, 0), 32));
@@ -436,6 +437,32 @@ struct Cells<float, HD, EXACT, NT> {
   }
 };
 
+// A lane's part of a row of Q as it lies in memory: elements 16 j ... + 7 of row type R
+// (float, _Float16, or uint16_t for bf16), zeros from element `n` on and where `live`
+// is false. All loads come before the first value is needed.
+template <typename R, int NK, bool EXACT>
+struct Column {
+  static constexpr int V = std::is_same_v<R, float> ? 2 : 1;
+  u32x4 u[NK][V];
+  __device__ __forceinline__ Column(const void *q, int64_t i, bool live, int n) {
+    const R *const row = static_cast<const R *>(q) + i;
+#pragma unroll
+    for (int j = 0; j < NK; ++j)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        u[j][v] = u32x4{0, 0, 0, 0};
+        if (live && (EXACT || 16 * j < n)) u[j][v] = *reinterpret_cast<const u32x4 *>(row + 16 * j + 4 * v);
+      }
+  }
+  __device__ __forceinline__ float get(int j, int k) const {
+    const uint32_t w = V == 2 ? u[j][k >> 2][k & 3] : u[j][0][k >> 1];
+    if constexpr (std::is_same_v<R, float>) return __builtin_bit_cast(float, w);
+    if constexpr (std::is_same_v<R, uint16_t>) return __builtin_bit_cast(float, k & 1 ? w & 0xffff0000u : w << 16);
+    const h2 h = __builtin_bit_cast(h2, w);
+    return k & 1 ? (float)h.y : (float)h.x;
+  }
+};
+
 // WC waves share a step's columns, 32 each; 4 / WC waves its positions. Steps go
 // through LDS as f16 numbers, on 32x32x16 products: scores^T = K Q^T, weights in
 // place, numerators^T += V^T W (a lane's scores are positions 8 (r / 4) + 4 (lane /
@@ -449,8 +476,12 @@ struct Cells<float, HD, EXACT, NT> {
 // (`top_o`): the largest weight times V, not the largest weight, lies near the top of
 // f16. 8-bit pools, whose powers lie between 2^-32 and 2^8: weights carry the inverse
 // of the largest power that the column has seen (`v_exp`), one instruction a score.
+// f32 pools, and heads of more than 128 elements, take one work-group a CU: two left
+// their waves too few registers (f32, one step of 8 rows: 18 us with spills).
+constexpr int tree_groups_a_cu(bool wide, int hd) { return wide || hd > 128 ? 1 : 2; }
+
 template <typename T, int HD, bool EXACT, bool FULL, int WC>
-__global__ void __launch_bounds__(kTreeThreads, HD > 128 ? 1 : 2)
+__global__ void __launch_bounds__(kTreeThreads, tree_groups_a_cu(std::is_same_v<T, float>, HD))
 tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   constexpr int NC = HD / 32, NK = HD / 16, WP = kTreeWaves / WC, U = 2 / WP;
   constexpr bool PAIRS = kPairs<T>, BYTES = std::is_same_v<T, int8_t>, WIDE = PAIRS && !BYTES;
@@ -462,8 +493,8 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   constexpr int FOLD = NC * 16 + 4;  // floats that a lane hands over where waves share columns
   // Few columns (WC 2) are bound by the pool's bytes: two steps ahead of the products,
   // in registers that Q leaves free in LDS.
-  constexpr int AHEAD = WC == 2 && !PAIRS ? 2 : 1;
-  constexpr bool Q_LDS = AHEAD == 2 && HD > 64;
+  constexpr int AHEAD = WC == 2 && !BYTES ? 2 : 1;
+  constexpr bool Q_LDS = WC == 2 && !PAIRS && HD > 64;
   constexpr int Q_BYTES = Q_LDS ? 32 * WC * K_PITCH : 16;
   static_assert(WP == 1 || (kTreeWaves - WC) * 64 * FOLD * 4 <= STEP_BYTES, "the fold fits the step's memory");
   __shared__ __align__(16) char lds[STEP_BYTES];
@@ -511,7 +542,7 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   const int64_t me = share * a.n_kv_heads + kvh;
   int64_t at = share * per;
   const int64_t end = min(total, at + per);
-  if (tid == 0) a.ends[4 * me] = -1;
+  if (tid == 0) a.ends[8 * me] = a.ends[8 * me + 4] = -1;  // (none, until one is met)
 
   while (at < end) {
     __syncthreads();  // s_found, and the step's memory, have been read
@@ -544,11 +575,11 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
     const int s_first = (int)(off - (int64_t)tile * ts.steps);
     const int s_last = (int)min((int64_t)ts.steps, s_first + (end - at));
     const int32_t r0 = tile * a.rows_per_tile;
-    if (tid == 0 && s_first > 0 && s_last == ts.steps) {
-      int64_t *const e = a.ends + 4 * me;
-      e[0] = rows.row0 + r0;
-      e[1] = min(a.rows_per_tile, rows.count - r0);
-      e[2] = (at - s_first) / per;
+    if (tid == 0 && s_last - s_first < ts.steps) {
+      const int64_t begin = at - s_first;
+      reinterpret_cast<i32x4 *>(a.ends)[2 * me + (s_first > 0 ? 0 : 1)] =
+          i32x4{(int)rows.row0 + r0, min(a.rows_per_tile, rows.count - r0), (int)(begin / per),
+                (int)((begin + ts.steps - 1) / per)};
     }
     at += s_last - s_first;
 
@@ -575,6 +606,12 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) load(steps[k], block_of(s_first + k));
 
+    // Table entries outside the pool are reported where a row sees a position of
+    // their block; the steps read block 0 in their place.
+    const int32_t blocks_end = (min(rows.len, ts.first + kTreeTokens * s_last) + 15) >> 4;
+    int32_t block = ((ts.first + kTreeTokens * s_first) >> 4) + tid;
+    int32_t entry = block < blocks_end ? tab[block] : 0;
+
     // the lane's column
     const int c = cw * 32 + col, rr = c / group;
     const bool live = rr < a.rows_per_tile && r0 + rr < rows.count;
@@ -593,33 +630,18 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
       from_max = __builtin_amdgcn_readfirstlane(max(max(s_from[0], s_from[1]), max(s_from[2], s_from[3])));
     }
 
-    // Table entries outside the pool are reported where a row sees a position of
-    // their block; the steps read block 0 in their place.
-    for (int32_t t = ts.first + kTreeTokens * s_first + 16 * tid; t < min(rows.len, ts.first + kTreeTokens * s_last);
-         t += 16 * kTreeThreads) {
-      if ((uint32_t)tab[t >> 4] < (uint32_t)n_blocks) continue;
-      bool needed = false;
-      for (int32_t r = 0; r < a.rows_per_tile && r0 + r < rows.count; ++r) {
-        TreeView v = tree_view(a, rows, r0 + r);
-        v.ctx = ts.ctx;
-        needed |= (v.sees32(t) & 0xffffu) != 0;
-      }
-      if (needed) report_fault(a.status, kFaultTable, seq);
-    }
-
     // Q columns, times a power of two and the scale's sign
     h8 qh[Q_LDS ? 1 : NK], ql[FULL && !Q_LDS ? NK : 1];
     char *const qp = lds_q + (Q_LDS ? (32 * cw + col) * K_PITCH + 16 * half : 0);
-    int q_exp;
-    {
-      float x[NK][8], amax = 0.f;
-      const int64_t q0 = (row * a.n_heads + head) * (int64_t)a.head_dim;
+    int q_exp = 0;
+    auto lay_out = [&](auto tag) {
+      const Column<decltype(tag), NK, EXACT> x(a.q, (row * a.n_heads + head) * (int64_t)a.head_dim + 8 * half, live,
+                                               a.head_dim - 8 * half);
+      float amax = 0.f;
 #pragma unroll
-      for (int j = 0; j < NK; ++j) {
-        load_row8(a, q0 + 16 * j + 8 * half, live && (EXACT || 16 * j + 8 * half < a.head_dim), x[j]);
+      for (int j = 0; j < NK; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) amax = __builtin_fmaxf(amax, __builtin_fabsf(x[j][i]));
-      }
+        for (int i = 0; i < 8; ++i) amax = __builtin_fmaxf(amax, __builtin_fabsf(x.get(j, i)));
       amax = halves_reduce<true>(amax);
       // (at most 100: a smaller row's scores are nothing beside their rounding)
       q_exp = amax > 0.f && amax < INFINITY ? min(10 - __builtin_amdgcn_frexp_expf(amax), 100) : 0;
@@ -628,7 +650,7 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
         h8 hi8, lo8;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float y = __builtin_amdgcn_ldexpf(x[j][i], q_exp);
+          const float y = __builtin_amdgcn_ldexpf(x.get(j, i), q_exp);
           _Float16 hi, lo;
           split2(a.scale < 0.f ? -y : y, hi, lo);
           hi8[i] = hi;
@@ -642,6 +664,19 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
           if constexpr (FULL) ql[j] = lo8;
         }
       }
+    };
+    if (FULL && a.row_type == LTKV_ROWS_F32) lay_out(float{});
+    else if (a.row_type == LTKV_ROWS_F16) lay_out(_Float16{});
+    else lay_out(uint16_t{});
+    for (; block < blocks_end; block += kTreeThreads, entry = block < blocks_end ? tab[block] : 0) {
+      if ((uint32_t)entry < (uint32_t)n_blocks) continue;
+      bool needed = false;
+      for (int32_t r = 0; r < a.rows_per_tile && r0 + r < rows.count; ++r) {
+        TreeView v = tree_view(a, rows, r0 + r);
+        v.ctx = ts.ctx;
+        needed |= (v.sees32(16 * block) & 0xffffu) != 0;
+      }
+      if (needed) report_fault(a.status, kFaultTable, seq);
     }
     const bool cap = a.softcap > 0.f;
     const float scale = __builtin_fabsf(a.scale);
@@ -956,45 +991,82 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   }
 }
 
-// A work-group a slice of a tile that lies in several shares: their averages,
-// weighted by their sums against the largest reference, in order, four parts' loads
-// at a time.
-__global__ void __launch_bounds__(kTreeThreads) tree_merge_kernel(TreeArgs a, int slices) {
-  const int64_t me = blockIdx.x / (uint32_t)slices, share = me / a.n_kv_heads;
-  const int64_t *const e = a.ends + 4 * me;
-  const int64_t row0 = e[0];
-  if (row0 < 0) return;
-  const int rows = (int)e[1], kvh = (int)(me - share * a.n_kv_heads), group = a.n_heads / a.n_kv_heads;
-  const int64_t first = e[2], columns = (int64_t)a.rows_per_tile * group;
-  const int x0 = ((int)(blockIdx.x % (uint32_t)slices) * kTreeThreads + (int)threadIdx.x) * 4;
-  const int c = x0 / a.head_dim, d = x0 - c * a.head_dim;
-  if (c >= rows * group) return;
-  constexpr int AHEAD = 4;
+// A running average of the parts of a tile, weighted by their sums against the
+// largest reference. (x stays an average, no larger than its V.)
+struct TreeFold {
   float mx = -INFINITY, l = 0.f;
   f32x4 x = {};
-  for (int64_t w = first; w <= share; w += AHEAD) {
-    f32x2 ml[AHEAD];
-    f32x4 o[AHEAD];
+  __device__ __forceinline__ void add(float m, float sum, const f32x4 &o) {
+    const float next = __builtin_fmaxf(mx, m), ref = next == -INFINITY ? 0.f : next;
+    const float kept = l * __builtin_amdgcn_exp2f(mx - ref), p = sum * __builtin_amdgcn_exp2f(m - ref);
+    l = kept + p;
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    x = x * (kept * inv) + o * (p * inv);
+    mx = next;
+  }
+};
+
+// The parts of a tile are folded by the work-groups that have them, each an equal
+// piece of its elements (kMergeGroups work-groups a share and kv head; a share has at
+// most two such tiles, its first and its last). A thread takes four elements of some
+// parts, in order; where the parts are many and the elements few, threads share the
+// parts and their averages are folded in LDS. One tree of 8 rows over 4000 positions
+// lies in 63 shares: TIME_ONE; 64 trees of up to 16 rows in two or three: TIME_MANY.
+constexpr int kMergeGroups = 4;
+
+__global__ void __launch_bounds__(kTreeThreads) tree_merge_kernel(TreeArgs a) {
+  __shared__ float s_fold[6][kTreeThreads];
+  const int tid = (int)threadIdx.x;
+  const int tile = (int)(blockIdx.x / kMergeGroups), me = tile >> 1, share = me / a.n_kv_heads;
+  const i32x4 r = reinterpret_cast<const i32x4 *>(a.ends)[tile];
+  const int kvh = me - share * a.n_kv_heads, group = a.n_heads / a.n_kv_heads, columns = a.rows_per_tile * group;
+  const int row0 = r.x, first = r.z, parts = r.w - first + 1;
+  if (row0 < 0) return;
+  const int all = r.y * group * a.head_dim / 4, pieces = parts * kMergeGroups;
+  const int piece = (share - first) * kMergeGroups + (int)(blockIdx.x % kMergeGroups);
+  const int v0 = all * piece / pieces, n = all * (piece + 1) / pieces - v0;
+  if (n == 0) return;
+  // `lanes` elements by `sets` of parts
+  int shift = 0;
+  while (1 << shift < n && 1 << shift < kTreeThreads) ++shift;
+  const int lanes = 1 << shift, sets = kTreeThreads >> shift, set = tid >> shift, lane = tid & (lanes - 1);
+  const int each = (parts + sets - 1) >> (8 - shift), w0 = first + set * each, w1 = min(w0 + each, first + parts);
+  static_assert(kTreeThreads == 256, "sets are 2^(8 - shift)");
+  for (int v = lane; v < ((n + lanes - 1) & ~(lanes - 1)); v += lanes) {
+    const int x0 = 4 * (v0 + min(v, n - 1)), c = x0 / a.head_dim, d = x0 - c * a.head_dim;
+    constexpr int AHEAD = 4;
+    TreeFold fold;
+    for (int w = w0; w < w1; w += AHEAD) {
+      f32x2 ml[AHEAD];
+      f32x4 o[AHEAD];
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const int64_t v = min(w + k, share);
-      const int64_t column = (2 * (v * a.n_kv_heads + kvh) + (v == first ? 1 : 0)) * columns + c;
-      ml[k] = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * column);
-      o[k] = *reinterpret_cast<const f32x4 *>(a.part_o + column * a.head_dim + d);
-      if (w + k > share) ml[k] = f32x2{-INFINITY, 0.f};
+      for (int i = 0; i < AHEAD; ++i) {
+        const int p = min(w + i, w1 - 1);
+        const int64_t column = (2 * (p * a.n_kv_heads + kvh) + (p == first ? 1 : 0)) * columns + c;
+        ml[i] = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * column);
+        o[i] = *reinterpret_cast<const f32x4 *>(a.part_o + column * a.head_dim + d);
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (w + i < w1) fold.add(ml[i].x, ml[i].y, o[i]);
     }
+    for (int half = sets >> 1; half > 0; half >>= 1) {
+      __syncthreads();  // the last round has been read
+      s_fold[0][tid] = fold.mx;
+      s_fold[1][tid] = fold.l;
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const float next = __builtin_fmaxf(mx, ml[k].x), ref = next == -INFINITY ? 0.f : next;
-      const float kept = l * __builtin_amdgcn_exp2f(mx - ref), p = ml[k].y * __builtin_amdgcn_exp2f(ml[k].x - ref);
-      l = kept + p;
-      const float inv = l != 0.f ? 1.f / l : 0.f;  // (x stays an average, no larger than its V)
-      x = x * (kept * inv) + o[k] * (p * inv);
-      mx = next;
+      for (int i = 0; i < 4; ++i) s_fold[2 + i][tid] = fold.x[i];
+      __syncthreads();
+      if (set < half) {
+        const int t = tid + half * lanes;
+        fold.add(s_fold[0][t], s_fold[1][t], f32x4{s_fold[2][t], s_fold[3][t], s_fold[4][t], s_fold[5][t]});
+      }
+    }
+    if (set == 0 && v < n) {
+      const int rr = c / group;
+      store_row4(a, (((int64_t)row0 + rr) * a.n_heads + (int64_t)kvh * group + (c - rr * group)) * a.head_dim + d, fold.x);
     }
   }
-  const int rr = c / group;
-  store_row4(a, ((row0 + rr) * a.n_heads + (int64_t)kvh * group + (c - rr * group)) * a.head_dim + d, x);
 }
 
 bool tree_tiles_supported(const TreeArgs &a) {
@@ -1027,24 +1099,25 @@ hipError_t launch_tiles_of(const PoolGeom &g, const TreeArgs &a, hipStream_t s) 
 
 }  // namespace
 
-int64_t tree_workspace(int, TreeArgs &a) {
+int64_t tree_workspace(int elem, TreeArgs &a) {
   a.rows_per_tile = a.shares = 0;
   if (!tree_tiles_supported(a) || a.max_len == 0) return 0;  // (max_len 0: a cache without blocks)
   const int group = a.n_heads / a.n_kv_heads;
   a.rows_per_tile = (int)std::min<int64_t>(a.max_rows, 32 * kTreeWaves / group);
-  // two work-groups a CU, or as many as there can be steps
+  // as many work-groups as a CU holds at a time, or as there can be steps
   const int64_t tiles = a.n_rows / a.rows_per_tile + a.n;
   const int64_t steps = tiles * std::max<int64_t>((a.max_len + kTreeTokens - 1) / kTreeTokens, 1);
-  const int64_t resident = std::max<int64_t>(2 * a.cu_count / a.n_kv_heads / 8 * 8, 8);
+  const int64_t resident =
+      std::max<int64_t>(tree_groups_a_cu(elem == 4, a.head_dim) * a.cu_count / a.n_kv_heads / 8 * 8, 8);
   a.shares = (int)std::min<int64_t>(resident, (steps + 7) / 8 * 8);
   const int64_t groups = (int64_t)a.shares * a.n_kv_heads;
-  return 2 * groups * a.rows_per_tile * group * (a.head_dim + 2) * 4 + groups * 4 * 8;
+  return 2 * groups * a.rows_per_tile * group * (a.head_dim + 2) * 4 + groups * 8 * 4;
 }
 
 void tree_partials(TreeArgs &a, uint8_t *base) {
-  a.ends = reinterpret_cast<int64_t *>(base);
+  a.ends = reinterpret_cast<int32_t *>(base);
   const int64_t groups = (int64_t)a.shares * a.n_kv_heads;
-  a.part_o = reinterpret_cast<float *>(base + groups * 4 * 8);
+  a.part_o = reinterpret_cast<float *>(base + groups * 8 * 4);
   a.part_ml = a.part_o + 2 * groups * a.rows_per_tile * (a.n_heads / a.n_kv_heads) * a.head_dim;
 }
 
@@ -1061,9 +1134,7 @@ hipError_t launch_tree_attention(const PoolGeom &g, const TreeArgs &a, hipStream
   if (const hipError_t e = by_element(g.elem, [&](auto tag) { return launch_tiles_of<decltype(tag)>(g, a, s); });
       e != hipSuccess)
     return e;
-  const int columns = a.rows_per_tile * (a.n_heads / a.n_kv_heads);
-  const int slices = (columns * a.head_dim + 4 * kTreeThreads - 1) / (4 * kTreeThreads);
-  tree_merge_kernel<<<(unsigned)(a.shares * a.n_kv_heads * slices), kTreeThreads, 0, s>>>(a, slices);
+  tree_merge_kernel<<<(unsigned)(2 * a.shares * a.n_kv_heads * kMergeGroups), kTreeThreads, 0, s>>>(a);
   return hipGetLastError();
 }
 
