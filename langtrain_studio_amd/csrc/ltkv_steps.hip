@@ -36,41 +36,34 @@ rope_table_kernel(const double *__restrict__ inv_freq, float magnitude, int half
 struct F16Row {};
 struct Bf16Row {};
 
-// N (4 or 8) elements of a row as f32.
+// N (4 or 8) elements of a row as they lie in memory, read as f32 values.
 template <typename R, int N>
-__device__ __forceinline__ void load_row(const void *row, int64_t e, float (&x)[N]) {
-  if constexpr (std::is_same_v<R, float>) {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const f32x4 u = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(row) + e + i);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[i + k] = u[k];
-    }
-  } else {
-    uint32_t w[N / 2];
-    const uint16_t *src = static_cast<const uint16_t *>(row) + e;
-    if constexpr (N == 8) {
-      const u32x4 u = *reinterpret_cast<const u32x4 *>(src);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) w[k] = u[k];
-    } else {
+struct Elements {
+  static constexpr int WORDS = std::is_same_v<R, float> ? N : N / 2;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const char *row, int64_t e) {
+    const char *src = row + e * (std::is_same_v<R, float> ? 4 : 2);
+    if constexpr (WORDS == 2) {
       const u32x2 u = *reinterpret_cast<const u32x2 *>(src);
       w[0] = u.x;
       w[1] = u.y;
-    }
+    } else {
 #pragma unroll
-    for (int k = 0; k < N / 2; ++k) {
-      if constexpr (std::is_same_v<R, F16Row>) {
-        const h2 h = __builtin_bit_cast(h2, w[k]);
-        x[2 * k] = (float)h.x;
-        x[2 * k + 1] = (float)h.y;
-      } else {
-        x[2 * k] = __builtin_bit_cast(float, w[k] << 16);
-        x[2 * k + 1] = __builtin_bit_cast(float, w[k] & 0xffff0000u);
+      for (int i = 0; i < WORDS; i += 4) {
+        const u32x4 u = *reinterpret_cast<const u32x4 *>(src + 4 * i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[i + k] = u[k];
       }
     }
   }
-}
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (std::is_same_v<R, float>) return __builtin_bit_cast(float, w[i]);
+    if constexpr (std::is_same_v<R, Bf16Row>)
+      return __builtin_bit_cast(float, i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    const h2 h = __builtin_bit_cast(h2, w[i >> 1]);
+    return i & 1 ? (float)h.y : (float)h.x;
+  }
+};
 
 // 8 f32 values as elements of a row.
 template <typename R>
@@ -106,78 +99,112 @@ constexpr int kInterleaved = 0, kHalves = 1, kHalvesOfFour = 2;
 // (a slice) for several heads, so that their cosines and sines are read once, and
 // a wave whole heads: with d_q_out == d_q every element of a head is read before
 // one is written. Every lane of the four that share a group of a quantised row
-// takes the same path. Pairs' partners are read a second time, through L1.
+// takes the same path. Pairs' partners are read a second time, through L1. The loads
+// of kHeads heads come before the first is needed.
+constexpr int kHeads = 4;
+
 template <int ELEM, typename R, int PAIRS>
 __global__ void __launch_bounds__(256)
 write_rope_rows_kernel(void *__restrict__ kpool, void *__restrict__ vpool, void *__restrict__ kscale,
                        void *__restrict__ vscale, RopeRows a, RopeGeom r, int kv_dim, int64_t n_cells, int team) {
 #pragma clang fp contract(off)
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-  const int64_t row = (int64_t)blockIdx.x * (256 / team) + (int)threadIdx.x / team;
+  constexpr int SIZE = std::is_same_v<R, float> ? 4 : 2;
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int waves = team >> 6, wave_of_team = wave % waves;
+  const int64_t row = (int64_t)blockIdx.x * (4 / waves) + wave / waves;
   if (row >= a.n) return;
-  const int wave_of_team = wave % (team >> 6), waves = team >> 6;
-  const int32_t pos = a.positions[row], s = a.slots[row];
+  const int32_t pos = scalar_read(a.positions, row), s = scalar_read(a.slots, row);
   if (pos < 0 || pos >= r.max_pos) return;
   const bool cell = s >= 0 && (int64_t)s < n_cells;
   const int slices = r.head_dim >> 3, per_wave = 64 / slices;
   const int hl = lane / slices, slice = lane - hl * slices, e = slice * 8;
   const int half = r.rope_dim >> 1;
-  const char *const krow = static_cast<const char *>(a.k) + row * a.src_stride * (std::is_same_v<R, float> ? 4 : 2);
-  const char *const vrow = static_cast<const char *>(a.v) + row * a.src_stride * (std::is_same_v<R, float> ? 4 : 2);
-  const char *const qrow = static_cast<const char *>(a.q) + row * a.q_stride * (std::is_same_v<R, float> ? 4 : 2);
-  char *const orow = static_cast<char *>(a.q_out) + row * a.out_stride * (std::is_same_v<R, float> ? 4 : 2);
+  const char *const krow = static_cast<const char *>(a.k) + row * a.src_stride * SIZE;
+  const char *const vrow = static_cast<const char *>(a.v) + row * a.src_stride * SIZE;
+  const char *const qrow = static_cast<const char *>(a.q) + row * a.q_stride * SIZE;
+  char *const orow = static_cast<char *>(a.q_out) + row * a.out_stride * SIZE;
+  const int v0 = wave_of_team * 64 + lane, v_end = cell ? kv_dim >> 3 : 0;
+  Elements<R, 8> v;
+  if (v0 < v_end) v.load(vrow, 8 * v0);
   if (hl < per_wave) {
-    // (cosine, sine) of element i's pair, sine negative where the element is its first member
     const bool turns = e < r.rope_dim;
+    // (cosine, sine) of element i's pair, sine negative where the element is its first member
     float c[8], sn[8];
     if (turns) {
       const float *cs = r.table + (int64_t)pos * half * 2;
+      if constexpr (PAIRS == kInterleaved) {
+        const f32x4 u = *reinterpret_cast<const f32x4 *>(cs + e), w = *reinterpret_cast<const f32x4 *>(cs + e + 4);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int x = e + i;
-        const int pair = PAIRS == kInterleaved ? x >> 1 : x < half ? x : x - half;
-        const bool first = PAIRS == kInterleaved ? (x & 1) == 0 : x < half;
-        c[i] = cs[2 * pair];
-        sn[i] = first ? -cs[2 * pair + 1] : cs[2 * pair + 1];
+        for (int i = 0; i < 8; ++i) {
+          const f32x4 &x = i < 4 ? u : w;
+          c[i] = x[2 * (i >> 1 & 1)];
+          sn[i] = i & 1 ? x[2 * (i >> 1 & 1) + 1] : -x[2 * (i >> 1 & 1) + 1];
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {  // 4 elements on one side each
+          const int x = e + 4 * q;
+          const bool low = x < half;
+          const float *const at = cs + 2 * (low ? x : x - half);
+          const f32x4 u = *reinterpret_cast<const f32x4 *>(at), w = *reinterpret_cast<const f32x4 *>(at + 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float y = i < 2 ? u[2 * i + 1] : w[2 * i - 3];
+            c[4 * q + i] = i < 2 ? u[2 * i] : w[2 * i - 4];
+            sn[4 * q + i] = low ? -y : y;
+          }
+        }
       }
     }
     const int n_kv = kv_dim / r.head_dim, heads = n_kv + (a.q ? a.n_heads : 0);
-    for (int h = cell ? 0 : n_kv; h < heads; h += waves * per_wave) {
-      const int mine = h + wave_of_team * per_wave + hl;
-      if (mine >= heads) break;
-      const bool is_q = mine >= n_kv;
-      const char *src = is_q ? qrow : krow;
-      const int64_t at = (int64_t)(is_q ? mine - n_kv : mine) * r.head_dim + e;
-      float x[8];
-      load_row<R, 8>(src, at, x);
-      if (turns) {
-        float y[8];  // the elements' partners
-        if constexpr (PAIRS == kInterleaved) {
+    const int step = waves * per_wave;
+    for (int h = (cell ? 0 : n_kv) + wave_of_team * per_wave + hl; h < heads; h += kHeads * step) {
+      Elements<R, 8> x[kHeads], y[kHeads];
+      Elements<R, 4> z[kHeads][2];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-        } else if constexpr (PAIRS == kHalves) {
-          load_row<R, 8>(src, at + (e < half ? half : -half), y);
-        } else {
+      for (int k = 0; k < kHeads; ++k) {
+        const int mine = h + k * step;
+        if (mine >= heads) break;
+        const char *src = mine >= n_kv ? qrow : krow;
+        const int64_t at = (int64_t)(mine >= n_kv ? mine - n_kv : mine) * r.head_dim + e;
+        x[k].load(src, at);
+        if (turns) {  // the elements' partners
+          if constexpr (PAIRS == kHalves) y[k].load(src, at + (e < half ? half : -half));
+          if constexpr (PAIRS == kHalvesOfFour) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            float z[4];
-            load_row<R, 4>(src, at + 4 * q + (e + 4 * q < half ? half : -half), z);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[4 * q + i] = z[i];
+            for (int q = 0; q < 2; ++q) z[k][q].load(src, at + 4 * q + (e + 4 * q < half ? half : -half));
           }
         }
-        // first members a c - b s, second ones a s + b c = b c + a s
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * c[i] + y[i] * sn[i];
       }
-      if (is_q) store_row<R>(orow, at, x);
-      else store_cell<ELEM>(kpool, kscale, s, (int)at, kv_dim, x);
+#pragma unroll
+      for (int k = 0; k < kHeads; ++k) {
+        const int mine = h + k * step;
+        if (mine >= heads) break;
+        const bool is_q = mine >= n_kv;
+        const int64_t at = (int64_t)(is_q ? mine - n_kv : mine) * r.head_dim + e;
+        float o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = x[k].get(i);
+        if (turns) {
+          // first members a c - b s, second ones a s + b c = b c + a s
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float p = PAIRS == kInterleaved ? x[k].get(i ^ 1)
+                            : PAIRS == kHalves    ? y[k].get(i)
+                                                  : z[k][i >> 2].get(i & 3);
+            o[i] = o[i] * c[i] + p * sn[i];
+          }
+        }
+        if (is_q) store_row<R>(orow, at, o);
+        else store_cell<ELEM>(kpool, kscale, s, (int)at, kv_dim, o);
+      }
     }
   }
-  if (!cell) return;
-  for (int u = wave_of_team * 64 + lane; u < kv_dim >> 3; u += team) {
+  for (int u = v0; u < v_end; u += team) {
+    if (u != v0) v.load(vrow, 8 * u);
     float x[8];
-    load_row<R, 8>(vrow, 8 * u, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = v.get(i);
     store_cell<ELEM>(vpool, vscale, s, 8 * u, kv_dim, x);
   }
 }

@@ -1012,7 +1012,7 @@ struct TreeFold {
 // parts, in order; where the parts are many and the elements few, threads share the
 // parts and their averages are folded in LDS. One tree of 8 rows over 4000 positions
 // lies in 63 shares: TIME_ONE; 64 trees of up to 16 rows in two or three: TIME_MANY.
-constexpr int kMergeGroups = 4;
+constexpr int kMergeGroups = 2;
 
 __global__ void __launch_bounds__(kTreeThreads) tree_merge_kernel(TreeArgs a) {
   __shared__ float s_fold[6][kTreeThreads];
