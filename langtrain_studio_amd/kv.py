@@ -72,6 +72,33 @@ def _dev_ptr(t, dtype, name: str, device: int) -> int:
     return t.data_ptr()
 
 
+_types = None
+
+
+def _row_types() -> dict:
+    """LTKV_ROWS_* code of each torch type that rows may have."""
+    global _types
+    if _types is None:
+        import torch
+
+        _types = {torch.float32: _lib.ROWS_F32, torch.float16: _lib.ROWS_F16, torch.bfloat16: _lib.ROWS_BF16}
+    return _types
+
+
+def _int32_parts(sizes, device):
+    """int32 tensors of these sizes in one allocation, and their addresses (each
+    16-byte aligned)."""
+    import torch
+
+    starts, total = [], 0
+    for size in sizes:
+        starts.append(total)
+        total += -(-size // 4) * 4
+    buf = torch.empty((total,), dtype=torch.int32, device=device)
+    base = buf.data_ptr()
+    return [buf[at:at + size] for at, size in zip(starts, sizes)], [base + 4 * at for at in starts]
+
+
 class StepLayout(NamedTuple):
     """The device arrays of a step (KvCache.step_layout), int32."""
 
@@ -81,6 +108,13 @@ class StepLayout(NamedTuple):
     slot_mapping: "object"  # [n_tokens]: each token's cell, -1 behind the last token
     positions: "object"     # [n_tokens]: each token's position, -1 behind the last token
     masks: "object" = None  # [n_tokens][words]: a drafted token's ancestors and itself
+
+
+class _OwnLayout(StepLayout):
+    """A layout as step_layout made it: its sizes and the addresses of its arrays."""
+
+    sizes = None
+    pointers = None
 
 
 class AcceptedTree(NamedTuple):
@@ -340,22 +374,26 @@ class KvCache:
         import torch
 
         n = slot_mapping.numel()
-        types = self._row_types()
-        if k.dtype not in types:
-            raise TypeError(f"k must be float32, float16 or bfloat16, got {k.dtype}")
-        if k.dim() != 2 or k.shape != v.shape or k.shape[0] != n or k.shape[1] != self.kv_dim:
+        dtype, dev = k.dtype, self.device
+        code = _row_types().get(dtype)
+        if code is None:
+            raise TypeError(f"k must be float32, float16 or bfloat16, got {dtype}")
+        shape = k.shape
+        if len(shape) != 2 or shape != v.shape or shape[0] != n or shape[1] != self._kv_dim:
             raise ValueError("k and v must be [n][kv_dim] and match slot_mapping")
         if positions.numel() != n:
             raise ValueError("positions must match slot_mapping")
 
         def rows(t, name):
-            if t.dtype is not k.dtype:
-                raise TypeError(f"{name} must be {k.dtype}, got {t.dtype}")
-            if not t.is_cuda or t.get_device() != self.device:
+            if t.dtype is not dtype:
+                raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+            if not t.is_cuda or t.get_device() != dev:
                 raise ValueError(f"{name} must be on the cache's device")
-            if t.shape[0] > 0 and t.stride(1) != 1 or t.stride(0) < 0:
+            across, along = t.stride()
+            if along != 1 or across < 0:
                 raise ValueError(f"{name} must have rows of unit stride")
-            return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else -(-max(t.shape[1], 1) // 8) * 8
+            # (the stride of a single row may be anything)
+            return t.data_ptr(), across if n > 1 else -(-t.shape[1] // 8) * 8
 
         kp, ks = rows(k, "k")
         vp, vs = rows(v, "v")
@@ -364,29 +402,21 @@ class KvCache:
         qp = op = None
         qs = os = 0
         if q is not None:
-            if q.dim() != 2 or q.shape[0] != n:
+            shape = q.shape
+            if len(shape) != 2 or shape[0] != n or (self._rope_dims and n_heads * self._rope_dims != shape[1]):
                 raise ValueError("q must be [n][n_heads*head_dim]")
             if out is None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            elif out.shape != q.shape:
+                out = torch.empty(shape, dtype=q.dtype, device=q.device)
+            elif out.shape != shape:
                 raise ValueError("out must match q")
             qp, qs = rows(q, "q")
-            op, os = rows(out, "out")
-            if n_heads < 0 or (self._rope_dims and n_heads * self._rope_dims != q.shape[1]):
-                raise ValueError("q must be [n][n_heads*head_dim]")
+            op, os = (qp, qs) if out is q else rows(out, "out")
         elif out is not None:
             raise ValueError("out without q")
         _check(self._lib.ltkv_write_rope_rows(
-            self._h, layer, n, _dev_ptr(slot_mapping, torch.int32, "slot_mapping", self.device),
-            _dev_ptr(positions, torch.int32, "positions", self.device), types[k.dtype], kp, vp, ks, qp, qs, n_heads,
-            op, os))
+            self._h, layer, n, _dev_ptr(slot_mapping, torch.int32, "slot_mapping", dev),
+            _dev_ptr(positions, torch.int32, "positions", dev), code, kp, vp, ks, qp, qs, n_heads, op, os))
         return out
-
-    @staticmethod
-    def _row_types() -> dict:
-        import torch
-
-        return {torch.float32: _lib.ROWS_F32, torch.float16: _lib.ROWS_F16, torch.bfloat16: _lib.ROWS_BF16}
 
     def copy_blocks(self, pairs) -> None:
         """Kernel 2: copy block pairs[i,0] -> pairs[i,1] (all layers, K and V)."""
@@ -448,7 +478,7 @@ class KvCache:
         import torch
 
         n = lens.numel()
-        types = self._row_types()
+        types = _row_types()
         if q.dim() != 2 or q.shape[1] != n_heads * head_dim:
             raise ValueError("q must be [n_rows][n_heads*head_dim]")
         if q.dtype not in types:
@@ -502,7 +532,7 @@ class KvCache:
         import torch
 
         n = lens.numel()
-        types = self._row_types()
+        types = _row_types()
         if q.dim() != 2 or q.shape[1] != n_heads * head_dim:
             raise ValueError("q must be [n_rows][n_heads*head_dim]")
         if q.dtype not in types:
@@ -555,17 +585,29 @@ class KvCache:
             raise ValueError("rows, lens and counts must have equal length")
         if parents is not None and parents.numel() != n_tokens:
             raise ValueError("parents must have n_tokens entries")
-
-        def new(*shape):
-            return torch.empty(shape, dtype=torch.int32, device=rows.device)
-
-        shapes = [(n + 1,), (n,), (n, table_stride), (n_tokens,), (n_tokens,),
-                  (n_tokens, mask_words) if parents is not None else None]
+        int32, dev = torch.int32, self.device
+        sizes = (n, n_tokens, table_stride, mask_words if parents is not None else None, dev)
         if out is None:
-            out = StepLayout(*(None if s is None else new(*s) for s in shapes))
-        for name, t, s in zip(StepLayout._fields, out, shapes):
-            if (t is None) != (s is None) or (t is not None and tuple(t.shape) != s):
-                raise ValueError(f"out.{name} must have shape {s}")
+            parts, pointers = _int32_parts(
+                [n + 1, n, n * table_stride, n_tokens, n_tokens] +
+                ([n_tokens * mask_words] if parents is not None else []), rows.device)
+            parts[2] = parts[2].view(n, table_stride)
+            if parents is not None:
+                parts[5] = parts[5].view(n_tokens, mask_words)
+            else:
+                parts.append(None)
+                pointers.append(None)
+            out = _OwnLayout(*parts)
+            out.sizes, out.pointers = sizes, pointers
+        pointers = out.pointers if isinstance(out, _OwnLayout) and out.sizes == sizes else None
+        if pointers is None:  # arrays of the caller's own
+            shapes = [(n + 1,), (n,), (n, table_stride), (n_tokens,), (n_tokens,),
+                      (n_tokens, mask_words) if parents is not None else None]
+            for name, t, shape in zip(StepLayout._fields, out, shapes):
+                if (t is None) != (shape is None) or (t is not None and tuple(t.shape) != shape):
+                    raise ValueError(f"out.{name} must have shape {shape}")
+            pointers = [None if t is None else _dev_ptr(t, int32, f"out.{name}", dev)
+                        for name, t in zip(StepLayout._fields, out)]
         if n == 0:  # nothing to lay out: every token is behind the last one
             out.row_starts.zero_()
             for t in (out.slot_mapping, out.positions):
@@ -573,14 +615,11 @@ class KvCache:
             if out.masks is not None:
                 out.masks.zero_()
             return out
-
-        def ptr(t, name):
-            return None if t is None else _dev_ptr(t, torch.int32, name, self.device)
-
         _check(self._lib.ltkv_step_layout(
-            self._h, n, ptr(rows, "rows"), ptr(lens, "lens"), ptr(counts, "counts"), n_tokens, table_stride,
-            ptr(parents, "parents"), mask_words if parents is not None else 0,
-            *(ptr(t, f"out.{name}") for name, t in zip(StepLayout._fields, out))))
+            self._h, n, _dev_ptr(rows, int32, "rows", dev), _dev_ptr(lens, int32, "lens", dev),
+            None if counts is None else _dev_ptr(counts, int32, "counts", dev), n_tokens, table_stride,
+            None if parents is None else _dev_ptr(parents, int32, "parents", dev),
+            mask_words if parents is not None else 0, *pointers))
         return out
 
     def accept_tree(self, tables, lens, row_starts, parents, tokens, targets,
@@ -600,21 +639,25 @@ class KvCache:
             raise ValueError("row_starts must have one entry per sequence and one more")
         if parents.numel() != n_rows or targets.numel() != n_rows:
             raise ValueError("parents, tokens and targets must have equal length")
+        int32, dev = torch.int32, self.device
         sizes = (n, n_rows, n, n)
         if out is None:
-            out = AcceptedTree(*(torch.empty((s,), dtype=torch.int32, device=lens.device) for s in sizes))
-        for name, t, s in zip(AcceptedTree._fields, out, sizes):
-            if t.numel() != s:
-                raise ValueError(f"out.{name} must have {s} entries")
+            parts, pointers = _int32_parts(sizes, lens.device)
+            out = AcceptedTree(*parts)
+        else:
+            pointers = []
+            for name, t, size in zip(AcceptedTree._fields, out, sizes):
+                if t.numel() != size:
+                    raise ValueError(f"out.{name} must have {size} entries")
+                pointers.append(_dev_ptr(t, int32, f"out.{name}", dev))
         if n == 0:
             out.path.fill_(-1)
             return out
-        args = dict(tables=tables, lens=lens, row_starts=row_starts, parents=parents, tokens=tokens, targets=targets,
-                    **{f"out.{name}": t for name, t in zip(AcceptedTree._fields, out)})
-        p = {name: _dev_ptr(t, torch.int32, name, self.device) for name, t in args.items()}
         _check(self._lib.ltkv_accept_tree(
-            self._h, n, n_rows, p["tables"], tables.shape[1], p["lens"], p["row_starts"], p["parents"], p["tokens"],
-            p["targets"], p["out.accepted"], p["out.path"], p["out.next"], p["out.lens"]))
+            self._h, n, n_rows, _dev_ptr(tables, int32, "tables", dev), tables.shape[1],
+            _dev_ptr(lens, int32, "lens", dev), _dev_ptr(row_starts, int32, "row_starts", dev),
+            _dev_ptr(parents, int32, "parents", dev), _dev_ptr(tokens, int32, "tokens", dev),
+            _dev_ptr(targets, int32, "targets", dev), *pointers))
         return out
 
     def _zeros_like(self, t):
