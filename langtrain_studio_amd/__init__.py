@@ -10,8 +10,8 @@ C ABI in include/ltkv.h). This package is its Python face:
   ``Model::forward`` (engine/crates/native/src/model.rs:380-475).
 """
 
-from .kv import BLOCK, KvCache, KvCacheFull, KvError, NonContiguous  # noqa: F401
-from .backend import BatchToken, PagedKvBackend, StepPlan  # noqa: F401
+from .kv import BLOCK, AcceptedTree, KvCache, KvCacheFull, KvError, NonContiguous, StepLayout  # noqa: F401
+from .backend import BatchToken, Drafts, DraftStep, PagedKvBackend, StepPlan  # noqa: F401
 
-__all__ = ["BLOCK", "KvCache", "KvCacheFull", "KvError", "NonContiguous", "BatchToken",
-           "PagedKvBackend", "StepPlan"]
+__all__ = ["BLOCK", "AcceptedTree", "KvCache", "KvCacheFull", "KvError", "NonContiguous", "StepLayout", "BatchToken",
+           "Drafts", "DraftStep", "PagedKvBackend", "StepPlan"]

@@ -8,6 +8,10 @@ KV segment of ``decode`` (model.rs:380-475): claim every token's cell first
 (copy-on-write copies land before any write), then per layer write K/V and
 run GQA attention over the paged rows. Projections, RoPE and the rest of the
 transformer stay with the caller.
+
+``begin_drafts``, ``draft_layer`` and ``accept`` are its step with drafted tokens,
+which the reference does not have: trees of drafts are appended and attended in
+one pass, and the path that the model agrees with is kept.
 """
 
 from __future__ import annotations
@@ -19,7 +23,7 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import _lib
-from .kv import BLOCK, KvCache
+from .kv import BLOCK, AcceptedTree, KvCache, StepLayout
 
 
 @dataclass(frozen=True)
@@ -45,6 +49,30 @@ class StepPlan:
     planned: bool = False   # the cache holds this step's attention plan ("planned")
     decode_only: bool = False  # one token per sequence: write and attention fuse into one launch
     upload: "object" = None    # (raw stream, event) of an upload still to be waited for on other streams
+
+
+@dataclass(frozen=True)
+class Drafts:
+    """One sequence's drafted tokens: its pending token (0, a root) and drafts,
+    each behind its parent, which comes before it."""
+
+    seq: int
+    parents: Sequence[int]
+
+
+@dataclass
+class DraftStep:
+    """Device-resident description of a claimed step with drafted tokens."""
+
+    n: int                   # rows of all sequences
+    seqs: list               # sequence of each entry
+    lens: list               # lengths in front of the drafts
+    ends: list               # and behind them
+    max_rows: int
+    layout: StepLayout       # row starts, lengths, tables, cells, positions, masks
+    parents: "object"        # torch.int32 [n]
+    upload: "object" = None  # as StepPlan's
+
 
 DESCRIPTORS = ("tables", "resident", "planned")
 
@@ -181,3 +209,77 @@ class PagedKvBackend:
                                                  self.scale, out=out)
         return self.kv.decode_attention(layer, q, plan.tables, plan.lens, self.n_heads, self.head_dim,
                                         self.scale, out=out)
+
+    # ---- steps with drafted tokens
+    def begin_drafts(self, drafts: Sequence[Drafts]) -> DraftStep:
+        """Claims the cells of every sequence's drafted tokens behind its length
+        and lays the step out on the device. All or nothing: where a claim fails
+        (KvCacheFull) the sequences are as they were. Not inside a stream
+        capture."""
+        import torch
+
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("begin_drafts cannot be captured: begin the step before the capture, capture its layers")
+        counts = [len(d.parents) for d in drafts]
+        n = sum(counts)
+        if n > self._n_batch:
+            raise ValueError(f"{n} drafted tokens exceed n_batch {self._n_batch}")
+        seqs = [d.seq for d in drafts]
+        if len(set(seqs)) != len(seqs) or any(m == 0 for m in counts):
+            raise ValueError("drafts need distinct sequences with at least one token each")
+        for d in drafts:
+            if d.parents[0] != -1 or any(not 0 <= p < j for j, p in enumerate(d.parents) if j):
+                raise ValueError(f"parents of sequence {d.seq}: the first is -1, the others name an earlier token")
+        lens = [self.kv.len(s) for s in seqs]
+        try:
+            if n:
+                self.kv.append_batch(np.repeat(np.array(seqs, np.uint32), counts),
+                                     np.concatenate([c + np.arange(m, dtype=np.uint64) for c, m in zip(lens, counts)]))
+        except Exception:
+            for s, c in zip(seqs, lens):
+                self.kv.truncate(s, c)
+            raise
+        words = (max(counts, default=1) + 31) // 32
+        stride = max([1] + [-(-(c + m) // BLOCK) for c, m in zip(lens, counts)])
+        arrays = [self.kv.seq_rows(seqs), np.array(lens, np.int32), np.array(counts, np.int32),
+                  np.array([p for d in drafts for p in d.parents], np.int32)]
+        (rows, d_lens, d_counts, parents), upload = self._upload(arrays)
+        layout = self.kv.step_layout(rows, d_lens, d_counts, n, stride, parents=parents, mask_words=words)
+        return DraftStep(n=n, seqs=seqs, lens=lens, ends=[c + m for c, m in zip(lens, counts)],
+                         max_rows=max(counts, default=0), layout=layout, parents=parents, upload=upload)
+
+    def draft_layer(self, step: DraftStep, layer: int, q, k, v, out: Optional[object] = None, rotate: bool = True,
+                    softcap: float = 0.0, window: int = 0):
+        """One layer of a step with drafted tokens: k and v ([n][kv_dim]) into the
+        claimed cells, then attention of q ([n][n_heads*head_dim]) over each
+        token's context and ancestors. With rotate the rows are f32, f16 or bf16
+        projections and turn by the cache's RoPE table (kv.rope_init_scaled);
+        else k and v are f32 rows with RoPE applied."""
+        if step.upload is not None and step.upload[0] != self.kv._stream:  # the cache changed streams since
+            _lib.wait_event(step.upload[1])
+            step.upload = None
+        at = step.layout
+        if rotate:
+            q = self.kv.write_rope_rows(layer, at.slot_mapping, at.positions, k, v, q=q, n_heads=self.n_heads)
+        else:
+            self.kv.write_batch(layer, at.slot_mapping, k, v)
+        return self.kv.tree_attention(layer, q, at.tables, at.lens, self.n_heads, self.head_dim, at.row_starts,
+                                      positions=at.positions, masks=at.masks, max_rows=max(step.max_rows, 1),
+                                      scale=self.scale, softcap=softcap, window=window, out=out)
+
+    def accept(self, step: DraftStep, tokens, targets) -> tuple[list, AcceptedTree]:
+        """Keeps the path of every tree that the model agrees with: tokens and
+        targets (int32 [n] on the device) are the drafted tokens and what the model
+        chose behind each. Waits for the device, and truncates the sequences to
+        what was kept; returns the tokens kept of each sequence, and the arrays on
+        the device (the token behind them is next)."""
+        at = step.layout
+        for s, end in zip(step.seqs, step.ends):
+            if self.kv.len(s) != end:
+                raise RuntimeError(f"sequence {s} changed since its drafts were begun")
+        done = self.kv.accept_tree(at.tables, at.lens, at.row_starts, step.parents, tokens, targets)
+        self.kv.synchronize()
+        kept = done.accepted.tolist()
+        for s, c, m in zip(step.seqs, step.lens, kept):
+            self.kv.truncate(s, c + m)
+        return kept, done
