@@ -169,12 +169,11 @@ write_kernel(uint8_t *__restrict__ kpool, uint8_t *__restrict__ vpool,
 // ----------------------------------------------------------------------------
 // Kernel 1 for q8_0 cells: each 32-element group of a K or V row becomes 32
 // int8 quants in the cell and its scale d, rounded to f16, in the scale pool
-// (the Q8_0 block of quant.rs:188-193: f16 d + 32 int8).
+// (the Q8_0 block of quant.rs:188-193: f16 d + 32 int8); q4_0 cells hold nibbles.
+// 4 lanes per 32-element group of K or V, two 16-byte loads and one 8-byte (4-byte)
+// store per lane. q4_0: ~9 500 rows of 2 x 1024 elements in 15.8 us (89 MB, 5.6
+// TB/s), bound by the reads; a row a wave and a division an element took 23 us.
 // ----------------------------------------------------------------------------
-// Kernel 1 for q8_0 and q4_0 cells: 4 lanes per 32-element group of K or V, two
-// 16-byte loads and one 8-byte (4-byte) store per lane. q4_0: ~9 500 rows of 2 x
-// 1024 elements in 15.8 us (89 MB, 5.6 TB/s), bound by the reads; a row a wave
-// and a division an element took 23 us.
 template <int BITS>
 __global__ void __launch_bounds__(256)
 write_quant_kernel(int8_t *__restrict__ kpool, int8_t *__restrict__ vpool, uint16_t *__restrict__ kscale,
