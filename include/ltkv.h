@@ -434,8 +434,10 @@ LTKV_API int ltkv_scored_attention(ltkv_cache *c, size_t layer, size_t n, size_t
  * a row that sees an infinity or NaN gives is not specified (it is not finite
  * where a visible V is not).
  * f32 rows are computed to f32 accuracy, f16 and bf16 rows with weights (and V of
- * f32 and Q8_0 pools) rounded to f16, summed in f32. Elements of f32 and Q8_0 pools
- * keep 22 bits down to 2^16 below the largest of their row's head.
+ * f32 and Q8_0 pools) rounded to f16, summed in f32. An element of K or V keeps 22
+ * bits down to 2^16 below the largest of its position's head (f32 pools: of its
+ * block's 16 positions where every row of a tile sees them), V also only down to
+ * 2^16 below the largest that the row sees, and fewer below that.
  * max_rows: the most rows of one sequence, which sizes the tiles (one with more is
  * computed all the same). head_dim a multiple of 8 up to 256 and groups of up to
  * 64 run on the matrix cores, others on a generic kernel; head_dim up to 1024. Rows
@@ -481,7 +483,7 @@ LTKV_API int ltkv_step_layout(ltkv_cache *c, size_t n, const int32_t *d_rows, co
  * chose d_targets[j] behind it. Token 0 is kept; from a kept token the lowest
  * child whose token is the kept one's target is kept next, until there is none.
  * The K and V rows of the kept tokens move together, the k-th to position C + k;
- * cells behind them hold what they held. Outputs: d_accepted [n] how many were
+ * cells behind them hold what they held. No sequence may come twice. Outputs: d_accepted [n] how many were
  * kept (0 without rows), d_path [n_rows] the kept tokens in order, -1 behind them
  * and in rows of no request; d_next [n] the last one's target (-1 without rows);
  * d_new_lens [n] the length after it (truncate the sequences to it). Blocks shared

@@ -174,9 +174,9 @@ struct TreeSeq {
   int32_t steps, tiles;
 };
 
-__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int64_t i) {
+__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, const SeqRows &rows) {
   TreeSeq s;
-  s.rows = seq_rows(a, i);
+  s.rows = rows;
   s.ctx = s.rows.len - s.rows.count;
   // no row sees a position in front of the window of the context's end
   s.first = a.window > 0 ? (int32_t)max((int64_t)s.ctx - a.window + 1, (int64_t)0) & ~15 : 0;
@@ -185,9 +185,15 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int64_t i) {
   return s;
 }
 
-__device__ __forceinline__ int64_t tree_steps(const TreeArgs &a, int64_t i) {
-  const TreeSeq s = tree_seq(a, i);
+__device__ __forceinline__ int64_t tree_steps(const TreeArgs &a, const SeqRows &rows) {
+  const TreeSeq s = tree_seq(a, rows);
   return (int64_t)s.steps * s.tiles;
+}
+
+__device__ __forceinline__ void keep_rows(int32_t (&to)[3], const SeqRows &r) {
+  to[0] = (int32_t)r.row0;
+  to[1] = r.count;
+  to[2] = r.len;
 }
 
 __device__ __forceinline__ int64_t uniform64(int64_t x) {
@@ -362,7 +368,8 @@ struct Cells<int8_t, HD, EXACT, NT> {
   // 2^-22 of the largest scale).
   // Returns the largest power of the lane's positions.
   template <int PLANES>
-  __device__ __forceinline__ float put(char *lds, int plane, int pitch, int lane, uint32_t bad, float *pow) const {
+  __device__ __forceinline__ float put(char *lds, int plane, int pitch, int lane, uint32_t bad, float *pow,
+                                       bool) const {
     float most = 0.f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -412,28 +419,50 @@ struct Cells<float, HD, EXACT, NT> {
     for (int j = 0; j < N; ++j) b |= top_bits(j) >= 0x7f800000u ? 1u << j : 0u;
     return b;
   }
-  // (powers of at least 2^-100: smaller values are nothing beside their products' rounding)
+  // Powers of at least 2^-100: smaller values are nothing beside their products'
+  // rounding. Each position has its own where a row does not see all of the step;
+  // else the block's 16 share one (a reduction instead of eight). Parts by
+  // truncation, two an instruction.
   template <int PLANES>
-  __device__ __forceinline__ float put(char *lds, int plane, int pitch, int lane, uint32_t bad, float *pow) const {
+  __device__ __forceinline__ float put(char *lds, int plane, int pitch, int lane, uint32_t bad, float *pow,
+                                       bool apart) const {
+    int e[N];
+    if (apart) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) e[j] = exponent(lanes_max<ROW>(__builtin_bit_cast(float, min(top_bits(j), 0x7f7fffffu))));
+    } else {
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j) top = max(top, top_bits(j));
+      const int all = exponent(lanes_max<64>(__builtin_bit_cast(float, min(top, 0x7f7fffffu))));
+#pragma unroll
+      for (int j = 0; j < N; ++j) e[j] = all;
+    }
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const float top = lanes_max<ROW>(__builtin_bit_cast(float, min(top_bits(j), 0x7f7fffffu)));
-      const int e = top > 0.f ? max(__builtin_amdgcn_frexp_expf(top) - 15, -100) : -100;
-      if (lane % ROW == 0) pow[row(lane, j)] = __builtin_amdgcn_ldexpf(1.f, e);
-      h4 hi, lo;
+      if (lane % ROW == 0) pow[row(lane, j)] = __builtin_amdgcn_ldexpf(1.f, e[j]);
+      h2 hi[2], lo[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        _Float16 a, b;
-        const uint32_t u = bad >> j & 1 ? 0u : x[j][i];
-        split2(__builtin_amdgcn_ldexpf(__builtin_bit_cast(float, u), -e), a, b);
-        hi[i] = a;
-        lo[i] = b;
+      for (int i = 0; i < 2; ++i) {
+        float v[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t u = bad >> j & 1 ? 0u : x[j][2 * i + k];
+          v[k] = __builtin_amdgcn_ldexpf(__builtin_bit_cast(float, u), -e[j]);
+        }
+        hi[i] = PLANES == 1 ? h2{(_Float16)v[0], (_Float16)v[1]}
+                            : __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(v[0], v[1]));
+        lo[i] = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi[i].x, -1.f, v[0]),
+                                                                  __builtin_fmaf((float)hi[i].y, -1.f, v[1])));
       }
       char *const to = lds + row(lane, j) * pitch + lane % ROW * 8;
-      *reinterpret_cast<h4 *>(to) = hi;
-      if constexpr (PLANES == 2) *reinterpret_cast<h4 *>(to + plane) = lo;
+      *reinterpret_cast<h4 *>(to) = h4{hi[0].x, hi[0].y, hi[1].x, hi[1].y};
+      if constexpr (PLANES == 2) *reinterpret_cast<h4 *>(to + plane) = h4{lo[0].x, lo[0].y, lo[1].x, lo[1].y};
     }
     return 0.f;
+  }
+  static __device__ __forceinline__ int exponent(float top) {
+    return top > 0.f ? max(__builtin_amdgcn_frexp_expf(top) - 15, -100) : -100;
   }
 };
 
@@ -503,8 +532,8 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   __shared__ uint32_t s_bad[kTreeWaves];  // bit p: V of position 16 wave + p has an infinity or NaN
   __shared__ int64_t s_begin[kTreeThreads + 1];
   __shared__ int64_t s_sum[kTreeWaves];
-  __shared__ int64_t s_found[2];
-  __shared__ TreeSeq s_seq;
+  __shared__ int64_t s_found[3];
+  __shared__ int32_t s_rows[kTreeThreads][3];  // of the last sequence that a thread looked at: first row, rows, length
   __shared__ int32_t s_from[kTreeWaves];
   __shared__ float s_top[kTreeWaves];  // 8-bit pools: the largest power of a wave's positions' V
   char *const lds_k = lds, *const lds_v = lds + K_PLANES * K_BYTES;
@@ -519,7 +548,11 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   const int64_t i0 = min((int64_t)tid * each, a.n), i1 = min(i0 + each, a.n);
   {
     int64_t sum = 0;
-    for (int64_t i = i0; i < i1; ++i) sum += tree_steps(a, i);
+    for (int64_t i = i0; i < i1; ++i) {
+      const SeqRows r = seq_rows(a, i);
+      keep_rows(s_rows[tid], r);
+      sum += tree_steps(a, r);
+    }
     int64_t upto = sum;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -547,29 +580,24 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   while (at < end) {
     __syncthreads();  // s_found, and the step's memory, have been read
     if (s_begin[tid] <= at && at < s_begin[tid + 1]) {
-      int64_t begin = s_begin[tid];
-      for (int64_t i = i0; i < i1; ++i) {
-        const TreeSeq x = tree_seq(a, i);
-        const int64_t next = begin + (int64_t)x.steps * x.tiles;
-        if (at < next) {
-          s_found[0] = i;
-          s_found[1] = begin;
-          s_seq = x;
-          break;
-        }
+      int64_t begin = s_begin[tid], i = i0;
+      for (; i + 1 < i1; ++i) {  // (a single sequence lies there already)
+        const SeqRows r = seq_rows(a, i);
+        keep_rows(s_rows[tid], r);
+        const int64_t next = begin + tree_steps(a, r);
+        if (at < next) break;
         begin = next;
       }
+      if (i0 + 1 < i1 && i + 1 == i1) keep_rows(s_rows[tid], seq_rows(a, i));
+      s_found[0] = i;
+      s_found[1] = begin;
+      s_found[2] = tid;
     }
     __syncthreads();
     const int64_t seq = uniform64(s_found[0]), off = at - uniform64(s_found[1]);
-    TreeSeq ts;
-    ts.rows.row0 = uniform64(s_seq.rows.row0);
-    ts.rows.count = __builtin_amdgcn_readfirstlane(s_seq.rows.count);
-    ts.rows.len = __builtin_amdgcn_readfirstlane(s_seq.rows.len);
-    ts.ctx = __builtin_amdgcn_readfirstlane(s_seq.ctx);
-    ts.first = __builtin_amdgcn_readfirstlane(s_seq.first);
-    ts.steps = __builtin_amdgcn_readfirstlane(s_seq.steps);
-    ts.tiles = __builtin_amdgcn_readfirstlane(s_seq.tiles);
+    const int32_t *const found = s_rows[s_found[2]];
+    const TreeSeq ts = tree_seq(a, SeqRows{__builtin_amdgcn_readfirstlane(found[0]), __builtin_amdgcn_readfirstlane(found[1]),
+                                           __builtin_amdgcn_readfirstlane(found[2])});
     const SeqRows rows = ts.rows;
     const int tile = (int)(off / ts.steps);
     const int s_first = (int)(off - (int64_t)tile * ts.steps);
@@ -708,9 +736,10 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
         }
       }
       if constexpr (PAIRS) {
-        cells.k.template put<2>(lds_k + 16 * wave * K_PITCH, K_BYTES, K_PITCH, lane, 0, s_kpow + 16 * wave);
+        cells.k.template put<2>(lds_k + 16 * wave * K_PITCH, K_BYTES, K_PITCH, lane, 0, s_kpow + 16 * wave, partial);
         const float v_top =
-            cells.v.template put<V_PLANES>(lds_v + 16 * wave * V_PITCH, V_BYTES, V_PITCH, lane, bad, s_vpow + 16 * wave);
+            cells.v.template put<V_PLANES>(lds_v + 16 * wave * V_PITCH, V_BYTES, V_PITCH, lane, bad, s_vpow + 16 * wave,
+                                              partial);
         if constexpr (BYTES) {
           const float x = lanes_max<64>(v_top);
           if (lane == 0) s_top[wave] = x;
@@ -1011,7 +1040,8 @@ struct TreeFold {
 // most two such tiles, its first and its last). A thread takes four elements of some
 // parts, in order; where the parts are many and the elements few, threads share the
 // parts and their averages are folded in LDS. One tree of 8 rows over 4000 positions
-// lies in 63 shares: TIME_ONE; 64 trees of up to 16 rows in two or three: TIME_MANY.
+// lies in 63 shares: 7.9 us (one work-group a share 6.8, four 11.6); 64 trees of up to
+// 16 rows in two or three: 10.2 us (10.6, 10.6).
 constexpr int kMergeGroups = 2;
 
 __global__ void __launch_bounds__(kTreeThreads) tree_merge_kernel(TreeArgs a) {
