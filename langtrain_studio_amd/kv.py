@@ -599,8 +599,10 @@ class KvCache:
                 pointers.append(None)
             out = _OwnLayout(*parts)
             out.sizes, out.pointers = sizes, pointers
-        pointers = out.pointers if isinstance(out, _OwnLayout) and out.sizes == sizes else None
-        if pointers is None:  # arrays of the caller's own
+        pointers = None
+        if isinstance(out, _OwnLayout) and out.sizes == sizes and out.row_starts.data_ptr() == out.pointers[0]:
+            pointers = out.pointers
+        else:  # arrays of the caller's own (or a copy of a layout)
             shapes = [(n + 1,), (n,), (n, table_stride), (n_tokens,), (n_tokens,),
                       (n_tokens, mask_words) if parents is not None else None]
             for name, t, shape in zip(StepLayout._fields, out, shapes):

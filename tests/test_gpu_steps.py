@@ -3,6 +3,7 @@ appends of rows of any type, and acceptance, against plain restatements."""
 
 from __future__ import annotations
 
+import copy
 import math
 
 import numpy as np
@@ -157,6 +158,14 @@ def test_layout_follows_the_tables(gpu):
     again = kv.step_layout(rows, lens, counts, 4, 4, out=out)
     kv.synchronize()
     assert again is out
+    copied = copy.deepcopy(out)  # a copy's arrays are its own
+    for t in (out.lens, copied.lens):
+        t.zero_()
+    torch.cuda.synchronize()
+    kv.step_layout(rows, lens, counts, 4, 4, out=copied)
+    kv.synchronize()
+    assert down(copied.lens).tolist() == [22, 10] and down(out.lens).tolist() == [0, 0]
+    out = copied
     for name, g, w in zip(out._fields, out, layout_of(kv, [20, 9], [2, 1], 4, 4)):
         if g is not None:
             np.testing.assert_array_equal(down(g), w, err_msg=name)
