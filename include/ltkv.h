@@ -483,12 +483,13 @@ LTKV_API int ltkv_step_layout(ltkv_cache *c, size_t n, const int32_t *d_rows, co
  * chose d_targets[j] behind it. Token 0 is kept; from a kept token the lowest
  * child whose token is the kept one's target is kept next, until there is none.
  * The K and V rows of the kept tokens move together, the k-th to position C + k;
- * cells behind them hold what they held. No sequence may come twice. Outputs: d_accepted [n] how many were
- * kept (0 without rows), d_path [n_rows] the kept tokens in order, -1 behind them
- * and in rows of no request; d_next [n] the last one's target (-1 without rows);
- * d_new_lens [n] the length after it (truncate the sequences to it). Blocks shared
- * with other sequences must have been copied, as appending the drafts does. A
- * table entry outside the pool moves nothing and is reported by ltkv_synchronize.
+ * cells behind them hold what they held. No sequence may come twice. Outputs:
+ * d_accepted [n] how many were kept (0 without rows), d_path [n_rows] the kept
+ * tokens in order, -1 behind them and in rows of no request; d_next [n] the last
+ * one's target (-1 without rows); d_new_lens [n] the length after it (truncate the
+ * sequences to it). Blocks shared with other sequences must have been copied, as
+ * appending the drafts does. A table entry outside the pool moves nothing and is
+ * reported by ltkv_synchronize.
  * Inputs and outputs may not overlap. */
 LTKV_API int ltkv_accept_tree(ltkv_cache *c, size_t n, size_t n_rows, const int32_t *d_tables,
                               size_t table_stride, const int32_t *d_lens, const int32_t *d_row_starts,

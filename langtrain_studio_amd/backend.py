@@ -255,8 +255,6 @@ class PagedKvBackend:
         token's context and ancestors. With rotate the rows are f32, f16 or bf16
         projections and turn by the cache's RoPE table (kv.rope_init_scaled);
         else k and v are f32 rows with RoPE applied."""
-        import torch
-
         if step.upload is not None and step.upload[0] != self.kv._stream:  # the cache changed streams since
             _lib.wait_event(step.upload[1])
             step.upload = None
@@ -266,7 +264,7 @@ class PagedKvBackend:
         else:
             self.kv.write_batch(layer, at.slot_mapping, k, v)
         if out is None:
-            out = torch.empty_like(q)  # (every row is a sequence's)
+            out = self.kv._empty(q.shape, q.dtype)  # (every row is a sequence's)
         return self.kv.tree_attention(layer, q, at.tables, at.lens, self.n_heads, self.head_dim, at.row_starts,
                                       positions=at.positions, masks=at.masks, max_rows=max(step.max_rows, 1),
                                       scale=self.scale, softcap=softcap, window=window, out=out)

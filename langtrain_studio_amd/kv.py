@@ -85,16 +85,16 @@ def _row_types() -> dict:
     return _types
 
 
-def _int32_parts(sizes, device):
-    """int32 tensors of these sizes in one allocation, and their addresses (each
-    16-byte aligned)."""
+def _int32_parts(sizes, empty):
+    """int32 tensors of these sizes in one allocation of empty(shape, dtype), and
+    their addresses (each 16-byte aligned)."""
     import torch
 
     starts, total = [], 0
     for size in sizes:
         starts.append(total)
         total += -(-size // 4) * 4
-    buf = torch.empty((total,), dtype=torch.int32, device=device)
+    buf = empty((total,), torch.int32)
     base = buf.data_ptr()
     return [buf[at:at + size] for at, size in zip(starts, sizes)], [base + 4 * at for at in starts]
 
@@ -406,7 +406,7 @@ class KvCache:
             if len(shape) != 2 or shape[0] != n or (self._rope_dims and n_heads * self._rope_dims != shape[1]):
                 raise ValueError("q must be [n][n_heads*head_dim]")
             if out is None:
-                out = torch.empty(shape, dtype=q.dtype, device=q.device)
+                out = self._empty(shape, q.dtype)
             elif out.shape != shape:
                 raise ValueError("out must match q")
             qp, qs = rows(q, "q")
@@ -590,7 +590,7 @@ class KvCache:
         if out is None:
             parts, pointers = _int32_parts(
                 [n + 1, n, n * table_stride, n_tokens, n_tokens] +
-                ([n_tokens * mask_words] if parents is not None else []), rows.device)
+                ([n_tokens * mask_words] if parents is not None else []), self._empty)
             parts[2] = parts[2].view(n, table_stride)
             if parents is not None:
                 parts[5] = parts[5].view(n_tokens, mask_words)
@@ -611,12 +611,15 @@ class KvCache:
             pointers = [None if t is None else _dev_ptr(t, int32, f"out.{name}", dev)
                         for name, t in zip(StepLayout._fields, out)]
         if n == 0:  # nothing to lay out: every token is behind the last one
-            out.row_starts.zero_()
-            for t in (out.slot_mapping, out.positions):
-                t.fill_(-1)
-            if out.masks is not None:
-                out.masks.zero_()
+            with self._ordered():
+                out.row_starts.zero_()
+                for t in (out.slot_mapping, out.positions):
+                    t.fill_(-1)
+                if out.masks is not None:
+                    out.masks.zero_()
             return out
+        if n_tokens == 0:  # (empty tensors have no address)
+            parents, pointers = None, [*pointers[:5], None]
         _check(self._lib.ltkv_step_layout(
             self._h, n, _dev_ptr(rows, int32, "rows", dev), _dev_ptr(lens, int32, "lens", dev),
             None if counts is None else _dev_ptr(counts, int32, "counts", dev), n_tokens, table_stride,
@@ -644,7 +647,7 @@ class KvCache:
         int32, dev = torch.int32, self.device
         sizes = (n, n_rows, n, n)
         if out is None:
-            parts, pointers = _int32_parts(sizes, lens.device)
+            parts, pointers = _int32_parts(sizes, self._empty)
             out = AcceptedTree(*parts)
         else:
             pointers = []
@@ -653,13 +656,38 @@ class KvCache:
                     raise ValueError(f"out.{name} must have {size} entries")
                 pointers.append(_dev_ptr(t, int32, f"out.{name}", dev))
         if n == 0:
-            out.path.fill_(-1)
+            with self._ordered():
+                out.path.fill_(-1)
             return out
         _check(self._lib.ltkv_accept_tree(
             self._h, n, n_rows, _dev_ptr(tables, int32, "tables", dev), tables.shape[1],
             _dev_ptr(lens, int32, "lens", dev), _dev_ptr(row_starts, int32, "row_starts", dev),
             _dev_ptr(parents, int32, "parents", dev), _dev_ptr(tokens, int32, "tokens", dev),
             _dev_ptr(targets, int32, "targets", dev), *pointers))
+        return out
+
+    def _ordered(self):
+        """Context in which torch works on the cache's stream, in order with its
+        launches."""
+        import torch
+
+        if not self._stream:  # (the null stream; ExternalStream(0) is a new one)
+            return torch.cuda.stream(torch.cuda.default_stream(self.device))
+        return torch.cuda.stream(torch.cuda.ExternalStream(self._stream, device=self.device))
+
+    def _empty(self, shape, dtype):
+        """Memory whose earlier use is in order with the cache's launches, whatever
+        the current stream is."""
+        import torch
+
+        if self.device is None:  # (the call refuses)
+            return torch.empty(shape, dtype=dtype)
+        current = torch.cuda.current_stream(self.device)
+        if current.cuda_stream == self._stream:
+            return torch.empty(shape, dtype=dtype, device=current.device)
+        with self._ordered():
+            out = torch.empty(shape, dtype=dtype, device=current.device)
+        out.record_stream(current)  # the caller's: the memory is not reused under its work
         return out
 
     def _zeros_like(self, t):
@@ -672,10 +700,7 @@ class KvCache:
         current = torch.cuda.current_stream(self.device)
         if current.cuda_stream == self._stream:
             return torch.zeros_like(t)
-        own = torch.cuda.default_stream(self.device)  # (the null stream; ExternalStream(0) is a new one)
-        if self._stream:
-            own = torch.cuda.ExternalStream(self._stream, device=self.device)
-        with torch.cuda.stream(own):
+        with self._ordered():
             out = torch.zeros_like(t)
         out.record_stream(current)  # the caller's: the memory is not reused under its work
         return out

@@ -171,6 +171,57 @@ def test_layout_follows_the_tables(gpu):
             np.testing.assert_array_equal(down(g), w, err_msg=name)
 
 
+def test_layout_without_tokens(gpu):
+    """Requests that get no tokens (with and without parents), and no requests."""
+    import torch
+
+    kv = cache([17, 5])
+    rows = kv.seq_rows(np.arange(2))
+    empty = torch.empty(0, dtype=torch.int32, device="cuda")
+    for parents, words in ((None, 0), (empty, 2)):
+        got = kv.step_layout(up(rows, np.int32), up([17, 5], np.int32), up([0, 0], np.int32), 0, 2, parents=parents,
+                             mask_words=words)
+        kv.synchronize()
+        assert down(got.row_starts).tolist() == [0, 0, 0] and down(got.lens).tolist() == [17, 5]
+        assert down(got.tables).tolist() == [list(kv.block_table(0)), [kv.block_table(1)[0], -1]]
+    got = kv.step_layout(empty, empty, empty, 3, 2, parents=up([-1, 0, 0], np.int32), mask_words=1)
+    kv.synchronize()
+    assert down(got.row_starts).tolist() == [0] and down(got.slot_mapping).tolist() == [-1] * 3
+    assert down(got.masks).tolist() == [[0]] * 3
+    done = kv.accept_tree(empty.view(0, 1), empty, up([0], np.int32), *[up([0, 0], np.int32)] * 3)
+    kv.synchronize()
+    assert down(done.path).tolist() == [-1, -1] and done.accepted.numel() == 0
+
+
+def test_outputs_do_not_take_memory_in_use_on_the_current_stream(gpu):
+    """New outputs of a cache on another stream than the current one lie in none of
+    the memory that work of the current stream still reads."""
+    import torch
+
+    n = 1 << 16
+    kv = cache([n + 64], kvd=32, stream=torch.cuda.Stream())
+    rows, lens = up(kv.seq_rows(np.arange(1)), np.int32), up([0], np.int32)
+    counts = up([n], np.int32)
+    stride = n // BLOCK + 4
+    big = torch.ones(1 << 28, device="cuda")
+    want = kv.step_layout(rows, lens, counts, n, stride)  # (its kernel and memory are there)
+    kv.synchronize()
+    size = want.row_starts.untyped_storage().nbytes() // 4
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        held = torch.full((size,), 7, dtype=torch.int32, device="cuda")
+        for _ in range(40):  # some 15 ms of work in front of the copy
+            big.mul_(1.0)
+        copied = held + 0
+        del held
+        got = kv.step_layout(rows, lens, counts, n, stride)
+    torch.cuda.synchronize()
+    assert bool((copied == 7).all())
+    for a, b in zip(got[:5], want[:5]):
+        assert torch.equal(a, b)
+
+
 def test_layout_refusals(gpu):
     import torch
 
