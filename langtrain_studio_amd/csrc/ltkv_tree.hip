@@ -507,6 +507,16 @@ struct Column {
 // of the largest power that the column has seen (`v_exp`), one instruction a score.
 // f32 pools, and heads of more than 128 elements, take one work-group a CU: two left
 // their waves too few registers (f32, one step of 8 rows: 18 us with spills).
+//
+// Measured (32/8 heads of 128 unless said): 64 trees of 10 to 16 bf16 rows behind 2048
+// to 4096 positions of an f16 cache 171-179 us (842 MB, 4.9 TB/s), bound by the reads:
+// loads alone with the same pieces take 138 us, and a tile's end costs a work-group 7
+// to 10 us (Q is read behind the K and V on their way). 8 trees of 40 to 48 f32 rows
+// behind 32 000 positions of a q8_0 cache (28/4 heads) 570-620 us: three products of
+// pairs (486 GFLOP: products 42% of the cycles, vector instructions 40%, partly
+// overlapped). 16 trees of 64 f16 rows, capped, over a 4-bit cache in a window of 2048:
+// 90 us, vector instructions 52% (cap and softmax). One tree of 8 rows behind 400
+// positions: 8.7 us, latency.
 constexpr int tree_groups_a_cu(bool wide, int hd) { return wide || hd > 128 ? 1 : 2; }
 
 template <typename T, int HD, bool EXACT, bool FULL, int WC>

@@ -385,6 +385,31 @@ def test_types(gpu, shape, d, half, dtype, rows):
     assert torch.equal(out, wide.to(out.dtype))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "q8_0"])
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("shape,d", [((8, 2, 128), 128), ((9, 3, 64), 40), ((1, 1, 32), 32)])
+@pytest.mark.parametrize("n", [1025, 2560, 2563])
+def test_many_rows(gpu, n, shape, d, half, dtype):
+    """A call of many rows gives the bits of calls of a few."""
+    import torch
+
+    heads, kvh, hd = shape
+    few, slots, positions, q, k, v = rope_case(dtype, "bf16", shape, d, half, "yarn", n, 7)
+    many = rope_case(dtype, "bf16", shape, d, half, "yarn", n, 7)[0]
+    sd, pd = up(slots, np.int32), up(positions, np.int32)
+    out = many.write_rope_rows(0, sd, pd, k, v, q=q, n_heads=heads)
+    parts = [few.write_rope_rows(0, sd[i:i + 400], pd[i:i + 400], k[i:i + 400], v[i:i + 400], q=q[i:i + 400],
+                                 n_heads=heads) for i in range(0, n, 400)]
+    for c in (few, many):
+        c.synchronize()
+    assert torch.equal(out, torch.cat(parts))
+    for a, b in zip(many.read_pool(0), few.read_pool(0)):
+        np.testing.assert_array_equal(a, b)
+    if dtype == "q8_0":
+        for a, b in zip(many.read_scales(0), few.read_scales(0)):
+            np.testing.assert_array_equal(a, b)
+
+
 def test_rope_rows_with_the_plain_table_match_write_rope(gpu):
     """On rope_init's table and f32 rows: write_rope's bits, in place too."""
     shape, n = (8, 2, 128), 20
