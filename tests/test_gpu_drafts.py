@@ -187,6 +187,118 @@ def test_captured_layers(gpu):
         b.kv.synchronize()
 
 
+def test_captured_acceptance(gpu):
+    """Layers and the acceptance in one graph, replayed with other choices of the
+    model: paths, lengths and the moved rows are those of eager calls."""
+    import torch
+
+    from langtrain_studio_amd import AcceptedTree, Drafts
+
+    side = torch.cuda.Stream()
+    rng = np.random.default_rng(5)
+    trees = [random_tree(rng, 24, 0.3), random_tree(rng, 9, 0.2)]
+    tokens = rng.integers(0, 3, 33)
+    made = []
+    for _ in range(2):  # a cache that replays and one that is eager
+        b = backend("q8_0", stream=side)
+        with torch.cuda.stream(side):
+            cells = b.kv.append_batch(np.zeros(37, np.uint32), np.arange(37, dtype=np.uint64))
+            for layer in range(LAYERS):
+                _, k, v = rows_of(np.arange(37), layer, torch.float32)
+                b.kv.write_rope_rows(layer, up(cells, np.int32), up(np.arange(37), np.int32), k, v)
+            step = b.begin_drafts([Drafts(0, trees[0]), Drafts(1, trees[1])])
+        rows = [rows_of(tokens, layer, torch.bfloat16) for layer in range(LAYERS)]
+        made.append((b, step, rows, up(tokens, np.int32), up(np.zeros(33), np.int32),
+                     AcceptedTree(*[torch.empty(m, dtype=torch.int32, device="cuda") for m in (2, 33, 2, 2)]),
+                     [torch.empty_like(x[0]) for x in rows]))
+    torch.cuda.synchronize()
+
+    def run(b, step, rows, drafted, targets, done, outs):
+        at = step.layout
+        for layer in range(LAYERS):
+            b.draft_layer(step, layer, *rows[layer], out=outs[layer])
+        b.kv.accept_tree(at.tables, at.lens, at.row_starts, step.parents, drafted, targets, out=done)
+
+    with torch.cuda.stream(side):
+        for x in made:
+            run(*x)  # (sizes what is sized on demand)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        run(*made[0])
+    kept = set()
+    for turn in range(4):
+        targets = up(rng.integers(0, 3, 33), np.int32)
+        for x in made:
+            x[4].copy_(targets)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            run(*made[1])
+        for x in made:
+            x[0].kv.synchronize()
+        for g, w in zip(made[0][5], made[1][5]):
+            assert torch.equal(g, w), turn
+        kept.add(tuple(made[0][5].accepted.tolist()))
+        for layer in range(LAYERS):
+            assert torch.equal(made[0][6][layer], made[1][6][layer])
+            for x, y in zip(made[0][0].kv.read_pool(layer), made[1][0].kv.read_pool(layer)):
+                np.testing.assert_array_equal(x, y)
+    assert len(kept) > 1
+
+
+@pytest.mark.parametrize("shape", [(8, 8, 128), (51, 51, 20)])
+@pytest.mark.parametrize("dtype,size", [("f16", 2), ("f32", 4), ("q8_0", 1), ("q4_0", 0.5)])
+def test_cells_past_32_bits(gpu, dtype, size, shape):
+    """Rows that lie more than 2^32 bytes behind a pool's start: the same bits as in a
+    small cache."""
+    import torch
+
+    from langtrain_studio_amd import KvCache
+
+    heads, kvh, hd = shape
+    kvd = heads * hd
+    if kvd % 32 and dtype in ("q8_0", "q4_0"):
+        kvd, kvh = 1280, 64  # (whole groups)
+        heads = kvh
+    blocks = int((1 << 32) / (kvd * size * BLOCK)) + 40
+    rng = np.random.default_rng(6)
+    ctx, new = 53, 13
+    parents = random_tree(rng, new, 0.4)
+    n = ctx + new
+    x = [up(rng.standard_normal((n, kvd)), np.float32).to(torch.bfloat16) for _ in range(3)]
+    tokens, targets = (up(rng.integers(0, 2, new), np.int32) for _ in range(2))
+    results = []
+    for total in (40, blocks):
+        kv = KvCache(1, kvd, total * BLOCK, dtype=dtype)
+        order = np.arange(total)[::-1].copy()
+        kv.init_free_order(order)
+        cells = kv.append_batch(np.zeros(n, np.uint32), np.arange(n, dtype=np.uint64))
+        if min(kv.block_table(0)) < total - 40:  # (the other end is handed out first)
+            kv = KvCache(1, kvd, total * BLOCK, dtype=dtype)
+            kv.init_free_order(order[::-1].copy())
+            cells = kv.append_batch(np.zeros(n, np.uint32), np.arange(n, dtype=np.uint64))
+        assert min(kv.block_table(0)) >= total - 40
+        if hd % 8 == 0:
+            kv.rope_init_scaled(10000.0, hd, hd, True, 128)
+            kv.write_rope_rows(0, up(cells, np.int32), up(np.arange(n), np.int32), x[1], x[2])
+        else:
+            kv.write_batch(0, up(cells, np.int32), x[1].float(), x[2].float())
+        at = kv.step_layout(up(kv.seq_rows(np.arange(1)), np.int32), up([ctx], np.int32), up([new], np.int32), new, 6,
+                            parents=up(parents, np.int32), mask_words=1)
+        out = kv.tree_attention(0, x[0][:new], at.tables, at.lens, heads, hd, at.row_starts, masks=at.masks)
+        done = kv.accept_tree(at.tables, at.lens, at.row_starts, up(parents, np.int32), tokens, targets)
+        got = [torch.zeros((n, kvd), device="cuda") for _ in range(2)]
+        kv.gather_values(0, at.tables, at.lens, torch.zeros(1, dtype=torch.int64, device="cuda"), *got)
+        kv.synchronize()
+        results.append([out, *done, *got])
+        del kv
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    assert bool(results[0][0].float().isfinite().all()) and bool((results[0][0] != 0).any())
+
+
 def test_captured_before_its_partials_exist(gpu):
     """A capture that would have to grow the partials is refused, and works after
     one eager call."""
