@@ -497,9 +497,9 @@ struct Column {
 // place, numerators^T += V^T W (a lane's scores are positions 8 (r / 4) + 4 (lane /
 // 32) + r % 4 of its column, which is the second product's operand layout when its
 // 16 positions are taken as 4 (lane / 32) ... + 3 and 8 + 4 (lane / 32) ... + 3: no
-// exchange). FULL (f32 rows, and any rows with a cap over kShortCap): Q and the
-// weights as hi + lo pairs; else Q as it is (times a power of two), the weights and V
-// rounded to f16.
+// exchange). FULL (f32 rows, f16 rows on pools of pairs, and any rows with a cap
+// over kShortCap): Q and the weights as hi + lo pairs; else Q as it is (times a power of
+// two), the weights and V rounded to f16.
 // Of pairs (kPairs) the scores are multiplied by their position's power of two, and
 // so are the weights. f32 pools: a column's numerators have a reference of their own
 // (`top_o`): the largest weight times V, not the largest weight, lies near the top of
@@ -1122,7 +1122,12 @@ int tile_waves(const TreeArgs &a) {
 
 template <typename T, int HD, bool EXACT, int WC>
 hipError_t launch_tiles(const PoolGeom &g, const TreeArgs &a, hipStream_t s) {
-  const bool full = a.row_type == LTKV_ROWS_F32 || a.softcap > kShortCap;
+  // f16 rows on pools of pairs too: weights and V rounded to f16 would each be off by
+  // as much as their output's rounding (relative error 3.2e-4 against 2.1e-4), which
+  // bf16 rows do not see. 8 trees of 8 rows behind 8000 positions, q8_0: 72 us (59 with
+  // them rounded); of 44 behind 32 000 (28/4 heads): 600-630 us (450-490).
+  const bool full = a.row_type == LTKV_ROWS_F32 || a.softcap > kShortCap ||
+                    (kPairs<T> && a.row_type == LTKV_ROWS_F16);
   const auto kernel = full ? tree_tile_kernel<T, HD, EXACT, true, WC> : tree_tile_kernel<T, HD, EXACT, false, WC>;
   kernel<<<(unsigned)(a.shares * a.n_kv_heads), kTreeThreads, 0, s>>>(a, g.n_blocks, g.kv_dim);
   return hipGetLastError();

@@ -103,6 +103,22 @@ def test_row_types(gpu, shape, dtype, how, rows):
     Trees(shape, dtype, [0, 40, 300, 129], [4, 20, 9, 33], 2, rows=rows).check(**HOW[how])
 
 
+@pytest.mark.parametrize("how", ["plain", "both"])
+@pytest.mark.parametrize("dtype", ["f32", "q8_0"])
+@pytest.mark.parametrize("shape", [(8, 2, 128), (9, 3, 64), (6, 2, 96), (2, 2, 256), (3, 1, 20 + 12)])
+def test_f16_rows_on_pools_of_pairs(gpu, shape, dtype, how):
+    """f16 rows of f32 and 8-bit pools are the f32 rows' results, rounded once."""
+    import torch
+
+    t = Trees(shape, dtype, [300, 7, 65], [9, 20, 1], 12, rows="f16")
+    args, kwargs = t.args(), dict(masks=up(t.masks, np.int32), positions=up(t.positions, np.int32), max_rows=20,
+                                  **HOW[how])
+    got = t.kv.tree_attention(0, *args, **kwargs)
+    want = t.kv.tree_attention(0, args[0].float(), *args[1:], **kwargs)
+    t.kv.synchronize()
+    assert got.dtype is torch.float16 and torch.equal(got, want.half())
+
+
 @pytest.mark.parametrize("dtype", ["f16", "q8_0"])
 @pytest.mark.parametrize("new", [[64, 31, 65], [130, 1, 200], [333, 0, 17]])
 def test_wide_trees(gpu, dtype, new):
