@@ -316,8 +316,11 @@ accept_tree_kernel(AcceptArgs a, int64_t n_blocks, int kv_dim, int elem) {
   const int part = (int)(blockIdx.x - seq * per_seq), layer = part >> 1;
   const bool is_v = part & 1, first = part == 0;
   const int64_t lo = scalar_read(a.row_starts, seq), hi = scalar_read(a.row_starts, seq + 1);
-  const int64_t row0 = lo < 0 ? 0 : lo > a.n_rows ? a.n_rows : lo, row1 = hi > a.n_rows ? a.n_rows : hi;
-  const int32_t m = (int32_t)(row1 > row0 ? row1 - row0 : 0);
+  // starts outside [0, n_rows], or falling ones, give fewer rows, never a row
+  // outside the call's or one that another request has in front
+  const int64_t row0 = lo < 0 ? 0 : lo > a.n_rows ? a.n_rows : lo;
+  const int64_t row1 = hi > a.n_rows ? a.n_rows : hi < row0 ? row0 : hi;
+  const int32_t m = (int32_t)(row1 - row0);
   const int64_t len = scalar_read(a.lens, seq), base = len - m;
   const int32_t *tab = a.tables + seq * a.table_stride;
   if (first) {  // rows of no request
