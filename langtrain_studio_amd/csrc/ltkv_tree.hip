@@ -92,7 +92,9 @@ __global__ void __launch_bounds__(kAnyThreads) tree_any_kernel(TreeArgs a, int64
   float m = -INFINITY, l = 0.f, o[kAnyD];
 #pragma unroll
   for (int k = 0; k < kAnyD; ++k) o[k] = 0.f;
-  for (int32_t t0 = view.from & ~15; t0 < view.len; t0 += kAnyThreads) {
+  // (the window bounds the context alone: a row's drafts lie behind its end, however
+  // far behind them the row's position is)
+  for (int32_t t0 = min(view.from, max(shift, 0)) & ~15; t0 < view.len; t0 += kAnyThreads) {
     const int n_tok = min(view.len - t0, kAnyThreads);
     const bool seen = t < n_tok && (view.sees32(t0 + (t & ~31)) >> (t & 31) & 1);
     __syncthreads();  // sblk and sp of the last round have been read
