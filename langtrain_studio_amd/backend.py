@@ -71,7 +71,7 @@ class DraftStep:
     max_rows: int
     layout: StepLayout       # row starts, lengths, tables, cells, positions, masks
     parents: "object"        # torch.int32 [n]
-    upload: "object" = None  # as StepPlan's
+    ready: "object" = None   # (raw stream, event) behind the layout, to be waited for on other streams
 
 
 DESCRIPTORS = ("tables", "resident", "planned")
@@ -243,10 +243,22 @@ class PagedKvBackend:
         stride = max([1] + [-(-(c + m) // BLOCK) for c, m in zip(lens, counts)])
         arrays = [self.kv.seq_rows(seqs), np.array(lens, np.int32), np.array(counts, np.int32),
                   np.array([p for d in drafts for p in d.parents], np.int32)]
-        (rows, d_lens, d_counts, parents), upload = self._upload(arrays)
+        (rows, d_lens, d_counts, parents), _ = self._upload(arrays)
         layout = self.kv.step_layout(rows, d_lens, d_counts, n, stride, parents=parents, mask_words=words)
+        # (behind the layout, not the upload: the step's arrays are written on the cache's stream)
+        made = torch.cuda.Event()
+        with self.kv._ordered():
+            made.record()
         return DraftStep(n=n, seqs=seqs, lens=lens, ends=[c + m for c, m in zip(lens, counts)],
-                         max_rows=max(counts, default=0), layout=layout, parents=parents, upload=upload)
+                         max_rows=max(counts, default=0), layout=layout, parents=parents,
+                         ready=(self.kv._stream, made))
+
+    def _wait_for(self, step: DraftStep) -> None:
+        """The step's arrays are there for the cache's stream (waits on the host
+        where the cache changed streams since the step was begun)."""
+        if step.ready is not None and step.ready[0] != self.kv._stream:
+            _lib.wait_event(step.ready[1])
+            step.ready = None
 
     def draft_layer(self, step: DraftStep, layer: int, q, k, v, out: Optional[object] = None, rotate: bool = True,
                     softcap: float = 0.0, window: int = 0):
@@ -255,9 +267,7 @@ class PagedKvBackend:
         token's context and ancestors. With rotate the rows are f32, f16 or bf16
         projections and turn by the cache's RoPE table (kv.rope_init_scaled);
         else k and v are f32 rows with RoPE applied."""
-        if step.upload is not None and step.upload[0] != self.kv._stream:  # the cache changed streams since
-            _lib.wait_event(step.upload[1])
-            step.upload = None
+        self._wait_for(step)
         at = step.layout
         if rotate:
             q = self.kv.write_rope_rows(layer, at.slot_mapping, at.positions, k, v, q=q, n_heads=self.n_heads)
@@ -279,6 +289,7 @@ class PagedKvBackend:
         for s, end in zip(step.seqs, step.ends):
             if self.kv.len(s) != end:
                 raise RuntimeError(f"sequence {s} changed since its drafts were begun")
+        self._wait_for(step)
         done = self.kv.accept_tree(at.tables, at.lens, at.row_starts, step.parents, tokens, targets)
         self.kv.synchronize()
         kept = done.accepted.tolist()

@@ -54,20 +54,13 @@ def test_steps_on_moved_streams(gpu, moved, current):
             torch.cuda.synchronize()
         elif moved == "layer":
             b.kv.set_stream(side)
-        outs = [b.draft_layer(step, layer, *rows[layer]) for layer in range(LAYERS)]
+        if not wait and moved == "accept":  # no layer in between: the paths alone
+            b.kv.set_stream(side)
+            outs = []
+        else:
+            outs = [b.draft_layer(step, layer, *rows[layer]) for layer in range(LAYERS)]
         if wait:
             torch.cuda.synchronize()
-        elif moved == "accept":
-            # a second step's layout waits on the old stream; its acceptance comes on the new one
-            torch.cuda.synchronize()
-            with torch.cuda.stream(own):
-                for _ in range(40):
-                    big.mul_(1.0)
-            for s, end in zip(step.seqs, step.lens):
-                b.kv.truncate(s, end)
-            with torch.cuda.stream(own if current == "same" else side):
-                step = b.begin_drafts([Drafts(0, trees[0]), Drafts(1, trees[1])])
-            b.kv.set_stream(side)
         kept, done = b.accept(step, drafted, wanted)
         torch.cuda.synchronize()
         n = [b.kv.len(s) for s in (0, 1)]
@@ -83,5 +76,8 @@ def test_steps_on_moved_streams(gpu, moved, current):
     assert kept == kept2 and max(kept) > 1
     for a, b in zip(arrays, arrays2):
         assert torch.equal(a, b)
+    if moved == "accept":  # (its rows were never written)
+        return
+    assert len(arrays) == len(arrays2) == 4 + LAYERS
     for a, b in zip(pools, pools2):
         np.testing.assert_array_equal(a, b)
