@@ -69,6 +69,7 @@ class DraftStep:
     lens: list               # lengths in front of the drafts
     ends: list               # and behind them
     max_rows: int
+    positions: int           # positions up to its deepest token
     layout: StepLayout       # row starts, lengths, tables, cells, positions, masks
     parents: "object"        # torch.int32 [n]
     ready: "object" = None   # (raw stream, event) behind the layout, to be waited for on other streams
@@ -227,9 +228,14 @@ class PagedKvBackend:
         seqs = [d.seq for d in drafts]
         if len(set(seqs)) != len(seqs) or any(m == 0 for m in counts):
             raise ValueError("drafts need distinct sequences with at least one token each")
+        deepest = []
         for d in drafts:
             if d.parents[0] != -1 or any(not 0 <= p < j for j, p in enumerate(d.parents) if j):
                 raise ValueError(f"parents of sequence {d.seq}: the first is -1, the others name an earlier token")
+            depth = [0] * len(d.parents)
+            for j, p in enumerate(d.parents):
+                depth[j] = depth[p] + 1 if j else 0
+            deepest.append(max(depth))
         lens = [self.kv.len(s) for s in seqs]
         try:
             if n:
@@ -250,8 +256,9 @@ class PagedKvBackend:
         with self.kv._ordered():
             made.record()
         return DraftStep(n=n, seqs=seqs, lens=lens, ends=[c + m for c, m in zip(lens, counts)],
-                         max_rows=max(counts, default=0), layout=layout, parents=parents,
-                         ready=(self.kv._stream, made))
+                         max_rows=max(counts, default=0),
+                         positions=max((c + m + 1 for c, m in zip(lens, deepest)), default=0),
+                         layout=layout, parents=parents, ready=(self.kv._stream, made))
 
     def _wait_for(self, step: DraftStep) -> None:
         """The step's arrays are there for the cache's stream (waits on the host
@@ -265,12 +272,17 @@ class PagedKvBackend:
         """One layer of a step with drafted tokens: k and v ([n][kv_dim]) into the
         claimed cells, then attention of q ([n][n_heads*head_dim]) over each
         token's context and ancestors. With rotate the rows are f32, f16 or bf16
-        projections and turn by the cache's RoPE table (kv.rope_init_scaled);
-        else k and v are f32 rows with RoPE applied."""
+        projections and turn by the cache's RoPE table (kv.rope_init_scaled), which
+        has to reach the step's deepest token; else k and v are f32 rows with RoPE
+        applied."""
+        if rotate and 0 < self.kv._rope_positions < step.positions:
+            raise ValueError(f"the step reaches position {step.positions - 1}, the RoPE table "
+                             f"{self.kv._rope_positions} positions")
         self._wait_for(step)
         at = step.layout
-        if rotate:
-            q = self.kv.write_rope_rows(layer, at.slot_mapping, at.positions, k, v, q=q, n_heads=self.n_heads)
+        if rotate:  # (every token has a position in the table: all rows of q are written)
+            q = self.kv.write_rope_rows(layer, at.slot_mapping, at.positions, k, v, q=q, n_heads=self.n_heads,
+                                        out=self.kv._empty(q.shape, q.dtype))
         else:
             self.kv.write_batch(layer, at.slot_mapping, k, v)
         if out is None:

@@ -153,7 +153,7 @@ class KvCache:
         self.n_blocks = self._lib.ltkv_n_blocks(h)
         self._kv_dim = self._lib.ltkv_kv_dim(h)
         self._plan_shape = None
-        self._rope_dims = 0  # head_dim of the RoPE table
+        self._rope_dims = self._rope_positions = 0  # head_dim and positions of the RoPE table
         self._stream = 0
         if stream is not None:
             self.set_stream(stream)
@@ -314,7 +314,7 @@ class KvCache:
         """RoPE table of Model::rope (model.rs:263-265, 291-308) for write_rope."""
         _check(self._lib.ltkv_rope_init(self._h, float(base), rope_dim, head_dim, 1 if neox else 0,
                                         max_positions))
-        self._rope_dims = head_dim
+        self._rope_dims, self._rope_positions = head_dim, max_positions
 
     def write_rope(self, layer: int, slot_mapping, positions, k, v, q=None, n_heads: int = 0) -> None:
         """Kernel 1 with RoPE (model.rs:414-429): k rotated into its cell, v appended,
@@ -364,13 +364,15 @@ class KvCache:
             self._h, float(base), rope_dim, head_dim, 1 if neox else 0, max_positions, code, float(factor), original,
             float(lo if low is None else low), float(hi if high is None else high),
             None if divisors is None else _np_ptr(divisors), 0.0 if magnitude is None else float(magnitude)))
-        self._rope_dims = head_dim
+        self._rope_dims, self._rope_positions = head_dim, max_positions
 
     def write_rope_rows(self, layer: int, slot_mapping, positions, k, v, q=None, n_heads: int = 0, out=None):
         """write_rope for f32, f16 or bf16 rows: k rotated into its cell, v
         appended, and q ([n][n_heads*head_dim], optional) rotated into out, which
-        is returned (default: a new tensor; out=q rotates in place). Rows may be
-        columns of a wider tensor (unit stride within a row)."""
+        is returned (default: a new tensor; out=q rotates in place). A token whose
+        position is outside the RoPE table is skipped: no cell of it is written, and
+        its row of q is left as it was (zeros in a new out). Rows may be columns of a
+        wider tensor (unit stride within a row)."""
         import torch
 
         n = slot_mapping.numel()
@@ -406,7 +408,7 @@ class KvCache:
             if len(shape) != 2 or shape[0] != n or (self._rope_dims and n_heads * self._rope_dims != shape[1]):
                 raise ValueError("q must be [n][n_heads*head_dim]")
             if out is None:
-                out = self._empty(shape, q.dtype)
+                out = self._zeros_like(q)  # (rows of skipped tokens)
             elif out.shape != shape:
                 raise ValueError("out must match q")
             qp, qs = rows(q, "q")

@@ -7,7 +7,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from test_gpu_drafts import HD, HEADS, KVH, LAYERS, backend, rows_of
+from test_gpu_drafts import LAYERS, backend, rows_of
 from test_gpu_scored import BLOCK, held_rows
 from test_gpu_tree import up
 from tree_definition import random_tree
