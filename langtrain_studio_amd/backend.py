@@ -23,7 +23,7 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import _lib
-from .kv import BLOCK, AcceptedTree, KvCache, StepLayout
+from .kv import BLOCK, AcceptedTree, KvCache, KvCacheFull, StepLayout
 
 
 @dataclass(frozen=True)
@@ -214,9 +214,10 @@ class PagedKvBackend:
     # ---- steps with drafted tokens
     def begin_drafts(self, drafts: Sequence[Drafts]) -> DraftStep:
         """Claims the cells of every sequence's drafted tokens behind its length
-        and lays the step out on the device. All or nothing: where a claim fails
-        (KvCacheFull) the sequences are as they were. Not inside a stream
-        capture."""
+        and lays the step out on the device. All or nothing: where the cache has no
+        room (KvCacheFull) nothing was claimed or copied, and after any other
+        failure the sequences have their lengths back (a block that was copied on
+        write then stays copied). Not inside a stream capture."""
         import torch
 
         if torch.cuda.is_current_stream_capturing():
@@ -237,20 +238,21 @@ class PagedKvBackend:
                 depth[j] = depth[p] + 1 if j else 0
             deepest.append(max(depth))
         lens = [self.kv.len(s) for s in seqs]
+        words = (max(counts, default=1) + 31) // 32
+        stride = max([1] + [-(-(c + m) // BLOCK) for c, m in zip(lens, counts)])
+        self._check_room(seqs, lens, counts)
         try:
             if n:
                 self.kv.append_batch(np.repeat(np.array(seqs, np.uint32), counts),
                                      np.concatenate([c + np.arange(m, dtype=np.uint64) for c, m in zip(lens, counts)]))
-        except Exception:
+            arrays = [self.kv.seq_rows(seqs), np.array(lens, np.int32), np.array(counts, np.int32),
+                      np.array([p for d in drafts for p in d.parents], np.int32)]
+            (rows, d_lens, d_counts, parents), _ = self._upload(arrays)
+            layout = self.kv.step_layout(rows, d_lens, d_counts, n, stride, parents=parents, mask_words=words)
+        except BaseException:
             for s, c in zip(seqs, lens):
                 self.kv.truncate(s, c)
             raise
-        words = (max(counts, default=1) + 31) // 32
-        stride = max([1] + [-(-(c + m) // BLOCK) for c, m in zip(lens, counts)])
-        arrays = [self.kv.seq_rows(seqs), np.array(lens, np.int32), np.array(counts, np.int32),
-                  np.array([p for d in drafts for p in d.parents], np.int32)]
-        (rows, d_lens, d_counts, parents), _ = self._upload(arrays)
-        layout = self.kv.step_layout(rows, d_lens, d_counts, n, stride, parents=parents, mask_words=words)
         # (behind the layout, not the upload: the step's arrays are written on the cache's stream)
         made = torch.cuda.Event()
         with self.kv._ordered():
@@ -259,6 +261,23 @@ class PagedKvBackend:
                          max_rows=max(counts, default=0),
                          positions=max((c + m + 1 for c, m in zip(lens, deepest)), default=0),
                          layout=layout, parents=parents, ready=(self.kv._stream, made))
+
+    def _check_room(self, seqs, lens, counts) -> None:
+        """KvCacheFull where the claims of these tokens would not fit: before the
+        first, since a block that a claim copied on write stays copied."""
+        free = self.kv.free_blocks()
+        # (all partial blocks copied: an upper bound)
+        new = sum(-(-(c + m) // BLOCK) - -(-c // BLOCK) for c, m in zip(lens, counts))
+        if new + sum(c % BLOCK != 0 for c in lens) <= free:
+            return
+        owners = {}  # of the partial blocks: a claim copies one that has other owners left
+        for s, c in zip(seqs, lens):
+            if c % BLOCK:
+                block = int(self.kv.block_table(s)[-1])
+                owners[block] = owners.get(block, self.kv.refcount(block)) - 1
+                new += owners[block] > 0
+        if new > free:
+            raise KvCacheFull(_lib.ERR_FULL, f"KV cache full: the drafts need {new} blocks, {free} are free")
 
     def _wait_for(self, step: DraftStep) -> None:
         """The step's arrays are there for the cache's stream (waits on the host
