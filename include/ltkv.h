@@ -219,7 +219,7 @@ LTKV_API int ltkv_write_rope(ltkv_cache *c, size_t layer, size_t n, const int32_
                     float *d_q, size_t q_stride, size_t n_heads);
 
 /* Scalings of rotary positions for contexts longer than a model was trained on
- * (ltkv_rope_init_scaled). With f_i = base^(-2i / rope_dim), pair i turns per
+ * (ltkv_rope_init_scaled64). With f_i = base^(-2i / rope_dim), pair i turns per
  * position by
  *   PLAIN   f_i;
  *   LINEAR  f_i / factor (positions squeezed into the trained range);
@@ -238,14 +238,21 @@ LTKV_API int ltkv_write_rope(ltkv_cache *c, size_t layer, size_t n, const int32_
 
 /* ltkv_rope_init with scaled frequencies and 64-bit angles: the table holds the
  * f32 values of cos and sin (pos * frequency, all in 64 bits) times the
- * magnitude. factor: of every scaling but PLAIN; original, low and high: of YARN
- * (usually low 1, high 32) and LLAMA3 (low 1, high 4), ignored by the others.
- * divisors (host, [rope_dim / 2], or null): each pair's frequency is divided by
- * its own as well. magnitude: of cosines and sines, 0 for the scaling's own.
+ * magnitude. numbers: host, four doubles, base, factor, low and high. factor: of
+ * every scaling but PLAIN; original, low and high: of YARN (usually low 1, high 32)
+ * and LLAMA3 (low 1, high 4), ignored by the others. divisors (host doubles,
+ * [rope_dim / 2], or null): each pair's frequency is divided by its own as well.
+ * magnitude: of cosines and sines, 0 for the scaling's own.
  * Replaces the cache's table for ltkv_write_rope and ltkv_write_rope_rows once
  * the stream is done with it; a captured append still names the old one. Not
  * under stream capture. No reference counterpart (its positions are unscaled,
  * model.rs:263-265). */
+LTKV_API int ltkv_rope_init_scaled64(ltkv_cache *c, size_t rope_dim, size_t head_dim, int neox,
+                                     size_t max_positions, int scaling, size_t original, const void *numbers,
+                                     const void *divisors, float magnitude);
+
+/* The same from f32 numbers, which are taken as they are: a factor of 1.3f is
+ * 1.2999999523, and pairs at position 131071 turn 4e-3 radians further than by 1.3. */
 LTKV_API int ltkv_rope_init_scaled(ltkv_cache *c, float base, size_t rope_dim, size_t head_dim, int neox,
                                    size_t max_positions, int scaling, float factor, size_t original,
                                    float low, float high, const float *divisors, float magnitude);

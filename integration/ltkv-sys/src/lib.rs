@@ -91,6 +91,9 @@ pub mod ffi {
         pub fn ltkv_write_rope(c: *mut ltkv_cache, layer: usize, n: usize, d_slot_mapping: *const i32,
                                d_positions: *const i32, d_k: *const f32, d_v: *const f32, src_stride: usize,
                                d_q: *mut f32, q_stride: usize, n_heads: usize) -> c_int;
+        pub fn ltkv_rope_init_scaled64(c: *mut ltkv_cache, rope_dim: usize, head_dim: usize, neox: c_int,
+                                       max_positions: usize, scaling: c_int, original: usize,
+                                       numbers: *const c_void, divisors: *const c_void, magnitude: f32) -> c_int;
         pub fn ltkv_rope_init_scaled(c: *mut ltkv_cache, base: f32, rope_dim: usize, head_dim: usize, neox: c_int,
                                      max_positions: usize, scaling: c_int, factor: f32, original: usize, low: f32,
                                      high: f32, divisors: *const f32, magnitude: f32) -> c_int;
@@ -208,10 +211,10 @@ impl RowType {
 #[derive(Clone, Copy, Debug)]
 pub struct RopeScaling {
     pub kind: c_int,
-    pub factor: f32,
+    pub factor: f64,
     pub original: usize,
-    pub low: f32,
-    pub high: f32,
+    pub low: f64,
+    pub high: f64,
     pub magnitude: f32,
 }
 
@@ -530,13 +533,14 @@ impl KvCache {
 
     /// `rope_init` with scaled frequencies and 64-bit angles; `divisors` is empty or
     /// has one entry per pair.
-    pub fn rope_init_scaled(&mut self, base: f32, rope_dim: usize, head_dim: usize, neox: bool, max_positions: usize,
-                            how: &RopeScaling, divisors: &[f32]) -> anyhow::Result<()> {
+    pub fn rope_init_scaled(&mut self, base: f64, rope_dim: usize, head_dim: usize, neox: bool, max_positions: usize,
+                            how: &RopeScaling, divisors: &[f64]) -> anyhow::Result<()> {
         anyhow::ensure!(divisors.is_empty() || divisors.len() == rope_dim / 2, "divisors need one entry per pair");
-        let d = if divisors.is_empty() { std::ptr::null() } else { divisors.as_ptr() };
+        let d = if divisors.is_empty() { std::ptr::null() } else { divisors.as_ptr() as *const c_void };
+        let numbers = [base, how.factor, how.low, how.high];
         check(unsafe {
-            ltkv_rope_init_scaled(self.raw, base, rope_dim, head_dim, neox as c_int, max_positions, how.kind, how.factor,
-                                  how.original, how.low, how.high, d, how.magnitude)
+            ltkv_rope_init_scaled64(self.raw, rope_dim, head_dim, neox as c_int, max_positions, how.kind, how.original,
+                                    numbers.as_ptr() as *const c_void, d, how.magnitude)
         })
     }
 

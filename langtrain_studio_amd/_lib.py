@@ -52,6 +52,7 @@ SIGNATURES = {
     "ltkv_rope_init": (_int, [_vp, _f32, _sz, _sz, _int, _sz]),
     "ltkv_write_rope": (_int, [_vp, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _sz]),
     "ltkv_rope_init_scaled": (_int, [_vp, _f32, _sz, _sz, _int, _sz, _int, _f32, _sz, _f32, _f32, _vp, _f32]),
+    "ltkv_rope_init_scaled64": (_int, [_vp, _sz, _sz, _int, _sz, _int, _sz, _vp, _vp, _f32]),
     "ltkv_write_rope_rows": (_int, [_vp, _sz, _sz, _vp, _vp, _int, _vp, _vp, _sz, _vp, _sz, _sz, _vp, _sz]),
     "ltkv_copy_blocks": (_int, [_vp, _sz, _vp]),
     "ltkv_gather": (_int, [_vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp]),

@@ -1540,11 +1540,12 @@ void rope_frequencies(std::vector<double> &f, double base, size_t rope_dim, int 
   }
 }
 
-}  // namespace
-
-int ltkv_rope_init_scaled(ltkv_cache *c, float base, size_t rope_dim, size_t head_dim, int neox, size_t max_positions,
-                          int scaling, float factor, size_t original, float low, float high, const float *divisors,
-                          float magnitude) {
+// The table of scaled frequencies (ltkv_rope_init_scaled64); `divisors` has rope_dim
+// / 2 entries, or is null.
+extern "C++" template <typename D>
+int rope_init_scaled(ltkv_cache *c, double base, size_t rope_dim, size_t head_dim, int neox, size_t max_positions,
+                     int scaling, double factor, size_t original, double low, double high, const D *divisors,
+                     float magnitude) {
   if (!c) return fail(LTKV_ERR_ARG, "cache is null");
   if (c->device == LTKV_NO_DEVICE) return no_device();
   if (head_dim == 0 || head_dim % 8 != 0 || c->kv_dim % head_dim != 0)
@@ -1554,16 +1555,16 @@ int ltkv_rope_init_scaled(ltkv_cache *c, float base, size_t rope_dim, size_t hea
   if (max_positions == 0 || max_positions > (size_t)INT32_MAX / 2 ||
       max_positions > ((size_t{1} << 32) - 256) / (rope_dim / 2))
     return fail(LTKV_ERR_ARG, "max_positions out of range");
-  if (!(base > 0.f) || std::isinf(base)) return fail(LTKV_ERR_ARG, "rope base must be positive");
+  if (!(base > 0.0) || std::isinf(base)) return fail(LTKV_ERR_ARG, "rope base must be positive");
   if (scaling < LTKV_ROPE_PLAIN || scaling > LTKV_ROPE_LLAMA3) return fail(LTKV_ERR_ARG, "unknown rope scaling %d", scaling);
-  if (scaling != LTKV_ROPE_PLAIN && (!(factor > 0.f) || std::isinf(factor)))
+  if (scaling != LTKV_ROPE_PLAIN && (!(factor > 0.0) || std::isinf(factor)))
     return fail(LTKV_ERR_ARG, "a rope scaling's factor must be positive");
   if (scaling == LTKV_ROPE_YARN || scaling == LTKV_ROPE_LLAMA3) {
     if (original == 0) return fail(LTKV_ERR_ARG, "this rope scaling needs the original context length");
-    if (!(low > 0.f) || !(high > low) || std::isinf(high))
+    if (!(low > 0.0) || !(high > low) || std::isinf(high))
       return fail(LTKV_ERR_ARG, "this rope scaling needs 0 < low < high");
   }
-  if (scaling == LTKV_ROPE_YARN && !(base > 1.f)) return fail(LTKV_ERR_ARG, "this rope scaling needs a base over 1");
+  if (scaling == LTKV_ROPE_YARN && !(base > 1.0)) return fail(LTKV_ERR_ARG, "this rope scaling needs a base over 1");
   if (!(magnitude >= 0.f) || std::isinf(magnitude))
     return fail(LTKV_ERR_ARG, "magnitude must be positive, or 0 for the scaling's own");
   std::vector<double> f;
@@ -1575,10 +1576,12 @@ int ltkv_rope_init_scaled(ltkv_cache *c, float base, size_t rope_dim, size_t hea
   }
   if (divisors) {
     for (size_t i = 0; i < f.size(); ++i) {
-      if (!(divisors[i] > 0.f) || std::isinf(divisors[i])) return fail(LTKV_ERR_ARG, "rope divisors must be positive");
+      if (!(divisors[i] > 0) || std::isinf(divisors[i])) return fail(LTKV_ERR_ARG, "rope divisors must be positive");
       f[i] /= (double)divisors[i];
     }
   }
+  for (const double x : f)
+    if (!std::isfinite(x * (double)max_positions)) return fail(LTKV_ERR_ARG, "rope frequencies out of range");
   DeviceGuard dg(c->device);
   if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
   if (capturing(c)) return fail(LTKV_ERR_ARG, "a rope table cannot be made under stream capture");
@@ -1607,6 +1610,23 @@ int ltkv_rope_init_scaled(ltkv_cache *c, float base, size_t rope_dim, size_t hea
   c->rope_geom.head_dim = (int)head_dim;
   c->rope_geom.neox = neox ? 1 : 0;
   return LTKV_OK;
+}
+
+}  // namespace
+
+int ltkv_rope_init_scaled64(ltkv_cache *c, size_t rope_dim, size_t head_dim, int neox, size_t max_positions, int scaling,
+                            size_t original, const void *numbers, const void *divisors, float magnitude) {
+  if (!numbers) return fail(LTKV_ERR_ARG, "numbers is null");
+  const double *x = static_cast<const double *>(numbers);
+  return rope_init_scaled(c, x[0], rope_dim, head_dim, neox, max_positions, scaling, x[1], original, x[2], x[3],
+                          static_cast<const double *>(divisors), magnitude);
+}
+
+int ltkv_rope_init_scaled(ltkv_cache *c, float base, size_t rope_dim, size_t head_dim, int neox, size_t max_positions,
+                          int scaling, float factor, size_t original, float low, float high, const float *divisors,
+                          float magnitude) {
+  return rope_init_scaled(c, base, rope_dim, head_dim, neox, max_positions, scaling, factor, original, low, high,
+                          divisors, magnitude);
 }
 
 int ltkv_write_rope_rows(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_slot_mapping,

@@ -341,7 +341,7 @@ class KvCache:
                          kind: str = "none", factor: float = 1.0, original: int = 0, low: Optional[float] = None,
                          high: Optional[float] = None, divisors=None, magnitude: Optional[float] = None) -> None:
         """rope_init with frequencies scaled for long contexts
-        (ltkv_rope_init_scaled): kind "none", "linear", "ntk", "yarn" or "llama3" by
+        (ltkv_rope_init_scaled64): kind "none", "linear", "ntk", "yarn" or "llama3" by
         `factor`; yarn and llama3 keep the frequencies of pairs that turn `high`
         (32; 4) times within `original` positions and scale those that turn up to
         `low` (1) times. divisors: one per pair. magnitude: of the cosines and
@@ -357,12 +357,12 @@ class KvCache:
             raise ValueError("magnitude must be positive")
         code, lo, hi = kinds[kind]
         if divisors is not None:
-            divisors = np.ascontiguousarray(divisors, dtype=np.float32).reshape(-1)
+            divisors = np.ascontiguousarray(divisors, dtype=np.float64).reshape(-1)
             if divisors.size != rope_dim // 2:
                 raise ValueError("divisors must have rope_dim / 2 entries")
-        _check(self._lib.ltkv_rope_init_scaled(
-            self._h, float(base), rope_dim, head_dim, 1 if neox else 0, max_positions, code, float(factor), original,
-            float(lo if low is None else low), float(hi if high is None else high),
+        numbers = np.array([base, factor, lo if low is None else low, hi if high is None else high], np.float64)
+        _check(self._lib.ltkv_rope_init_scaled64(
+            self._h, rope_dim, head_dim, 1 if neox else 0, max_positions, code, original, _np_ptr(numbers),
             None if divisors is None else _np_ptr(divisors), 0.0 if magnitude is None else float(magnitude)))
         self._rope_dims, self._rope_positions = head_dim, max_positions
 
