@@ -227,7 +227,8 @@ LTKV_API int ltkv_write_rope(ltkv_cache *c, size_t layer, size_t n, const int32_
  *   YARN    a blend of f_i / factor and f_i by how often the pair turns within
  *           `original` positions: f_i where that is `high` times or more, f_i /
  *           factor at `low` times or less, linear in i between (its ends rounded
- *           outward to whole pairs); cosines and sines times 1 + 0.1 ln(factor);
+ *           outward to whole pairs); cosines and sines times 1 + 0.1 ln(factor)
+ *           where factor is over 1;
  *   LLAMA3  the same blend, linear in the number of turns between `low` and
  *           `high`. */
 #define LTKV_ROPE_PLAIN 0

@@ -1536,7 +1536,7 @@ void rope_frequencies(std::vector<double> &f, double base, size_t rope_dim, int 
       const double blend = std::min(std::max(((double)i - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
       f[i] = f[i] / factor * blend + f[i] * (1.0 - blend);
     }
-    *magnitude = 0.1 * std::log(factor) + 1.0;
+    *magnitude = factor > 1.0 ? 0.1 * std::log(factor) + 1.0 : 1.0;  // (1 where no context is added)
   }
 }
 

@@ -64,3 +64,16 @@ def test_refusals(gpu):
         with pytest.raises(KvError, match=match):
             kv.rope_init_scaled(1e4, 64, 64, True, 1000, **how)
     assert _lib.load().ltkv_rope_init_scaled64(kv._h, 64, 64, 0, 100, 0, 0, None, None, 0.0) == _lib.ERR_ARG
+
+
+@pytest.mark.parametrize("factor,magnitude", [(0.25, 1.0), (1.0, 1.0), (1e-6, 1.0), (2.0, 0.1 * np.log(2.0) + 1.0)])
+def test_yarn_magnitudes(gpu, factor, magnitude):
+    """Contexts that are not stretched keep the rows' size; a magnitude given is taken."""
+    for own in (True, False):
+        kv, slots, positions, q, k, v = rope_case("f32", "f32", (4, 2, 64), 64, True, "none", 20, 5, top=500)
+        kv.rope_init_scaled(10000.0, 64, 64, True, 500, kind="yarn", factor=factor, original=128,
+                            magnitude=None if own else 0.75)
+        f, _ = frequencies(10000.0, 64, "yarn", factor, 128)
+        out = kv.write_rope_rows(0, up(slots, np.int32), up(positions, np.int32), k, v, q=q, n_heads=4)
+        kv.synchronize()
+        check_rotation(down(out), down(q), positions, 64, 64, True, f, magnitude if own else 0.75, "f32")
