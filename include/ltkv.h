@@ -432,9 +432,10 @@ LTKV_API int ltkv_scored_attention(ltkv_cache *c, size_t layer, size_t n, size_t
  *   row's position p = d_positions[row] (at least C; needed with a window only:
  *   for a tree it is C plus the row's depth);
  *   the rows' cells C + j for which bit j % 32 of word j / 32 of its mask is set
- *   (d_masks [n_rows][mask_words]; rows past the words are not seen; the window
- *   does not bound these). Without d_masks a row sees the rows up to its own, as
- *   in a prompt chunk.
+ *   (d_masks [n_rows][mask_words]; rows past the words are not seen). The window
+ *   does not bound these: where drafts may be as deep as it, bound the masks by
+ *   it first (ltkv_window_masks). Without d_masks a row sees all rows up to its own
+ *   (a prompt chunk whose rows the window bounds too is ltkv_scored_attention's).
  * The score of a position is scale * q.k, capped to softcap * tanh(s / softcap)
  * where softcap > 0 (caps over 2^96 count as that); the output is V weighted by the
  * softmax of the scores over what the row sees, zeros where that is nothing.
@@ -485,6 +486,16 @@ LTKV_API int ltkv_step_layout(ltkv_cache *c, size_t n, const int32_t *d_rows, co
                               const int32_t *d_parents, size_t mask_words, int32_t *d_row_starts,
                               int32_t *d_new_lens, int32_t *d_tables, int32_t *d_slot_mapping,
                               int32_t *d_positions, int32_t *d_masks);
+
+/* Masks for a layer with a window: d_out [n_rows][mask_words] gets the bits of
+ * d_masks that stand for rows less than `window` positions in front of the row
+ * that holds them, as a token decoded alone would see them. Sequence i (of n) has
+ * the rows [d_row_starts[i], d_row_starts[i+1]), at d_positions (ltkv_step_layout's).
+ * Bits of rows that the sequence does not have are cleared, and so are the masks of
+ * rows of no sequence. d_out may be d_masks, or apart from the inputs. */
+LTKV_API int ltkv_window_masks(ltkv_cache *c, size_t n, size_t n_rows, const int32_t *d_row_starts,
+                               const int32_t *d_positions, const int32_t *d_masks, size_t mask_words,
+                               size_t window, int32_t *d_out);
 
 /* Keeps what the model agrees with of every request's drafted tree, in all layers.
  * Request i's rows lie as in ltkv_tree_attention (d_lens with the drafts); its

@@ -136,6 +136,9 @@ pub mod ffi {
                                 d_counts: *const i32, n_tokens: usize, table_stride: usize, d_parents: *const i32,
                                 mask_words: usize, d_row_starts: *mut i32, d_new_lens: *mut i32, d_tables: *mut i32,
                                 d_slot_mapping: *mut i32, d_positions: *mut i32, d_masks: *mut i32) -> c_int;
+        pub fn ltkv_window_masks(c: *mut ltkv_cache, n: usize, n_rows: usize, d_row_starts: *const i32,
+                                 d_positions: *const i32, d_masks: *const i32, mask_words: usize, window: usize,
+                                 d_out: *mut i32) -> c_int;
         pub fn ltkv_accept_tree(c: *mut ltkv_cache, n: usize, n_rows: usize, d_tables: *const i32,
                                 table_stride: usize, d_lens: *const i32, d_row_starts: *const i32,
                                 d_parents: *const i32, d_tokens: *const i32, d_targets: *const i32,

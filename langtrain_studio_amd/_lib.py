@@ -66,6 +66,7 @@ SIGNATURES = {
     "ltkv_tree_attention": (_int, [_vp, _sz, _sz, _sz, _sz, _sz, _sz, _f32, _f32, _sz, _vp, _vp, _sz, _int, _vp, _vp,
                                    _sz, _vp, _vp, _vp]),
     "ltkv_step_layout": (_int, [_vp, _sz, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ltkv_window_masks": (_int, [_vp, _sz, _sz, _vp, _vp, _vp, _sz, _sz, _vp]),
     "ltkv_accept_tree": (_int, [_vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "ltkv_set_attention_partition": (_int, [_vp, _sz]),
     "ltkv_set_attention_engine": (_int, [_vp, _int]),

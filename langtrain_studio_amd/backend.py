@@ -70,6 +70,7 @@ class DraftStep:
     ends: list               # and behind them
     max_rows: int
     positions: int           # positions up to its deepest token
+    depth: int               # of the deepest token in its tree
     layout: StepLayout       # row starts, lengths, tables, cells, positions, masks
     parents: "object"        # torch.int32 [n]
     ready: "object" = None   # (raw stream, event) behind the layout, to be waited for on other streams
@@ -260,6 +261,7 @@ class PagedKvBackend:
         return DraftStep(n=n, seqs=seqs, lens=lens, ends=[c + m for c, m in zip(lens, counts)],
                          max_rows=max(counts, default=0),
                          positions=max((c + m + 1 for c, m in zip(lens, deepest)), default=0),
+                         depth=max(deepest, default=0),
                          layout=layout, parents=parents, ready=(self.kv._stream, made))
 
     def _check_room(self, seqs, lens, counts) -> None:
@@ -290,7 +292,8 @@ class PagedKvBackend:
                     softcap: float = 0.0, window: int = 0):
         """One layer of a step with drafted tokens: k and v ([n][kv_dim]) into the
         claimed cells, then attention of q ([n][n_heads*head_dim]) over each
-        token's context and ancestors. With rotate the rows are f32, f16 or bf16
+        token's context and ancestors, with window > 0 those less than that many
+        positions back. With rotate the rows are f32, f16 or bf16
         projections and turn by the cache's RoPE table (kv.rope_init_scaled), which
         has to reach the step's deepest token; else k and v are f32 rows with RoPE
         applied."""
@@ -306,8 +309,11 @@ class PagedKvBackend:
             self.kv.write_batch(layer, at.slot_mapping, k, v)
         if out is None:
             out = self.kv._empty(q.shape, q.dtype)  # (every row is a sequence's)
+        masks = at.masks
+        if 0 < window <= step.depth:  # (shallower trees lie inside the window)
+            masks = self.kv.window_masks(at.row_starts, at.positions, masks, window)
         return self.kv.tree_attention(layer, q, at.tables, at.lens, self.n_heads, self.head_dim, at.row_starts,
-                                      positions=at.positions, masks=at.masks, max_rows=max(step.max_rows, 1),
+                                      positions=at.positions, masks=masks, max_rows=max(step.max_rows, 1),
                                       scale=self.scale, softcap=softcap, window=window, out=out)
 
     def accept(self, step: DraftStep, tokens, targets) -> tuple[list, AcceptedTree]:

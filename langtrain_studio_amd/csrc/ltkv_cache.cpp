@@ -2229,6 +2229,30 @@ int ltkv_step_layout(ltkv_cache *c, size_t n, const int32_t *d_rows, const int32
   return LTKV_OK;
 }
 
+int ltkv_window_masks(ltkv_cache *c, size_t n, size_t n_rows, const int32_t *d_row_starts, const int32_t *d_positions,
+                      const int32_t *d_masks, size_t mask_words, size_t window, int32_t *d_out) {
+  if (!c) return fail(LTKV_ERR_ARG, "cache is null");
+  if (c->device == LTKV_NO_DEVICE) return no_device();
+  if (n_rows > (size_t)INT32_MAX / 2 || n > (size_t)INT32_MAX / 2 || mask_words > (size_t)INT32_MAX / 32)
+    return fail(LTKV_ERR_ARG, "%zu rows of %zu sequences are too many for one call", n_rows, n);
+  if (n == 0 || n_rows == 0) return LTKV_OK;
+  if (mask_words == 0) return fail(LTKV_ERR_ARG, "masks need at least one word a row");
+  if (window == 0) return fail(LTKV_ERR_ARG, "window must be > 0");
+  if (!d_row_starts || !d_positions || !d_masks || !d_out) return fail(LTKV_ERR_ARG, "null device pointer");
+  const size_t word = sizeof(int32_t), bytes = n_rows * mask_words * word;
+  if (overlap(d_out, bytes, d_row_starts, (n + 1) * word) || overlap(d_out, bytes, d_positions, n_rows * word) ||
+      (d_out != d_masks && overlap(d_out, bytes, d_masks, bytes)))
+    return fail(LTKV_ERR_ARG, "inputs and outputs overlap: they are read after others are written");
+  DeviceGuard dg(c->device);
+  if (!dg.ok) return fail(LTKV_ERR_HIP, "hipSetDevice(%d) failed", c->device);
+  const ltkv::WindowMasks a{d_row_starts, d_positions, d_masks, (int64_t)n, (int64_t)n_rows, (int64_t)mask_words,
+                            (int64_t)std::min<size_t>(window, (size_t)INT32_MAX), d_out};
+  const hipError_t e = ltkv::launch_window_masks(a, c->stream);
+  if (e == hipErrorInvalidValue) return fail(LTKV_ERR_ARG, "too many masks for one launch");
+  if (e != hipSuccess) return hip_fail(e, "window masks launch");
+  return LTKV_OK;
+}
+
 int ltkv_accept_tree(ltkv_cache *c, size_t n, size_t n_rows, const int32_t *d_tables, size_t table_stride,
                      const int32_t *d_lens, const int32_t *d_row_starts, const int32_t *d_parents,
                      const int32_t *d_tokens, const int32_t *d_targets, int32_t *d_accepted, int32_t *d_path,

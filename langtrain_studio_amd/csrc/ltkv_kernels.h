@@ -455,6 +455,15 @@ struct LayoutArgs {
 };
 hipError_t launch_step_layout(const LayoutArgs &a, hipStream_t s);
 
+// The masks of a step's rows without what lies `window` positions or more in front
+// of them (ltkv_window_masks).
+struct WindowMasks {
+  const int32_t *row_starts, *positions, *masks;
+  int64_t n, n_rows, words, window;
+  int32_t *out;
+};
+hipError_t launch_window_masks(const WindowMasks &a, hipStream_t s);
+
 // The accepted path of drafted trees and the move of its rows (ltkv_accept_tree).
 struct AcceptArgs {
   void *k, *v, *k_scale, *v_scale;  // whole pools

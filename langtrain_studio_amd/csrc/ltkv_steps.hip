@@ -4,6 +4,7 @@
 //   rope_table_kernel       cosines and sines of scaled rotary frequencies
 //   write_rope_rows_kernel  K rotated into its cells, V appended, Q rotated, for rows of any type
 //   step_layout_kernel      row starts, lengths, tables, slots, positions and masks of a step
+//   window_masks_kernel     a step's masks for a layer with a window
 //   accept_tree_kernel      the accepted path of every tree, and its rows moved together
 #include <hip/hip_runtime.h>
 
@@ -298,6 +299,32 @@ __global__ void __launch_bounds__(kStepThreads) step_layout_kernel(LayoutArgs a,
   }
 }
 
+// ---- masks of a layer with a window --------------------------------------------
+
+// A thread a word: the sequence by bisection, then the positions of the rows whose
+// bits are set. Bound by latency (one launch).
+__global__ void __launch_bounds__(256) window_masks_kernel(WindowMasks a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.n_rows * a.words) return;
+  const int64_t row = i / a.words, word = i - row * a.words;
+  int64_t lo = 0, hi = a.n;  // the last sequence whose first row is not behind the row
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) / 2;
+    if ((int64_t)a.row_starts[mid] <= row) lo = mid;
+    else hi = mid;
+  }
+  const int64_t row0 = a.row_starts[lo], row1 = a.row_starts[lo + 1];
+  uint32_t kept = 0;
+  if (row0 >= 0 && row >= row0 && row < row1) {
+    const int64_t from = (int64_t)a.positions[row] - a.window;  // positions up to it are not seen
+    for (uint32_t bits = (uint32_t)a.masks[i]; bits; bits &= bits - 1) {
+      const int64_t other = row0 + 32 * word + __builtin_ctz(bits);
+      if (other < row1 && other < a.n_rows && a.positions[other] > from) kept |= bits & -bits;
+    }
+  }
+  a.out[i] = (int32_t)kept;
+}
+
 // ---- acceptance --------------------------------------------------------------
 
 // Rows moved at a time: all of them are read before one is written, which is safe
@@ -476,6 +503,14 @@ hipError_t launch_step_layout(const LayoutArgs &a, hipStream_t s) {
   const int64_t wgs = (a.n + 1) * std::max(slices, 1);
   if (wgs >= (int64_t{1} << 24)) return hipErrorInvalidValue;
   step_layout_kernel<<<(unsigned)wgs, kStepThreads, 0, s>>>(a, std::max(slices, 1));
+  return hipGetLastError();
+}
+
+hipError_t launch_window_masks(const WindowMasks &a, hipStream_t s) {
+  const int64_t wgs = (a.n_rows * a.words + 255) / 256;
+  if (wgs <= 0) return hipSuccess;
+  if (wgs >= (int64_t{1} << 24)) return hipErrorInvalidValue;
+  window_masks_kernel<<<(unsigned)wgs, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 

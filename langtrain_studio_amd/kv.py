@@ -526,8 +526,9 @@ class KvCache:
         ([n_rows][n_heads*head_dim], f32, f16 or bf16), the last cells of its
         lens[i] positions. A row sees the context in front of them (with window >
         0: less than that many positions back from positions[row], int32
-        [n_rows]) and the rows whose bits its masks (int32 [n_rows][words]) hold;
-        without masks the rows up to its own. softcap > 0: scores become softcap
+        [n_rows]) and the rows whose bits its masks (int32 [n_rows][words]) hold,
+        window or not (window_masks bounds them by it); without masks the rows up
+        to its own. softcap > 0: scores become softcap
         * tanh(score / softcap). max_rows: the most rows of one sequence (a hint;
         default: as many as there are). Rows of no sequence are left as they were
         (zeros in a new out)."""
@@ -627,6 +628,38 @@ class KvCache:
             None if counts is None else _dev_ptr(counts, int32, "counts", dev), n_tokens, table_stride,
             None if parents is None else _dev_ptr(parents, int32, "parents", dev),
             mask_words if parents is not None else 0, *pointers))
+        return out
+
+    def window_masks(self, row_starts, positions, masks, window: int, out=None):
+        """masks (int32 [n_rows][words]) without the rows that lie `window`
+        positions or more in front of the one that sees them (ltkv_window_masks),
+        for the layers of a model that have a window. All int32 device tensors,
+        as step_layout gives them; out: a new tensor, or one to fill (masks
+        itself, too)."""
+        import torch
+
+        if masks.dim() != 2 or masks.shape[1] == 0:
+            raise ValueError("masks must be [n_rows][words], of at least one word")
+        n, n_rows = row_starts.numel() - 1, masks.shape[0]
+        if n < 0:
+            raise ValueError("row_starts must have one entry per sequence and one more")
+        if positions.numel() != n_rows:
+            raise ValueError("positions must have one entry per row")
+        if window <= 0:
+            raise ValueError("window must be positive")
+        int32, dev = torch.int32, self.device
+        if out is None:
+            out = self._empty(masks.shape, int32)
+        elif out.shape != masks.shape:
+            raise ValueError("out must match masks")
+        if n == 0 or n_rows == 0:
+            with self._ordered():
+                out.zero_()
+            return out
+        _check(self._lib.ltkv_window_masks(
+            self._h, n, n_rows, _dev_ptr(row_starts, int32, "row_starts", dev),
+            _dev_ptr(positions, int32, "positions", dev), _dev_ptr(masks, int32, "masks", dev), masks.shape[1], window,
+            _dev_ptr(out, int32, "out", dev)))
         return out
 
     def accept_tree(self, tables, lens, row_starts, parents, tokens, targets,
