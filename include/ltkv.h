@@ -442,12 +442,12 @@ LTKV_API int ltkv_scored_attention(ltkv_cache *c, size_t layer, size_t n, size_t
  * Positions a row does not see do not enter its result, whatever they hold; what
  * a row that sees an infinity or NaN gives is not specified (it is not finite
  * where a visible V is not).
- * f32 rows, and f16 rows on f32 and Q8_0 pools, are computed to f32 accuracy, other
- * rows with weights (and bf16 rows' V of f32 and Q8_0 pools) rounded to f16, summed
- * in f32. An element of K or V of these pools keeps 22 bits down to 2^16 below the
- * largest of its position's head (f32: of its block's 16 positions where every row of
- * a tile sees them), V also only down to 2^16 below the largest that the row sees, and
- * fewer below that.
+ * Rows of any type are computed to f32 accuracy and rounded to their type once
+ * (16-bit rows on F16 and Q4_0 pools with caps up to 256: the tanh to 3e-7). An
+ * element of K or V of an F32 pool keeps its bits down to 2^16 below the largest of
+ * its position's head (or of its block's 16 positions where every row of a tile sees
+ * them), Q8_0 and F32 V also only down to 2^16 below the largest that the row sees,
+ * and fewer below that.
  * max_rows: the most rows of one sequence, which sizes the tiles (one with more is
  * computed all the same). head_dim a multiple of 8 up to 256 and groups of up to
  * 64 run on the matrix cores, others on a generic kernel; head_dim up to 1024. Rows

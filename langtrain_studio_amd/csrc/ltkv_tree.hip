@@ -204,9 +204,9 @@ __device__ __forceinline__ int64_t uniform64(int64_t x) {
 }
 
 // What a position's K and V hold as products' operands: f16 and q4_0 cells are f16
-// numbers; q8_0 and f32 cells enter as f16 hi + lo pairs (22 bits) times a power of
-// two of the position's own, so that no row loses bits to a position that it does
-// not see.
+// numbers; q8_0 and f32 cells enter as f16 hi + lo pairs (a q8_0 element exactly, an
+// f32 one but for its last bit at most) times a power of two of the position's own, so that
+// no row loses bits to a position that it does not see.
 template <typename T>
 constexpr bool kPairs = std::is_same_v<T, int8_t> || std::is_same_v<T, float>;
 
@@ -369,7 +369,6 @@ struct Cells<int8_t, HD, EXACT, NT> {
   // the fused multiply-add gives exactly (d times a power of two is one too, down to
   // 2^-22 of the largest scale).
   // Returns the largest power of the lane's positions.
-  template <int PLANES>
   __device__ __forceinline__ float put(char *lds, int plane, int pitch, int lane, uint32_t bad, float *pow,
                                        bool) const {
     float most = 0.f;
@@ -386,7 +385,7 @@ struct Cells<int8_t, HD, EXACT, NT> {
         const h8 q = i8x8_to_h8(u32x2{x[j][2 * i], x[j][2 * i + 1]}), hi = q * d8;
         char *const to = lds + row(lane, j) * pitch + lane % ROW * (2 * E) + 16 * i;
         *reinterpret_cast<h8 *>(to) = hi;
-        if constexpr (PLANES == 2) *reinterpret_cast<h8 *>(to + plane) = __builtin_elementwise_fma(q, d8, -hi);
+        *reinterpret_cast<h8 *>(to + plane) = __builtin_elementwise_fma(q, d8, -hi);
       }
     }
     return most;
@@ -423,9 +422,9 @@ struct Cells<float, HD, EXACT, NT> {
   }
   // Powers of at least 2^-100: smaller values are nothing beside their products'
   // rounding. Each position has its own where a row does not see all of the step;
-  // else the block's 16 share one (a reduction instead of eight). Parts by
-  // truncation, two an instruction.
-  template <int PLANES>
+  // else the block's 16 share one (a reduction instead of eight). Parts to nearest: by
+  // truncation the largest term of the result's error (8 trees of 8 f32 rows behind
+  // 8000 positions: 7.2e-7, so 5.8e-7; 155 us, 160).
   __device__ __forceinline__ float put(char *lds, int plane, int pitch, int lane, uint32_t bad, float *pow,
                                        bool apart) const {
     int e[N];
@@ -452,14 +451,13 @@ struct Cells<float, HD, EXACT, NT> {
           const uint32_t u = bad >> j & 1 ? 0u : x[j][2 * i + k];
           v[k] = __builtin_amdgcn_ldexpf(__builtin_bit_cast(float, u), -e[j]);
         }
-        hi[i] = PLANES == 1 ? h2{(_Float16)v[0], (_Float16)v[1]}
-                            : __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(v[0], v[1]));
-        lo[i] = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi[i].x, -1.f, v[0]),
-                                                                  __builtin_fmaf((float)hi[i].y, -1.f, v[1])));
+        hi[i] = h2{(_Float16)v[0], (_Float16)v[1]};
+        lo[i] = h2{(_Float16)__builtin_fmaf((float)hi[i].x, -1.f, v[0]),
+                   (_Float16)__builtin_fmaf((float)hi[i].y, -1.f, v[1])};
       }
       char *const to = lds + row(lane, j) * pitch + lane % ROW * 8;
       *reinterpret_cast<h4 *>(to) = h4{hi[0].x, hi[0].y, hi[1].x, hi[1].y};
-      if constexpr (PLANES == 2) *reinterpret_cast<h4 *>(to + plane) = h4{lo[0].x, lo[0].y, lo[1].x, lo[1].y};
+      *reinterpret_cast<h4 *>(to + plane) = h4{lo[0].x, lo[0].y, lo[1].x, lo[1].y};
     }
     return 0.f;
   }
@@ -499,9 +497,13 @@ struct Column {
 // place, numerators^T += V^T W (a lane's scores are positions 8 (r / 4) + 4 (lane /
 // 32) + r % 4 of its column, which is the second product's operand layout when its
 // 16 positions are taken as 4 (lane / 32) ... + 3 and 8 + 4 (lane / 32) ... + 3: no
-// exchange). FULL (f32 rows, f16 rows on pools of pairs, and any rows with a cap
-// over kShortCap): Q and the weights as hi + lo pairs; else Q as it is (times a power of
-// two), the weights and V rounded to f16.
+// exchange). The weights enter as hi + lo pairs for rows of any type: rounded to f16,
+// they took f16 rows' error from 2.07e-4, the output's own rounding, to 2.44e-4 (16
+// trees of 64 rows over a 4-bit cache, capped; 104 us, 94 so) and bf16 rows' from
+// 1.66e-3 to 1.68e-3, and either off what f32 arithmetic gives by as much as its
+// rounding. FULL (f32 rows, and any rows with a cap over kShortCap): Q as hi + lo pairs
+// and the cap's tanh to f32 accuracy; else Q as it is, times a power of two, and on pools
+// that are no pairs the tanh off by up to 3e-7, below a sixth of a 16-bit row's rounding.
 // Of pairs (kPairs) the scores are multiplied by their position's power of two, and
 // so are the weights. f32 pools: a column's numerators have a reference of their own
 // (`top_o`): the largest weight times V, not the largest weight, lies near the top of
@@ -526,11 +528,11 @@ __global__ void __launch_bounds__(kTreeThreads, tree_groups_a_cu(std::is_same_v<
 tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   constexpr int NC = HD / 32, NK = HD / 16, WP = kTreeWaves / WC, U = 2 / WP;
   constexpr bool PAIRS = kPairs<T>, BYTES = std::is_same_v<T, int8_t>, WIDE = PAIRS && !BYTES;
-  constexpr int K_PLANES = PAIRS ? 2 : 1, V_PLANES = PAIRS && FULL ? 2 : 1;
+  constexpr int PLANES = PAIRS ? 2 : 1;
   constexpr int K_PITCH = HD * 2 + 16;  // rows 4 banks apart: 16-byte reads of 16 rows without conflicts
   constexpr int V_PITCH = HD * 2 + 64;  // rows 16 banks apart, for the transposing reads
   constexpr int K_BYTES = kTreeTokens * K_PITCH, V_BYTES = kTreeTokens * V_PITCH;
-  constexpr int STEP_BYTES = K_PLANES * K_BYTES + V_PLANES * V_BYTES;
+  constexpr int STEP_BYTES = PLANES * (K_BYTES + V_BYTES);
   constexpr int FOLD = NC * 16 + 4;  // floats that a lane hands over where waves share columns
   // Few columns (WC 2) are bound by the pool's bytes: two steps ahead of the products,
   // in registers that Q leaves free in LDS.
@@ -548,7 +550,7 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   __shared__ int32_t s_rows[kTreeThreads][3];  // of the last sequence that a thread looked at: first row, rows, length
   __shared__ int32_t s_from[kTreeWaves];
   __shared__ float s_top[kTreeWaves];  // 8-bit pools: the largest power of a wave's positions' V
-  char *const lds_k = lds, *const lds_v = lds + K_PLANES * K_BYTES;
+  char *const lds_k = lds, *const lds_v = lds + PLANES * K_BYTES;
 
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cw = wave % WC, pw = wave / WC;
@@ -748,10 +750,9 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
         }
       }
       if constexpr (PAIRS) {
-        cells.k.template put<2>(lds_k + 16 * wave * K_PITCH, K_BYTES, K_PITCH, lane, 0, s_kpow + 16 * wave, partial);
+        cells.k.put(lds_k + 16 * wave * K_PITCH, K_BYTES, K_PITCH, lane, 0, s_kpow + 16 * wave, partial);
         const float v_top =
-            cells.v.template put<V_PLANES>(lds_v + 16 * wave * V_PITCH, V_BYTES, V_PITCH, lane, bad, s_vpow + 16 * wave,
-                                              partial);
+            cells.v.put(lds_v + 16 * wave * V_PITCH, V_BYTES, V_PITCH, lane, bad, s_vpow + 16 * wave, partial);
         if constexpr (BYTES) {
           const float x = lanes_max<64>(v_top);
           if (lane == 0) s_top[wave] = x;
@@ -824,7 +825,7 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float x = sc[u][i] * to_x;
-            sc[u][i] = (FULL ? tanh_f32(x) : tanh_f16(x)) * cap_scale;
+            sc[u][i] = (FULL || PAIRS ? tanh_f32(x) : tanh_f16(x)) * cap_scale;
           }
         m = 1.f;
       }
@@ -885,7 +886,7 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           sc[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], m, base));
-          if constexpr (FULL || PAIRS) sum += sc[u][i];
+          sum += sc[u][i];
         }
       if constexpr (BYTES) {
 #pragma unroll
@@ -928,29 +929,26 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
       }
 #pragma unroll
       for (int p = 0; p < 2 * U; ++p) {  // 16 positions each
-        // hi parts of pairs by truncation (two an instruction; the lo parts take what
-        // is left), alone to nearest
+        // hi and lo parts of the weights. By truncation: the lo parts take what is left
+        // of hi, and 21 bits are past every other rounding but those of f32 pools.
         h8 wh, wl;
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
-          const float x = sc[p >> 1][8 * (p & 1) + i], y = sc[p >> 1][8 * (p & 1) + i + 1];
-          if constexpr (FULL) {
-            const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x, y));
-            const h2 lo = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi.x, -1.f, x),
-                                                                           __builtin_fmaf((float)hi.y, -1.f, y)));
-            wh[i] = hi.x;
-            wh[i + 1] = hi.y;
-            wl[i] = lo.x;
-            wl[i + 1] = lo.y;
+          float x = sc[p >> 1][8 * (p & 1) + i], y = sc[p >> 1][8 * (p & 1) + i + 1];
+          h2 hi, lo;
+          if constexpr (WIDE) {
+            asm("" : "+v"(x), "+v"(y));  // (f32 numbers, as in split2)
+            hi = h2{(_Float16)x, (_Float16)y};
+            lo = h2{(_Float16)__builtin_fmaf((float)hi.x, -1.f, x), (_Float16)__builtin_fmaf((float)hi.y, -1.f, y)};
           } else {
-            wh[i] = (_Float16)x;
-            wh[i + 1] = (_Float16)y;
+            hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x, y));
+            lo = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi.x, -1.f, x),
+                                                                   __builtin_fmaf((float)hi.y, -1.f, y)));
           }
-        }
-        if constexpr (!FULL && !PAIRS) {  // the weights as they enter the product, two an instruction
-          const h2 one = {(_Float16)1.f, (_Float16)1.f};
-#pragma unroll
-          for (int i = 0; i < 8; i += 2) sum = __builtin_amdgcn_fdot2(h2{wh[i], wh[i + 1]}, one, sum, false);
+          wh[i] = hi.x;
+          wh[i + 1] = hi.y;
+          wl[i] = lo.x;
+          wl[i + 1] = lo.y;
         }
         const char *vp = lds_v + (32 * pw * U + 16 * p + 4 * half + ((lane & 15) >> 2)) * V_PITCH +
                          (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
@@ -958,8 +956,8 @@ tree_tile_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
         for (int i = 0; i < NC; ++i) {
           const h8 x = read_tr2(vp + 64 * i, 8 * V_PITCH);
           o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wh, o[i], 0, 0, 0);
-          if constexpr (FULL) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wl, o[i], 0, 0, 0);
-          if constexpr (V_PLANES == 2) {
+          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wl, o[i], 0, 0, 0);
+          if constexpr (PAIRS) {
             const h8 y = read_tr2(vp + V_BYTES + 64 * i, 8 * V_PITCH);
             o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, wh, o[i], 0, 0, 0);
           }
@@ -1124,12 +1122,9 @@ int tile_waves(const TreeArgs &a) {
 
 template <typename T, int HD, bool EXACT, int WC>
 hipError_t launch_tiles(const PoolGeom &g, const TreeArgs &a, hipStream_t s) {
-  // f16 rows on pools of pairs too: weights and V rounded to f16 would each be off by
-  // as much as their output's rounding (relative error 3.2e-4 against 2.1e-4), which
-  // bf16 rows do not see. 8 trees of 8 rows behind 8000 positions, q8_0: 72 us (59 with
-  // them rounded); of 44 behind 32 000 (28/4 heads): 600-630 us (450-490).
-  const bool full = a.row_type == LTKV_ROWS_F32 || a.softcap > kShortCap ||
-                    (kPairs<T> && a.row_type == LTKV_ROWS_F16);
+  // (16-bit rows' Q has no lo part. 8 trees of 44 f16 rows behind 32 000 positions of
+  // a q8_0 cache, 28/4 heads: 550 us with the products of zeros, 510 without)
+  const bool full = a.row_type == LTKV_ROWS_F32 || a.softcap > kShortCap;
   const auto kernel = full ? tree_tile_kernel<T, HD, EXACT, true, WC> : tree_tile_kernel<T, HD, EXACT, false, WC>;
   kernel<<<(unsigned)(a.shares * a.n_kv_heads), kTreeThreads, 0, s>>>(a, g.n_blocks, g.kv_dim);
   return hipGetLastError();
