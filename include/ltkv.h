@@ -262,7 +262,7 @@ LTKV_API int ltkv_rope_init_scaled(ltkv_cache *c, float base, size_t rope_dim, s
  * elements): K rotated in f32 (each product and sum rounded, as there) and
  * stored as ltkv_write stores f32 rows; V stored so; Q, when d_q is not null,
  * rotated into d_q_out and rounded to row_type. d_q_out may be d_q with the same
- * stride, or rows apart from q, k and v (columns of one [q | k | v] buffer are). A
+ * stride, or rows apart from q, k and v (other columns of their buffer are). A
  * token with a position outside the table is skipped, Q too; one with a negative
  * or out-of-range cell rotates Q only. Row pointers 16-byte aligned, strides
  * whole 16-byte pieces, head_dim up to 512. No two rows may have one cell. */

@@ -1629,6 +1629,21 @@ int ltkv_rope_init_scaled(ltkv_cache *c, float base, size_t rope_dim, size_t hea
                           divisors, magnitude);
 }
 
+namespace {
+
+// Whether n rows of `a` elements every a_stride of them and n rows of b share no byte:
+// their memory is apart, or they are different columns of one buffer ([q | k | v] rows).
+bool rows_apart(const void *a, size_t a_stride, size_t a_len, const void *b, size_t b_stride, size_t b_len, size_t n,
+                size_t size) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  if (x >= y + ((n - 1) * b_stride + b_len) * size || y >= x + ((n - 1) * a_stride + a_len) * size) return true;
+  if (a_stride != b_stride) return false;
+  const size_t row = b_stride * size, at = x >= y ? (x - y) % row : (row - (y - x) % row) % row;  // of a in a row of b
+  return at >= b_len * size && at + a_len * size <= row;
+}
+
+}  // namespace
+
 int ltkv_write_rope_rows(ltkv_cache *c, size_t layer, size_t n, const int32_t *d_slot_mapping,
                          const int32_t *d_positions, int row_type, const void *d_k, const void *d_v, size_t src_stride,
                          const void *d_q, size_t q_stride, size_t n_heads, void *d_q_out, size_t q_out_stride) {
@@ -1657,29 +1672,14 @@ int ltkv_write_rope_rows(ltkv_cache *c, size_t layer, size_t n, const int32_t *d
     return fail(LTKV_ERR_ARG, "q strides must be >= n_heads * head_dim and whole 16-byte pieces");
   if (((uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_q | (uintptr_t)d_q_out) % 16 != 0)
     return fail(LTKV_ERR_ARG, "K/V/Q rows must be 16-byte aligned");
-  if (d_q && !(d_q == d_q_out && q_stride == q_out_stride)) {  // in place, or apart
-    // (rows of one buffer may interleave: q as columns of a wider output is refused too)
-    const uintptr_t in = (uintptr_t)d_q, out = (uintptr_t)d_q_out;
-    const size_t in_bytes = ((n - 1) * q_stride + n_heads * hd) * size;
-    const size_t out_bytes = ((n - 1) * q_out_stride + n_heads * hd) * size;
-    if (in < out + out_bytes && out < in + in_bytes)
-      return fail(LTKV_ERR_ARG, "q and its output overlap: they are the same rows or apart");
-  }
-  if (d_q) {  // K and V rows are read while Q's are written
-    const uintptr_t out = (uintptr_t)d_q_out;
-    const size_t out_bytes = ((n - 1) * q_out_stride + n_heads * hd) * size;
-    const size_t src_bytes = ((n - 1) * src_stride + c->kv_dim) * size;
-    for (const void *src : {d_k, d_v}) {
-      const uintptr_t in = (uintptr_t)src;
-      if (!(in < out + out_bytes && out < in + src_bytes)) continue;
-      // columns of one buffer ([q | k | v] rows): apart if a row's columns are
-      const bool columns = src_stride == q_out_stride;
-      const size_t row = q_out_stride * size;
-      const size_t at = columns ? (in >= out ? (in - out) % row : (row - (out - in) % row) % row) : 0;
-      if (!columns || at < n_heads * hd * size || at + c->kv_dim * size > row)
-        return fail(LTKV_ERR_ARG, "q's output overlaps the rows of K or V");
-    }
-  }
+  // Q in place or apart from its output; K and V, which are read while Q's rows are
+  // written, apart from it.
+  if (d_q && !(d_q == d_q_out && q_stride == q_out_stride) &&
+      !rows_apart(d_q, q_stride, n_heads * hd, d_q_out, q_out_stride, n_heads * hd, n, size))
+    return fail(LTKV_ERR_ARG, "q and its output overlap: they are the same rows or apart");
+  if (d_q && !(rows_apart(d_k, src_stride, c->kv_dim, d_q_out, q_out_stride, n_heads * hd, n, size) &&
+               rows_apart(d_v, src_stride, c->kv_dim, d_q_out, q_out_stride, n_heads * hd, n, size)))
+    return fail(LTKV_ERR_ARG, "q's output overlaps the rows of K or V");
   ltkv::RopeRows a{d_slot_mapping, d_positions, row_type, d_k, d_v, d_q, d_q_out, (int64_t)n, (int64_t)src_stride,
                    (int64_t)q_stride, (int64_t)q_out_stride, d_q ? (int)n_heads : 0};
   if (d_q && n_heads > (size_t)INT32_MAX / 2 - c->kv_dim) return fail(LTKV_ERR_ARG, "too many heads");
