@@ -233,7 +233,8 @@ __device__ __forceinline__ int32_t asked(const LayoutArgs &a, int64_t i) {
 }
 
 // A work-group takes a slice of a request's tokens and table entries; it adds up
-// the requests in front of its own by itself, so that the step is one launch. The
+// the requests in front of its own by itself, so that the step is one launch (for up
+// to some thousand requests: 4096 13 us, 16 384 93 us, growing with the square). The
 // last ones write the rows behind the last token. A token's mask is its way up
 // the tree: its bits fall from word to word, so no word is written twice. Bound by
 // latency (counts, then tables): 64 trees of 16 to 64 tokens 6.4 us, 48 prompts 4.3.
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(kStepThreads) step_layout_kernel(LayoutArgs a,
 // ---- masks of a layer with a window --------------------------------------------
 
 // A thread a word: the sequence by bisection, then the positions of the rows whose
-// bits are set. Bound by latency (one launch).
+// bits are set. Bound by latency: 5 us.
 __global__ void __launch_bounds__(256) window_masks_kernel(WindowMasks a) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= a.n_rows * a.words) return;
@@ -461,9 +462,15 @@ template <int ELEM, typename R>
 hipError_t launch_rope_rows_t(const PoolGeom &g, void *k_layer, void *v_layer, void *k_scale, void *v_scale,
                               const RopeRows &a, const RopeGeom &r, hipStream_t s) {
   // A token's waves: four while the tokens are few (a wave's loads then wait for one
-  // another), one where they fill the chip (32/8 heads of 128, bf16, into f16 cells, us
-  // with four, two and one: 256 tokens 5.0, 5.9, 8.2; 1000: 7.9, 7.8, 9.3; 2000: 12.2,
-  // 11.0, 12.1; 3000: 17.1, 15.0, 14.8; 13 000: 65, 57, 57).
+  // another), two where they begin to fill the chip, one behind that, which short rows
+  // gain by. Whole calls, us with four, two and one:
+  //              32/8 x 128 bf16, f16    32/8 x 96 f32, q8_0   32/4 x 64 bf16   9/3 x 64 f32
+  //   512 tokens  7.9   7.9   8.4         8.0   8.2   9.0      7.9  8.1  8.0    8.0  8.1  7.9
+  //   1024        7.9   7.9   9.1         9.3   9.6  10.6      7.9  7.9  7.9    7.9  7.7  8.2
+  //   2048       12.8  11.2  12.3        16.3  14.7  15.9      9.1  8.0  8.0    8.3  8.1  8.0
+  //   4800       24.9  22.2  21.2        31.9  29.5  28.5     17.6 13.9 12.7   14.9 11.2 10.8
+  //   13 000     64.7  57.2  57.4         103  89.0  88.5     39.7 28.5 25.9   36.8 25.1 22.7
+  //   24 000      123   108   114         184   153   153     70.1 48.8 43.0   64.5 42.8 35.6
   const int team = a.n <= 1024 ? 256 : a.n <= 2560 ? 128 : 64;
   const int64_t wgs = (a.n + 256 / team - 1) / (256 / team);
   if (wgs >= (int64_t{1} << 24)) return hipErrorInvalidValue;

@@ -68,7 +68,8 @@ constexpr int kAnyD = kAnyMaxHeadDim / kAnyThreads;
 // Any shape and pool: a work-group takes a (row, query head), 256 positions a
 // round, a score a thread, then each thread up to four output elements over the
 // round's visible positions. It serves shapes that the tile kernel does not, and
-// is bound by its scalar loads.
+// is bound by its scalar loads (8 trees of 8 rows behind 2000 positions: 71 heads of 64
+// over one 2.0 ms, where 64 heads on the tile kernel take 27 us; 8/2 heads of 320 1.3 ms).
 template <typename T>
 __global__ void __launch_bounds__(kAnyThreads) tree_any_kernel(TreeArgs a, int64_t n_blocks, int64_t kv_dim) {
   __shared__ float sq[kAnyMaxHeadDim];
@@ -241,7 +242,7 @@ __device__ __forceinline__ float lanes_max(float x) {
 // positions of one block, whose address is uniform. A load takes whole rows of the
 // head, ROW lanes each, 64 / ROW rows an instruction: with 64 bytes of 16 rows an
 // instruction, lines were fetched in two pieces (64 trees of up to 16 rows, f16: the
-// loads alone 197 us; so, past the caches, 160). EXACT: head_dim is HD, 64 or 128; else
+// kernel with nothing but its loads 197 us; so, past the caches, 160). EXACT: head_dim is HD, 64 or 128; else
 // elements past head_dim are zeros, and 8-bit and 4-bit chunks of 8 bring a scale
 // each (a head may begin inside a group of 32).
 // put() writes the positions' rows in LDS; `bad` has a bit for each load whose V
@@ -513,14 +514,15 @@ struct Column {
 // their waves too few registers (f32, one step of 8 rows: 18 us with spills).
 //
 // Measured (32/8 heads of 128 unless said): 64 trees of 10 to 16 bf16 rows behind 2048
-// to 4096 positions of an f16 cache 171-179 us (842 MB, 4.9 TB/s), bound by the reads:
-// loads alone with the same pieces take 138 us, and a tile's end costs a work-group 7
-// to 10 us (Q is read behind the K and V on their way). 8 trees of 40 to 48 f32 rows
-// behind 32 000 positions of a q8_0 cache (28/4 heads) 570-620 us: three products of
-// pairs (486 GFLOP: products 42% of the cycles, vector instructions 40%, partly
-// overlapped). 16 trees of 64 f16 rows, capped, over a 4-bit cache in a window of 2048:
-// 90 us, vector instructions 52% (cap and softmax). One tree of 8 rows behind 400
-// positions: 8.7 us, latency.
+// to 4096 positions of an f16 cache 172-184 us (842 MB read, 26 MB of parts written),
+// bound by the reads: a kernel of the same loads alone takes 138 us, and a tile's end
+// costs a work-group 7 to 10 us (Q is read behind the K and V on their way). 8 trees of
+// 40 to 48 f32 rows behind 32 000 positions of a q8_0 cache (28/4 heads) 570-620 us:
+// three products of pairs (486 GFLOP: products 42% of the cycles, vector instructions
+// 41%, partly overlapped). 16 trees of 64 f16 rows, capped, over a 4-bit cache in a
+// window of 2048: 102 us (vector instructions 53% of the cycles, products 25%, one after
+// the other; waves wait a third of their time; 85 parts of 32 tiles, 44 MB written). One
+// tree of 8 rows behind 400 positions: 8.7 us, latency.
 constexpr int tree_groups_a_cu(bool wide, int hd) { return wide || hd > 128 ? 1 : 2; }
 
 template <typename T, int HD, bool EXACT, bool FULL, int WC>
