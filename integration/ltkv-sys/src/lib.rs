@@ -611,6 +611,14 @@ impl KvCache {
                                d_row_starts, d_new_lens, d_tables, d_slot_mapping, d_positions, d_masks))
     }
 
+    /// A step's masks for a layer with a window (`ltkv_window_masks`); `d_out` may be
+    /// `d_masks`.
+    pub unsafe fn window_masks(&mut self, n: usize, n_rows: usize, d_row_starts: *const i32,
+                               d_positions: *const i32, d_masks: *const i32, mask_words: usize, window: usize,
+                               d_out: *mut i32) -> anyhow::Result<()> {
+        check(ltkv_window_masks(self.raw, n, n_rows, d_row_starts, d_positions, d_masks, mask_words, window, d_out))
+    }
+
     /// Keeps the path of every drafted tree that the model agrees with
     /// (`ltkv_accept_tree`); truncate the sequences to d_new_lens.
     pub unsafe fn accept_tree(&mut self, n: usize, n_rows: usize, d_tables: *const i32, table_stride: usize,

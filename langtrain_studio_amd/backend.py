@@ -154,6 +154,9 @@ class PagedKvBackend:
         buf.copy_(host[:total], non_blocking=ordered)
         if ordered:
             event.record(stream)
+        else:  # (the current stream's memory, which the cache's launches still read when the step is dropped)
+            with self.kv._ordered():
+                buf.record_stream(torch.cuda.current_stream(dev))
         views = [buf[o:o + a.size].view(a.shape) for a, o in zip(arrays, offs)]
         return views, (stream.cuda_stream, event) if ordered else None
 
@@ -321,7 +324,9 @@ class PagedKvBackend:
         targets (int32 [n] on the device) are the drafted tokens and what the model
         chose behind each. Waits for the device, and truncates the sequences to
         what was kept; returns the tokens kept of each sequence, and the arrays on
-        the device (the token behind them is next)."""
+        the device (the token behind them is next). Where the wait reports a fault the
+        sequences keep the step's cells, of whose rows some may have moved: truncate
+        them to step.lens."""
         at = step.layout
         for s, end in zip(step.seqs, step.ends):
             if self.kv.len(s) != end:

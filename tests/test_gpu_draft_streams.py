@@ -7,7 +7,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from test_gpu_drafts import LAYERS, backend, rows_of
+from test_gpu_drafts import HD, HEADS, KVH, LAYERS, backend, rows_of
 from test_gpu_scored import BLOCK, held_rows
 from test_gpu_tree import up
 from tree_definition import random_tree
@@ -81,3 +81,73 @@ def test_steps_on_moved_streams(gpu, moved, current):
     assert len(arrays) == len(arrays2) == 4 + LAYERS
     for a, b in zip(pools, pools2):
         np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("n", [1, 8])
+def test_uploads_outlive_their_step(gpu, n):
+    """A step begun on another stream than the cache's and dropped at once: its layout,
+    held back, still reads what was uploaded, whatever the current stream allocates."""
+    import torch
+
+    from langtrain_studio_amd import Drafts
+
+    own, side = torch.cuda.Stream(), torch.cuda.Stream()
+    big = torch.ones(1 << 28, device="cuda")
+    rng = np.random.default_rng(n)
+    trees = [random_tree(rng, 20, 0.3) for _ in range(n)]
+    want = None
+    for late in (False, True):
+        b = backend(stream=own)
+        for s in range(n):
+            b.kv.append_batch(np.full(s, s, np.uint32), np.arange(s, dtype=np.uint64))
+        torch.cuda.synchronize()
+        if late:
+            with torch.cuda.stream(own):
+                for _ in range(40):  # some 15 ms of work in front of the layout
+                    big.mul_(1.0)
+        with torch.cuda.stream(side):
+            step = b.begin_drafts([Drafts(s, p) for s, p in enumerate(trees)])
+            layout, size = step.layout, step.parents.untyped_storage().nbytes() // 4
+            del step
+            filled = [torch.full((size,), 99, dtype=torch.int32, device="cuda") for _ in range(8)]
+        torch.cuda.synchronize()
+        b.kv.synchronize()
+        got = [x.cpu() for x in layout]
+        want = want or got
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+        del filled
+
+
+@pytest.mark.parametrize("descriptor", ["tables", "resident"])
+def test_uploads_of_plain_steps_outlive_their_plan(gpu, descriptor):
+    import torch
+
+    from langtrain_studio_amd import BatchToken, PagedKvBackend
+
+    own, side = torch.cuda.Stream(), torch.cuda.Stream()
+    big = torch.ones(1 << 28, device="cuda")
+    n, want = 40, None
+    q, k, v = rows_of(range(n), 0, torch.float32)
+    for late in (False, True):
+        b = PagedKvBackend(LAYERS, HEADS, KVH, HD, 2000, n_seq_max=n, descriptor=descriptor, stream=own)
+        with torch.cuda.stream(side):
+            plan = b.begin_step([BatchToken(0, 0, s) for s in range(n)])
+        b.layer(plan, 0, q, k, v)  # (sizes what is sized on demand)
+        out = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        if late:
+            with torch.cuda.stream(own):
+                for _ in range(40):
+                    big.mul_(1.0)
+        with torch.cuda.stream(side):
+            plan = b.begin_step([BatchToken(0, 1, s) for s in range(n)])
+            size = plan.lens.untyped_storage().nbytes() // 4
+            b.layer(plan, 0, q, k, v, out=out)
+            del plan
+            filled = [torch.full((size,), 99, dtype=torch.int32, device="cuda") for _ in range(8)]
+        torch.cuda.synchronize()
+        b.kv.synchronize()
+        want = out if want is None else want
+        assert torch.equal(out, want)
+        del filled
